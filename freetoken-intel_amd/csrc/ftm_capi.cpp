@@ -48,6 +48,11 @@ int scratch_of_current_device(void** ptr) {
 
 bool dt_ok(int dt) { return dt == FTM_DT_F32 || dt == FTM_DT_F16 || dt == FTM_DT_BF16; }
 
+unsigned dt_bytes(int dt) { return dt == FTM_DT_F32 ? 4 : 2; }
+
+// Rows of dtype dt summed into (or a gradient taken from) tokens of dtype ot.
+bool row_dt_ok(int dt, int ot) { return dt_ok(dt) && dt_ok(ot) && (dt == ot || dt == FTM_DT_F32); }
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // Whether the register-dequant MFMA engine takes this projection (else the
@@ -421,6 +426,102 @@ int ftm_dequant(const ftm_proj* proj, int32_t slot, void* out, int32_t out_dtype
   if (!dt_ok(out_dtype)) return FTM_ERR_FORMAT;
   if (out == nullptr) return FTM_ERR_NULL;
   return hip_rc(launch_dequant(*proj, slot, out, out_dtype, transpose_out ? 1 : 0, (hipStream_t)stream));
+}
+
+int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride, int8_t* q,
+                   int64_t q_stride, float* scale, void* stream) {
+  if (!dt_ok(x_dtype)) return FTM_ERR_FORMAT;
+  if (rows < 0 || rows > INT32_MAX || K <= 0 || x_stride < 0 || q_stride < K) return FTM_ERR_DIM;
+  if (rows == 0) return FTM_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)x | (uint64_t)x_stride) % dt_bytes(x_dtype) != 0 || ((uintptr_t)scale & 3u) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_quant_int8(x, x_dtype, rows, K, x_stride, q, q_stride, scale, (hipStream_t)stream));
+}
+
+int ftm_w8a8_linear(const ftm_w8a8* call, void* stream) {
+  if (call == nullptr) return FTM_ERR_NULL;
+  const ftm_w8a8& c = *call;
+  if (c.K <= 0 || c.K > FTM_W8A8_MAX_K || c.N <= 0 || c.rows < 0 || c.rows > INT32_MAX || c.x_rows < 0 ||
+      c.x_rows > INT32_MAX || c.x_stride < 0 || c.w_stride < 0)
+    return FTM_ERR_DIM;
+  if (!dt_ok(c.w_scale_dtype) || !dt_ok(c.out_dtype) || (c.bias != nullptr && !dt_ok(c.bias_dtype)))
+    return FTM_ERR_FORMAT;
+  if (c.act < -1 || c.act > FTM_ACT_SWIGLU_OAI) return FTM_ERR_FORMAT;
+  if (c.act >= 0 && c.N % 2 != 0) return FTM_ERR_DIM;
+  if (c.w_packed && c.K % 4 != 0) return FTM_ERR_DIM;
+  if (c.num_experts < 1 || c.num_experts > kMaxExperts || (c.offsets == nullptr && c.num_experts != 1))
+    return FTM_ERR_DIM;
+  if (c.num_experts > 1 && c.w_stride < (int64_t)c.N * c.K) return FTM_ERR_DIM;
+  if (c.rows == 0) return FTM_OK;
+  if (c.out == nullptr || c.w == nullptr || c.w_scale == nullptr) return FTM_ERR_NULL;
+  // without an index every row of the output is one of x; with one x may be empty
+  if (c.row_index == nullptr && c.x_rows < c.rows) return FTM_ERR_DIM;
+  if (c.x_rows == 0) return FTM_ERR_DIM;
+  if (c.x == nullptr || c.x_scale == nullptr) return FTM_ERR_NULL;
+  if (c.x_rows > 1 && c.x_stride < c.K) return FTM_ERR_DIM;
+  if (((uintptr_t)c.x_scale & 3u) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_w8a8(c, (hipStream_t)stream));
+}
+
+size_t ftm_sort_workspace_bytes(int32_t T, int32_t k, int32_t num_experts) {
+  if (T <= 0 || k <= 0 || num_experts <= 0 || num_experts > kMaxExperts) return 0;
+  return sort_workspace_bytes((int64_t)T * k, num_experts);
+}
+
+int ftm_sort_tokens(const void* ids, int32_t ids_dtype, int32_t T, int32_t k, int32_t num_experts, int32_t* offsets,
+                    int32_t* row_of_pair, int32_t* pair_of_row, int32_t* token_of_row, void* workspace,
+                    size_t ws_bytes, void* stream) {
+  if (ids_dtype != FTM_ID_I32 && ids_dtype != FTM_ID_I64) return FTM_ERR_FORMAT;
+  if (T < 0 || k <= 0 || num_experts <= 0 || num_experts > kMaxExperts || (int64_t)T * k >= INT32_MAX)
+    return FTM_ERR_DIM;
+  if (offsets == nullptr) return FTM_ERR_NULL;
+  if (T > 0 && (ids == nullptr || row_of_pair == nullptr || pair_of_row == nullptr || token_of_row == nullptr))
+    return FTM_ERR_NULL;
+  const size_t need = sort_workspace_bytes((int64_t)T * k, num_experts);
+  if (need > 0 && (workspace == nullptr || ws_bytes < need)) return FTM_ERR_WORKSPACE;
+  if (need > 0 && ((uintptr_t)workspace & 3u) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_sort(ids, ids_dtype == FTM_ID_I64, (int64_t)T * k, k, num_experts, offsets, row_of_pair,
+                            pair_of_row, token_of_row, workspace, (hipStream_t)stream));
+}
+
+int ftm_gather_tokens(const void* x, int64_t x_stride, int32_t elem_bytes, int32_t H, const int32_t* row_of_pair,
+                      int32_t T, int32_t k, void* rows, void* stream) {
+  if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return FTM_ERR_FORMAT;
+  if (T < 0 || k <= 0 || H <= 0 || H > (1 << 28) || x_stride < 0 || (int64_t)T * k >= INT32_MAX) return FTM_ERR_DIM;
+  if (T == 0) return FTM_OK;
+  if (x == nullptr || row_of_pair == nullptr || rows == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)x | (uintptr_t)rows | (uint64_t)x_stride) % elem_bytes != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_gather(x, x_stride, elem_bytes, H, row_of_pair, T, k, rows, (hipStream_t)stream));
+}
+
+int ftm_combine_tokens(const void* rows, int32_t dtype, int64_t row_stride, const void* w, int32_t w_dtype,
+                       const int32_t* row_of_pair, int32_t T, int32_t k, int32_t H, void* out, int32_t out_dtype,
+                       void* stream) {
+  if (!row_dt_ok(dtype, out_dtype) || (w != nullptr && !dt_ok(w_dtype))) return FTM_ERR_FORMAT;
+  if (T < 0 || k <= 0 || H <= 0 || H > (1 << 28) || row_stride < 0 || (int64_t)T * k >= INT32_MAX) return FTM_ERR_DIM;
+  if (T == 0) return FTM_OK;
+  if (rows == nullptr || row_of_pair == nullptr || out == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)rows | (uint64_t)row_stride) % dt_bytes(dtype) != 0 || (uintptr_t)out % dt_bytes(out_dtype) != 0)
+    return FTM_ERR_ALIGN;
+  return hip_rc(launch_combine(rows, dtype, row_stride, w, w_dtype, row_of_pair, T, k, H, out, out_dtype,
+                               (hipStream_t)stream));
+}
+
+int ftm_combine_tokens_grad(const void* g, int32_t g_dtype, int64_t g_stride, const void* rows, int32_t dtype,
+                            int64_t row_stride, const void* w, int32_t w_dtype, const int32_t* row_of_pair,
+                            int32_t T, int32_t k, int32_t H, void* grad_rows, void* grad_w, void* stream) {
+  if (!row_dt_ok(dtype, g_dtype) || !dt_ok(w_dtype)) return FTM_ERR_FORMAT;
+  if (T < 0 || k <= 0 || H <= 0 || H > (1 << 28) || g_stride < 0 || row_stride < 0 || (int64_t)T * k >= INT32_MAX)
+    return FTM_ERR_DIM;
+  if (T == 0 || (grad_rows == nullptr && grad_w == nullptr)) return FTM_OK;
+  if (g == nullptr || row_of_pair == nullptr || (grad_w != nullptr && rows == nullptr) ||
+      (grad_rows != nullptr && w == nullptr))
+    return FTM_ERR_NULL;
+  if (((uintptr_t)g | (uint64_t)g_stride) % dt_bytes(g_dtype) != 0 || (uintptr_t)grad_rows % dt_bytes(dtype) != 0)
+    return FTM_ERR_ALIGN;
+  if (grad_w != nullptr && ((uintptr_t)rows | (uint64_t)row_stride) % dt_bytes(dtype) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_combine_grad(g, g_dtype, g_stride, rows, dtype, row_stride, w, w_dtype, row_of_pair, T, k, H,
+                                    grad_rows, grad_w, (hipStream_t)stream));
 }
 
 int ftm_copy_slots(void* dev_pool, const void* host_bank, int64_t row_bytes, const int32_t* evict_slots,

@@ -210,5 +210,20 @@ hipError_t launch_experts_generic(const ftm_moe_layer& L, const void* x, int T, 
                                   const WsLayout& wl, hipStream_t st);
 hipError_t launch_dequant(const ftm_proj& P, int slot, void* out, int out_dt, int transpose,
                           hipStream_t st);
+// ftm_w8a8.hip (strides in bytes)
+hipError_t launch_quant_int8(const void* x, int dt, int64_t rows, int K, int64_t x_stride, int8_t* q,
+                             int64_t q_stride, float* scale, hipStream_t st);
+hipError_t launch_w8a8(const ftm_w8a8& call, hipStream_t st);
+// ftm_sort.hip
+size_t sort_workspace_bytes(int64_t pairs, int E);
+hipError_t launch_sort(const void* ids, bool ids64, int64_t pairs, int k, int E, int32_t* offsets,
+                       int32_t* row_of_pair, int32_t* pair_of_row, int32_t* token_of_row, void* ws, hipStream_t st);
+hipError_t launch_gather(const void* x, int64_t x_stride, int elem, int H, const int32_t* row_of_pair, int T, int k,
+                         void* rows, hipStream_t st);
+hipError_t launch_combine(const void* rows, int dt, int64_t row_stride, const void* w, int w_dt,
+                          const int32_t* row_of_pair, int T, int k, int H, void* out, int out_dt, hipStream_t st);
+hipError_t launch_combine_grad(const void* g, int g_dt, int64_t g_stride, const void* rows, int dt, int64_t row_stride,
+                               const void* w, int w_dt, const int32_t* row_of_pair, int T, int k, int H,
+                               void* grad_rows, void* grad_w, hipStream_t st);
 
 }  // namespace ftm

@@ -26,6 +26,7 @@ import sys
 # them where both sit in one basic block.
 NEED = {
     "v_mfma_f32_16x16x32_bf16": 8,
+    "v_mfma_i32_16x16x64_i8": 8,
     "v_mfma_f32_16x16x4_f32": 10,
     "v_mfma_scale_f32_16x16x128_f8f6f4": 12,  # with an e4m3 operand (fp4 x fp4 would need fewer)
     "v_mfma_f32_32x32x1_2b_f32": 18,

@@ -9,6 +9,7 @@ binding (python/freetoken/kernel/cpu_moe.py:195-245), minus its JIT compiler.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -42,6 +43,11 @@ DT_BF16 = 2
 ROUTE_SOFTMAX_TOPK = 0
 ROUTE_SOFTMAX_TOPK_LOWP = 1
 ROUTE_TOPK_SOFTMAX = 2
+
+ID_I32 = 0
+ID_I64 = 1
+
+W8A8_MAX_K = 131071
 
 ACT_SILU = 0
 ACT_GELU = 1
@@ -124,6 +130,35 @@ class FtmMoeLayer(ctypes.Structure):
     ]
 
 
+class FtmW8A8(ctypes.Structure):
+    """``ftm_w8a8``: one int8 x int8 product, dense or grouped by expert."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("row_index", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("x_rows", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("w_stride", ctypes.c_int64),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("num_experts", ctypes.c_int32),
+        ("w_packed", ctypes.c_int32),
+        ("w_scale_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("act_alpha", ctypes.c_float),
+        ("act_limit", ctypes.c_float),
+    ]
+
+
 # Every symbol include/ftmoe.h declares (tests check the export table against this).
 EXPORTED = (
     "ftm_version",
@@ -138,6 +173,13 @@ EXPORTED = (
     "ftm_linear",
     "ftm_expert_forward",
     "ftm_dequant",
+    "ftm_quant_int8",
+    "ftm_w8a8_linear",
+    "ftm_sort_workspace_bytes",
+    "ftm_sort_tokens",
+    "ftm_gather_tokens",
+    "ftm_combine_tokens",
+    "ftm_combine_tokens_grad",
     "ftm_lru_ensure",
     "ftm_lru_materialize",
     "ftm_copy_slots",
@@ -199,6 +241,20 @@ def lib() -> ctypes.CDLL:
     L.ftm_expert_forward.argtypes = [P_layer, i32, vp, i32, vp, vp, sz, vp]
     L.ftm_dequant.restype = ctypes.c_int
     L.ftm_dequant.argtypes = [P_proj, i32, vp, i32, i32, vp]
+    L.ftm_quant_int8.restype = ctypes.c_int
+    L.ftm_quant_int8.argtypes = [vp, i32, i64, i32, i64, vp, i64, vp, vp]
+    L.ftm_w8a8_linear.restype = ctypes.c_int
+    L.ftm_w8a8_linear.argtypes = [ctypes.POINTER(FtmW8A8), vp]
+    L.ftm_sort_workspace_bytes.restype = sz
+    L.ftm_sort_workspace_bytes.argtypes = [i32, i32, i32]
+    L.ftm_sort_tokens.restype = ctypes.c_int
+    L.ftm_sort_tokens.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, sz, vp]
+    L.ftm_gather_tokens.restype = ctypes.c_int
+    L.ftm_gather_tokens.argtypes = [vp, i64, i32, i32, vp, i32, i32, vp, vp]
+    L.ftm_combine_tokens.restype = ctypes.c_int
+    L.ftm_combine_tokens.argtypes = [vp, i32, i64, vp, i32, vp, i32, i32, i32, vp, i32, vp]
+    L.ftm_combine_tokens_grad.restype = ctypes.c_int
+    L.ftm_combine_tokens_grad.argtypes = [vp, i32, i64, vp, i32, i64, vp, i32, vp, i32, i32, i32, vp, vp, vp]
     L.ftm_lru_ensure.restype = ctypes.c_int
     L.ftm_lru_ensure.argtypes = [i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]
     L.ftm_lru_materialize.restype = ctypes.c_int
@@ -258,6 +314,24 @@ def stream_of(t) -> int:
     import torch
 
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device_of(t):
+    """The context a launch on ``t``'s stream needs: ``t``'s device current."""
+    import torch
+
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def require_same_device(t, others) -> None:
+    """``others``: (name, tensor or None) pairs that have to be on ``t``'s device."""
+    for name, o in others:
+        if o is not None and o.device != t.device:
+            require_gpu(o, name)
+            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
 
 
 def ptr(t) -> Optional[int]:

@@ -265,6 +265,87 @@ int ftm_expert_forward(const ftm_moe_layer* layer, int32_t slot, const void* x,
 int ftm_dequant(const ftm_proj* proj, int32_t slot, void* out, int32_t out_dtype,
                 int32_t transpose_out, void* stream);
 
+/* ---- int8 activations x int8 weights ----
+ * The reference has INT8 weights under wide activations only (fused_int8_linear
+ * above); these take the activations in int8 too, one scale per token. */
+
+/* Quantise rows x [rows, K] (x_stride bytes apart) to int8: scale[m] =
+ * fp32(max_k |x[m, k]| / 127), the maximum taken as at least 1e-12; q[m, k] =
+ * the whole number nearest x[m, k] / scale[m], ties to even (q_stride bytes
+ * between rows).  A row with an infinity or NaN gets the scale NaN and codes 0. */
+int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride,
+                   int8_t* q, int64_t q_stride, float* scale, void* stream);
+
+/* One product: out[m, n] = (sum_k x[i, k] w[n, k]) * x_scale[i] * w_scale[n]
+ * (+ bias[n]), i = m or row_index[m], the sum exact in int32 (K <= 131071), one
+ * rounding to out_dtype.  With act >= 0 the weight rows [0, N/2) are gate and
+ * [N/2, N) up and out[m, n] = act(gate) * up, n < N/2.
+ * Grouped (offsets not NULL): rows [offsets[e], offsets[e+1]) take weight e;
+ * the other rows, and rows whose row_index names no row of x, become zeros. */
+typedef struct ftm_w8a8 {
+  const int8_t* x;         /* [x_rows, K], rows x_stride bytes apart */
+  const float* x_scale;    /* [x_rows] */
+  const void* w;           /* int8 [N, K] per expert; w_packed: int32 [N, K/4], bytes + 128 */
+  const void* w_scale;     /* [N] per expert, w_scale_dtype */
+  const void* bias;        /* [N] per expert, bias_dtype, or NULL */
+  void* out;               /* [rows, N] (act: [rows, N/2]), out_dtype */
+  const int32_t* offsets;  /* device [num_experts + 1], or NULL: one weight */
+  const int32_t* row_index;/* device [rows]: row of x of each output row, or NULL: the same row */
+  int64_t rows;            /* output rows */
+  int64_t x_rows;
+  int64_t x_stride;
+  int64_t w_stride;        /* bytes between the experts' weights */
+  int32_t N;
+  int32_t K;
+  int32_t num_experts;     /* <= 512; 1 without offsets */
+  int32_t w_packed;
+  int32_t w_scale_dtype;
+  int32_t bias_dtype;
+  int32_t out_dtype;
+  int32_t act;             /* FTM_ACT_*, or -1: none */
+  float act_alpha;         /* FTM_ACT_SWIGLU_OAI */
+  float act_limit;
+} ftm_w8a8;
+#define FTM_W8A8_MAX_K 131071
+int ftm_w8a8_linear(const ftm_w8a8* call, void* stream);
+
+/* ---- (token, expert) pairs sorted by expert, and back ----
+ * ids [T, k] int32 or int64 (ids_dtype: FTM_ID_*).  Pair p = t k + j.  The rows
+ * of expert e, [offsets[e], offsets[e+1]), are its pairs in order of p; the
+ * pairs whose id is outside [0, E) follow in rows [offsets[E], T k).
+ * row_of_pair[p] and pair_of_row[row] are inverse to each other and hold the
+ * complement (~row, ~p) for a pair without an expert; token_of_row[row] = p / k,
+ * or -1.  The workspace needs no initial value; one call uses it at a time.
+ * The grouping of python/freetoken/kernel/triton/fused_moe.py:106-133 as a
+ * table, without its host loop. */
+#define FTM_ID_I32 0
+#define FTM_ID_I64 1
+size_t ftm_sort_workspace_bytes(int32_t T, int32_t k, int32_t num_experts);
+int ftm_sort_tokens(const void* ids, int32_t ids_dtype, int32_t T, int32_t k, int32_t num_experts,
+                    int32_t* offsets, int32_t* row_of_pair, int32_t* pair_of_row, int32_t* token_of_row,
+                    void* workspace, size_t ws_bytes, void* stream);
+
+/* rows[row_of_pair[t, j], :] = x[t, :] (x_stride bytes between tokens; elements
+ * of elem_bytes 1, 2 or 4); zeros in the rows of pairs without an expert. */
+int ftm_gather_tokens(const void* x, int64_t x_stride, int32_t elem_bytes, int32_t H,
+                      const int32_t* row_of_pair, int32_t T, int32_t k, void* rows, void* stream);
+
+/* out[t, :] = sum_j w[t, j] rows[row_of_pair[t, j], :] over the pairs with an
+ * expert, in order of j, fp32 sums, one rounding to out_dtype (dtype, or any
+ * from fp32 rows); w NULL: ones (the gradient of ftm_gather_tokens).  Replaces
+ * the weighted index_add of fused_moe.py:157-161, without atomics. */
+int ftm_combine_tokens(const void* rows, int32_t dtype, int64_t row_stride, const void* w, int32_t w_dtype,
+                       const int32_t* row_of_pair, int32_t T, int32_t k, int32_t H, void* out, int32_t out_dtype,
+                       void* stream);
+
+/* Its gradients for g = d out [T, H] (g_dtype, as out_dtype above): grad_rows[row_of_pair[t, j], :] = w[t, j]
+ * g[t, :] (zeros without an expert), grad_w[t, j] = g[t] . rows[row] (w_dtype; 0
+ * without an expert).  Either may be NULL (rows only serve grad_w, w grad_rows
+ * and the dtype). */
+int ftm_combine_tokens_grad(const void* g, int32_t g_dtype, int64_t g_stride, const void* rows, int32_t dtype,
+                            int64_t row_stride, const void* w, int32_t w_dtype, const int32_t* row_of_pair,
+                            int32_t T, int32_t k, int32_t H, void* grad_rows, void* grad_w, void* stream);
+
 /* ---- offload slot pool (python/freetoken/moe/offload_cache.py:218-694) ---- */
 
 /* Host-side global timestamp LRU over num_layers*E expert ids and S slots.
