@@ -191,6 +191,57 @@ int check_ws(const ftm_moe_layer* L, int T, const void* ws, size_t ws_bytes) {
   return FTM_OK;
 }
 
+int check_w8a8(const ftm_w8a8* call) {
+  if (call == nullptr) return FTM_ERR_NULL;
+  const ftm_w8a8& c = *call;
+  if (c.K <= 0 || c.K > FTM_W8A8_MAX_K || c.N <= 0 || c.rows < 0 || c.rows > INT32_MAX || c.x_rows < 0 ||
+      c.x_rows > INT32_MAX || c.x_stride < 0 || c.w_stride < 0)
+    return FTM_ERR_DIM;
+  if (!dt_ok(c.w_scale_dtype) || !dt_ok(c.out_dtype) || (c.bias != nullptr && !dt_ok(c.bias_dtype)))
+    return FTM_ERR_FORMAT;
+  if (c.act < -1 || c.act > FTM_ACT_SWIGLU_OAI) return FTM_ERR_FORMAT;
+  if (c.act >= 0 && c.N % 2 != 0) return FTM_ERR_DIM;
+  if (c.w_packed && c.K % 4 != 0) return FTM_ERR_DIM;
+  if (c.num_experts < 1 || c.num_experts > kMaxExperts || (c.offsets == nullptr && c.num_experts != 1))
+    return FTM_ERR_DIM;
+  if (c.num_experts > 1 && c.w_stride < (int64_t)c.N * c.K) return FTM_ERR_DIM;
+  if (c.rows == 0) return FTM_OK;
+  if (c.out == nullptr || c.w == nullptr || c.w_scale == nullptr) return FTM_ERR_NULL;
+  // without an index every row of the output is one of x
+  if (c.row_index == nullptr && c.x_rows < c.rows) return FTM_ERR_DIM;
+  if (c.x_rows == 0) return FTM_ERR_DIM;
+  if (c.x == nullptr || c.x_scale == nullptr) return FTM_ERR_NULL;
+  if (c.x_rows > 1 && c.x_stride < c.K) return FTM_ERR_DIM;
+  if (((uintptr_t)c.x_scale & 3u) != 0) return FTM_ERR_ALIGN;
+  return FTM_OK;
+}
+
+// Workspace of ftm_w8a8_moe_forward.
+struct W8a8MoeLayout {
+  size_t offsets, row_of_pair, pair_of_row, token_of_row, codes, scales, h, y, sort, total;
+};
+W8a8MoeLayout w8a8_moe_layout(int T, int k, int E, int H, int I) {
+  W8a8MoeLayout w;
+  const size_t P = (size_t)T * k, cx = (size_t)T * H, ch = P * I;
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o = align_up(o + bytes, 256);
+    return at;
+  };
+  w.offsets = take(4 * (size_t)(E + 1));
+  w.row_of_pair = take(4 * P);
+  w.pair_of_row = take(4 * P);
+  w.token_of_row = take(4 * P);
+  w.codes = take(cx > ch ? cx : ch);  // of x, then of h
+  w.scales = take(4 * P);
+  w.h = take(4 * P * I);
+  w.y = take(4 * P * H);
+  w.sort = take(sort_workspace_bytes((int64_t)P, E));
+  w.total = o;
+  return w;
+}
+
 int hip_rc(hipError_t e) { return e == hipSuccess ? FTM_OK : FTM_ERR_HIP; }
 
 }  // namespace
@@ -439,28 +490,70 @@ int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int6
 }
 
 int ftm_w8a8_linear(const ftm_w8a8* call, void* stream) {
+  const int rc = check_w8a8(call);
+  if (rc != FTM_OK || call->rows == 0) return rc;
+  return hip_rc(launch_w8a8(*call, (hipStream_t)stream));
+}
+
+int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w8a8* call, void* stream) {
+  int rc = check_w8a8(call);
+  if (rc != FTM_OK) return rc;
+  if (call->x_stride != call->K) return FTM_ERR_DIM;
+  if (call->rows == 0) return FTM_OK;
+  rc = ftm_quant_int8(x, x_dtype, call->x_rows, call->K, x_stride, const_cast<int8_t*>(call->x), call->K,
+                      const_cast<float*>(call->x_scale), stream);
+  if (rc != FTM_OK) return rc;
+  return hip_rc(launch_w8a8(*call, (hipStream_t)stream));
+}
+
+size_t ftm_w8a8_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter) {
+  if (T <= 0 || k <= 0 || num_experts <= 0 || num_experts > kMaxExperts || hidden <= 0 || inter <= 0) return 0;
+  return w8a8_moe_layout(T, k, num_experts, hidden, inter).total;
+}
+
+int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_bytes, void* stream) {
   if (call == nullptr) return FTM_ERR_NULL;
-  const ftm_w8a8& c = *call;
-  if (c.K <= 0 || c.K > FTM_W8A8_MAX_K || c.N <= 0 || c.rows < 0 || c.rows > INT32_MAX || c.x_rows < 0 ||
-      c.x_rows > INT32_MAX || c.x_stride < 0 || c.w_stride < 0)
+  const ftm_w8a8_moe& c = *call;
+  const int T = c.T, k = c.k, E = c.num_experts, H = c.hidden, I = c.inter;
+  if (T < 0 || k <= 0 || E <= 0 || E > kMaxExperts || H <= 0 || I <= 0 || I > FTM_W8A8_MAX_K || H > FTM_W8A8_MAX_K ||
+      (int64_t)T * k >= INT32_MAX || c.x_stride < 0)
     return FTM_ERR_DIM;
-  if (!dt_ok(c.w_scale_dtype) || !dt_ok(c.out_dtype) || (c.bias != nullptr && !dt_ok(c.bias_dtype)))
-    return FTM_ERR_FORMAT;
-  if (c.act < -1 || c.act > FTM_ACT_SWIGLU_OAI) return FTM_ERR_FORMAT;
-  if (c.act >= 0 && c.N % 2 != 0) return FTM_ERR_DIM;
-  if (c.w_packed && c.K % 4 != 0) return FTM_ERR_DIM;
-  if (c.num_experts < 1 || c.num_experts > kMaxExperts || (c.offsets == nullptr && c.num_experts != 1))
-    return FTM_ERR_DIM;
-  if (c.num_experts > 1 && c.w_stride < (int64_t)c.N * c.K) return FTM_ERR_DIM;
-  if (c.rows == 0) return FTM_OK;
-  if (c.out == nullptr || c.w == nullptr || c.w_scale == nullptr) return FTM_ERR_NULL;
-  // without an index every row of the output is one of x; with one x may be empty
-  if (c.row_index == nullptr && c.x_rows < c.rows) return FTM_ERR_DIM;
-  if (c.x_rows == 0) return FTM_ERR_DIM;
-  if (c.x == nullptr || c.x_scale == nullptr) return FTM_ERR_NULL;
-  if (c.x_rows > 1 && c.x_stride < c.K) return FTM_ERR_DIM;
-  if (((uintptr_t)c.x_scale & 3u) != 0) return FTM_ERR_ALIGN;
-  return hip_rc(launch_w8a8(c, (hipStream_t)stream));
+  if (!dt_ok(c.dtype) || !dt_ok(c.topk_w_dtype) || c.act < 0) return FTM_ERR_FORMAT;
+  if (T == 0) return FTM_OK;
+  if (c.x == nullptr || c.topk_ids == nullptr || c.topk_w == nullptr || c.out == nullptr) return FTM_ERR_NULL;
+  if (workspace == nullptr) return FTM_ERR_WORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return FTM_ERR_ALIGN;
+  const W8a8MoeLayout L = w8a8_moe_layout(T, k, E, H, I);
+  if (ws_bytes < L.total) return FTM_ERR_WORKSPACE;
+  char* ws = (char*)workspace;
+  const int P = T * k;
+  int32_t* offsets = (int32_t*)(ws + L.offsets);
+  int32_t* row_of_pair = (int32_t*)(ws + L.row_of_pair);
+  int32_t* pair_of_row = (int32_t*)(ws + L.pair_of_row);
+  int32_t* token_of_row = (int32_t*)(ws + L.token_of_row);
+  int8_t* q = (int8_t*)(ws + L.codes);
+  float* s = (float*)(ws + L.scales);
+  float *h = (float*)(ws + L.h), *y = (float*)(ws + L.y);
+  const ftm_w8a8 a = {q, s, c.w13, c.w13_scale, c.w13_bias, h, offsets, token_of_row, P, T, H, (int64_t)2 * I * H,
+                      2 * I, H, E, c.w13_packed, c.w13_scale_dtype, c.w13_bias_dtype, FTM_DT_F32, c.act, c.act_alpha,
+                      c.act_limit};
+  const ftm_w8a8 b = {q, s, c.w2, c.w2_scale, c.w2_bias, y, offsets, nullptr, P, P, I, (int64_t)H * I, H, I, E,
+                      c.w2_packed, c.w2_scale_dtype, c.w2_bias_dtype, FTM_DT_F32, -1, 0.0f, 0.0f};
+  // everything is checked before anything is launched
+  int rc = check_w8a8(&a);
+  if (rc == FTM_OK) rc = check_w8a8(&b);
+  if (rc != FTM_OK) return rc;
+  if (((uintptr_t)c.x | (uint64_t)c.x_stride | (uintptr_t)c.out) % dt_bytes(c.dtype) != 0) return FTM_ERR_ALIGN;
+  rc = ftm_sort_tokens(c.topk_ids, c.ids_dtype, T, k, E, offsets, row_of_pair, pair_of_row, token_of_row, ws + L.sort,
+                       L.total - L.sort, stream);
+  if (rc == FTM_OK) rc = ftm_quant_int8(c.x, c.dtype, T, H, c.x_stride, q, H, s, stream);
+  if (rc == FTM_OK) rc = ftm_w8a8_linear(&a, stream);
+  if (rc == FTM_OK) rc = ftm_quant_int8(h, FTM_DT_F32, P, I, (int64_t)I * 4, q, I, s, stream);
+  if (rc == FTM_OK) rc = ftm_w8a8_linear(&b, stream);
+  if (rc == FTM_OK)
+    rc = ftm_combine_tokens(y, FTM_DT_F32, (int64_t)H * 4, c.topk_w, c.topk_w_dtype, row_of_pair, T, k, H, c.out, c.dtype,
+                            stream);
+  return rc;
 }
 
 size_t ftm_sort_workspace_bytes(int32_t T, int32_t k, int32_t num_experts) {

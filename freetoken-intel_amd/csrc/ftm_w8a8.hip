@@ -2,7 +2,7 @@
 // the integer product with one scale per token and one per output channel,
 // dense or grouped by expert (rows sorted by expert, one weight per expert).
 //
-//   s_m = fp32(max_k |x_mk| / 127), q_mk = the whole number nearest x_mk / s_m
+//   s_m = max_k |x_mk| * (1 / 127), both fp32, q_mk = the whole number nearest x_mk / s_m
 //   y_mn = (sum_k q_mk w_nk) s_m t_n (+ b_n), optionally h = act(gate) * up
 //
 // The sum is exact in int32 (K <= 131071, checked by the callers), so its order
@@ -39,7 +39,10 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
   return up(up(at(0), at(16)), up(at(32), at(48)));
 }
 
-// A row's scale and the factor of its first guess; a row with a value that is
+// A row's scale and the factor of its first guess.  The product with the fp32
+// nearest 1 / 127, not a division: what torch makes of `amax / 127` on the GPU, so
+// the codes are those of a torch quantiser there (where the scales are an ulp
+// apart, quotients of bf16 values that end in .5 round to other codes).  A row with a value that is
 // not finite gets the scale NaN and codes 0, so its outputs are NaN and no
 // other row's change.
 struct QuantScale {
@@ -47,7 +50,7 @@ struct QuantScale {
 };
 __device__ __forceinline__ QuantScale quant_scale(uint32_t max_bits) {
   if (max_bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.0f};
-  const float s = fmaxf(__uint_as_float(max_bits), 1e-12f) / 127.0f;
+  const float s = fmaxf(__uint_as_float(max_bits), 1e-12f) * (1.0f / 127.0f);
   return {s, 1.0f / s};
 }
 // The whole number nearest x / s, ties to even, for the exact quotient: the
@@ -201,74 +204,90 @@ struct RowTile {
   int cnt, e;
 };
 
-// Row tile `t` of height BM.  Dense: the t-th BM rows.  Grouped: the experts'
-// row tiles in order of the experts, then tiles over the rows of no expert.
-// Every wave finds it by itself: eight experts a lane, one prefix sum over the
-// wave.  The offsets are clamped to [0, rows], so a bad table reads and writes
-// no other memory.
+// Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
+// lanes (DPP row_shr, zeros shifted in), then the rows before.
+__device__ __forceinline__ int wave_prefix_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31);
+  const int c = __builtin_amdgcn_readlane(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
+// The experts' rows cut into tiles of height BM, in order of the experts, found by
+// every wave for itself: eight experts a lane, one prefix sum over the wave.
+// The offsets are clamped to [0, rows], so a bad table reads and writes no
+// other memory.
 template <int BM>
-__device__ __forceinline__ RowTile row_tile(const ftm_w8a8& c, int t) {
-  RowTile r;
-  if (c.offsets == nullptr) {
-    r.row0 = (int64_t)t * BM;
-    const int64_t left = c.rows - r.row0;
-    r.cnt = left < BM ? (int)left : BM;
-    r.e = 0;
-    return r;
-  }
-  const int lane = threadIdx.x & 63, E = c.num_experts, P = (int)c.rows;
-  int lo[9], tiles[8], sum = 0;
+struct RowScan {
+  int lo[9];  // first rows of the lane's eight experts, and the end of the last
+  int first;  // tiles of the experts before them
+  int total;  // tiles of all experts
+
+  __device__ __forceinline__ static int tiles(int begin, int end) { return end > begin ? (end - begin + BM - 1) / BM : 0; }
+
+  __device__ __forceinline__ explicit RowScan(const ftm_w8a8& c) {
+    const int lane = threadIdx.x & 63, E = c.num_experts, P = (int)c.rows;
 #pragma unroll
-  for (int i = 0; i < 9; ++i) {
-    const int e = 8 * lane + i;
-    const int o = c.offsets[e < E ? e : E];
-    lo[i] = o < 0 ? 0 : o > P ? P : o;
-  }
+    for (int i = 0; i < 9; ++i) {
+      const int e = 8 * lane + i;
+      const int o = c.offsets[e < E ? e : E];
+      lo[i] = o < 0 ? 0 : o > P ? P : o;
+    }
+    int sum = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = lo[i + 1] - lo[i];
-    tiles[i] = n > 0 ? (n + BM - 1) / BM : 0;
-    sum += tiles[i];
+    for (int i = 0; i < 8; ++i) sum += tiles(lo[i], lo[i + 1]);
+    const int upto = wave_prefix_sum(sum);
+    first = upto - sum;
+    total = __builtin_amdgcn_readlane(upto, 63);
   }
-  int upto = sum;  // inclusive prefix sum over the lanes
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int v = __shfl_up(upto, d);
-    upto += lane >= d ? v : 0;
-  }
-  const int total = __builtin_amdgcn_readlane(upto, 63);
-  const uint64_t in = __ballot(t >= upto - sum && t < upto);
-  if (in != 0) {
-    const int src = __builtin_ctzll(in);
-    int before = upto - sum, e = 0, m = 0, begin = 0, end = 0;
+
+  // Tile t < total.
+  __device__ __forceinline__ RowTile tile(int t) const {
+    int before = first, e = -1, m = 0, begin = 0, end = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool here = t >= before && t < before + tiles[i];
-      e = here ? 8 * lane + i : e;
+      const int n = tiles(lo[i], lo[i + 1]);
+      const bool here = t >= before && t < before + n;
+      e = here ? 8 * (int)(threadIdx.x & 63) + i : e;
       m = here ? t - before : m;
       begin = here ? lo[i] : begin;
       end = here ? lo[i + 1] : end;
-      before += tiles[i];
+      before += n;
     }
+    const int src = __builtin_ctzll(__ballot(e >= 0));
     e = __builtin_amdgcn_readlane(e, src);
-    m = __builtin_amdgcn_readlane(m, src);
-    begin = __builtin_amdgcn_readlane(begin, src) + m * BM;
+    begin = __builtin_amdgcn_readlane(begin, src) + BM * __builtin_amdgcn_readlane(m, src);
     end = __builtin_amdgcn_readlane(end, src);
-    r.row0 = begin;
-    r.cnt = end - begin < BM ? end - begin : BM;
-    r.e = e;
-    return r;
+    return {begin, end - begin < BM ? end - begin : BM, e};
   }
-  // the rows of no expert: before the first offset and behind the last
-  const int head = __builtin_amdgcn_readlane(lo[0], 0), tail = __builtin_amdgcn_readlane(lo[8], 63);
-  const int head_tiles = (head + BM - 1) / BM;
-  const int u = t - total;
-  const int begin = u < head_tiles ? u * BM : tail + (u - head_tiles) * BM;
-  const int end = u < head_tiles ? head : P;
-  r.row0 = begin;
-  r.cnt = end - begin < BM ? (end > begin ? end - begin : 0) : BM;
-  r.e = -1;
-  return r;
+
+  // The rows of no expert: before the first offset and from the last on.
+  __device__ __forceinline__ int head() const { return __builtin_amdgcn_readlane(lo[0], 0); }
+  __device__ __forceinline__ int tail() const { return __builtin_amdgcn_readlane(lo[8], 63); }
+};
+
+// Tile t of a dense product.
+template <int BM>
+__device__ __forceinline__ RowTile dense_tile(const ftm_w8a8& c, int t) {
+  const int64_t row0 = (int64_t)t * BM, left = c.rows - row0;
+  return {row0, left < BM ? (int)left : BM, 0};
+}
+
+// Row tile t: dense, or of a grouped product the experts' and behind them those
+// over the rows of no expert.
+template <int BM>
+__device__ __forceinline__ RowTile row_tile(const ftm_w8a8& c, int t) {
+  if (c.offsets == nullptr) return dense_tile<BM>(c, t);
+  const RowScan<BM> scan(c);
+  if (t < scan.total) return scan.tile(t);
+  const int head = scan.head(), head_tiles = (head + BM - 1) / BM, u = t - scan.total;
+  const int begin = u < head_tiles ? u * BM : scan.tail() + (u - head_tiles) * BM;
+  const int end = u < head_tiles ? head : (int)c.rows;
+  return {begin, end - begin < BM ? (end > begin ? end - begin : 0) : BM, -1};
 }
 
 // Row tiles that row_tile<BM> can name: each expert ends in one partly filled
@@ -299,28 +318,118 @@ __device__ __forceinline__ Channel channel(const ftm_w8a8& c, int e, int n) {
   const int64_t i = (int64_t)e * c.N + n;
   return {load_scalar(c.w_scale, i, c.w_scale_dtype), c.bias != nullptr ? load_scalar(c.bias, i, c.bias_dtype) : 0.0f};
 }
+// The same as raw bits, requested ahead of their use (converting would wait for
+// the load).
+struct ChannelBits {
+  uint32_t t, b;
+};
+// Raw bits of N neighbouring entries (index capped at `last`).
+template <int N>
+__device__ __forceinline__ void load_run(const void* p, int64_t base, int first, int last, int dt, uint32_t* bits) {
+  if (dt == FTM_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits[i] = ((const uint32_t*)p)[base + (first + i < last ? first + i : last)];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits[i] = ((const uint16_t*)p)[base + (first + i < last ? first + i : last)];
+  }
+}
+
+__device__ __forceinline__ Channel channel(const ftm_w8a8& c, ChannelBits r) {
+  return {bits_to_f32(opaque_bits(r.t), c.w_scale_dtype), bits_to_f32(opaque_bits(r.b), c.bias_dtype)};
+}
 __device__ __forceinline__ float scaled(int sum, float s, Channel ch) {
   return fmaf((float)sum * s, ch.t, ch.b);
 }
 
+// Slot s of row r of a 128-byte wide LDS stage holds 16-byte piece s ^ swz(r): the
+// 16 rows of one operand read (128 bytes apart, 256 bytes of banks) hit distinct
+// banks.
+constexpr int kRow = 128;
+__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
+typedef __attribute__((address_space(3))) void* LPtr;
+
+// The results of a row tile: N neighbouring channels from n0 on of one row at a
+// time, through a buffer that drops rows past the tile; channels past the last
+// take an offset past its end, so there is no branch around a store.
+template <int N>
+struct RowOut {
+  Rsrc res;
+  int NO, n0, dt;
+  bool vec;  // 16 bytes (four 16-bit values: 8) a store
+  __device__ __forceinline__ RowOut(const ftm_w8a8& c, const RowTile& t, int NO_, int n0_) : NO(NO_), n0(n0_), dt(c.out_dtype) {
+    const int esz = dt == FTM_DT_F32 ? 4 : 2;
+    res = make_rsrc((char*)c.out + t.row0 * NO * esz, (uint32_t)(t.cnt * NO) * (uint32_t)esz);
+    vec = NO % (dt == FTM_DT_F32 || N == 4 ? 4 : 8) == 0 && ((uintptr_t)c.out & 15u) == 0;
+  }
+  __device__ __forceinline__ uint32_t half2(float a, float b) const {
+    return dt == FTM_DT_BF16 ? pack_bf16x2(a, b) : (uint32_t)f32_to_f16(a) | ((uint32_t)f32_to_f16(b) << 16);
+  }
+  __device__ __forceinline__ void store(int row, const float (&y)[N]) const {
+    const uint32_t at = (uint32_t)(row * NO + n0);
+    if (dt == FTM_DT_F32) {
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              (u32x4){__float_as_uint(y[i]), __float_as_uint(y[i + 1]), __float_as_uint(y[i + 2]), __float_as_uint(y[i + 3])},
+              res, n0 + i < NO ? 4u * (at + i) : kOOB, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[i]), res, n0 + i < NO ? 4u * (at + i) : kOOB, 0, 0);
+      }
+      return;
+    }
+    uint32_t h[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) h[i] = half2(y[2 * i], y[2 * i + 1]);
+    if (vec) {
+      if constexpr (N == 4) {
+        __builtin_amdgcn_raw_buffer_store_b64((u32x2){h[0], h[1]}, res, n0 < NO ? 2u * at : kOOB, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 8)
+          __builtin_amdgcn_raw_buffer_store_b128((u32x4){h[i / 2], h[i / 2 + 1], h[i / 2 + 2], h[i / 2 + 3]}, res,
+                                                 n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(h[i / 2] >> (16 * (i & 1))), res,
+                                              n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
+    }
+  }
+};
+
+// f(activation) with the selection outside the loops (-1: none).
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  if (act < 0) f(std::integral_constant<int, -1>{});
+  else if (act == FTM_ACT_SILU) f(std::integral_constant<int, FTM_ACT_SILU>{});
+  else if (act == FTM_ACT_GELU) f(std::integral_constant<int, FTM_ACT_GELU>{});
+  else if (act == FTM_ACT_RELU) f(std::integral_constant<int, FTM_ACT_RELU>{});
+  else f(std::integral_constant<int, FTM_ACT_SWIGLU_OAI>{});
+}
+
 // ------------------------------------------------------------------ K split over the waves
-// A workgroup's tile of 16 MT tokens x 16 NT weight rows (with an activation:
-// NT / 2 blocks of gate rows and the up rows that belong to them); each of the
-// NW waves takes a part of K over the whole tile, straight from memory into
-// registers, and the waves' sums meet in LDS.  No barrier in the K loop, so a
-// wave keeps its loads in flight; the tokens are read once a column of tiles,
-// from L2.  For few rows (weights bound it) and for grids too small for the
-// LDS tiles.
-template <int MT, int NT, int NW, bool PACKED>
+// A workgroup's tile of 16 MT tokens x 16 NT weight rows (with an activation 8
+// gate rows and their 8 up rows a block); each of the NW waves takes a run of
+// K over the whole tile through an LDS ring of its own (S stages of 128 K), and
+// the waves' sums meet in LDS.  No barrier in the K loop.  For few rows, and
+// for grids too small for the tiles that share a ring.  The copies go to LDS
+// because eight neighbouring lanes then read 128 bytes of one row: loads in
+// operand layout touch another row with every lane, and a CU looks up four
+// times as many cache lines for them.
+template <int MT, int NT, int NW, int S, bool PACKED>
 __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, int ntiles) {
-  constexpr int BM = 16 * MT;
-  constexpr int U = MT * NT >= 8 ? 2 : 4;  // K steps of 64 in a register set
-  extern __shared__ int red[];            // [NW][MT * NT * 4][64]
+  constexpr int BM = 16 * MT, kStage = (MT + NT) * 16 * kRow, NC = 2 * (MT + NT);
+  extern __shared__ char lds[];  // [NW][S][kStage], then the sums [NW][MT * NT * 4][64]
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const RowTile rt = row_tile<BM>(c, item / ntiles);
   if (rt.cnt <= 0) return;
   const bool act = c.act >= 0;
-  const int NO = out_cols(c);
+  const int NO = out_cols(c), K = c.K;
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = act ? 8 * NT : 16 * NT;  // output channels of the tile
@@ -331,93 +440,400 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
-  if (rt.e >= 0) {
-    const int K = c.K;
-    const int per = ((K + 64 * NW - 1) / (64 * NW)) * 64;  // K of a wave
-    const int k_lo = wave * per, k_hi = k_lo + per < K ? k_lo + per : K;
-    // rows past the tile read a row inside it (their results are dropped)
-    const char* xrow[MT];
+  // the scales of the blocks this wave finishes (below): requested behind the
+  // first copies and ahead of the K loop
+  constexpr int kParts = (MT * NT + NW - 1) / NW;
+  float xscale[kParts];
+  uint32_t tb[kParts][8] = {}, bb[kParts][8] = {};  // scales and biases: four channels, their up rows
+  bool live[kParts];
+  auto request_scales = [&] {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int r = 16 * i + m;
-      const int64_t s = source_row(c, rt.row0 + (r < rt.cnt ? r : 0));
-      xrow[i] = (const char*)c.x + (s < 0 ? 0 : s) * c.x_stride;
+    for (int p = 0; p < kParts; ++p) {
+      const int f = p * NW + wave, r = 16 * (f / NT) + m, j = f % NT;
+      const int64_t src = f < MT * NT && r < rt.cnt && rt.e >= 0 ? source_row(c, rt.row0 + r) : -1;
+      live[p] = src >= 0;
+      xscale[p] = src >= 0 ? c.x_scale[src] : 0.0f;
+      if (rt.e < 0) continue;
+      const int n = n0 + (act ? 8 * j + 4 * (g & 1) : 16 * j + 4 * g);
+      const int64_t at = (int64_t)rt.e * c.N;
+      load_run<4>(c.w_scale, at, n, NO - 1, c.w_scale_dtype, tb[p]);
+      if (act) load_run<4>(c.w_scale, at + NO, n, NO - 1, c.w_scale_dtype, tb[p] + 4);
+      if (c.bias == nullptr) continue;
+      load_run<4>(c.bias, at, n, NO - 1, c.bias_dtype, bb[p]);
+      if (act) load_run<4>(c.bias, at + NO, n, NO - 1, c.bias_dtype, bb[p] + 4);
     }
-    // the tile's weight rows, from n0 (and, with an activation, N/2 + n0) on;
-    // rows past the last read zeros
-    const char* wbase = (const char*)c.w + (int64_t)rt.e * c.w_stride;
-    const uint32_t bytes = (uint32_t)ncol * (uint32_t)K;
-    const Rsrc w0 = make_rsrc(wbase + (int64_t)n0 * K, bytes);
-    const Rsrc w1 = make_rsrc(wbase + (int64_t)((act ? NO : 0) + n0) * K, bytes);
-    struct Set {
-      u32x4 x[U][MT], w[U][NT];
-    };
-    auto load = [&](Set& s, int k) {
+  };
+  const int nsteps = (K + 127) / 128, per = (nsteps + NW - 1) / NW;
+  const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
+  if (rt.e >= 0 && lo < hi) {
+    // copies of 8 rows, a 16-byte piece a lane; rows past the tile copy one
+    // inside it, pieces past K what follows the row (their weights are made
+    // zero).  Tokens: offsets from the tile's first row, or, read through an
+    // index, from x's; weights from the tile's first row (and the up rows N/2 on)
+    const bool indexed = c.row_index != nullptr;
+    const char* xbase = (const char*)c.x + (indexed ? 0 : rt.row0 * c.x_stride);
+    const Rsrc xres = make_rsrc(xbase, (uint32_t)((indexed ? c.x_rows - 1 : (int64_t)rt.cnt - 1) * c.x_stride + K));
+    const char* wbase = (const char*)c.w + (int64_t)rt.e * c.w_stride + (int64_t)n0 * K;
+    const Rsrc wres = make_rsrc(wbase, (uint32_t)((act ? NO : 0) + ncol) * (uint32_t)K);
+    uint32_t xoff[2 * MT], woff[2 * NT];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kk = k + 64 * u + 16 * g;
-        const bool in = kk < k_hi;
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      int n = act ? 8 * (i >> 1) + (r & 7) : r;
+      n = n < ncol ? n : ncol - 1;
+      woff[i] = (uint32_t)(n + (act && (i & 1) ? NO : 0)) * (uint32_t)K + 16u * (uint32_t)((lane & 7) ^ swz(r));
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      int64_t s = r < rt.cnt ? r : 0;
+      if (indexed) {
+        s = source_row(c, rt.row0 + s);
+        s = s < 0 ? 0 : s;
+      }
+      xoff[i] = (uint32_t)(s * c.x_stride) + 16u * (uint32_t)((lane & 7) ^ swz(r));
+    }
+    char* ring = lds + wave * (S * kStage);
+    auto issue = [&](int step, int slot) {
+      const uint32_t k0 = (uint32_t)(step < hi ? step : hi - 1) * 128u;
+      char* st = ring + slot * kStage;
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + 1024 * (2 * MT + i)), 16, (int)(woff[i] + k0), 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * i), 16, (int)(xoff[i] + k0), 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(lo + i, i);
+    request_scales();
+    int slot = 0;
+    for (int step = lo; step < hi; ++step) {
+      issue(step + S - 1, slot == 0 ? S - 1 : slot - 1);
+      wait_vm<(S - 1) * NC>();  // this step's copies have landed
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = ring + slot * kStage;
+      auto piece = [&](int r, int q) { return *(const u32x4*)(st + r * kRow + 16 * ((4 * q + g) ^ swz(r))); };
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const bool in = step * 128 + 64 * q + 16 * g < K;
+        u32x4 w[NT], x[MT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const bool up = j >= NT / 2 && NT > 1;
-          const int jr = (act && up ? j - NT / 2 : j) * 16 + m;
-          s.w[u][j] = bload16(act && up ? w1 : w0, in ? (uint32_t)jr * (uint32_t)K + (uint32_t)kk : kOOB);
+          // past K the weights have to be zero; packed bytes are offset by 128
+          const u32x4 v = piece(16 * (MT + j) + m, q);
+          w[j] = in ? (PACKED ? v ^ 0x80808080u : v) : (u32x4){0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) s.x[u][i] = *(const u32x4*)(xrow[i] + (in ? kk : 0));
+        for (int i = 0; i < MT; ++i) x[i] = piece(16 * i + m, q);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][j] = mfma_i8(w[j], x[i], acc[i][j]);
       }
-    };
-    auto mma = [&](const Set& s, int k) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // packed bytes are offset by 128; past K both forms have to be zero
-        const uint32_t flip = PACKED && k + 64 * u + 16 * g < k_hi ? 0x80808080u : 0u;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          u32x4 w = s.w[u][j];
-          if constexpr (PACKED) w ^= flip;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][j] = mfma_i8(w, s.x[u][i], acc[i][j]);
-        }
-      }
-    };
-    Set s0, s1;
-    load(s0, k_lo);
-    for (int k = k_lo; k < k_hi; k += 128 * U) {
-      load(s1, k + 64 * U);
-      mma(s0, k);
-      load(s0, k + 128 * U);
-      mma(s1, k + 64 * U);
+      __builtin_amdgcn_sched_barrier(0);  // the next copies overwrite what these products have read
+      slot = slot == S - 1 ? 0 : slot + 1;
     }
+    wait_vm<0>();  // the copies past the last step, before the sums take their place
+  } else {
+    request_scales();
   }
+  i32x4* red = (i32x4*)lds;  // [NW][MT * NT][64]
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) red[((wave * MT * NT + i * NT + j) * 4 + r) * 64 + lane] = acc[i][j][r];
+    for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  // sum of (token row, weight row) of the tile over the waves
-  auto total = [&](int row, int n) {
-    const int at = (((row >> 4) * NT + (n >> 4)) * 4 + (n & 3)) * 64 + (row & 15) + 16 * ((n >> 2) & 3);
-    int v = 0;
+  // The waves share the blocks; a lane has four neighbouring weight rows of one
+  // token (with an activation the lanes of 8..15 pass: those are the up rows of
+  // the others)
+  if (act && g >= 2) return;
+  with_act(c.act, [&](auto a) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) v += red[w * MT * NT * 256 + at];
-    return v;
-  };
-  for (int i = threadIdx.x; i < rt.cnt * cols; i += 64 * NW) {
-    const int row = i / cols, n = i % cols;
-    if (n >= ncol) continue;
-    const int64_t orow = rt.row0 + row;
-    float y = 0.0f;
-    const int64_t src = rt.e >= 0 ? source_row(c, orow) : -1;
-    if (src >= 0) {
-      const float s = c.x_scale[src];
-      y = scaled(total(row, n), s, channel(c, rt.e, n0 + n));
-      if (act)
-        y = act_fn(c.act, y, scaled(total(row, n + 8 * NT), s, channel(c, rt.e, NO + n0 + n)), c.act_alpha, c.act_limit);
+    for (int p = 0; p < kParts; ++p) {
+      constexpr int A = decltype(a)::value;
+      const int f = p * NW + wave;
+      if (MT * NT % NW != 0 && f >= MT * NT) continue;
+      i32x4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        u += red[(w * MT * NT + f) * 64 + lane];
+        if constexpr (A >= 0) v += red[(w * MT * NT + f) * 64 + lane + 32];
+      }
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = scaled(u[r], xscale[p], channel(c, {tb[p][r], bb[p][r]}));
+        if constexpr (A >= 0)
+          y[r] = act_fn(A, y[r], scaled(v[r], xscale[p], channel(c, {tb[p][4 + r], bb[p][4 + r]})), c.act_alpha, c.act_limit);
+        y[r] = live[p] ? y[r] : 0.0f;
+      }
+      RowOut<4>(c, rt, NO, n0 + (act ? 8 : 16) * (f % NT) + 4 * g).store(16 * (f / NT) + m, y);
     }
-    store_scalar(c.out, orow * NO + n0 + n, c.out_dtype, y);
+  });
+}
+
+// ------------------------------------------------------------------ LDS tiles
+// A tile is BM = 16 MI WM tokens x 256 weight rows (with an activation 128 gate
+// rows and their up rows): 4 WM waves of 16 MI tokens x 64 weight rows each over
+// the whole K.  Tokens and weights go through a ring of S LDS stages of 128 K,
+// filled by direct copies S steps ahead, one barrier a step.  A workgroup takes
+// one tile after another, and the copies run on from tile to tile: the first
+// stages of the next are under way during the last products and the epilogue
+// of this one.
+
+// The order of a dense product's tiles: groups of eight row tiles, their columns
+// one after another, so that the tiles in flight on one XCD share both operands.
+template <int BM>
+__device__ __forceinline__ RowTile dense_item(const ftm_w8a8& c, int item, int mtiles, int ntiles, int& nt) {
+  const int per = 8 * ntiles, first = item / per * 8;
+  const int rows = mtiles - first < 8 ? mtiles - first : 8;
+  nt = item % per / rows;
+  return dense_tile<BM>(c, first + item % per % rows);
+}
+
+// The lane's number, anew: what is computed from it inside a loop is not kept in
+// registers over the loop.
+__device__ __forceinline__ int opaque_lane() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
+__global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtiles, int ntiles) {
+  constexpr int BM = 16 * MI * WM;
+  constexpr int kX = BM * kRow, kStage = kX + 256 * kRow;
+  constexpr int NX = BM / 8 / (4 * WM), NB = 32 / (4 * WM);  // 1 KiB copies a wave and step: tokens, weights
+  constexpr int kCols = ACT ? 128 : 256;                     // output channels of the tile
+  constexpr int kAhead = 3;                                  // row blocks read ahead of their products
+  static_assert(2 * MI % (kAhead + 1) == 0, "a step leaves its row blocks where it found them");
+  static_assert(kAhead <= MI && MI >= 4, "the next step's first weights take registers that are done");
+  extern __shared__ char lds[];
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / 4, wn = wave % 4;
+  const int NO = out_cols(c), K = c.K;
+  const int nsteps = (K + 127) / 128, nrun = nsteps > S ? nsteps : S;  // steps past K multiply zeros
+  const bool indexed = GROUPED && c.row_index != nullptr;
+
+  // this workgroup's items: every (workgroups per XCD)-th of its XCD's run
+  using Scan = std::conditional_t<GROUPED, RowScan<BM>, int>;
+  const Scan scan = [&] {
+    if constexpr (GROUPED) return RowScan<BM>(c);
+    else return 0;
+  }();
+  int row_tiles = mtiles;
+  if constexpr (GROUPED) row_tiles = scan.total;
+  const int items = row_tiles * ntiles, xcd = blockIdx.x & 7, rem = items & 7;
+  const int begin = xcd * (items >> 3) + (xcd < rem ? xcd : rem), end = begin + (items >> 3) + (xcd < rem ? 1 : 0);
+  struct Tile {
+    RowTile rt;
+    int n;  // first output channel
+  };
+  auto tile_at = [&](int item) __attribute__((always_inline)) {
+    Tile t;
+    int nt;
+    if constexpr (GROUPED) {
+      nt = item % ntiles;
+      t.rt = scan.tile(item / ntiles);
+    } else {
+      t.rt = dense_item<BM>(c, item, mtiles, ntiles, nt);
+    }
+    t.n = nt * kCols;
+    return t;
+  };
+  int item = begin + (blockIdx.x >> 3);
+  if (item < end) {
+    Tile cur = tile_at(item);
+    // A wave's copies: 8 rows each, a 16-byte piece a lane; rows past the tile
+    // copy one inside it, pieces past K what follows the row (their weights are
+    // made zero).  Tokens: offsets from the tile's first row, or, read through an
+    // index, from x's; weights from the tile's first gate row, so that 32 bits
+    // reach them (the launch sees to it).
+    Rsrc xres, wres;
+    uint32_t xoff[NX], woff[NB];
+    int ix[NX], er[MI];  // rows of x: of the copies, of the results' tokens
+    auto copy_rows = [&](const Tile& t) __attribute__((always_inline)) {
+      const int lane = opaque_lane();
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int r = 8 * (wave * NX + i) + (lane >> 3), in = r < t.rt.cnt ? r : 0;
+        ix[i] = indexed ? c.row_index[t.rt.row0 + in] : in;
+      }
+    };
+    auto result_rows = [&](const Tile& t) __attribute__((always_inline)) {
+      const int m = opaque_lane() & 15;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = 16 * (wm * MI + i) + m, in = r < t.rt.cnt ? r : 0;
+        er[i] = indexed ? c.row_index[t.rt.row0 + in] : (int)t.rt.row0 + in;
+      }
+    };
+    auto aim = [&](const Tile& t) __attribute__((always_inline)) {
+      const int lane = opaque_lane();
+      xres = make_rsrc((const char*)c.x + (indexed ? 0 : t.rt.row0 * c.x_stride),
+                       (uint32_t)((indexed ? c.x_rows - 1 : (int64_t)t.rt.cnt - 1) * c.x_stride + K));
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int r = 8 * (wave * NX + i) + (lane >> 3);
+        const bool ok = !indexed || (ix[i] >= 0 && ix[i] < c.x_rows);
+        xoff[i] = (uint32_t)((ok ? ix[i] : 0) * c.x_stride) + 16u * (uint32_t)((lane & 7) ^ swz(r));
+      }
+      const int cols = NO - t.n < kCols ? NO - t.n : kCols;
+      wres = make_rsrc((const char*)c.w + (int64_t)t.rt.e * c.w_stride + (int64_t)t.n * K,
+                       (uint32_t)((ACT ? NO : 0) + cols) * (uint32_t)K);
+      // Weight row of LDS row r: wave r / 64 of the columns; its operand block j = r
+      // % 64 / 16, operand row o = r % 16 is channel 16 (o / 4) + 4 j + o % 4, so that
+      // a lane's results are 16 neighbours (with an activation: 8 (o / 4) + 4 (j % 2)
+      // + o % 4 of gate, j < 2, and of up); rows past the last copy it
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int r = 8 * (wave * NB + i) + (lane >> 3), j = (r >> 4) & 3, o = r & 15;
+        int n = (r >> 6) * (kCols / 4) + (ACT ? 8 * (o >> 2) + 4 * (j & 1) : 16 * (o >> 2) + 4 * j) + (o & 3);
+        n = n < cols ? n : cols - 1;
+        woff[i] = (uint32_t)(n + (ACT && j >= 2 ? NO : 0)) * (uint32_t)K + 16u * (uint32_t)((lane & 7) ^ swz(r));
+      }
+    };
+    auto issue = [&](int kb, int slot) __attribute__((always_inline)) {
+      const uint32_t k0 = (uint32_t)(kb < nsteps ? kb : nsteps - 1) * 128u;
+      char* st = lds + slot * kStage;
+#pragma unroll
+      for (int i = 0; i < NX; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * (wave * NX + i)), 16, (int)(xoff[i] + k0), 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + i)), 16, (int)(woff[i] + k0), 0, 0,
+                                                 0);
+    };
+    i32x4 acc[MI][4];
+    u32x4 b[2][4], x[kAhead + 1];
+    auto piece = [&](int slot, int r, int q) __attribute__((always_inline)) {
+      return *(const u32x4*)(lds + slot * kStage + r * kRow + 16 * ((4 * q + g) ^ swz(r)));
+    };
+    auto xfrag = [&](int slot, int at) __attribute__((always_inline)) { return piece(slot, 16 * (wm * MI + at % MI) + m, at / MI); };
+    auto wfrag = [&](int slot, int j, int q) __attribute__((always_inline)) { return piece(slot, BM + 64 * wn + 16 * j + m, q); };
+    // Products of step kb, whose first operands are in registers; the rest is
+    // read kAhead row blocks ahead.  Once every wave has read the last of them,
+    // the stage's slot takes the copies of step kb + S (`ahead`: its number in the
+    // tile that the copies are at) and the first operands of step kb + 1, whose
+    // copies have landed, are read under the products left.
+    auto step = [&](int kb, int ahead, int slot) __attribute__((always_inline)) {
+      const int next = slot == S - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if constexpr (PACKED || TAIL) {
+          // packed bytes are offset by 128; past K the weights have to be zero
+          const bool in = !TAIL || kb * 128 + 64 * q + 16 * g < K;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const u32x4 v = PACKED ? b[q][j] ^ 0x80808080u : b[q][j];
+            b[q][j] = in ? v : (u32x4){0, 0, 0, 0};
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int at = MI * q + i;
+          if (at == 2 * MI - kAhead) {
+            wait_vm<(S - 2) * (NX + NB)>();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            issue(ahead, slot);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[0][j] = wfrag(next, j, 0);
+          }
+          const int a = at + kAhead;
+          x[a % (kAhead + 1)] = a < 2 * MI ? xfrag(slot, a) : xfrag(next, a - 2 * MI);
+          if (q == 0 && i >= MI - 4) b[1][i - (MI - 4)] = wfrag(slot, i - (MI - 4), 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(b[q][j], x[at % (kAhead + 1)], acc[i][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    copy_rows(cur);
+    aim(cur);
+#pragma unroll
+    for (int i = 0; i < S; ++i) issue(i, i);
+    wait_vm<(S - 1) * (NX + NB)>();
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[0][j] = wfrag(0, j, 0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) x[i] = xfrag(0, i);
+    int slot = 0;
+    for (;;) {
+      const int after = item + (int)(gridDim.x >> 3);
+      const Tile next = after < end ? tile_at(after) : cur;  // (the last tile's copies go on over it: nothing reads them)
+      result_rows(cur);
+      copy_rows(next);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+      for (int kb = 0; kb < nrun; ++kb) {
+        if (kb == nrun - S) aim(next);  // from here on the copies are the next tile's
+        step(kb, kb + S < nrun ? kb + S : kb + S - nrun, slot);
+        slot = slot == S - 1 ? 0 : slot + 1;
+      }
+      // a lane's channels: 16 (with an activation 8, and their up rows) from n0 on
+      constexpr int CN = ACT ? 8 : 16;
+      const int el = opaque_lane(), em = el & 15;
+      const int n0 = cur.n + wn * (kCols / 4) + CN * (el >> 4);
+      uint32_t tb[16];
+      float xs[MI];
+      {
+        const int64_t cb = (int64_t)cur.rt.e * c.N;
+        load_run<CN>(c.w_scale, cb, n0, NO - 1, c.w_scale_dtype, tb);
+        if constexpr (ACT) load_run<CN>(c.w_scale, cb + NO, n0, NO - 1, c.w_scale_dtype, tb + 8);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xs[i] = c.x_scale[er[i] >= 0 && er[i] < c.x_rows ? er[i] : 0];
+      }
+      uint32_t bb[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      if (c.bias != nullptr) {
+        const int64_t cb = (int64_t)cur.rt.e * c.N;
+        load_run<CN>(c.bias, cb, n0, NO - 1, c.bias_dtype, bb);
+        if constexpr (ACT) load_run<CN>(c.bias, cb + NO, n0, NO - 1, c.bias_dtype, bb + 8);
+      }
+      float cs[16], cb[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const Channel ch = channel(c, ChannelBits{tb[i], bb[i]});
+        cs[i] = ch.t, cb[i] = ch.b;
+      }
+      const RowOut<CN> out(c, cur.rt, NO, n0);
+      with_act(ACT ? c.act : -1, [&](auto a) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          // one row block after the other, so that their results do not all sit in
+          // registers at once
+          asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]) : : "memory");
+          const bool live = er[i] >= 0 && er[i] < c.x_rows;
+          float y[CN];
+#pragma unroll
+          for (int n = 0; n < CN; ++n) {
+            y[n] = scaled(acc[i][n >> 2][n & 3], xs[i], {cs[n], cb[n]});
+            if constexpr (ACT)
+              y[n] = act_fn(decltype(a)::value, y[n], scaled(acc[i][2 + (n >> 2)][n & 3], xs[i], {cs[8 + n], cb[8 + n]}),
+                            c.act_alpha, c.act_limit);
+            y[n] = live ? y[n] : 0.0f;
+          }
+          out.store(16 * (wm * MI + i) + em, y);
+        }
+      });
+      if (after >= end) break;
+      cur = next;
+      item = after;
+    }
+    wait_vm<0>();  // the copies past the last step, before the LDS is given back
+  }
+  if constexpr (GROUPED) {  // rows of no expert
+    const int head = scan.head(), tail = scan.tail(), none = head + ((int)c.rows - tail);
+    for (int z = blockIdx.x; z < none; z += gridDim.x) {
+      const int64_t row = z < head ? z : tail + (z - head);
+      for (int n = threadIdx.x; n < NO; n += 256 * WM) store_scalar(c.out, row * NO + n, c.out_dtype, 0.0f);
+    }
   }
 }
 
@@ -469,35 +885,129 @@ __global__ __launch_bounds__(256) void k_w8a8_any(ftm_w8a8 c, int mtiles, int nt
 
 namespace {
 
-template <int MT, int NT, int NW>
+template <int MT, int NT, int NW, int S, bool PACKED>
 hipError_t split(const ftm_w8a8& c, hipStream_t st) {
-  const int NO = out_cols(c);
+  constexpr int ring = NW * S * (MT + NT) * 16 * kRow, sums = NW * MT * NT * 1024;
+  constexpr int lds = ring > sums ? ring : sums;
   const int cols = c.act >= 0 ? 8 * NT : 16 * NT;
-  const int64_t mt = row_tiles(c, 16 * MT), nt = (NO + cols - 1) / cols;
+  const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + cols - 1) / cols;
   if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
-  const size_t lds = (size_t)NW * MT * NT * 1024;
-  const dim3 grid((unsigned)(mt * nt)), wg(64 * NW);
-  if (c.w_packed) k_w8a8_split<MT, NT, NW, true><<<grid, wg, lds, st>>>(c, (int)mt, (int)nt);
-  else k_w8a8_split<MT, NT, NW, false><<<grid, wg, lds, st>>>(c, (int)mt, (int)nt);
+  static DeviceBits lds_set{0};
+  const hipError_t e = allow_lds(lds_set, (const void*)k_w8a8_split<MT, NT, NW, S, PACKED>, lds);
+  if (e != hipSuccess) return e;
+  k_w8a8_split<MT, NT, NW, S, PACKED><<<dim3((unsigned)(mt * nt)), dim3(64 * NW), lds, st>>>(c, (int)mt, (int)nt);
   return hipGetLastError();
+}
+template <int MT, int NT, int NW, int S>
+hipError_t split(const ftm_w8a8& c, hipStream_t st) {
+  return c.w_packed ? split<MT, NT, NW, S, true>(c, st) : split<MT, NT, NW, S, false>(c, st);
+}
+
+constexpr int kCUs = 256;
+
+template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
+hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
+  constexpr int BM = 16 * MI * WM, lds = S * (BM + 256) * kRow;
+  constexpr int resident = kCUs * (2 * lds <= 160 * 1024 ? 2 : 1);  // workgroups the chip holds at once
+  const int cols = ACT ? 128 : 256;
+  const int64_t mt = row_tiles(c, BM), nt = (out_cols(c) + cols - 1) / cols;
+  if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w8a8_tile<WM, MI, S, PACKED, ACT, TAIL, GROUPED>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, lds);
+  if (e != hipSuccess) return e;
+  const int64_t grid = mt * nt < resident ? (mt * nt + 7) / 8 * 8 : resident;  // the same for every XCD
+  kernel<<<dim3((unsigned)grid), dim3(256 * WM), lds, st>>>(c, (int)mt, (int)nt);
+  return hipGetLastError();
+}
+template <int WM, int MI, int S, bool ACT, bool GROUPED>
+hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
+  if (c.K % 128 != 0 || c.K < 128 * S)
+    return c.w_packed ? tile<WM, MI, S, true, ACT, true, GROUPED>(c, st) : tile<WM, MI, S, false, ACT, true, GROUPED>(c, st);
+  return c.w_packed ? tile<WM, MI, S, true, ACT, false, GROUPED>(c, st) : tile<WM, MI, S, false, ACT, false, GROUPED>(c, st);
+}
+template <int WM, int MI, int S, bool GROUPED>
+hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
+  return c.act >= 0 ? tile<WM, MI, S, true, GROUPED>(c, st) : tile<WM, MI, S, false, GROUPED>(c, st);
+}
+
+// us on MI355X beside each rule: 'split' 64 x 64 is k_w8a8_split's tile of 64
+// tokens and 64 weight rows, 'tile' 64 k_w8a8_tile's of 64 tokens.
+
+// The split tile of up to 64 tokens whose columns give every CU one workgroup at
+// most (wider tiles read the tokens less often, but their CUs stay idle), or
+// none: 33-512 rows, 64 x 16 / 64 x 32 / 64 x 64 / tile 64: 64 of 4096 x 4096 7.8 /
+// 9.5 / 15.6 / 26, 128 13.8 / 10.0 / 15.8 / 26, 256 26 / 18.4 / 17.9 / 26, 512 50 /
+// 35 / 33 / 27, 64 of 4096 x 12288 25.6 / 22.4 / 19.3 / 38.
+bool split64(const ftm_w8a8& c, int64_t row_tiles, hipStream_t st, hipError_t& e) {
+  const int64_t blocks = row_tiles * ((c.N + 15) / 16);  // of 16 weight rows
+  if (blocks <= kCUs) e = split<4, 1, 4, 3>(c, st);
+  else if (blocks <= 2 * kCUs) e = split<4, 2, 4, 2>(c, st);
+  else if (blocks <= 6 * kCUs) e = split<4, 4, 4, 2>(c, st);
+  else return false;
+  return true;
+}
+
+hipError_t dense(const ftm_w8a8& c, hipStream_t st) {
+  const int64_t M = c.rows, blocks = (c.N + 15) / 16;
+  // Few rows: the weights' stream.  16 x 16 with four or two stages, 16 rows of
+  // 11008 x 4096 11.7 / 12.4, of 4096 x 12288 13.7 / 12.5; 32 x 16 / 32 x 32, 32
+  // rows of 4096 x 4096 5.8 / 7.2, of 4096 x 12288 16.3 / 14.8
+  if (M <= 16) return blocks <= 2 * kCUs ? split<1, 1, 4, 4>(c, st) : split<1, 1, 4, 2>(c, st);
+  if (M <= 32) return blocks <= 2 * kCUs ? split<2, 1, 4, 3>(c, st) : split<2, 2, 4, 2>(c, st);
+  hipError_t e = hipSuccess;
+  if (c.row_index != nullptr || split64(c, (M + 63) / 64, st, e)) return c.row_index != nullptr ? split<4, 4, 4, 2>(c, st) : e;
+  // The largest tile reads its operands least often, but a launch takes whole
+  // rounds of them: rounds x the time of one, in that of a 256-token tile (1;
+  // 128 tokens 0.6; two of 64 on a CU 0.68, one 0.58; 8192 rows of 8192 x 8192
+  // 460 / 558 / 625, 1024 of 4096 x 4096 50 / 33 / 30)
+  const int64_t nt = (c.N + 255) / 256;
+  auto rounds = [&](int rows, int at_once) { return (double)(((M + rows - 1) / rows * nt + at_once - 1) / at_once); };
+  const double t256 = rounds(256, kCUs), t128 = 0.6 * rounds(128, kCUs);
+  const double t64 = rounds(64, kCUs) <= 1 ? 0.58 : 0.68 * rounds(64, 2 * kCUs);
+  if (t256 <= t128 && t256 <= t64) return tile<2, 8, 2, false>(c, st);
+  return t128 <= t64 ? tile<2, 4, 3, false>(c, st) : tile<1, 4, 2, false>(c, st);
+}
+
+hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
+  // experts with rows, at most, and the rows of each if all have as many
+  const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
+  const int64_t tiles = hit * ((seg + 63) / 64) * ((c.N + 255) / 256);
+  // Too few tiles for the chip: K split.  16 x 32 / tile 64, 1 token over 8 of 256
+  // experts of 2048 x 1024 (32 tiles) 7.5 / 18.6, 4 tokens (128) 17.7 / 20.5, 16
+  // tokens (512) 49 / 33; 4 tokens over 32 of 128 experts of 768 x 2048 (256) 15.1 / 14.8
+  if (tiles < kCUs) {
+    if (seg <= 16) return split<1, 2, 4, 2>(c, st);
+    if (seg <= 32) return split<2, 2, 4, 2>(c, st);
+    hipError_t e = hipSuccess;
+    if (split64(c, hit * ((seg + 63) / 64), st, e)) return e;
+  }
+  // 64 / 128 tokens a tile, 2048 tokens over 128 experts (128 rows each) of 2048
+  // x 1536 123 / 142, 4 of 32 (256 rows each) of 2880 x 5760 337 / 283
+  return seg < 192 ? tile<1, 4, 2, true>(c, st) : tile<2, 4, 3, true>(c, st);
 }
 
 }  // namespace
 
+// Whether a tile's 32-bit offsets reach its tokens (256 rows from its first, or
+// all of x where they are read through an index), its weight rows and its results.
+static bool offsets_ok(const ftm_w8a8& c) {
+  const int64_t rows = c.row_index != nullptr ? c.x_rows : c.x_rows < 256 ? c.x_rows : 256;
+  const int64_t wrows = 256 + (c.act >= 0 ? c.N / 2 : 0);
+  return (rows - 1) * c.x_stride + c.K + 256 < INT32_MAX && wrows * c.K + 256 < INT32_MAX &&
+         4 * 256 * (int64_t)c.N < INT32_MAX;
+}
+
 hipError_t launch_w8a8(const ftm_w8a8& c, hipStream_t st) {
   const bool aligned = c.K % 16 == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15u) == 0 && (c.x_stride & 15) == 0 &&
                        (c.offsets == nullptr || (c.w_stride & 15) == 0);
-  if (!aligned) {
+  if (!aligned || !offsets_ok(c)) {
     const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + 15) / 16;
     if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
     k_w8a8_any<<<dim3((unsigned)(mt * nt)), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
     return hipGetLastError();
   }
-  // rows an expert gets on average
-  const int64_t seg = c.offsets == nullptr ? c.rows : c.rows / (c.rows < c.num_experts ? c.rows : c.num_experts);
-  if (seg <= 16) return split<1, 2, 4>(c, st);
-  if (seg <= 32) return split<2, 2, 4>(c, st);
-  return split<4, 2, 4>(c, st);
+  return c.offsets != nullptr ? grouped(c, st) : dense(c, st);
 }
 
 }  // namespace ftm

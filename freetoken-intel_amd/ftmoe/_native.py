@@ -9,7 +9,6 @@ binding (python/freetoken/kernel/cpu_moe.py:195-245), minus its JIT compiler.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -159,6 +158,18 @@ class FtmW8A8(ctypes.Structure):
     ]
 
 
+class FtmW8A8Moe(ctypes.Structure):
+    """``ftm_w8a8_moe``: one call of the routed experts, int8 x int8."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "topk_ids", "topk_w", "out", "w13", "w13_scale", "w13_bias", "w2",
+                                                "w2_scale", "w2_bias")]
+                + [("x_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("T", "k", "num_experts", "hidden", "inter", "dtype", "ids_dtype",
+                                                 "topk_w_dtype", "w13_packed", "w2_packed", "w13_scale_dtype",
+                                                 "w13_bias_dtype", "w2_scale_dtype", "w2_bias_dtype", "act")]
+                + [("act_alpha", ctypes.c_float), ("act_limit", ctypes.c_float)])
+
+
 # Every symbol include/ftmoe.h declares (tests check the export table against this).
 EXPORTED = (
     "ftm_version",
@@ -175,6 +186,9 @@ EXPORTED = (
     "ftm_dequant",
     "ftm_quant_int8",
     "ftm_w8a8_linear",
+    "ftm_w8a8_linear_dynamic",
+    "ftm_w8a8_moe_workspace_bytes",
+    "ftm_w8a8_moe_forward",
     "ftm_sort_workspace_bytes",
     "ftm_sort_tokens",
     "ftm_gather_tokens",
@@ -245,6 +259,12 @@ def lib() -> ctypes.CDLL:
     L.ftm_quant_int8.argtypes = [vp, i32, i64, i32, i64, vp, i64, vp, vp]
     L.ftm_w8a8_linear.restype = ctypes.c_int
     L.ftm_w8a8_linear.argtypes = [ctypes.POINTER(FtmW8A8), vp]
+    L.ftm_w8a8_linear_dynamic.restype = ctypes.c_int
+    L.ftm_w8a8_linear_dynamic.argtypes = [vp, i32, i64, ctypes.POINTER(FtmW8A8), vp]
+    L.ftm_w8a8_moe_workspace_bytes.restype = sz
+    L.ftm_w8a8_moe_workspace_bytes.argtypes = [i32] * 5
+    L.ftm_w8a8_moe_forward.restype = ctypes.c_int
+    L.ftm_w8a8_moe_forward.argtypes = [ctypes.POINTER(FtmW8A8Moe), vp, sz, vp]
     L.ftm_sort_workspace_bytes.restype = sz
     L.ftm_sort_workspace_bytes.argtypes = [i32, i32, i32]
     L.ftm_sort_tokens.restype = ctypes.c_int
@@ -316,14 +336,26 @@ def stream_of(t) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-_SAME_DEVICE = contextlib.nullcontext()
+_raw_stream = None  # device index -> its current stream, without a Stream object around it
 
 
-def on_device_of(t):
-    """The context a launch on ``t``'s stream needs: ``t``'s device current."""
+def launch(what: str, fn, t, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``t``'s device, which is made
+    current for the call; raises :class:`FtmError` for an error code."""
+    global _raw_stream
     import torch
 
-    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    if _raw_stream is None:
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda i: torch.cuda.current_stream(i).cuda_stream)
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc < 0:
+        raise FtmError(what, rc)
 
 
 def require_same_device(t, others) -> None:

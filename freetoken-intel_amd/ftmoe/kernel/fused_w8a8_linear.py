@@ -6,8 +6,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _native as nat
-from .w8a8_linear import quantize_int8_token, w8a8_linear
+from .w8a8_linear import _product
 
 
 def fused_w8a8_linear(
@@ -20,11 +19,7 @@ def fused_w8a8_linear(
 ) -> torch.Tensor:
     """``quantize_int8_token(x)`` times ``weight`` (int8 ``[N, K]`` or packed int32
     ``[N, K/4]``, ``weight_scale [N]``) ``(+ bias)``, in ``out_dtype`` (default: x's)."""
-    if x.dim() != 2:
-        raise ValueError(f"x must be [M, K], got {tuple(x.shape)}")
-    nat.require_gpu(x, "x")
-    q, s = quantize_int8_token(x)
-    return w8a8_linear(q, s, weight, weight_scale, bias=bias, out_dtype=out_dtype if out_dtype is not None else x.dtype)
+    return _product(x, None, weight, weight_scale, bias=bias, out_dtype=out_dtype if out_dtype is not None else x.dtype)
 
 
 def fused_w8a8_expert_forward(
@@ -36,18 +31,18 @@ def fused_w8a8_expert_forward(
     *,
     intermediate: int,
     activation: str = "silu",
+    swiglu_alpha: float = 1.702,
+    swiglu_limit: float = 7.0,
     out_dtype: torch.dtype | None = None,
 ) -> torch.Tensor:
     """One expert: ``down(act(gate(x)) * up(x))``, x and ``h`` each quantised by token
     (``h`` from fp32)."""
     if weight_gate_up.shape[0] != 2 * intermediate:
         raise ValueError(f"weight_gate_up must have {2 * intermediate} rows, got {weight_gate_up.shape[0]}")
-    if x.dim() != 2:
-        raise ValueError(f"x must be [M, K], got {tuple(x.shape)}")
-    q, s = quantize_int8_token(x)
-    h = w8a8_linear(q, s, weight_gate_up, weight_scale_gate_up, activation=activation, out_dtype=torch.float32)
-    q, s = quantize_int8_token(h)
-    return w8a8_linear(q, s, weight_down, weight_scale_down, out_dtype=out_dtype if out_dtype is not None else x.dtype)
+    h = _product(x, None, weight_gate_up, weight_scale_gate_up, bias=None, activation=activation,
+                 alpha=swiglu_alpha, limit=swiglu_limit, out_dtype=torch.float32)
+    return _product(h, None, weight_down, weight_scale_down, bias=None,
+                    out_dtype=out_dtype if out_dtype is not None else x.dtype)
 
 
 __all__ = ["fused_w8a8_linear", "fused_w8a8_expert_forward"]

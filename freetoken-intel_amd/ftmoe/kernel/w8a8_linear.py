@@ -19,99 +19,134 @@ import torch
 from .. import _native as nat
 from ..layer import ACTIVATIONS
 
-_SCALE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+_DT = {torch.float32: nat.DT_F32, torch.float16: nat.DT_F16, torch.bfloat16: nat.DT_BF16}
+
+
+def _dt(dtype, name: str) -> int:
+    code = _DT.get(dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {dtype}")
+    return code
 
 
 def quantize_int8_token(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``x [..., K]`` (fp32, fp16 or bf16) -> (int8 codes ``[..., K]``, fp32 scales
-    ``[...]``): scale = max |x| / 127 of the row (the maximum at least 1e-12), code
-    = the whole number nearest x / scale, ties to even.  A row with an infinity or
+    ``[...]``): scale = max |x| / 127 of the row (the maximum at least 1e-12; times the
+    fp32 nearest 1 / 127, as torch divides by a number on the GPU), code = the whole
+    number nearest x / scale, ties to even.  A row with an infinity or
     NaN gets the scale NaN and codes 0: its products are NaN, no other row's are."""
     nat.require_gpu(x, "x")
-    dt = nat.dtype_code(x.dtype)
+    dt = _dt(x.dtype, "x")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., K] with K > 0, got {tuple(x.shape)}")
     lead, K = x.shape[:-1], x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1 and K > 1:
-        x2 = x2.contiguous()
-    rows = x2.shape[0]
-    q = torch.empty((*lead, K), dtype=torch.int8, device=x.device)
+    x2 = rows_of(x if x.dim() == 2 else x.reshape(-1, K))
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    if rows == 0:
-        return q, scale
-    with nat.on_device_of(x):
-        rc = nat.lib().ftm_quant_int8(x2.data_ptr(), dt, rows, K, x2.stride(0) * x2.element_size(), q.data_ptr(), K,
-                                      scale.data_ptr(), nat.stream_of(x))
-    nat.check(rc, "ftm_quant_int8")
+    if x2.shape[0]:
+        nat.launch("ftm_quant_int8", nat.lib().ftm_quant_int8, x2, x2.data_ptr(), dt, x2.shape[0], K,
+                   x2.stride(0) * x2.element_size(), q.data_ptr(), K, scale.data_ptr())
     return q, scale
 
 
-def _weight(weight: torch.Tensor, K: int, dim: int) -> tuple[torch.Tensor, int]:
-    """(contiguous weight, packed) after the checks the formats share."""
-    if weight.dtype not in (torch.int8, torch.int32):
-        raise TypeError(f"weight must be int8 or packed int32, got {weight.dtype}")
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t [n, H]`` with neighbouring elements of a row side by side."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def weight_of(weight: torch.Tensor, K: int, dim: int, name: str = "weight") -> tuple[torch.Tensor, int]:
+    """(contiguous weight, whether it is packed) for activations of K channels."""
+    if weight.dtype == torch.int8:
+        packed, k = 0, weight.shape[-1] if weight.dim() else 0
+    elif weight.dtype == torch.int32:
+        packed, k = 1, 4 * weight.shape[-1] if weight.dim() else 0
+    else:
+        raise TypeError(f"{name} must be int8 or packed int32, got {weight.dtype}")
     if weight.dim() != dim:
-        raise ValueError(f"weight must have {dim} dimensions, got shape {tuple(weight.shape)}")
-    packed = weight.dtype == torch.int32
-    k = weight.shape[-1] * (4 if packed else 1)
+        raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(weight.shape)}")
     if k != K:
-        raise ValueError(f"x's K={K} does not match the weight's K={k}")
+        raise ValueError(f"x's K={K} does not match the {name}'s K={k}")
     if K > nat.W8A8_MAX_K:
         raise ValueError(f"K={K} exceeds {nat.W8A8_MAX_K}: int32 sums of int8 products could overflow")
-    return weight.contiguous(), int(packed)
+    return weight.contiguous(), packed
 
 
-def _per_channel(t: torch.Tensor, shape: tuple, name: str) -> torch.Tensor:
-    if t.dtype not in _SCALE_DTYPES:
-        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    if tuple(t.shape) != shape and (name != "weight_scale" or tuple(t.shape) != (*shape, 1)):
+def scale_of(t: torch.Tensor, shape, name: str) -> tuple[torch.Tensor, int]:
+    """(contiguous scales of ``shape`` -- or with a last 1, one group a row --, their dtype code)."""
+    code = _dt(t.dtype, name)
+    if t.shape != shape and t.shape != (*shape, 1):
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
-    return t.contiguous()
+    return t.contiguous(), code
 
 
-def _product(x_int8, x_scale, weight, weight_scale, *, offsets, row_index, bias, activation, swiglu_alpha,
-             swiglu_limit, out_dtype) -> torch.Tensor:
-    nat.require_gpu(x_int8, "x_int8")
-    nat.require_same_device(x_int8, (("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale),
-                                     ("bias", bias), ("offsets", offsets), ("row_index", row_index)))
-    if x_int8.dtype != torch.int8:
-        raise TypeError(f"x_int8 must be int8, got {x_int8.dtype}")
-    if x_int8.dim() != 2 or x_int8.shape[1] == 0:
-        raise ValueError(f"x_int8 must be [M, K] with K > 0, got {tuple(x_int8.shape)}")
-    M, K = x_int8.shape
-    if x_scale.dtype != torch.float32:
-        raise TypeError(f"x_scale must be float32, got {x_scale.dtype}")
-    if tuple(x_scale.shape) not in ((M,), (M, 1)):
-        raise ValueError(f"x_scale must be [{M}], got {tuple(x_scale.shape)}")
-    w, packed = _weight(weight, K, 2 if offsets is None else 3)
-    N = w.shape[-2]
-    ws = _per_channel(weight_scale, tuple(w.shape[:-1]), "weight_scale")
-    b = _per_channel(bias, tuple(w.shape[:-1]), "bias") if bias is not None else None
+def bias_of(t: Optional[torch.Tensor], shape, name: str) -> tuple[Optional[torch.Tensor], int]:
+    if t is None:
+        return None, 0
+    code = _dt(t.dtype, name)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    return t.contiguous(), code
+
+
+def activation_code(activation: str) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unsupported MoE activation: {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _product(x, x_scale, weight, weight_scale, *, bias, out_dtype, offsets=None, row_index=None, activation=None,
+             alpha=0.0, limit=0.0) -> torch.Tensor:
+    """The call behind the products: x int8 with x_scale, or (x_scale None) wide x that the
+    same call quantises."""
+    nat.require_gpu(x, "x_int8" if x_scale is not None else "x")
+    nat.require_same_device(x, (("weight", weight), ("weight_scale", weight_scale), ("x_scale", x_scale),
+                                ("bias", bias), ("offsets", offsets), ("row_index", row_index)))
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x must be [M, K] with K > 0, got {tuple(x.shape)}")
+    M, K = x.shape
+    if x_scale is None:
+        x_dt = _dt(x.dtype, "x")
+    else:
+        if x.dtype != torch.int8:
+            raise TypeError(f"x_int8 must be int8, got {x.dtype}")
+        if x_scale.dtype != torch.float32:
+            raise TypeError(f"x_scale must be float32, got {x_scale.dtype}")
+        if x_scale.shape != (M,) and x_scale.shape != (M, 1):
+            raise ValueError(f"x_scale must be [{M}], got {tuple(x_scale.shape)}")
+        x_scale = x_scale.contiguous()
+    w, packed = weight_of(weight, K, 2 if offsets is None else 3)
+    lead = w.shape[:-1]
+    N = lead[-1]
+    ws, ws_dt = scale_of(weight_scale, lead, "weight_scale")
+    b, b_dt = bias_of(bias, lead, "bias")
+    out_dt = _dt(out_dtype, "out_dtype")
     act = -1
     if activation is not None:
-        if activation not in ACTIVATIONS:
-            raise ValueError(f"unsupported MoE activation: {activation!r}")
+        act = activation_code(activation)
         if N % 2:
             raise ValueError(f"a gated activation needs an even number of weight rows (gate, then up), got {N}")
-        act = ACTIVATIONS[activation]
-    if x_int8.stride(1) != 1 and K > 1:
-        x_int8 = x_int8.contiguous()
-    x_scale = x_scale.contiguous()
+    x = rows_of(x)
     rows = M if row_index is None else row_index.shape[0]
-    out = torch.empty((rows, N // 2 if act >= 0 else N), dtype=out_dtype, device=x_int8.device)
+    out = torch.empty((rows, N // 2 if act >= 0 else N), dtype=out_dtype, device=x.device)
     if out.numel() == 0:
         return out
     if M == 0:  # an index into no rows
         return out.zero_()
-    c = nat.FtmW8A8(x_int8.data_ptr(), x_scale.data_ptr(), w.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(),
-                    nat.ptr(offsets), nat.ptr(row_index), rows, M, x_int8.stride(0), N * K, N, K,
-                    1 if offsets is None else w.shape[0], packed, nat.dtype_code(ws.dtype),
-                    nat.dtype_code(b.dtype) if b is not None else 0, nat.dtype_code(out_dtype), act,
-                    swiglu_alpha, swiglu_limit)
-    with nat.on_device_of(x_int8):
-        rc = nat.lib().ftm_w8a8_linear(ctypes.byref(c), nat.stream_of(x_int8))
-    nat.check(rc, "ftm_w8a8_linear")
+    if x_scale is None:  # codes, then the scales on a 4-byte border
+        at = (M * K + 3) // 4 * 4
+        scratch = torch.empty(at + 4 * M, dtype=torch.uint8, device=x.device).data_ptr()
+        q, s, stride = scratch, scratch + at, K
+    else:
+        q, s, stride = x.data_ptr(), x_scale.data_ptr(), x.stride(0)
+    c = nat.FtmW8A8(q, s, w.data_ptr(), ws.data_ptr(), None if b is None else b.data_ptr(), out.data_ptr(),
+                    None if offsets is None else offsets.data_ptr(), None if row_index is None else row_index.data_ptr(),
+                    rows, M, stride, N * K, N, K, 1 if offsets is None else lead[0], packed, ws_dt, b_dt, out_dt, act,
+                    alpha, limit)
+    if x_scale is None:
+        nat.launch("ftm_w8a8_linear_dynamic", nat.lib().ftm_w8a8_linear_dynamic, x, x.data_ptr(), x_dt,
+                   x.stride(0) * x.element_size(), ctypes.byref(c))
+    else:
+        nat.launch("ftm_w8a8_linear", nat.lib().ftm_w8a8_linear, x, ctypes.byref(c))
     return out
 
 
@@ -134,8 +169,8 @@ def w8a8_linear(
     ``[N, 1]``).  With ``activation`` (as :class:`~ftmoe.layer.MoeLayer` names them) the
     weight's first N/2 rows are gate and the others up, and the result is
     ``act(gate) * up`` ``[M, N/2]``."""
-    return _product(x_int8, x_scale, weight, weight_scale, offsets=None, row_index=None, bias=bias,
-                    activation=activation, swiglu_alpha=swiglu_alpha, swiglu_limit=swiglu_limit, out_dtype=out_dtype)
+    return _product(x_int8, x_scale, weight, weight_scale, bias=bias, activation=activation, alpha=swiglu_alpha,
+                    limit=swiglu_limit, out_dtype=out_dtype)
 
 
 def w8a8_grouped_linear(
@@ -169,12 +204,13 @@ def w8a8_grouped_linear(
             raise TypeError(f"{name} must be int32, got {t.dtype}")
         if t.dim() != 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous and have one dimension, got {tuple(t.shape)}")
-    if weight.dim() == 3 and offsets.shape[0] != weight.shape[0] + 1:
-        raise ValueError(f"offsets must have {weight.shape[0] + 1} entries, got {offsets.shape[0]}")
-    if not 1 <= offsets.shape[0] - 1 <= 512:
-        raise ValueError(f"between 1 and 512 experts, got {offsets.shape[0] - 1}")
+    E = offsets.shape[0] - 1
+    if weight.dim() == 3 and weight.shape[0] != E:
+        raise ValueError(f"offsets must have {weight.shape[0] + 1} entries, got {E + 1}")
+    if not 1 <= E <= 512:
+        raise ValueError(f"between 1 and 512 experts, got {E}")
     return _product(x_int8, x_scale, weight, weight_scale, offsets=offsets, row_index=row_index, bias=bias,
-                    activation=activation, swiglu_alpha=swiglu_alpha, swiglu_limit=swiglu_limit, out_dtype=out_dtype)
+                    activation=activation, alpha=swiglu_alpha, limit=swiglu_limit, out_dtype=out_dtype)
 
 
 __all__ = ["quantize_int8_token", "w8a8_linear", "w8a8_grouped_linear"]

@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
 
-_ID_DTYPES = {torch.int32: nat.ID_I32, torch.int64: nat.ID_I64}
+ID_DTYPES = {torch.int32: nat.ID_I32, torch.int64: nat.ID_I64}
 
 
 @dataclass(frozen=True)
@@ -40,7 +40,7 @@ def sort_tokens(topk_ids: torch.Tensor, num_experts: int) -> TokenSort:
     """Sort the pairs of ``topk_ids [T, k]`` (int32 or int64) by expert, stably.  An id
     outside ``[0, num_experts)`` is a pair without an expert; ``num_experts`` <= 512."""
     nat.require_gpu(topk_ids, "topk_ids")
-    if topk_ids.dtype not in _ID_DTYPES:
+    if topk_ids.dtype not in ID_DTYPES:
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     if topk_ids.dim() != 2 or topk_ids.shape[1] == 0:
         raise ValueError(f"topk_ids must be [T, k] with k > 0, got {tuple(topk_ids.shape)}")
@@ -58,11 +58,9 @@ def sort_tokens(topk_ids: torch.Tensor, num_experts: int) -> TokenSort:
     token_of_row = torch.empty(T * k, dtype=torch.int32, device=dev)
     need = L.ftm_sort_workspace_bytes(T, k, E)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with nat.on_device_of(ids):
-        rc = L.ftm_sort_tokens(ids.data_ptr(), _ID_DTYPES[ids.dtype], T, k, E, offsets.data_ptr(),
-                               row_of_pair.data_ptr(), pair_of_row.data_ptr(), token_of_row.data_ptr(), nat.ptr(ws),
-                               need, nat.stream_of(ids))
-    nat.check(rc, "ftm_sort_tokens")
+    nat.launch("ftm_sort_tokens", L.ftm_sort_tokens, ids, ids.data_ptr(), ID_DTYPES[ids.dtype], T, k, E,
+               offsets.data_ptr(), row_of_pair.data_ptr(), pair_of_row.data_ptr(), token_of_row.data_ptr(),
+               nat.ptr(ws), need)
     return TokenSort(E, offsets, row_of_pair, pair_of_row, token_of_row)
 
 
@@ -87,10 +85,8 @@ def _gather(x: torch.Tensor, sort: TokenSort) -> torch.Tensor:
     rows = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
     if rows.numel() == 0:
         return rows
-    with nat.on_device_of(x):
-        rc = nat.lib().ftm_gather_tokens(x.data_ptr(), x.stride(0) * size, size, H, sort.row_of_pair.data_ptr(), T, k,
-                                         rows.data_ptr(), nat.stream_of(x))
-    nat.check(rc, "ftm_gather_tokens")
+    nat.launch("ftm_gather_tokens", nat.lib().ftm_gather_tokens, x, x.data_ptr(), x.stride(0) * size, size, H,
+               sort.row_of_pair.data_ptr(), T, k, rows.data_ptr())
     return rows
 
 
@@ -102,13 +98,9 @@ def _combine(rows: torch.Tensor, w: Optional[torch.Tensor], sort: TokenSort, out
     if out.numel() == 0:
         return out
     w = w.contiguous() if w is not None else None
-    with nat.on_device_of(rows):
-        rc = nat.lib().ftm_combine_tokens(rows.data_ptr(), nat.dtype_code(rows.dtype),
-                                          rows.stride(0) * rows.element_size(), nat.ptr(w),
-                                          nat.dtype_code(w.dtype) if w is not None else 0,
-                                          sort.row_of_pair.data_ptr(), T, k, H, out.data_ptr(),
-                                          nat.dtype_code(out_dtype), nat.stream_of(rows))
-    nat.check(rc, "ftm_combine_tokens")
+    nat.launch("ftm_combine_tokens", nat.lib().ftm_combine_tokens, rows, rows.data_ptr(), nat.dtype_code(rows.dtype),
+               rows.stride(0) * rows.element_size(), nat.ptr(w), nat.dtype_code(w.dtype) if w is not None else 0,
+               sort.row_of_pair.data_ptr(), T, k, H, out.data_ptr(), nat.dtype_code(out_dtype))
     return out
 
 
@@ -144,13 +136,10 @@ class _Combine(torch.autograd.Function):
         grad_w = torch.empty((T, k), dtype=w.dtype, device=w.device) if want_w else None
         if T == 0 or H == 0:
             return grad_rows, None if grad_w is None else grad_w.zero_(), None, None
-        with nat.on_device_of(rows):
-            rc = nat.lib().ftm_combine_tokens_grad(
-                g.data_ptr(), nat.dtype_code(g.dtype), g.stride(0) * g.element_size(), rows.data_ptr(),
-                nat.dtype_code(rows.dtype), rows.stride(0) * rows.element_size(), wc.data_ptr(),
-                nat.dtype_code(w.dtype), sort.row_of_pair.data_ptr(), T, k, H, nat.ptr(grad_rows), nat.ptr(grad_w),
-                nat.stream_of(rows))
-        nat.check(rc, "ftm_combine_tokens_grad")
+        nat.launch("ftm_combine_tokens_grad", nat.lib().ftm_combine_tokens_grad, rows, g.data_ptr(),
+                   nat.dtype_code(g.dtype), g.stride(0) * g.element_size(), rows.data_ptr(),
+                   nat.dtype_code(rows.dtype), rows.stride(0) * rows.element_size(), wc.data_ptr(),
+                   nat.dtype_code(w.dtype), sort.row_of_pair.data_ptr(), T, k, H, nat.ptr(grad_rows), nat.ptr(grad_w))
         return grad_rows, grad_w, None, None
 
 

@@ -270,8 +270,8 @@ int ftm_dequant(const ftm_proj* proj, int32_t slot, void* out, int32_t out_dtype
  * above); these take the activations in int8 too, one scale per token. */
 
 /* Quantise rows x [rows, K] (x_stride bytes apart) to int8: scale[m] =
- * fp32(max_k |x[m, k]| / 127), the maximum taken as at least 1e-12; q[m, k] =
- * the whole number nearest x[m, k] / scale[m], ties to even (q_stride bytes
+ * max_k |x[m, k]| * fp32(1 / 127) in fp32, the maximum taken as at least 1e-12
+ * (the value of torch's amax / 127 on the GPU); q[m, k] = the whole number nearest x[m, k] / scale[m], ties to even (q_stride bytes
  * between rows).  A row with an infinity or NaN gets the scale NaN and codes 0. */
 int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride,
                    int8_t* q, int64_t q_stride, float* scale, void* stream);
@@ -309,6 +309,11 @@ typedef struct ftm_w8a8 {
 #define FTM_W8A8_MAX_K 131071
 int ftm_w8a8_linear(const ftm_w8a8* call, void* stream);
 
+/* ftm_quant_int8 of x [call->x_rows, K] and ftm_w8a8_linear over its codes:
+ * call->x [x_rows, K] (x_stride K) and call->x_scale are scratch that the call
+ * writes first. */
+int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w8a8* call, void* stream);
+
 /* ---- (token, expert) pairs sorted by expert, and back ----
  * ids [T, k] int32 or int64 (ids_dtype: FTM_ID_*).  Pair p = t k + j.  The rows
  * of expert e, [offsets[e], offsets[e+1]), are its pairs in order of p; the
@@ -345,6 +350,45 @@ int ftm_combine_tokens(const void* rows, int32_t dtype, int64_t row_stride, cons
 int ftm_combine_tokens_grad(const void* g, int32_t g_dtype, int64_t g_stride, const void* rows, int32_t dtype,
                             int64_t row_stride, const void* w, int32_t w_dtype, const int32_t* row_of_pair,
                             int32_t T, int32_t k, int32_t H, void* grad_rows, void* grad_w, void* stream);
+
+/* Routed experts, int8 x int8: sort the pairs of topk_ids, quantise x [T, H],
+ * w13 with its activation, quantise h (fp32), w2, and the rows (fp32) back with
+ * topk_w [T, k], rounded once to dtype (x and out).  w13 / w2: the weights, as
+ * ftm_w8a8's w, w_scale, bias with their strides and dtypes; N and K are the
+ * layer's (w13 [2 inter, hidden], w2 [hidden, inter]).  The workspace needs no
+ * initial value; one call uses it at a time. */
+typedef struct ftm_w8a8_moe {
+  const void* x;          /* [T, hidden], x_stride bytes apart */
+  const void* topk_ids;   /* [T, k], ids_dtype; outside [0, E): no expert */
+  const void* topk_w;     /* [T, k], topk_w_dtype */
+  void* out;              /* [T, hidden] */
+  const void* w13;
+  const void* w13_scale;
+  const void* w13_bias;   /* or NULL */
+  const void* w2;
+  const void* w2_scale;
+  const void* w2_bias;    /* or NULL */
+  int64_t x_stride;
+  int32_t T;
+  int32_t k;
+  int32_t num_experts;
+  int32_t hidden;
+  int32_t inter;
+  int32_t dtype;
+  int32_t ids_dtype;
+  int32_t topk_w_dtype;
+  int32_t w13_packed;
+  int32_t w2_packed;
+  int32_t w13_scale_dtype;
+  int32_t w13_bias_dtype;
+  int32_t w2_scale_dtype;
+  int32_t w2_bias_dtype;
+  int32_t act;            /* FTM_ACT_* */
+  float act_alpha;
+  float act_limit;
+} ftm_w8a8_moe;
+size_t ftm_w8a8_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter);
+int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---- offload slot pool (python/freetoken/moe/offload_cache.py:218-694) ---- */
 

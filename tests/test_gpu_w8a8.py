@@ -58,9 +58,12 @@ def exact(q, s, w, ws, bias=None):
 
 
 # ------------------------------------------------------------------ quantiser
+INV = torch.ones(()) / 127  # the fp32 nearest 1 / 127, by which the scale is defined
+
+
 def exact_quantise(x):
     xc = x.cpu()
-    s = xc.float().abs().amax(dim=-1).clamp_min(1e-12) / 127
+    s = xc.float().abs().amax(dim=-1).clamp_min(1e-12) * INV
     q = (xc.double() / s.double().unsqueeze(-1)).round()
     return q.to(torch.int8), s
 
@@ -83,13 +86,25 @@ def test_quantiser_borders(gpu):
     n = torch.arange(-127, 127, dtype=torch.float64) + 0.5
     for s in (2.0 ** -3, 0.1, 0.37, 1.7e-5, 3.3e7):
         top = torch.tensor(127 * s, dtype=torch.float32)
-        sc = (top / 127).double()
+        sc = (top * INV).double()
         b = (n * sc).float()
         x = torch.cat([top.reshape(1), b, torch.nextafter(b, torch.tensor(math.inf)),
                        torch.nextafter(b, torch.tensor(-math.inf))])[None]
         q, sg = quantize_int8_token(x.to(gpu))
         rq, rs = exact_quantise(x)
         assert torch.equal(sg.cpu(), rs) and torch.equal(q.cpu(), rq), s
+
+
+def test_quantiser_is_torchs_on_the_gpu(gpu):
+    """bf16 values, whose quotients often end in .5: the codes of ``quantize_int8_channel``
+    on the GPU wherever its fp32 quotient is not the one that a border needs."""
+    x = torch.randn(500, 512, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(gpu)
+    q, s = quantize_int8_token(x)
+    tq, ts = quant.quantize_int8_channel(x)
+    assert torch.equal(s, ts)
+    quotient = x.double() / s.double()[:, None]
+    sure = ((quotient - quotient.floor()) - 0.5).abs() > 127 * U
+    assert torch.equal(q[sure], tq[sure])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -106,7 +121,7 @@ def test_quantiser_rows_apart(gpu, dtype, K):
     q, s = quantize_int8_token(bad)
     for r in (0, 2, 3):
         assert torch.isnan(s[r]) and not q[r].any()
-    assert not q[4].any() and s[4].item() == torch.tensor(1e-12).div(127).item()
+    assert not q[4].any() and s[4].item() == (torch.tensor(1e-12) * INV).item()
     for r in (1, 5):
         assert torch.equal(q[r], ref_q[r]) and s[r] == ref_s[r]
 
@@ -373,7 +388,7 @@ def moe_inputs(gpu, T, E, H, I, k, dtype, seed=0, drop=False):
 
 def exact_moe(x, w1, s1, w2, s2, ids, tw):
     def quantise(v):
-        s = (v.abs().amax(dim=1).clamp_min(1e-12).float() / 127).double()
+        s = (v.abs().amax(dim=1).clamp_min(1e-12).float() * INV.to(v.device)).double()
         return (v / s[:, None]).round().clamp(-127, 127) * s[:, None]
 
     out = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
