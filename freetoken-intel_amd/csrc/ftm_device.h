@@ -207,6 +207,19 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
   return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
 }
 
+// Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
+// lanes (DPP row_shr, zeros shifted in), then the rows before.
+__device__ __forceinline__ int wave_prefix_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31);
+  const int c = __builtin_amdgcn_readlane(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
 __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 32));
   v = fmaxf(v, __shfl_xor(v, 16));

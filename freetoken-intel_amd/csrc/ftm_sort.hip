@@ -16,21 +16,23 @@ namespace ftm {
 namespace {
 
 constexpr int kSortWaves = 16;
-constexpr int kSortKeys = kMaxExperts + 1;  // the last: no expert
-constexpr int kSortOne = 8192;              // pairs that one workgroup sorts
-constexpr int kSortBlocks = 128;            // workgroups above that, at most
-constexpr int kSortPer = 4096;              // pairs a workgroup, at least
+constexpr int kSortWg = 64 * kSortWaves;  // threads and pairs of one round of a workgroup
+constexpr int kSortOne = 4 * kSortWg;     // pairs that one workgroup sorts by itself
 
-inline int64_t sort_per(int64_t P) {
-  const int64_t per = (P + kSortBlocks - 1) / kSortBlocks;
-  return per < kSortPer ? kSortPer : (per + 1023) / 1024 * 1024;
+// Pairs a workgroup takes: up to four rounds by itself, one of several takes
+// one round, four where there are more than 256 of them otherwise (every one reads
+// all counts).
+inline int sort_rounds(int64_t P) {
+  const int64_t r = (P + kSortWg - 1) / kSortWg;
+  if (P <= kSortOne) return r <= 1 ? 1 : r <= 2 ? 2 : 4;
+  return r <= 256 ? 1 : 4;
 }
 
 }  // namespace
 
 template <class ID>
-__device__ __forceinline__ int sort_key(const ID* ids, int64_t p, int64_t end, int E) {
-  const ID v = p < end ? ids[p] : (ID)-1;
+__device__ __forceinline__ int sort_key(const ID* ids, int64_t p, int64_t P, int E) {
+  const ID v = p < P ? ids[p] : (ID)-1;
   return v >= 0 && v < (ID)E ? (int)v : E;
 }
 
@@ -44,61 +46,77 @@ __device__ __forceinline__ uint64_t same_key(int key, int bits, uint64_t live) {
   return m;
 }
 
-// Counts of a workgroup's pairs by wave and key: each wave walks a run of its
-// own, one leader lane a key adds the number of lanes that share it, so the
+// Pairs of one workgroup: wave w's run is pairs 64 R w .. of the workgroup's, 64 a
+// round.  hist[w][key] counts the wave's; a lane's rank is the number of pairs
+// before it in its run with its key.  One lane a key adds for the others, so the
 // order of the pairs is kept and no atomics are used.
-template <class ID>
-__device__ __forceinline__ void sort_count(const ID* ids, int64_t lo, int64_t hi, int64_t run, int E, int bits,
-                                           int (*hist)[kSortKeys]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = threadIdx.x; i < kSortWaves * kSortKeys; i += 64 * kSortWaves) ((int*)hist)[i] = 0;
-  __syncthreads();
-  const int64_t w_lo = lo + wave * run, w_hi = w_lo + run < hi ? w_lo + run : hi;
-  for (int64_t p0 = w_lo; p0 < w_hi; p0 += 64) {
-    const int64_t p = p0 + lane;
-    const int key = sort_key(ids, p, w_hi, E);
-    const uint64_t m = same_key(key, bits, __ballot(p < w_hi));
-    if (p < w_hi && (m & ((1ull << lane) - 1)) == 0) hist[wave][key] += __popcll(m);
+template <class ID, int R>
+struct SortRun {
+  int key[R], rank[R];
+  int64_t p0;  // the lane's pair of the first round
+
+  __device__ __forceinline__ SortRun(const ID* ids, int64_t P, int E, int bits, int* hist) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    p0 = (int64_t)blockIdx.x * (R * kSortWg) + wave * (64 * R) + lane;
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = sort_key(ids, p0 + 64 * r, P, E);
+    for (int i = threadIdx.x; i < kSortWaves * (E + 1); i += kSortWg) hist[i] = 0;
+    __syncthreads();
+    int* mine = hist + wave * (E + 1);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = p0 + 64 * r < P;
+      const uint64_t m = same_key(key[r], bits, __ballot(live));
+      rank[r] = live ? mine[key[r]] + __popcll(m & ((1ull << lane) - 1)) : 0;
+      __builtin_amdgcn_wave_barrier();
+      // the last lane of a key, once every lane has read the count (the wave runs
+      // in step, its LDS accesses in order)
+      if (live && (m >> lane) == 1) mine[key[r]] = rank[r] + 1;
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
   }
-  __syncthreads();
-}
+};
 
 // counts[b][key] of workgroup b's pairs.
-template <class ID>
-__global__ __launch_bounds__(64 * kSortWaves) void k_sort_count(const ID* ids, int64_t P, int64_t per, int E, int bits,
-                                                                int32_t* counts) {
-  __shared__ int hist[kSortWaves][kSortKeys];
-  const int64_t lo = blockIdx.x * per, hi = lo + per < P ? lo + per : P;
-  sort_count(ids, lo, hi, per / kSortWaves, E, bits, hist);
-  for (int e = threadIdx.x; e <= E; e += 64 * kSortWaves) {
+template <class ID, int R>
+__global__ __launch_bounds__(kSortWg) void k_sort_count(const ID* ids, int64_t P, int E, int bits, int32_t* counts) {
+  __shared__ int hist[kSortWaves * (kMaxExperts + 1)];
+  const SortRun<ID, R> run(ids, P, E, bits, hist);
+  for (int e = threadIdx.x; e <= E; e += kSortWg) {
     int n = 0;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) n += hist[w][e];
+    for (int w = 0; w < kSortWaves; ++w) n += hist[w * (E + 1) + e];
     counts[(int64_t)blockIdx.x * (E + 1) + e] = n;
   }
 }
 
 // The rows of workgroup b's pairs: the keys' totals over all workgroups and
-// those before b (counts; none: one workgroup sorts everything), their prefix
-// sum, then a second walk in the order of the first.
-template <class ID>
-__global__ __launch_bounds__(64 * kSortWaves) void k_sort_place(const ID* ids, int64_t P, int64_t per, int E, int bits,
-                                                                int k, const int32_t* counts, int blocks,
-                                                                int32_t* offsets, int32_t* row_of_pair,
-                                                                int32_t* pair_of_row, int32_t* token_of_row) {
-  __shared__ int hist[kSortWaves][kSortKeys];
-  __shared__ int total[64 * 9], mine[64 * 9];
+// those before b (counts; null: this one sorts everything) and their prefix sum
+// give the first row of every wave's pairs of every key; a pair's rank is added.
+template <class ID, int R>
+__global__ __launch_bounds__(kSortWg) void k_sort_place(const ID* ids, int64_t P, int E, int bits, int k,
+                                                        const int32_t* counts, int32_t* offsets, int32_t* row_of_pair,
+                                                        int32_t* pair_of_row, int32_t* token_of_row) {
+  __shared__ int hist[kSortWaves * (kMaxExperts + 1)];
+  __shared__ int total[64 * 9], first[64 * 9];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t lo = blockIdx.x * per, hi = lo + per < P ? lo + per : P;
-  const int64_t run = per / kSortWaves;
-  sort_count(ids, lo, hi, run, E, bits, hist);
-  for (int e = threadIdx.x; e < 64 * 9; e += 64 * kSortWaves) {
+  const SortRun<ID, R> run(ids, P, E, bits, hist);
+  for (int e = threadIdx.x; e < 64 * 9; e += kSortWg) {
     int all = 0, before = 0;
     if (e <= E) {
-      if (counts == nullptr) {
-        for (int w = 0; w < kSortWaves; ++w) all += hist[w][e];
-      } else {
-        for (int b = 0; b < blocks; ++b) {
+      int own = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) {  // the waves' counts become their starts
+        const int n = hist[w * (E + 1) + e];
+        hist[w * (E + 1) + e] = own;
+        own += n;
+      }
+      all = own;
+      if (counts != nullptr) {
+        all = 0;
+#pragma unroll 8
+        for (int b = 0; b < (int)gridDim.x; ++b) {
           const int n = counts[(int64_t)b * (E + 1) + e];
           all += n;
           before += b < (int)blockIdx.x ? n : 0;
@@ -106,7 +124,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_sort_place(const ID* ids, i
       }
     }
     total[e] = all;
-    mine[e] = before;
+    first[e] = before;
   }
   __syncthreads();
   if (wave == 0) {  // exclusive prefix sum over the keys, nine a lane
@@ -116,54 +134,31 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_sort_place(const ID* ids, i
       v[i] = total[9 * lane + i];
       sum += v[i];
     }
-    int upto = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      upto += lane >= d ? o : 0;
-    }
-    int at = upto - sum;
+    int at = wave_prefix_sum(sum) - sum;
 #pragma unroll
     for (int i = 0; i < 9; ++i) {
       const int e = 9 * lane + i;
       if (blockIdx.x == 0 && e <= E) offsets[e] = at;
-      mine[e] += at;
+      first[e] += at;
       at += v[i];
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += 64 * kSortWaves) {  // first row of every wave's pairs of key e
-    int at = mine[e];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      const int n = hist[w][e];
-      hist[w][e] = at;
-      at += n;
-    }
-  }
-  __syncthreads();
-  const int64_t w_lo = lo + wave * run, w_hi = w_lo + run < hi ? w_lo + run : hi;
-  for (int64_t p0 = w_lo; p0 < w_hi; p0 += 64) {
-    const int64_t p = p0 + lane;
-    const int key = sort_key(ids, p, w_hi, E);
-    const uint64_t m = same_key(key, bits, __ballot(p < w_hi));
-    const uint64_t lower = m & ((1ull << lane) - 1);
-    if (p >= w_hi) continue;
-    const int first = hist[wave][key];
-    const int row = first + __popcll(lower);
+  for (int r = 0; r < R; ++r) {
+    const int64_t p = run.p0 + 64 * r;
+    if (p >= P) continue;
+    const int key = run.key[r], row = first[key] + hist[wave * (E + 1) + key] + run.rank[r];
     const bool here = key < E;
     row_of_pair[p] = here ? row : ~row;
     pair_of_row[row] = here ? (int)p : ~(int)p;
     token_of_row[row] = here ? (int)p / k : -1;
-    // the last lane of a key moves its first row on for the next 64 pairs
-    // (every lane has read it: the wave runs in step, LDS in order)
-    if ((m >> lane) == 1) hist[wave][key] = row + 1;
   }
 }
 
 size_t sort_workspace_bytes(int64_t P, int E) {
   if (P <= kSortOne) return 0;
-  const int64_t per = sort_per(P);
+  const int64_t per = (int64_t)sort_rounds(P) * kSortWg;
   return (size_t)((P + per - 1) / per) * (size_t)(E + 1) * 4;
 }
 
@@ -172,20 +167,26 @@ static hipError_t sort_ids(const ID* ids, int64_t P, int k, int E, int32_t* offs
                            int32_t* pair_of_row, int32_t* token_of_row, int32_t* counts, hipStream_t st) {
   int bits = 1;
   while ((E >> bits) != 0) ++bits;
-  const dim3 wg(64 * kSortWaves);
+  const int rounds = sort_rounds(P);
+  const int64_t per = (int64_t)rounds * kSortWg;
+  const dim3 grid((unsigned)(P > 0 ? (P + per - 1) / per : 1)), wg(kSortWg);
+  auto place = [&](auto r, const int32_t* n) {
+    k_sort_place<ID, decltype(r)::value><<<grid, wg, 0, st>>>(ids, P, E, bits, k, n, offsets, row_of_pair, pair_of_row,
+                                                              token_of_row);
+  };
+  using std::integral_constant;
   if (P <= kSortOne) {
-    const int64_t per = (P + 64 * kSortWaves - 1) / (64 * kSortWaves) * (64 * kSortWaves);
-    k_sort_place<ID><<<dim3(1), wg, 0, st>>>(ids, P, per > 0 ? per : 64 * kSortWaves, E, bits, k, nullptr, 1, offsets,
-                                             row_of_pair, pair_of_row, token_of_row);
+    if (rounds == 1) place(integral_constant<int, 1>{}, nullptr);
+    else if (rounds == 2) place(integral_constant<int, 2>{}, nullptr);
+    else place(integral_constant<int, 4>{}, nullptr);
     return hipGetLastError();
   }
-  const int64_t per = sort_per(P);
-  const int blocks = (int)((P + per - 1) / per);
-  k_sort_count<ID><<<dim3(blocks), wg, 0, st>>>(ids, P, per, E, bits, counts);
+  if (rounds == 1) k_sort_count<ID, 1><<<grid, wg, 0, st>>>(ids, P, E, bits, counts);
+  else k_sort_count<ID, 4><<<grid, wg, 0, st>>>(ids, P, E, bits, counts);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  k_sort_place<ID><<<dim3(blocks), wg, 0, st>>>(ids, P, per, E, bits, k, counts, blocks, offsets, row_of_pair,
-                                                pair_of_row, token_of_row);
+  if (rounds == 1) place(integral_constant<int, 1>{}, counts);
+  else place(integral_constant<int, 4>{}, counts);
   return hipGetLastError();
 }
 
@@ -197,12 +198,30 @@ hipError_t launch_sort(const void* ids, bool ids64, int64_t P, int k, int E, int
 }
 
 // ------------------------------------------------------------------ rows out of tokens
-// A pair's row: [0, rows), its complement for a pair without an expert; an
-// entry of a table that names neither is left out (~rows).
-__device__ __forceinline__ int pair_row(const int32_t* row_of_pair, int64_t p, int rows) {
-  const int r = row_of_pair[p];
-  return (r < 0 ? ~r : r) < rows ? r : ~rows;
-}
+// Rows and weights of up to eight pairs of a token, in scalar registers: eight
+// lanes request them at once (one after another each would cost its latency).
+// A row is in [0, rows) or, for a pair without an expert, its complement; an
+// entry of a table that names neither, and entries past k, become ~rows.  To be
+// built where every lane of the wave is active: a lane that is not has no entry.
+struct TokenRows {
+  int row[8];
+  float w[8];
+  __device__ __forceinline__ TokenRows(const int32_t* row_of_pair, const void* weights, int w_dt, int64_t p, int n, int rows) {
+    const int l = threadIdx.x & 7;
+    int r = ~rows;
+    float wt = 1.0f;
+    if (l < n) {
+      r = row_of_pair[p + l];
+      r = (r < 0 ? ~r : r) < rows ? r : ~rows;
+      if (weights != nullptr) wt = load_scalar(weights, p + l, w_dt);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      row[j] = __builtin_amdgcn_readlane(r, j);
+      w[j] = readlane_f(wt, j);
+    }
+  }
+};
 
 // One workgroup a token: its row is read once and written to the rows of its k
 // pairs (zeros where a pair has no expert).  Bound by the writes.
@@ -212,11 +231,15 @@ __global__ __launch_bounds__(256) void k_gather_tokens(const char* x, int64_t x_
   const int64_t t = blockIdx.x;
   const int P = (int)gridDim.x * k;
   const V* src = (const V*)(x + t * x_stride);
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const V v = src[i];
-    for (int j = 0; j < k; ++j) {
-      const int r = pair_row(row_of_pair, t * k + j, P);
-      if (r != ~P) rows[(int64_t)(r < 0 ? ~r : r) * n + i] = r < 0 ? V{} : v;
+  for (int j0 = 0; j0 < k; j0 += 8) {
+    const TokenRows to(row_of_pair, nullptr, 0, t * k + j0, k - j0, P);
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const V v = src[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = to.row[j];
+        if (r != ~P) rows[(int64_t)(r < 0 ? ~r : r) * n + i] = r < 0 ? V{} : v;
+      }
     }
   }
 }
@@ -235,24 +258,32 @@ hipError_t launch_gather(const void* x, int64_t x_stride, int elem, int H, const
 }
 
 // ------------------------------------------------------------------ rows back into tokens
-// N neighbouring values of a row as fp32: 1, or 4 or 8 in one load of up to 16 bytes.
+// N neighbouring values of a row: 1, or 4 or 8 in one access of up to 16 bytes.
+// Loads are requested raw and converted at their use, through buffers of one
+// row each (zeros past its end, and everywhere for a row that is not there), so
+// that nothing stands between the requests of several rows.
 template <int DT, int N>
 struct RowVec {
   static constexpr int kBytes = N * (DT == FTM_DT_F32 ? 4 : 2);
-  using Raw = std::conditional_t<kBytes == 16, u32x4, u32x2>;
-  __device__ __forceinline__ static void load(const char* p, int64_t i, float (&f)[N]) {
+  using Raw = std::conditional_t<N == 1, uint32_t, std::conditional_t<kBytes == 16, u32x4, u32x2>>;
+  __device__ __forceinline__ static Rsrc row(const char* base, int64_t stride, int r, int n) {
+    return make_rsrc(base + (r >= 0 ? r : 0) * stride, r >= 0 ? (uint32_t)n * kBytes : 0u);
+  }
+  __device__ __forceinline__ static Raw request(Rsrc res, int i) {
+    const uint32_t off = (uint32_t)i * kBytes;
+    if constexpr (kBytes == 16) return __builtin_amdgcn_raw_buffer_load_b128(res, off, 0, 0);
+    else if constexpr (kBytes == 8) return __builtin_amdgcn_raw_buffer_load_b64(res, off, 0, 0);
+    else if constexpr (kBytes == 4) return bload4(res, off);
+    else return bload2(res, off);
+  }
+  __device__ __forceinline__ static void values(Raw v, float (&f)[N]) {
     if constexpr (N == 1) {
-      f[0] = load_scalar(p, i, DT);
+      f[0] = bits_to_f32(v, DT);
     } else {
-      const Raw v = ((const Raw*)p)[i];
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        if constexpr (DT == FTM_DT_F32) {
-          f[n] = __uint_as_float(v[n]);
-        } else {
-          const uint32_t h = (v[n >> 1] >> (16 * (n & 1))) & 0xffffu;
-          f[n] = DT == FTM_DT_F16 ? f16_to_f32((uint16_t)h) : __uint_as_float(h << 16);
-        }
+        if constexpr (DT == FTM_DT_F32) f[n] = __uint_as_float(v[n]);
+        else f[n] = bits_to_f32((v[n >> 1] >> (16 * (n & 1))) & 0xffffu, DT);
       }
     }
   }
@@ -279,21 +310,30 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const char* rows, int64_
                                                         const int32_t* row_of_pair, int k, int n, char* out,
                                                         int64_t out_stride) {
   const int64_t t = blockIdx.x;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  const int P = (int)gridDim.x * k;
+  // every lane takes part in each round of the loop (TokenRows asks lanes 0..7),
+  // those past the row without loads
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + threadIdx.x;
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0f;
-#pragma unroll 8
-    for (int j = 0; j < k; ++j) {
-      const int r = pair_row(row_of_pair, t * k + j, (int)gridDim.x * k);
-      if (r < 0) continue;
-      const float wt = w != nullptr ? load_scalar(w, t * k + j, w_dt) : 1.0f;
-      float v[N];
-      RowVec<DT, N>::load(rows + (int64_t)r * row_stride, i, v);
+    for (int j0 = 0; j0 < k; j0 += 8) {
+      const TokenRows from(row_of_pair, w, w_dt, t * k + j0, k - j0, P);
+      using V = RowVec<DT, N>;
+      typename V::Raw raw[8];
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = fmaf(wt, v[e], acc[e]);
+      for (int j = 0; j < 8; ++j) raw[j] = V::request(V::row(rows, row_stride, from.row[j], n), i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v[N];
+        V::values(raw[j], v);
+        const float wt = from.row[j] >= 0 ? from.w[j] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = fmaf(wt, v[e], acc[e]);
+      }
     }
-    RowVec<OT, N>::store(out + t * out_stride, i, acc);
+    if (i < n) RowVec<OT, N>::store(out + t * out_stride, i, acc);
   }
 }
 
@@ -311,32 +351,38 @@ __global__ __launch_bounds__(256) void k_combine_grad(const char* g, int64_t g_s
   const int P = (int)gridDim.x * k;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int j0 = 0; j0 < k; j0 += 8) {
-    float dot[8];
-    int r[8];
-    float wt[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      dot[j] = 0.0f;
-      const bool in = j0 + j < k;
-      r[j] = in ? pair_row(row_of_pair, t * k + j0 + j, P) : ~P;
-      wt[j] = in && grad_rows != nullptr && r[j] >= 0 ? load_scalar(w, t * k + j0 + j, w_dt) : 0.0f;
-    }
+    const TokenRows to(row_of_pair, grad_rows != nullptr ? w : nullptr, w_dt, t * k + j0, k - j0, P);
+    float dot[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int i = threadIdx.x; i < n; i += 256) {
-      float gv[N];
-      RowVec<OT, N>::load(g + t * g_stride, i, gv);
+      using V = RowVec<DT, N>;
+      using G = RowVec<OT, N>;
+      const typename G::Raw graw = G::request(G::row(g + t * g_stride, 0, 0, n), i);
+      typename V::Raw raw[8];
+      if (grad_w != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (r[j] == ~P) continue;
-        float v[N];
-        if (grad_w != nullptr && r[j] >= 0) {
-          RowVec<DT, N>::load(rows + (int64_t)r[j] * row_stride, i, v);
+        for (int j = 0; j < 8; ++j) raw[j] = V::request(V::row(rows, row_stride, to.row[j], n), i);
+      }
+      float gv[N];
+      G::values(graw, gv);
+      if (grad_rows != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = to.row[j];
+          if (r == ~P) continue;
+          float v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = r >= 0 ? to.w[j] * gv[e] : 0.0f;
+          V::store(grad_rows + (int64_t)(r < 0 ? ~r : r) * grad_stride, i, v);
+        }
+      }
+      if (grad_w != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (to.row[j] < 0) continue;  // (g may hold infinities: 0 in their place is not the same)
+          float v[N];
+          V::values(raw[j], v);
 #pragma unroll
           for (int e = 0; e < N; ++e) dot[j] = fmaf(gv[e], v[e], dot[j]);
-        }
-        if (grad_rows != nullptr) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) v[e] = r[j] >= 0 ? wt[j] * gv[e] : 0.0f;
-          RowVec<DT, N>::store(grad_rows + (int64_t)(r[j] < 0 ? ~r[j] : r[j]) * grad_stride, i, v);
         }
       }
     }

@@ -204,19 +204,6 @@ struct RowTile {
   int cnt, e;
 };
 
-// Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
-// lanes (DPP row_shr, zeros shifted in), then the rows before.
-__device__ __forceinline__ int wave_prefix_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31);
-  const int c = __builtin_amdgcn_readlane(v, 47);
-  const int row = (threadIdx.x & 63) >> 4;
-  return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
-}
-
 // The experts' rows cut into tiles of height BM, in order of the experts, found by
 // every wave for itself: eight experts a lane, one prefix sum over the wave.
 // The offsets are clamped to [0, rows], so a bad table reads and writes no
@@ -349,18 +336,18 @@ constexpr int kRow = 128;
 __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 typedef __attribute__((address_space(3))) void* LPtr;
 
-// The results of a row tile: N neighbouring channels from n0 on of one row at a
-// time, through a buffer that drops rows past the tile; channels past the last
-// take an offset past its end, so there is no branch around a store.
+// The results of a row tile: N = 4 or 2 neighbouring channels from n0 on of one row
+// at a time, through a buffer that drops rows past the tile; channels past the
+// last take an offset past its end, so there is no branch around a store.
 template <int N>
 struct RowOut {
   Rsrc res;
   int NO, n0, dt;
-  bool vec;  // 16 bytes (four 16-bit values: 8) a store
+  bool vec;  // all N in one store
   __device__ __forceinline__ RowOut(const ftm_w8a8& c, const RowTile& t, int NO_, int n0_) : NO(NO_), n0(n0_), dt(c.out_dtype) {
     const int esz = dt == FTM_DT_F32 ? 4 : 2;
     res = make_rsrc((char*)c.out + t.row0 * NO * esz, (uint32_t)(t.cnt * NO) * (uint32_t)esz);
-    vec = NO % (dt == FTM_DT_F32 || N == 4 ? 4 : 8) == 0 && ((uintptr_t)c.out & 15u) == 0;
+    vec = NO % N == 0 && ((uintptr_t)c.out & 15u) == 0;
   }
   __device__ __forceinline__ uint32_t half2(float a, float b) const {
     return dt == FTM_DT_BF16 ? pack_bf16x2(a, b) : (uint32_t)f32_to_f16(a) | ((uint32_t)f32_to_f16(b) << 16);
@@ -368,12 +355,14 @@ struct RowOut {
   __device__ __forceinline__ void store(int row, const float (&y)[N]) const {
     const uint32_t at = (uint32_t)(row * NO + n0);
     if (dt == FTM_DT_F32) {
+      const uint32_t off = n0 < NO ? 4u * at : kOOB;
       if (vec) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
+        if constexpr (N == 4)
           __builtin_amdgcn_raw_buffer_store_b128(
-              (u32x4){__float_as_uint(y[i]), __float_as_uint(y[i + 1]), __float_as_uint(y[i + 2]), __float_as_uint(y[i + 3])},
-              res, n0 + i < NO ? 4u * (at + i) : kOOB, 0, 0);
+              (u32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])}, res, off, 0,
+              0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(y[0]), __float_as_uint(y[1])}, res, off, 0, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -381,23 +370,16 @@ struct RowOut {
       }
       return;
     }
-    uint32_t h[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) h[i] = half2(y[2 * i], y[2 * i + 1]);
+    const uint32_t off = n0 < NO ? 2u * at : kOOB;
     if (vec) {
-      if constexpr (N == 4) {
-        __builtin_amdgcn_raw_buffer_store_b64((u32x2){h[0], h[1]}, res, n0 < NO ? 2u * at : kOOB, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 8)
-          __builtin_amdgcn_raw_buffer_store_b128((u32x4){h[i / 2], h[i / 2 + 1], h[i / 2 + 2], h[i / 2 + 3]}, res,
-                                                 n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
-      }
+      if constexpr (N == 4)
+        __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(h[i / 2] >> (16 * (i & 1))), res,
-                                              n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)half2(y[i], 0.0f), res, n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
     }
   }
 };
@@ -654,21 +636,13 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
     // reach them (the launch sees to it).
     Rsrc xres, wres;
     uint32_t xoff[NX], woff[NB];
-    int ix[NX], er[MI];  // rows of x: of the copies, of the results' tokens
+    int ix[NX];  // rows of x that the copies read
     auto copy_rows = [&](const Tile& t) __attribute__((always_inline)) {
       const int lane = opaque_lane();
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         const int r = 8 * (wave * NX + i) + (lane >> 3), in = r < t.rt.cnt ? r : 0;
         ix[i] = indexed ? c.row_index[t.rt.row0 + in] : in;
-      }
-    };
-    auto result_rows = [&](const Tile& t) __attribute__((always_inline)) {
-      const int m = opaque_lane() & 15;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int r = 16 * (wm * MI + i) + m, in = r < t.rt.cnt ? r : 0;
-        er[i] = indexed ? c.row_index[t.rt.row0 + in] : (int)t.rt.row0 + in;
       }
     };
     auto aim = [&](const Tile& t) __attribute__((always_inline)) {
@@ -685,13 +659,13 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
       wres = make_rsrc((const char*)c.w + (int64_t)t.rt.e * c.w_stride + (int64_t)t.n * K,
                        (uint32_t)((ACT ? NO : 0) + cols) * (uint32_t)K);
       // Weight row of LDS row r: wave r / 64 of the columns; its operand block j = r
-      // % 64 / 16, operand row o = r % 16 is channel 16 (o / 4) + 4 j + o % 4, so that
-      // a lane's results are 16 neighbours (with an activation: 8 (o / 4) + 4 (j % 2)
-      // + o % 4 of gate, j < 2, and of up); rows past the last copy it
+      // % 64 / 16, operand row o = r % 16 is channel 4 o + j, so that a lane's
+      // results are four neighbours, its neighbour's the next (with an activation: 2 o
+      // + j % 2 of gate, j < 2, and of up); rows past the last copy it
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int r = 8 * (wave * NB + i) + (lane >> 3), j = (r >> 4) & 3, o = r & 15;
-        int n = (r >> 6) * (kCols / 4) + (ACT ? 8 * (o >> 2) + 4 * (j & 1) : 16 * (o >> 2) + 4 * j) + (o & 3);
+        int n = (r >> 6) * (kCols / 4) + (ACT ? 2 * o + (j & 1) : 4 * o + j);
         n = n < cols ? n : cols - 1;
         woff[i] = (uint32_t)(n + (ACT && j >= 2 ? NO : 0)) * (uint32_t)K + 16u * (uint32_t)((lane & 7) ^ swz(r));
       }
@@ -747,7 +721,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
           if (q == 0 && i >= MI - 4) b[1][i - (MI - 4)] = wfrag(slot, i - (MI - 4), 1);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(b[q][j], x[at % (kAhead + 1)], acc[i][j]);
+          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(x[at % (kAhead + 1)], b[q][j], acc[i][j]);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -766,7 +740,6 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
     for (;;) {
       const int after = item + (int)(gridDim.x >> 3);
       const Tile next = after < end ? tile_at(after) : cur;  // (the last tile's copies go on over it: nothing reads them)
-      result_rows(cur);
       copy_rows(next);
 #pragma unroll
       for (int i = 0; i < MI; ++i)
@@ -777,31 +750,36 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
         step(kb, kb + S < nrun ? kb + S : kb + S - nrun, slot);
         slot = slot == S - 1 ? 0 : slot + 1;
       }
-      // a lane's channels: 16 (with an activation 8, and their up rows) from n0 on
-      constexpr int CN = ACT ? 8 : 16;
-      const int el = opaque_lane(), em = el & 15;
-      const int n0 = cur.n + wn * (kCols / 4) + CN * (el >> 4);
-      uint32_t tb[16];
-      float xs[MI];
-      {
-        const int64_t cb = (int64_t)cur.rt.e * c.N;
-        load_run<CN>(c.w_scale, cb, n0, NO - 1, c.w_scale_dtype, tb);
-        if constexpr (ACT) load_run<CN>(c.w_scale, cb + NO, n0, NO - 1, c.w_scale_dtype, tb + 8);
+      // A lane has tokens 16 i + 4 g + r (r 0..3) and CN neighbouring channels from
+      // n0 on (with an activation two, and their up rows)
+      constexpr int CN = ACT ? 2 : 4;
+      const int el = opaque_lane(), eg = el >> 4;
+      const int n0 = cur.n + wn * (kCols / 4) + CN * (el & 15);
+      const int t0 = 16 * wm * MI + 4 * eg;
+      int er[MI][4];
+      float xs[MI][4];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) xs[i] = c.x_scale[er[i] >= 0 && er[i] < c.x_rows ? er[i] : 0];
-      }
-      uint32_t bb[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = t0 + 16 * i + r, in = t < cur.rt.cnt ? t : 0;
+          er[i][r] = indexed ? c.row_index[cur.rt.row0 + in] : (int)cur.rt.row0 + in;
+        }
+      uint32_t tb[4], bb[4] = {0, 0, 0, 0};
+      const int64_t at = (int64_t)cur.rt.e * c.N;
+      load_run<CN>(c.w_scale, at, n0, NO - 1, c.w_scale_dtype, tb);
+      if constexpr (ACT) load_run<CN>(c.w_scale, at + NO, n0, NO - 1, c.w_scale_dtype, tb + 2);
       if (c.bias != nullptr) {
-        const int64_t cb = (int64_t)cur.rt.e * c.N;
-        load_run<CN>(c.bias, cb, n0, NO - 1, c.bias_dtype, bb);
-        if constexpr (ACT) load_run<CN>(c.bias, cb + NO, n0, NO - 1, c.bias_dtype, bb + 8);
+        load_run<CN>(c.bias, at, n0, NO - 1, c.bias_dtype, bb);
+        if constexpr (ACT) load_run<CN>(c.bias, at + NO, n0, NO - 1, c.bias_dtype, bb + 2);
       }
-      float cs[16], cb[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const Channel ch = channel(c, ChannelBits{tb[i], bb[i]});
-        cs[i] = ch.t, cb[i] = ch.b;
-      }
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) xs[i][r] = c.x_scale[er[i][r] >= 0 && er[i][r] < c.x_rows ? er[i][r] : 0];
+      Channel ch[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) ch[n] = channel(c, ChannelBits{tb[n], bb[n]});
       const RowOut<CN> out(c, cur.rt, NO, n0);
       with_act(ACT ? c.act : -1, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll
@@ -809,17 +787,20 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
           // one row block after the other, so that their results do not all sit in
           // registers at once
           asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]) : : "memory");
-          const bool live = er[i] >= 0 && er[i] < c.x_rows;
-          float y[CN];
 #pragma unroll
-          for (int n = 0; n < CN; ++n) {
-            y[n] = scaled(acc[i][n >> 2][n & 3], xs[i], {cs[n], cb[n]});
-            if constexpr (ACT)
-              y[n] = act_fn(decltype(a)::value, y[n], scaled(acc[i][2 + (n >> 2)][n & 3], xs[i], {cs[8 + n], cb[8 + n]}),
-                            c.act_alpha, c.act_limit);
-            y[n] = live ? y[n] : 0.0f;
+          for (int r = 0; r < 4; ++r) {
+            const bool live = !GROUPED || (er[i][r] >= 0 && er[i][r] < c.x_rows);
+            float y[CN];
+#pragma unroll
+            for (int n = 0; n < CN; ++n) {
+              y[n] = scaled(acc[i][n][r], xs[i][r], ch[n]);
+              if constexpr (ACT)
+                y[n] = act_fn(decltype(a)::value, y[n], scaled(acc[i][2 + n][r], xs[i][r], ch[2 + n]), c.act_alpha,
+                              c.act_limit);
+              y[n] = live ? y[n] : 0.0f;
+            }
+            out.store(t0 + 16 * i + r, y);
           }
-          out.store(16 * (wm * MI + i) + em, y);
         }
       });
       if (after >= end) break;
