@@ -496,14 +496,14 @@ int ftm_w8a8_linear(const ftm_w8a8* call, void* stream) {
 }
 
 int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w8a8* call, void* stream) {
-  int rc = check_w8a8(call);
+  const int rc = check_w8a8(call);
   if (rc != FTM_OK) return rc;
-  if (call->x_stride != call->K) return FTM_ERR_DIM;
+  if (!dt_ok(x_dtype)) return FTM_ERR_FORMAT;
+  if (call->x_stride != call->K || x_stride < 0) return FTM_ERR_DIM;
   if (call->rows == 0) return FTM_OK;
-  rc = ftm_quant_int8(x, x_dtype, call->x_rows, call->K, x_stride, const_cast<int8_t*>(call->x), call->K,
-                      const_cast<float*>(call->x_scale), stream);
-  if (rc != FTM_OK) return rc;
-  return hip_rc(launch_w8a8(*call, (hipStream_t)stream));
+  if (x == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)x | (uint64_t)x_stride) % dt_bytes(x_dtype) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_w8a8_dynamic(*call, x, x_dtype, x_stride, (hipStream_t)stream));
 }
 
 size_t ftm_w8a8_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter) {
@@ -519,6 +519,7 @@ int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_by
       (int64_t)T * k >= INT32_MAX || c.x_stride < 0)
     return FTM_ERR_DIM;
   if (!dt_ok(c.dtype) || !dt_ok(c.topk_w_dtype) || c.act < 0) return FTM_ERR_FORMAT;
+  if (c.ids_dtype != FTM_ID_I32 && c.ids_dtype != FTM_ID_I64) return FTM_ERR_FORMAT;
   if (T == 0) return FTM_OK;
   if (c.x == nullptr || c.topk_ids == nullptr || c.topk_w == nullptr || c.out == nullptr) return FTM_ERR_NULL;
   if (workspace == nullptr) return FTM_ERR_WORKSPACE;
@@ -546,10 +547,8 @@ int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_by
   if (((uintptr_t)c.x | (uint64_t)c.x_stride | (uintptr_t)c.out) % dt_bytes(c.dtype) != 0) return FTM_ERR_ALIGN;
   rc = ftm_sort_tokens(c.topk_ids, c.ids_dtype, T, k, E, offsets, row_of_pair, pair_of_row, token_of_row, ws + L.sort,
                        L.total - L.sort, stream);
-  if (rc == FTM_OK) rc = ftm_quant_int8(c.x, c.dtype, T, H, c.x_stride, q, H, s, stream);
-  if (rc == FTM_OK) rc = ftm_w8a8_linear(&a, stream);
-  if (rc == FTM_OK) rc = ftm_quant_int8(h, FTM_DT_F32, P, I, (int64_t)I * 4, q, I, s, stream);
-  if (rc == FTM_OK) rc = ftm_w8a8_linear(&b, stream);
+  if (rc == FTM_OK) rc = ftm_w8a8_linear_dynamic(c.x, c.dtype, c.x_stride, &a, stream);
+  if (rc == FTM_OK) rc = ftm_w8a8_linear_dynamic(h, FTM_DT_F32, (int64_t)I * 4, &b, stream);
   if (rc == FTM_OK)
     rc = ftm_combine_tokens(y, FTM_DT_F32, (int64_t)H * 4, c.topk_w, c.topk_w_dtype, row_of_pair, T, k, H, c.out, c.dtype,
                             stream);

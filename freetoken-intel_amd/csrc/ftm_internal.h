@@ -214,6 +214,8 @@ hipError_t launch_dequant(const ftm_proj& P, int slot, void* out, int out_dt, in
 hipError_t launch_quant_int8(const void* x, int dt, int64_t rows, int K, int64_t x_stride, int8_t* q,
                              int64_t q_stride, float* scale, hipStream_t st);
 hipError_t launch_w8a8(const ftm_w8a8& call, hipStream_t st);
+// ... of x still wide (call.x and call.x_scale: scratch for its codes)
+hipError_t launch_w8a8_dynamic(const ftm_w8a8& call, const void* x, int x_dt, int64_t x_stride, hipStream_t st);
 // ftm_sort.hip
 size_t sort_workspace_bytes(int64_t pairs, int E);
 hipError_t launch_sort(const void* ids, bool ids64, int64_t pairs, int k, int E, int32_t* offsets,

@@ -26,6 +26,14 @@ __device__ __forceinline__ i32x4 mfma_i8(u32x4 a, u32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
+// A weight operand for the product: packed bytes are offset by 128, and past K (keep
+// 0, else all ones) it has to be zero.  Bit operations: a choice would be a branch
+// between the MFMA and what it reads.
+template <bool PACKED>
+__device__ __forceinline__ u32x4 weight_operand(u32x4 v, uint32_t keep) {
+  return PACKED ? (v ^ 0x80808080u) & keep : v & keep;
+}
+
 // ------------------------------------------------------------------ quantiser
 // Largest |x| of a wave as fp32 bits (unsigned order: NaN above infinity above
 // every finite value, so a row with either is recognised).
@@ -395,6 +403,101 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 }
 
 // ------------------------------------------------------------------ K split over the waves
+// One 16 x 16 block of results that a wave finishes from the waves' sums: a lane
+// has weight rows 4 g .. 4 g + 3 of token m (with an activation rows 0..7 of a block
+// are gate channels, 8..15 their up rows, and only lanes of the first eight have
+// results).
+struct SplitBlock {
+  uint32_t t[8], b[8];  // scales and biases of its four channels, and of their up rows
+  float xscale;         // the token's
+  bool live;            // it names a row of x
+
+  __device__ __forceinline__ void request(const ftm_w8a8& c, const RowTile& rt, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = b[i] = 0;
+    if (rt.e < 0) return;
+    const int last = out_cols(c) - 1;
+    const int64_t at = (int64_t)rt.e * c.N;
+    load_run<4>(c.w_scale, at, n, last, c.w_scale_dtype, t);
+    if (c.act >= 0) load_run<4>(c.w_scale, at + last + 1, n, last, c.w_scale_dtype, t + 4);
+    if (c.bias == nullptr) return;
+    load_run<4>(c.bias, at, n, last, c.bias_dtype, b);
+    if (c.act >= 0) load_run<4>(c.bias, at + last + 1, n, last, c.bias_dtype, b + 4);
+  }
+};
+
+template <int NT>
+__device__ __forceinline__ int split_channel(const ftm_w8a8& c, int n0, int block, int g) {
+  return n0 + (c.act >= 0 ? 8 * (block % NT) + 4 * (g & 1) : 16 * (block % NT) + 4 * g);
+}
+
+// The waves' sums of the tile's MT x NT blocks, through LDS (which they may
+// overwrite), and the results.
+template <int MT, int NT, int NW, int PARTS>
+__device__ __forceinline__ void split_finish(const ftm_w8a8& c, const RowTile& rt, char* lds, int n0,
+                                             const i32x4 (&acc)[MT][NT], const SplitBlock (&blocks)[PARTS]) {
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  i32x4* red = (i32x4*)lds;  // [NW][MT * NT][64]
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  if (c.act >= 0 && g >= 2) return;
+  with_act(c.act, [&](auto a) {
+    constexpr int A = decltype(a)::value;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const int f = p * NW + wave;
+      if (MT * NT % NW != 0 && f >= MT * NT) continue;
+      i32x4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        u += red[(w * MT * NT + f) * 64 + lane];
+        if constexpr (A >= 0) v += red[(w * MT * NT + f) * 64 + lane + 32];
+      }
+      const SplitBlock& k = blocks[p];
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = scaled(u[r], k.xscale, channel(c, {k.t[r], k.b[r]}));
+        if constexpr (A >= 0)
+          y[r] = act_fn(A, y[r], scaled(v[r], k.xscale, channel(c, {k.t[4 + r], k.b[4 + r]})), c.act_alpha, c.act_limit);
+        y[r] = k.live ? y[r] : 0.0f;
+      }
+      RowOut<4>(c, rt, out_cols(c), split_channel<NT>(c, n0, f, g)).store(16 * (f / NT) + m, y);
+    }
+  });
+}
+
+// The weight rows of a split tile: copies of 8 rows, a 16-byte piece a lane, from
+// the tile's first row (and the up rows N / 2 on); rows past the last copy it.
+template <int NT>
+struct SplitWeights {
+  Rsrc res;
+  uint32_t off[2 * NT];
+  __device__ __forceinline__ SplitWeights(const ftm_w8a8& c, const RowTile& rt, int n0, int ncol) {
+    const bool act = c.act >= 0;
+    const int lane = threadIdx.x & 63, NO = out_cols(c);
+    res = make_rsrc((const char*)c.w + (int64_t)rt.e * c.w_stride + (int64_t)n0 * c.K,
+                    (uint32_t)((act ? NO : 0) + ncol) * (uint32_t)c.K);
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      int n = act ? 8 * (i >> 1) + (r & 7) : r;
+      n = n < ncol ? n : ncol - 1;
+      off[i] = (uint32_t)(n + (act && (i & 1) ? NO : 0)) * (uint32_t)c.K + 16u * (uint32_t)((lane & 7) ^ swz(r));
+    }
+  }
+  __device__ __forceinline__ void issue(char* at, uint32_t k0) const {
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LPtr)(at + 1024 * i), 16, (int)(off[i] + k0), 0, 0, 0);
+  }
+};
+
 // A workgroup's tile of 16 MT tokens x 16 NT weight rows (with an activation 8
 // gate rows and their 8 up rows a block); each of the NW waves takes a run of
 // K over the whole tile through an LDS ring of its own (S stages of 128 K), and
@@ -406,15 +509,15 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 template <int MT, int NT, int NW, int S, bool PACKED>
 __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, int ntiles) {
   constexpr int BM = 16 * MT, kStage = (MT + NT) * 16 * kRow, NC = 2 * (MT + NT);
-  extern __shared__ char lds[];  // [NW][S][kStage], then the sums [NW][MT * NT * 4][64]
+  constexpr int kParts = (MT * NT + NW - 1) / NW;
+  extern __shared__ char lds[];  // [NW][S][kStage], then the sums
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const RowTile rt = row_tile<BM>(c, item / ntiles);
   if (rt.cnt <= 0) return;
-  const bool act = c.act >= 0;
   const int NO = out_cols(c), K = c.K;
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int cols = act ? 8 * NT : 16 * NT;  // output channels of the tile
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT;  // output channels of the tile
   const int n0 = (item % ntiles) * cols;
   const int ncol = NO - n0 < cols ? NO - n0 : cols;
   i32x4 acc[MT][NT];
@@ -422,49 +525,28 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
-  // the scales of the blocks this wave finishes (below): requested behind the
-  // first copies and ahead of the K loop
-  constexpr int kParts = (MT * NT + NW - 1) / NW;
-  float xscale[kParts];
-  uint32_t tb[kParts][8] = {}, bb[kParts][8] = {};  // scales and biases: four channels, their up rows
-  bool live[kParts];
+  SplitBlock blocks[kParts];
   auto request_scales = [&] {
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
-      const int f = p * NW + wave, r = 16 * (f / NT) + m, j = f % NT;
+      const int f = p * NW + wave, r = 16 * (f / NT) + m;
       const int64_t src = f < MT * NT && r < rt.cnt && rt.e >= 0 ? source_row(c, rt.row0 + r) : -1;
-      live[p] = src >= 0;
-      xscale[p] = src >= 0 ? c.x_scale[src] : 0.0f;
-      if (rt.e < 0) continue;
-      const int n = n0 + (act ? 8 * j + 4 * (g & 1) : 16 * j + 4 * g);
-      const int64_t at = (int64_t)rt.e * c.N;
-      load_run<4>(c.w_scale, at, n, NO - 1, c.w_scale_dtype, tb[p]);
-      if (act) load_run<4>(c.w_scale, at + NO, n, NO - 1, c.w_scale_dtype, tb[p] + 4);
-      if (c.bias == nullptr) continue;
-      load_run<4>(c.bias, at, n, NO - 1, c.bias_dtype, bb[p]);
-      if (act) load_run<4>(c.bias, at + NO, n, NO - 1, c.bias_dtype, bb[p] + 4);
+      blocks[p].live = src >= 0;
+      blocks[p].xscale = src >= 0 ? c.x_scale[src] : 0.0f;
+      blocks[p].request(c, rt, split_channel<NT>(c, n0, f, g));
     }
   };
   const int nsteps = (K + 127) / 128, per = (nsteps + NW - 1) / NW;
   const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
   if (rt.e >= 0 && lo < hi) {
-    // copies of 8 rows, a 16-byte piece a lane; rows past the tile copy one
-    // inside it, pieces past K what follows the row (their weights are made
-    // zero).  Tokens: offsets from the tile's first row, or, read through an
-    // index, from x's; weights from the tile's first row (and the up rows N/2 on)
+    // rows past the tile copy one inside it, pieces past K what follows the row
+    // (their weights are made zero); offsets from the tile's first token, or, read
+    // through an index, from x's
     const bool indexed = c.row_index != nullptr;
     const char* xbase = (const char*)c.x + (indexed ? 0 : rt.row0 * c.x_stride);
     const Rsrc xres = make_rsrc(xbase, (uint32_t)((indexed ? c.x_rows - 1 : (int64_t)rt.cnt - 1) * c.x_stride + K));
-    const char* wbase = (const char*)c.w + (int64_t)rt.e * c.w_stride + (int64_t)n0 * K;
-    const Rsrc wres = make_rsrc(wbase, (uint32_t)((act ? NO : 0) + ncol) * (uint32_t)K);
-    uint32_t xoff[2 * MT], woff[2 * NT];
-#pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
-      const int r = 8 * i + (lane >> 3);
-      int n = act ? 8 * (i >> 1) + (r & 7) : r;
-      n = n < ncol ? n : ncol - 1;
-      woff[i] = (uint32_t)(n + (act && (i & 1) ? NO : 0)) * (uint32_t)K + 16u * (uint32_t)((lane & 7) ^ swz(r));
-    }
+    const SplitWeights<NT> weights(c, rt, n0, ncol);
+    uint32_t xoff[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
       const int r = 8 * i + (lane >> 3);
@@ -479,33 +561,28 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, 
     auto issue = [&](int step, int slot) {
       const uint32_t k0 = (uint32_t)(step < hi ? step : hi - 1) * 128u;
       char* st = ring + slot * kStage;
-#pragma unroll
-      for (int i = 0; i < 2 * NT; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + 1024 * (2 * MT + i)), 16, (int)(woff[i] + k0), 0, 0, 0);
+      weights.issue(st + 2048 * MT, k0);
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * i), 16, (int)(xoff[i] + k0), 0, 0, 0);
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) issue(lo + i, i);
-    request_scales();
+    request_scales();  // behind the first copies and ahead of the K loop
     int slot = 0;
     for (int step = lo; step < hi; ++step) {
       issue(step + S - 1, slot == 0 ? S - 1 : slot - 1);
       wait_vm<(S - 1) * NC>();  // this step's copies have landed
+      asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       const char* st = ring + slot * kStage;
       auto piece = [&](int r, int q) { return *(const u32x4*)(st + r * kRow + 16 * ((4 * q + g) ^ swz(r))); };
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const bool in = step * 128 + 64 * q + 16 * g < K;
+        const uint32_t keep = step * 128 + 64 * q + 16 * g < K ? ~0u : 0u;
         u32x4 w[NT], x[MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          // past K the weights have to be zero; packed bytes are offset by 128
-          const u32x4 v = piece(16 * (MT + j) + m, q);
-          w[j] = in ? (PACKED ? v ^ 0x80808080u : v) : (u32x4){0, 0, 0, 0};
-        }
+        for (int j = 0; j < NT; ++j) w[j] = weight_operand<PACKED>(piece(16 * (MT + j) + m, q), keep);
 #pragma unroll
         for (int i = 0; i < MT; ++i) x[i] = piece(16 * i + m, q);
 #pragma unroll
@@ -520,40 +597,106 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, 
   } else {
     request_scales();
   }
-  i32x4* red = (i32x4*)lds;  // [NW][MT * NT][64]
-  __syncthreads();
+  split_finish<MT, NT, NW>(c, rt, lds, n0, acc, blocks);
+}
+
+// The same for at most 16 tokens a tile whose values are still wide (XDT; x_stride
+// bytes between rows): every workgroup quantises its tokens itself, each wave the
+// K that it multiplies, into LDS, while its first weights are under way.  The
+// codes and scales are the quantiser's; the launch that would write them is
+// saved (the figures are at launch_w8a8_dynamic).
+template <int XDT, int NT, int S, bool PACKED>
+__global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, int64_t x_stride, int lds_rows, int ntiles) {
+  using V = QuantVec<XDT>;
+  constexpr int kStage = NT * 16 * kRow, NC = 2 * NT;
+  extern __shared__ char lds[];  // [4][S][kStage], then [step][lds_rows][kRow] codes
+  __shared__ uint32_t maxima[4][16];
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const RowTile rt = row_tile<16>(c, item / ntiles);
+  if (rt.cnt <= 0) return;
+  const int NO = out_cols(c), K = c.K;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT;
+  const int n0 = (item % ntiles) * cols;
+  const int ncol = NO - n0 < cols ? NO - n0 : cols;
+  i32x4 acc[1][NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int j = 0; j < NT; ++j) acc[0][j] = (i32x4){0, 0, 0, 0};
+  SplitBlock blocks[1];
+  const int nsteps = (K + 127) / 128, per = (nsteps + 3) / 4;
+  const int lo = wave * per < nsteps ? wave * per : nsteps, hi = lo + per < nsteps ? lo + per : nsteps;
+  const int64_t src = m < rt.cnt && rt.e >= 0 ? source_row(c, rt.row0 + m) : -1;  // of row m
+  blocks[0].live = src >= 0;
+  blocks[0].xscale = 0.0f;
+  if (rt.e >= 0) {
+    const SplitWeights<NT> weights(c, rt, n0, ncol);
+    char* ring = lds + wave * (S * kStage);
+    char* codes = lds + 4 * S * kStage;
+    auto issue = [&](int step, int slot) {
+      weights.issue(ring + slot * kStage, (uint32_t)(step < hi ? step : nsteps - 1) * 128u);
+    };
 #pragma unroll
-    for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  // The waves share the blocks; a lane has four neighbouring weight rows of one
-  // token (with an activation the lanes of 8..15 pass: those are the up rows of
-  // the others)
-  if (act && g >= 2) return;
-  with_act(c.act, [&](auto a) {
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      constexpr int A = decltype(a)::value;
-      const int f = p * NW + wave;
-      if (MT * NT % NW != 0 && f >= MT * NT) continue;
-      i32x4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        u += red[(w * MT * NT + f) * 64 + lane];
-        if constexpr (A >= 0) v += red[(w * MT * NT + f) * 64 + lane + 32];
+    for (int i = 0; i < S - 1; ++i) issue(lo + i, i);
+    blocks[0].request(c, rt, split_channel<NT>(c, n0, wave, g));
+    // the largest of each row: this wave's K, then all waves'
+    const int k_hi = hi * 128 < K ? hi * 128 : K;
+    auto row_at = [&](int r) {
+      const int s = __builtin_amdgcn_readlane((int)src, r);
+      return x + (int64_t)(s < 0 ? 0 : s) * x_stride;
+    };
+    uint32_t mine = 0;
+    for (int r = 0; r < rt.cnt; ++r) {
+      const char* p = row_at(r);
+      uint32_t v = 0;
+      for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN) {
+        const uint32_t b = V::max_bits(*(const u32x4*)(p + (int64_t)k * (16 / V::kN)));
+        v = b > v ? b : v;
       }
-      float y[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        y[r] = scaled(u[r], xscale[p], channel(c, {tb[p][r], bb[p][r]}));
-        if constexpr (A >= 0)
-          y[r] = act_fn(A, y[r], scaled(v[r], xscale[p], channel(c, {tb[p][4 + r], bb[p][4 + r]})), c.act_alpha, c.act_limit);
-        y[r] = live[p] ? y[r] : 0.0f;
-      }
-      RowOut<4>(c, rt, NO, n0 + (act ? 8 : 16) * (f % NT) + 4 * g).store(16 * (f / NT) + m, y);
+      v = wave_max_bits(v);
+      mine = m == r ? v : mine;
     }
-  });
+    if (lane < 16) maxima[wave][lane] = mine;
+    __syncthreads();
+    uint32_t top = maxima[0][m];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = maxima[w][m] > top ? maxima[w][m] : top;
+    const QuantScale own = quant_scale(top);  // of row m
+    blocks[0].xscale = own.s;
+    for (int r = 0; r < rt.cnt; ++r) {
+      const char* p = row_at(r);
+      const QuantScale qs = {readlane_f(own.s, r), readlane_f(own.inv, r)};
+      for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN)
+        V::store((int8_t*)codes + ((k >> 7) * lds_rows + r) * kRow + 16 * (((k >> 4) & 7) ^ swz(r)) + (k & 15),
+                 *(const u32x4*)(p + (int64_t)k * (16 / V::kN)), qs);
+    }
+    __builtin_amdgcn_wave_barrier();
+    const int xr = m < rt.cnt ? m : 0;
+    int slot = 0;
+    for (int step = lo; step < hi; ++step) {
+      issue(step + S - 1, slot == 0 ? S - 1 : slot - 1);
+      wait_vm<(S - 1) * NC>();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = ring + slot * kStage;
+      const char* xt = codes + step * lds_rows * kRow;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t keep = step * 128 + 64 * q + 16 * g < K ? ~0u : 0u;
+        const u32x4 xv = *(const u32x4*)(xt + xr * kRow + 16 * ((4 * q + g) ^ swz(xr)));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int r = 16 * j + m;
+          const u32x4 v = *(const u32x4*)(st + r * kRow + 16 * ((4 * q + g) ^ swz(r)));
+          acc[0][j] = mfma_i8(weight_operand<PACKED>(v, keep), xv, acc[0][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      slot = slot == S - 1 ? 0 : slot + 1;
+    }
+    wait_vm<0>();
+  }
+  split_finish<1, NT, 4>(c, rt, lds, n0, acc, blocks);
 }
 
 // ------------------------------------------------------------------ LDS tiles
@@ -698,13 +841,9 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if constexpr (PACKED || TAIL) {
-          // packed bytes are offset by 128; past K the weights have to be zero
-          const bool in = !TAIL || kb * 128 + 64 * q + 16 * g < K;
+          const uint32_t keep = !TAIL || kb * 128 + 64 * q + 16 * g < K ? ~0u : 0u;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const u32x4 v = PACKED ? b[q][j] ^ 0x80808080u : b[q][j];
-            b[q][j] = in ? v : (u32x4){0, 0, 0, 0};
-          }
+          for (int j = 0; j < 4; ++j) b[q][j] = weight_operand<PACKED>(b[q][j], keep);
         }
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -885,6 +1024,28 @@ hipError_t split(const ftm_w8a8& c, hipStream_t st) {
 }
 
 constexpr int kCUs = 256;
+constexpr int kWideCodes = 64 * 1024;  // bytes of codes in LDS at most
+
+// k_w8a8_wide with one block of 16 weight rows (with an activation, grouped: two) a
+// tile.
+template <int XDT, int NT, bool PACKED>
+hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, int lds_rows, hipStream_t st) {
+  constexpr int S = NT == 1 ? 4 : 2, ring = 4 * S * NT * 16 * kRow;
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = ring + lds_rows * ((c.K + 127) / 128) * kRow;
+  const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + cols - 1) / cols;
+  if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w8a8_wide<XDT, NT, S, PACKED>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, ring + kWideCodes);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (const char*)x, x_stride, lds_rows, (int)nt);
+  return hipGetLastError();
+}
+template <int XDT>
+hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, int lds_rows, hipStream_t st) {
+  if (c.offsets == nullptr) return c.w_packed ? wide<XDT, 1, true>(c, x, x_stride, lds_rows, st) : wide<XDT, 1, false>(c, x, x_stride, lds_rows, st);
+  return c.w_packed ? wide<XDT, 2, true>(c, x, x_stride, lds_rows, st) : wide<XDT, 2, false>(c, x, x_stride, lds_rows, st);
+}
 
 template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
 hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
@@ -979,16 +1140,46 @@ static bool offsets_ok(const ftm_w8a8& c) {
          4 * 256 * (int64_t)c.N < INT32_MAX;
 }
 
+// What the fast kernels need of a call's layout.
+static bool aligned_call(const ftm_w8a8& c) {
+  return c.K % 16 == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15u) == 0 && (c.x_stride & 15) == 0 &&
+         (c.offsets == nullptr || (c.w_stride & 15) == 0) && offsets_ok(c);
+}
+
 hipError_t launch_w8a8(const ftm_w8a8& c, hipStream_t st) {
-  const bool aligned = c.K % 16 == 0 && (((uintptr_t)c.x | (uintptr_t)c.w) & 15u) == 0 && (c.x_stride & 15) == 0 &&
-                       (c.offsets == nullptr || (c.w_stride & 15) == 0);
-  if (!aligned || !offsets_ok(c)) {
+  if (!aligned_call(c)) {
     const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + 15) / 16;
     if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
     k_w8a8_any<<<dim3((unsigned)(mt * nt)), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
     return hipGetLastError();
   }
   return c.offsets != nullptr ? grouped(c, st) : dense(c, st);
+}
+
+hipError_t launch_w8a8_dynamic(const ftm_w8a8& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {
+  const bool in = aligned_call(c) && ((uintptr_t)x & 15u) == 0 && (x_stride & 15) == 0;
+  bool few;
+  int lds_rows = 16;
+  if (c.offsets == nullptr) {
+    // every workgroup quantises all tokens, which pays while they are few: 1 / 2 / 4 /
+    // 8 tokens of 2048 x 1536 4.6 / 5.6 / 7.6 / 11.7 us, two launches 7.5 / 7.7 /
+    // 7.8 / 7.7 and about 3 more of the host's; one of 11008 x 4096 14.9 / 14.7
+    few = c.rows <= 4 && c.rows * c.K <= 8192;
+    lds_rows = (int)c.rows;
+  } else {
+    // up to two rows an expert on average, and a grid that would split K anyway (4
+    // tokens through 16 experts of 1024 x 512 with the host 25 us, in six launches 32)
+    const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts;
+    few = c.rows <= 2 * hit && hit * ((c.N + 255) / 256) < kCUs;
+  }
+  if (in && few && (int64_t)lds_rows * ((c.K + 127) / 128) * kRow <= kWideCodes) {
+    if (dt == FTM_DT_F32) return wide<FTM_DT_F32>(c, x, x_stride, lds_rows, st);
+    if (dt == FTM_DT_F16) return wide<FTM_DT_F16>(c, x, x_stride, lds_rows, st);
+    return wide<FTM_DT_BF16>(c, x, x_stride, lds_rows, st);
+  }
+  const hipError_t e = launch_quant_int8(x, dt, c.x_rows, c.K, x_stride, const_cast<int8_t*>(c.x), c.K,
+                                         const_cast<float*>(c.x_scale), st);
+  return e != hipSuccess ? e : launch_w8a8(c, st);
 }
 
 }  // namespace ftm

@@ -12,8 +12,9 @@ import ctypes
 import torch
 
 from .. import _native as nat
+from ..layout import rows_of
 from ..moe.token_sort import ID_DTYPES
-from .w8a8_linear import activation_code, bias_of, rows_of, scale_of, weight_of
+from .w8a8_linear import activation_code, bias_of, scale_of, weight_of
 
 
 def fused_w8a8_moe(

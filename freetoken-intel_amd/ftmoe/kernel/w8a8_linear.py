@@ -18,6 +18,7 @@ import torch
 
 from .. import _native as nat
 from ..layer import ACTIVATIONS
+from ..layout import rows_of
 
 _DT = {torch.float32: nat.DT_F32, torch.float16: nat.DT_F16, torch.bfloat16: nat.DT_BF16}
 
@@ -47,11 +48,6 @@ def quantize_int8_token(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         nat.launch("ftm_quant_int8", nat.lib().ftm_quant_int8, x2, x2.data_ptr(), dt, x2.shape[0], K,
                    x2.stride(0) * x2.element_size(), q.data_ptr(), K, scale.data_ptr())
     return q, scale
-
-
-def rows_of(t: torch.Tensor) -> torch.Tensor:
-    """``t [n, H]`` with neighbouring elements of a row side by side."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def weight_of(weight: torch.Tensor, K: int, dim: int, name: str = "weight") -> tuple[torch.Tensor, int]:

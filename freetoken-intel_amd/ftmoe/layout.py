@@ -1,0 +1,9 @@
+"""Tensor layouts that the kernels take."""
+from __future__ import annotations
+
+import torch
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t [n, H]`` with neighbouring elements of a row side by side (rows may lie apart)."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()

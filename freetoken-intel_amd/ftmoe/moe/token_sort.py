@@ -15,6 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
+from ..layout import rows_of
 
 ID_DTYPES = {torch.int32: nat.ID_I32, torch.int64: nat.ID_I64}
 
@@ -73,14 +74,9 @@ def _check_sort(sort: TokenSort, t: torch.Tensor, name: str) -> None:
         raise ValueError(f"the sort is on {r.device}, {name} on {t.device}")
 
 
-def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t [n, H]`` with neighbouring elements of a row side by side."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
 def _gather(x: torch.Tensor, sort: TokenSort) -> torch.Tensor:
     T, k = sort.row_of_pair.shape
-    x = _unit_rows(x)
+    x = rows_of(x)
     H, size = x.shape[1], x.element_size()
     rows = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
     if rows.numel() == 0:
@@ -92,7 +88,7 @@ def _gather(x: torch.Tensor, sort: TokenSort) -> torch.Tensor:
 
 def _combine(rows: torch.Tensor, w: Optional[torch.Tensor], sort: TokenSort, out_dtype: torch.dtype) -> torch.Tensor:
     T, k = sort.row_of_pair.shape
-    rows = _unit_rows(rows)
+    rows = rows_of(rows)
     H = rows.shape[1]
     out = torch.empty((T, H), dtype=out_dtype, device=rows.device)
     if out.numel() == 0:
@@ -104,6 +100,17 @@ def _combine(rows: torch.Tensor, w: Optional[torch.Tensor], sort: TokenSort, out
     return out
 
 
+def _first_only(backward):
+    """``backward``, refusing a second derivative; the wrapper that refuses it costs more
+    than a small backward itself, so it is passed only where one may follow."""
+    once = once_differentiable(backward)
+
+    def run(ctx, g):
+        return once(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+    return run
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, sort):
@@ -111,7 +118,7 @@ class _Gather(torch.autograd.Function):
         return _gather(x, sort)
 
     @staticmethod
-    @once_differentiable
+    @_first_only
     def backward(ctx, g):
         return _combine(g, None, ctx.sort, g.dtype), None
 
@@ -124,13 +131,13 @@ class _Combine(torch.autograd.Function):
         return _combine(rows, w, sort, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_only
     def backward(ctx, g):
         rows, w = ctx.saved_tensors
         sort = ctx.sort
         T, k = sort.row_of_pair.shape
         want_rows, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        g, rows, wc = _unit_rows(g), _unit_rows(rows), w.contiguous()
+        g, rows, wc = rows_of(g), rows_of(rows), w.contiguous()
         H = rows.shape[1]
         grad_rows = torch.empty((T * k, H), dtype=rows.dtype, device=rows.device) if want_rows else None
         grad_w = torch.empty((T, k), dtype=w.dtype, device=w.device) if want_w else None

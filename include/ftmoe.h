@@ -310,8 +310,8 @@ typedef struct ftm_w8a8 {
 int ftm_w8a8_linear(const ftm_w8a8* call, void* stream);
 
 /* ftm_quant_int8 of x [call->x_rows, K] and ftm_w8a8_linear over its codes:
- * call->x [x_rows, K] (x_stride K) and call->x_scale are scratch that the call
- * writes first. */
+ * call->x [x_rows, K] (x_stride K) and call->x_scale are scratch for them (for
+ * few rows the product quantises by itself and leaves the scratch as it is). */
 int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w8a8* call, void* stream);
 
 /* ---- (token, expert) pairs sorted by expert, and back ----

@@ -464,6 +464,47 @@ def test_expert_and_projection(gpu, dtype):
         fused_w8a8_expert_forward(x, w1[0], s1[0], w2[0], s2[0], intermediate=64)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 2048, 1536), (1, 16, 1), (2, 176, 33), (3, 1408, 64), (4, 2048, 40), (4, 48, 300),
+                                   (5, 64, 64), (1, 8192, 48), (1, 8208, 48), (2, 50, 20)])
+def test_projection_of_few_tokens(gpu, dtype, M, K, N):
+    """Few tokens are quantised inside the product: the bits of the two calls, rows with
+    infinities and NaN, rows apart, biased and packed."""
+    gen = torch.Generator(device=gpu).manual_seed(K)
+    big = torch.randn(M, 2 * K, generator=gen, device=gpu).to(dtype)
+    w, ws = codes((N, K), 1, gpu), scales((N,), 2, gpu)
+    b = torch.randn(N, generator=gen, device=gpu)
+    for x in (big[:, :K].contiguous(), big[:, K:], big[:, 1:K + 1]):
+        x = x.clone() if x.is_contiguous() else x
+        q, s = quantize_int8_token(x)
+        ref = w8a8_linear(q, s, w, ws, bias=b, out_dtype=torch.float32)
+        assert torch.equal(fused_w8a8_linear(x, w, ws, bias=b, out_dtype=torch.float32), ref)
+        if K % 4 == 0:
+            assert torch.equal(fused_w8a8_linear(x, quant.pack_int8_to_int32(w), ws, bias=b, out_dtype=torch.float32), ref)
+    bad = big[:, :K].contiguous()
+    ref = fused_w8a8_linear(bad, w, ws)
+    bad[M - 1, K // 2] = math.inf
+    bad[0, K - 1] = math.nan
+    got = fused_w8a8_linear(bad, w, ws)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[M - 1]).all() and torch.equal(got[1:-1], ref[1:-1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,E,H,I,k", [(1, 8, 128, 64, 2), (4, 16, 1024, 512, 2), (6, 64, 176, 48, 3), (2, 300, 256, 96, 8)])
+def test_moe_of_few_tokens_is_its_operators(gpu, dtype, T, E, H, I, k):
+    """Up to two rows an expert: both products quantise their rows themselves."""
+    x, w1, s1, w2, s2, ids, tw = moe_inputs(gpu, T, E, H, I, k, dtype, seed=3, drop=True)
+    if T > 1:
+        ids[1] = ids[0]  # an expert with several rows
+    sort = sort_tokens(ids, E)
+    q, s = quantize_int8_token(x)
+    h = w8a8_grouped_linear(q, s, sort.offsets, w1, s1, row_index=sort.token_of_row, activation="silu",
+                            out_dtype=torch.float32)
+    y = w8a8_grouped_linear(*quantize_int8_token(h), sort.offsets, w2, s2, out_dtype=torch.float32)
+    ref = combine_tokens(y, tw, sort, out_dtype=dtype)
+    assert torch.equal(fused_w8a8_moe(x, w1, s1, w2, s2, ids, tw), ref)
+
+
 def test_moe_in_a_graph_and_on_streams(gpu):
     """Captured and replayed over new inputs, with eager work between the replays; two
     streams at once."""

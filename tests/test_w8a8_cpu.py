@@ -51,6 +51,50 @@ def test_product_arguments():
     assert _call(rows=0, x_rows=0, out=None, x=None) == nat.OK
 
 
+def test_dynamic_product_arguments():
+    def call(x=P, dt=nat.DT_BF16, xs=128, **kw):
+        c = nat.FtmW8A8(P, P, P, P, None, P, None, None, 4, 4, 64, 0, 32, 64, 1, 0, nat.DT_F32, 0, nat.DT_BF16, -1, 0.0,
+                        0.0)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return nat.lib().ftm_w8a8_linear_dynamic(x, dt, xs, ctypes.byref(c), None)
+
+    assert nat.lib().ftm_w8a8_linear_dynamic(P, 0, 128, None, None) == nat.ERR_NULL
+    assert call(x=None) == nat.ERR_NULL and call(w=None) == nat.ERR_NULL and call(x_scale=None) == nat.ERR_NULL
+    assert call(dt=7) == nat.ERR_FORMAT
+    assert call(xs=-2) == nat.ERR_DIM and call(x_stride=128) == nat.ERR_DIM and call(K=0) == nat.ERR_DIM
+    assert call(x=P + 1) == nat.ERR_ALIGN and call(xs=127) == nat.ERR_ALIGN
+    assert call(rows=0, x_rows=0, x=None) == nat.OK
+
+
+def test_moe_arguments():
+    L = nat.lib()
+    need = L.ftm_w8a8_moe_workspace_bytes(4, 2, 8, 64, 32)
+    assert need > 0
+    for a in ((0, 2, 8, 64, 32), (4, 0, 8, 64, 32), (4, 2, 513, 64, 32), (4, 2, 8, 0, 32), (4, 2, 8, 64, 0)):
+        assert L.ftm_w8a8_moe_workspace_bytes(*a) == 0
+
+    def call(ws=P, n=need, **kw):
+        c = nat.FtmW8A8Moe(P, P, P, P, P, P, None, P, P, None, 128, 4, 2, 8, 64, 32, nat.DT_BF16, nat.ID_I32, nat.DT_F32,
+                           0, 0, nat.DT_F32, 0, nat.DT_F32, 0, nat.ACT_SILU, 0.0, 0.0)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return L.ftm_w8a8_moe_forward(ctypes.byref(c), ws, n, None)
+
+    assert L.ftm_w8a8_moe_forward(None, P, need, None) == nat.ERR_NULL
+    for k in ("x", "topk_ids", "topk_w", "out", "w13", "w13_scale", "w2", "w2_scale"):
+        assert call(**{k: None}) == nat.ERR_NULL, k
+    for kw in (dict(T=-1), dict(k=0), dict(num_experts=0), dict(num_experts=513), dict(hidden=0), dict(inter=0),
+               dict(hidden=nat.W8A8_MAX_K + 1), dict(x_stride=-2), dict(T=2**30, k=2)):
+        assert call(**kw) == nat.ERR_DIM, kw
+    for kw in (dict(dtype=9), dict(topk_w_dtype=9), dict(act=-1), dict(act=4), dict(w13_scale_dtype=9),
+               dict(w2_scale_dtype=9), dict(ids_dtype=5)):
+        assert call(**kw) == nat.ERR_FORMAT, kw
+    assert call(ws=None) == nat.ERR_WORKSPACE and call(n=need - 1) == nat.ERR_WORKSPACE
+    assert call(ws=P + 16) == nat.ERR_ALIGN and call(x=P + 1) == nat.ERR_ALIGN
+    assert call(T=0, x=None) == nat.OK
+
+
 def test_sort_arguments():
     L = nat.lib()
 
