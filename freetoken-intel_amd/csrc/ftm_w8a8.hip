@@ -600,19 +600,22 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_split(ftm_w8a8 c, int mtiles, 
   split_finish<MT, NT, NW>(c, rt, lds, n0, acc, blocks);
 }
 
-// The same for at most 16 tokens a tile whose values are still wide (XDT; x_stride
+constexpr int kWideRows = 4;
+constexpr int kWideK = 8192;  // their codes are kept in LDS
+
+// The same for at most kWideRows tokens a tile whose values are still wide (XDT; x_stride
 // bytes between rows): every workgroup quantises its tokens itself, each wave the
 // K that it multiplies, into LDS, while its first weights are under way.  The
 // codes and scales are the quantiser's; the launch that would write them is
 // saved (the figures are at launch_w8a8_dynamic).
 template <int XDT, int NT, int S, bool PACKED>
-__global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, int64_t x_stride, int lds_rows, int ntiles) {
+__global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, int64_t x_stride, int ntiles) {
   using V = QuantVec<XDT>;
   constexpr int kStage = NT * 16 * kRow, NC = 2 * NT;
-  extern __shared__ char lds[];  // [4][S][kStage], then [step][lds_rows][kRow] codes
+  extern __shared__ char lds[];  // [4][S][kStage], then [step][kWideRows][kRow] codes
   __shared__ uint32_t maxima[4][16];
   const int item = xcd_item(blockIdx.x, gridDim.x);
-  const RowTile rt = row_tile<16>(c, item / ntiles);
+  const RowTile rt = row_tile<kWideRows>(c, item / ntiles);
   if (rt.cnt <= 0) return;
   const int NO = out_cols(c), K = c.K;
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -645,16 +648,22 @@ __global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, in
       const int s = __builtin_amdgcn_readlane((int)src, r);
       return x + (int64_t)(s < 0 ? 0 : s) * x_stride;
     };
+    const char* p[kWideRows];
+#pragma unroll
+    for (int r = 0; r < kWideRows; ++r) p[r] = row_at(r);
+    uint32_t v[kWideRows] = {};
+    for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN)
+#pragma unroll
+      for (int r = 0; r < kWideRows; ++r)
+        if (r < rt.cnt) {
+          const uint32_t b = V::max_bits(*(const u32x4*)(p[r] + (int64_t)k * (16 / V::kN)));
+          v[r] = b > v[r] ? b : v[r];
+        }
     uint32_t mine = 0;
-    for (int r = 0; r < rt.cnt; ++r) {
-      const char* p = row_at(r);
-      uint32_t v = 0;
-      for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN) {
-        const uint32_t b = V::max_bits(*(const u32x4*)(p + (int64_t)k * (16 / V::kN)));
-        v = b > v ? b : v;
-      }
-      v = wave_max_bits(v);
-      mine = m == r ? v : mine;
+#pragma unroll
+    for (int r = 0; r < kWideRows; ++r) {
+      const uint32_t top = r < rt.cnt ? wave_max_bits(v[r]) : 0;
+      mine = m == r ? top : mine;
     }
     if (lane < 16) maxima[wave][lane] = mine;
     __syncthreads();
@@ -663,13 +672,14 @@ __global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, in
     for (int w = 1; w < 4; ++w) top = maxima[w][m] > top ? maxima[w][m] : top;
     const QuantScale own = quant_scale(top);  // of row m
     blocks[0].xscale = own.s;
-    for (int r = 0; r < rt.cnt; ++r) {
-      const char* p = row_at(r);
-      const QuantScale qs = {readlane_f(own.s, r), readlane_f(own.inv, r)};
-      for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN)
-        V::store((int8_t*)codes + ((k >> 7) * lds_rows + r) * kRow + 16 * (((k >> 4) & 7) ^ swz(r)) + (k & 15),
-                 *(const u32x4*)(p + (int64_t)k * (16 / V::kN)), qs);
-    }
+    for (int k = lo * 128 + lane * V::kN; k < k_hi; k += 64 * V::kN)
+#pragma unroll
+      for (int r = 0; r < kWideRows; ++r)
+        if (r < rt.cnt) {
+          const QuantScale qs = {readlane_f(own.s, r), readlane_f(own.inv, r)};
+          V::store((int8_t*)codes + ((k >> 7) * kWideRows + r) * kRow + 16 * (((k >> 4) & 7) ^ swz(r)) + (k & 15),
+                   *(const u32x4*)(p[r] + (int64_t)k * (16 / V::kN)), qs);
+        }
     __builtin_amdgcn_wave_barrier();
     const int xr = m < rt.cnt ? m : 0;
     int slot = 0;
@@ -679,7 +689,7 @@ __global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, in
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       const char* st = ring + slot * kStage;
-      const char* xt = codes + step * lds_rows * kRow;
+      const char* xt = codes + step * kWideRows * kRow;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const uint32_t keep = step * 128 + 64 * q + 16 * g < K ? ~0u : 0u;
@@ -1024,27 +1034,26 @@ hipError_t split(const ftm_w8a8& c, hipStream_t st) {
 }
 
 constexpr int kCUs = 256;
-constexpr int kWideCodes = 64 * 1024;  // bytes of codes in LDS at most
 
 // k_w8a8_wide with one block of 16 weight rows (with an activation, grouped: two) a
 // tile.
 template <int XDT, int NT, bool PACKED>
-hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, int lds_rows, hipStream_t st) {
+hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, hipStream_t st) {
   constexpr int S = NT == 1 ? 4 : 2, ring = 4 * S * NT * 16 * kRow;
-  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = ring + lds_rows * ((c.K + 127) / 128) * kRow;
-  const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + cols - 1) / cols;
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = ring + kWideRows * ((c.K + 127) / 128) * kRow;
+  const int64_t mt = row_tiles(c, kWideRows), nt = (out_cols(c) + cols - 1) / cols;
   if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
   static DeviceBits lds_set{0};
   const auto kernel = k_w8a8_wide<XDT, NT, S, PACKED>;
-  const hipError_t e = allow_lds(lds_set, (const void*)kernel, ring + kWideCodes);
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, ring + kWideRows * kWideK);
   if (e != hipSuccess) return e;
-  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (const char*)x, x_stride, lds_rows, (int)nt);
+  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (const char*)x, x_stride, (int)nt);
   return hipGetLastError();
 }
 template <int XDT>
-hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, int lds_rows, hipStream_t st) {
-  if (c.offsets == nullptr) return c.w_packed ? wide<XDT, 1, true>(c, x, x_stride, lds_rows, st) : wide<XDT, 1, false>(c, x, x_stride, lds_rows, st);
-  return c.w_packed ? wide<XDT, 2, true>(c, x, x_stride, lds_rows, st) : wide<XDT, 2, false>(c, x, x_stride, lds_rows, st);
+hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, hipStream_t st) {
+  if (c.offsets == nullptr) return c.w_packed ? wide<XDT, 1, true>(c, x, x_stride, st) : wide<XDT, 1, false>(c, x, x_stride, st);
+  return c.w_packed ? wide<XDT, 2, true>(c, x, x_stride, st) : wide<XDT, 2, false>(c, x, x_stride, st);
 }
 
 template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
@@ -1114,16 +1123,13 @@ hipError_t dense(const ftm_w8a8& c, hipStream_t st) {
 hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
   // experts with rows, at most, and the rows of each if all have as many
   const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
-  const int64_t tiles = hit * ((seg + 63) / 64) * ((c.N + 255) / 256);
-  // Too few tiles for the chip: K split.  16 x 32 / tile 64, 1 token over 8 of 256
-  // experts of 2048 x 1024 (32 tiles) 7.5 / 18.6, 4 tokens (128) 17.7 / 20.5, 16
-  // tokens (512) 49 / 33; 4 tokens over 32 of 128 experts of 768 x 2048 (256) 15.1 / 14.8
-  if (tiles < kCUs) {
-    if (seg <= 16) return split<1, 2, 4, 2>(c, st);
-    if (seg <= 32) return split<2, 2, 4, 2>(c, st);
-    hipError_t e = hipSuccess;
-    if (split64(c, hit * ((seg + 63) / 64), st, e)) return e;
-  }
+  const int64_t blocks = (hit + c.rows / 16) * ((c.N + 31) / 32);  // 16 x 32, the last of an expert partly filled
+  // Too few tiles to keep the memory busy: K split.  16 x 32 / tile 64, with the
+  // blocks of the first: 1 token over 8 of 256 experts of 2048 x 1024 (256) 7.5 /
+  // 18.6; 2 of 16 of 1024 x 1024, 128 tokens (1024) 12.2 / 15.4, 256 (1536) 15.3 /
+  // 15.5, 512 (2560) 23 / 15.6; 4 of 32 of 2048 x 1536, 8 tokens (1632) 21.8 / 23.9,
+  // 32 (1920) 28.9 / 28.9, 64 (2304) 32.3 / 29.3, 256 (4608) 48.5 / 29.4
+  if (blocks < 8 * kCUs) return split<1, 2, 4, 2>(c, st);
   // 64 / 128 tokens a tile, 2048 tokens over 128 experts (128 rows each) of 2048
   // x 1536 123 / 142, 4 of 32 (256 rows each) of 2880 x 5760 337 / 283
   return seg < 192 ? tile<1, 4, 2, true>(c, st) : tile<2, 4, 3, true>(c, st);
@@ -1159,23 +1165,23 @@ hipError_t launch_w8a8(const ftm_w8a8& c, hipStream_t st) {
 hipError_t launch_w8a8_dynamic(const ftm_w8a8& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {
   const bool in = aligned_call(c) && ((uintptr_t)x & 15u) == 0 && (x_stride & 15) == 0;
   bool few;
-  int lds_rows = 16;
   if (c.offsets == nullptr) {
-    // every workgroup quantises all tokens, which pays while they are few: 1 / 2 / 4 /
-    // 8 tokens of 2048 x 1536 4.6 / 5.6 / 7.6 / 11.7 us, two launches 7.5 / 7.7 /
-    // 7.8 / 7.7 and about 3 more of the host's; one of 11008 x 4096 14.9 / 14.7
-    few = c.rows <= 4 && c.rows * c.K <= 8192;
-    lds_rows = (int)c.rows;
+    // every workgroup quantises all tokens, which pays while they are few: 1 / 2 / 4
+    // tokens of 2048 x 1536 4.9 / 5.7 / 7.3 us, in two launches 7.7 / 7.8 / 7.9 and
+    // about 3 more of the host's; 1 / 2 / 4 of 4096 x 4096 6.3 / 7.9 / 11.2, two 7.6
+    few = c.rows <= kWideRows && c.rows * c.K <= 8192;
   } else {
-    // up to two rows an expert on average, and a grid that would split K anyway (4
-    // tokens through 16 experts of 1024 x 512 with the host 25 us, in six launches 32)
+    // up to one row an expert on average and three rounds of workgroups: both
+    // products with all else of the expert layer, here / in two launches each, 1 / 2
+    // tokens through 8 of 128 experts of 2048 x 768 25.3 / 29.1, 37.3 / 38.5, 4 through
+    // 2 of 16 of 1024 x 512 19.0 / 21.0, but 2 through 4 of 32 of 2880 x 2880 69 / 62
     const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts;
-    few = c.rows <= 2 * hit && hit * ((c.N + 255) / 256) < kCUs;
+    few = c.rows <= c.num_experts && hit * ((c.N + 31) / 32) <= 3 * kCUs;
   }
-  if (in && few && (int64_t)lds_rows * ((c.K + 127) / 128) * kRow <= kWideCodes) {
-    if (dt == FTM_DT_F32) return wide<FTM_DT_F32>(c, x, x_stride, lds_rows, st);
-    if (dt == FTM_DT_F16) return wide<FTM_DT_F16>(c, x, x_stride, lds_rows, st);
-    return wide<FTM_DT_BF16>(c, x, x_stride, lds_rows, st);
+  if (in && few && c.K <= kWideK && c.x_rows > 0) {
+    if (dt == FTM_DT_F32) return wide<FTM_DT_F32>(c, x, x_stride, st);
+    if (dt == FTM_DT_F16) return wide<FTM_DT_F16>(c, x, x_stride, st);
+    return wide<FTM_DT_BF16>(c, x, x_stride, st);
   }
   const hipError_t e = launch_quant_int8(x, dt, c.x_rows, c.K, x_stride, const_cast<int8_t*>(c.x), c.K,
                                          const_cast<float*>(c.x_scale), st);

@@ -115,11 +115,13 @@ class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, sort):
         ctx.sort = sort
+        ctx.save_for_backward(sort.row_of_pair)  # a later write to it is found
         return _gather(x, sort)
 
     @staticmethod
     @_first_only
     def backward(ctx, g):
+        ctx.saved_tensors
         return _combine(g, None, ctx.sort, g.dtype), None
 
 
@@ -127,15 +129,14 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w, sort, out_dtype):
         ctx.sort = sort
-        ctx.save_for_backward(rows, w)
+        ctx.save_for_backward(rows, w, sort.row_of_pair)
         return _combine(rows, w, sort, out_dtype)
 
     @staticmethod
     @_first_only
     def backward(ctx, g):
-        rows, w = ctx.saved_tensors
-        sort = ctx.sort
-        T, k = sort.row_of_pair.shape
+        rows, w, row_of_pair = ctx.saved_tensors
+        T, k = row_of_pair.shape
         want_rows, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         g, rows, wc = rows_of(g), rows_of(rows), w.contiguous()
         H = rows.shape[1]
@@ -146,7 +147,7 @@ class _Combine(torch.autograd.Function):
         nat.launch("ftm_combine_tokens_grad", nat.lib().ftm_combine_tokens_grad, rows, g.data_ptr(),
                    nat.dtype_code(g.dtype), g.stride(0) * g.element_size(), rows.data_ptr(),
                    nat.dtype_code(rows.dtype), rows.stride(0) * rows.element_size(), wc.data_ptr(),
-                   nat.dtype_code(w.dtype), sort.row_of_pair.data_ptr(), T, k, H, nat.ptr(grad_rows), nat.ptr(grad_w))
+                   nat.dtype_code(w.dtype), row_of_pair.data_ptr(), T, k, H, nat.ptr(grad_rows), nat.ptr(grad_w))
         return grad_rows, grad_w, None, None
 
 

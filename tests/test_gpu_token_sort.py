@@ -287,6 +287,39 @@ def test_gradients_of_broadcast_outputs(gpu):
         gx.sum().backward()
 
 
+def test_rows_past_32_bits(gpu):
+    """More than 2^32 bytes of rows, tokens and gradients: the last tokens against the same alone."""
+    T, k, H, E = 300000, 2, 8192, 9
+    ids = torch.arange(T * k, device=gpu).reshape(T, k) % E
+    sort = sort_tokens(ids, E)
+    x = torch.zeros(T, H, device=gpu, dtype=torch.bfloat16)
+    x[-9:] = torch.randn(9, H, generator=torch.Generator(device=gpu).manual_seed(4), device=gpu).to(torch.bfloat16)
+    rows = gather_tokens(x, sort)
+    at = sort.row_of_pair[-9:].reshape(-1).long()
+    assert torch.equal(rows[at], x[-9:].repeat_interleave(k, 0))
+    w = torch.rand(T, k, device=gpu)
+    small = sort_tokens(ids[-9:], E)
+    sr, sw = gather_tokens(x[-9:], small).requires_grad_(), w[-9:].clone().requires_grad_()
+    ref = combine_tokens(sr, sw, small)
+    rows.requires_grad_(), w.requires_grad_()
+    out = combine_tokens(rows, w, sort)
+    assert torch.equal(out[-9:], ref)
+    gr, gw = torch.autograd.grad(out, (rows, w), x)
+    sgr, sgw = torch.autograd.grad(ref, (sr, sw), x[-9:])
+    assert torch.equal(gw[-9:], sgw) and torch.equal(gr[at], sgr[small.row_of_pair.reshape(-1).long()])
+
+
+def test_gradient_after_the_order_changed(gpu):
+    """A write to the order between forward and backward is refused, not used."""
+    sort = sort_tokens(routing(8, 2, 4, 3).to(gpu), 4)
+    x = torch.randn(8, 16, device=gpu, requires_grad=True)
+    rows = gather_tokens(x, sort)
+    out = combine_tokens(rows, torch.rand(8, 2, device=gpu), sort)
+    sort.row_of_pair.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 # ------------------------------------------------------------------ together
 def test_training_step(gpu):
     """Tokens out, a dense expert each, rows back: values and gradients of tokens, router

@@ -305,7 +305,7 @@ GROUPS = {
 
 
 @pytest.mark.parametrize("name", sorted(GROUPS))
-@pytest.mark.parametrize("K,N", [(64, 48), (272, 33), (256, 300), (40, 10)])
+@pytest.mark.parametrize("K,N", [(64, 48), (272, 33), (256, 300), (40, 10), (384, 2100), (176, 1900)])
 @pytest.mark.parametrize("act", [None, "silu"])
 def test_grouped(gpu, name, K, N, act):
     """Every expert's rows are the dense product's bits, the rows of no expert zeros; packed
@@ -357,6 +357,54 @@ def test_grouped_rows_without_an_expert_are_not_read(gpu):
     s[43:] = math.nan
     out = w8a8_grouped_linear(q, s, off, codes((3, 32, 64), 3, gpu), scales((3, 32), 4, gpu))
     assert not out[43:].any() and not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_grouped_weights_past_32_bits(gpu, act):
+    """The last expert's weights, scales and rows lie more than 2^32 bytes behind the first's."""
+    E, N, K = 40, 8192, 16384
+    w, ws = torch.empty((E, N, K), dtype=torch.int8, device=gpu), scales((E, N), 4, gpu)
+    w[E - 1] = codes((N, K), 3, gpu)
+    w[0] = codes((N, K), 5, gpu)
+    for rows in (3, 70):  # split K, tiles
+        counts = [0] * E
+        counts[0] = counts[E - 1] = rows
+        off, P = segments(counts, gpu)
+        q, s = codes((P, K), 1, gpu), scales((P,), 2, gpu)
+        got = w8a8_grouped_linear(q, s, off, w, ws, activation=act)
+        for e, at in ((0, slice(0, rows)), (E - 1, slice(rows, P))):
+            assert torch.equal(got[at], w8a8_linear(q[at], s[at], w[e], ws[e], activation=act))
+
+
+@pytest.mark.parametrize("K,N", [(8192, 96), (8208, 40)])
+def test_rows_past_32_bits(gpu, K, N):
+    """Tokens of more than 2^32 bytes, dense, by expert and through an index; 2^31 results."""
+    M = 2**32 // K + 1000
+    x = torch.zeros((M, K), dtype=torch.float16, device=gpu)  # 2^33 bytes of values, 2^32 of codes
+    last = torch.randn(300, K, generator=torch.Generator(device=gpu).manual_seed(3), device=gpu).half()
+    x[-300:] = last
+    q, s = quantize_int8_token(x)
+    del x
+    lq, ls = quantize_int8_token(last)
+    assert torch.equal(q[-300:], lq) and torch.equal(s[-300:], ls)
+    w, ws = codes((2, N, K), 3, gpu), scales((2, N), 4, gpu)
+    ref = w8a8_linear(lq, ls, w[1], ws[1])
+    assert torch.equal(w8a8_linear(q, s, w[1], ws[1])[-300:], ref)
+    off = torch.tensor([0, 5, M], dtype=torch.int32, device=gpu)
+    assert torch.equal(w8a8_grouped_linear(q, s, off, w, ws)[-300:], ref)
+    idx = torch.arange(M - 300, M, dtype=torch.int32, device=gpu)
+    off = torch.tensor([0, 0, 300], dtype=torch.int32, device=gpu)
+    assert torch.equal(w8a8_grouped_linear(q, s, off, w, ws, row_index=idx), ref)
+
+
+@pytest.mark.parametrize("N", [16384, 16400])
+def test_results_past_32_bits(gpu, N):
+    M, K = 2**32 // (2 * N) + 300, 64
+    q, s = codes((M, K), 1, gpu), scales((M,), 2, gpu)
+    w, ws = codes((N, K), 3, gpu), scales((N,), 4, gpu)
+    got = w8a8_linear(q, s, w, ws, out_dtype=torch.bfloat16)
+    for at in (slice(0, 260), slice(M - 260, M)):
+        assert torch.equal(got[at], w8a8_linear(q[at], s[at], w, ws, out_dtype=torch.bfloat16))
 
 
 def test_grouped_refused(gpu):
@@ -490,7 +538,7 @@ def test_projection_of_few_tokens(gpu, dtype, M, K, N):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T,E,H,I,k", [(1, 8, 128, 64, 2), (4, 16, 1024, 512, 2), (6, 64, 176, 48, 3), (2, 300, 256, 96, 8)])
+@pytest.mark.parametrize("T,E,H,I,k", [(1, 8, 128, 64, 2), (4, 16, 1024, 512, 2), (8, 64, 176, 48, 3), (2, 300, 256, 96, 8)])
 def test_moe_of_few_tokens_is_its_operators(gpu, dtype, T, E, H, I, k):
     """Up to two rows an expert: both products quantise their rows themselves."""
     x, w1, s1, w2, s2, ids, tw = moe_inputs(gpu, T, E, H, I, k, dtype, seed=3, drop=True)
