@@ -240,24 +240,31 @@ struct RowScan {
     total = __builtin_amdgcn_readlane(upto, 63);
   }
 
-  // Tile t < total.
-  __device__ __forceinline__ RowTile tile(int t) const {
-    int before = first, e = -1, m = 0, begin = 0, end = 0;
+  // The expert of tile t < total: its rows, its tiles and the tiles before them.
+  struct Expert {
+    int e, begin, end, tiles, before;
+  };
+  __device__ __forceinline__ Expert expert(int t) const {
+    int before = first, e = -1, start = 0, begin = 0, end = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int n = tiles(lo[i], lo[i + 1]);
       const bool here = t >= before && t < before + n;
       e = here ? 8 * (int)(threadIdx.x & 63) + i : e;
-      m = here ? t - before : m;
+      start = here ? before : start;
       begin = here ? lo[i] : begin;
       end = here ? lo[i + 1] : end;
       before += n;
     }
     const int src = __builtin_ctzll(__ballot(e >= 0));
-    e = __builtin_amdgcn_readlane(e, src);
-    begin = __builtin_amdgcn_readlane(begin, src) + BM * __builtin_amdgcn_readlane(m, src);
+    begin = __builtin_amdgcn_readlane(begin, src);
     end = __builtin_amdgcn_readlane(end, src);
-    return {begin, end - begin < BM ? end - begin : BM, e};
+    return {__builtin_amdgcn_readlane(e, src), begin, end, tiles(begin, end), __builtin_amdgcn_readlane(start, src)};
+  }
+  // Its m-th tile.
+  __device__ __forceinline__ static RowTile tile(const Expert& x, int m) {
+    const int begin = x.begin + BM * m;
+    return {begin, x.end - begin < BM ? x.end - begin : BM, x.e};
   }
 
   // The rows of no expert: before the first offset and from the last on.
@@ -278,7 +285,10 @@ template <int BM>
 __device__ __forceinline__ RowTile row_tile(const ftm_w8a8& c, int t) {
   if (c.offsets == nullptr) return dense_tile<BM>(c, t);
   const RowScan<BM> scan(c);
-  if (t < scan.total) return scan.tile(t);
+  if (t < scan.total) {
+    const auto x = scan.expert(t);
+    return scan.tile(x, t - x.before);
+  }
   const int head = scan.head(), head_tiles = (head + BM - 1) / BM, u = t - scan.total;
   const int begin = u < head_tiles ? u * BM : scan.tail() + (u - head_tiles) * BM;
   const int end = u < head_tiles ? head : (int)c.rows;
@@ -718,15 +728,19 @@ __global__ __launch_bounds__(256) void k_w8a8_wide(ftm_w8a8 c, const char* x, in
 // stages of the next are under way during the last products and the epilogue
 // of this one.
 
-// The order of a dense product's tiles: groups of eight row tiles, their columns
-// one after another, so that the tiles in flight on one XCD share both operands.
-template <int BM>
-__device__ __forceinline__ RowTile dense_item(const ftm_w8a8& c, int item, int mtiles, int ntiles, int& nt) {
-  const int per = 8 * ntiles, first = item / per * 8;
-  const int rows = mtiles - first < 8 ? mtiles - first : 8;
-  nt = item % per / rows;
-  return dense_tile<BM>(c, first + item % per % rows);
-}
+// The order of a product's tiles (an expert's, grouped): groups of eight row tiles,
+// their columns one after another, so that the tiles in flight on one XCD share
+// both operands, and where a round of them ends inside an expert only the weights
+// of one column are read a second time.
+struct ItemOrder {
+  int m, nt;  // row tile, column
+  __device__ __forceinline__ ItemOrder(int item, int mtiles, int ntiles) {
+    const int per = 8 * ntiles, first = item / per * 8;
+    const int rows = mtiles - first < 8 ? mtiles - first : 8;
+    nt = item % per / rows;
+    m = first + item % per % rows;
+  }
+};
 
 // The lane's number, anew: what is computed from it inside a loop is not kept in
 // registers over the loop.
@@ -768,16 +782,14 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
     int n;  // first output channel
   };
   auto tile_at = [&](int item) __attribute__((always_inline)) {
-    Tile t;
-    int nt;
     if constexpr (GROUPED) {
-      nt = item % ntiles;
-      t.rt = scan.tile(item / ntiles);
+      const auto x = scan.expert(item / ntiles);
+      const ItemOrder o(item - x.before * ntiles, x.tiles, ntiles);
+      return Tile{scan.tile(x, o.m), o.nt * kCols};
     } else {
-      t.rt = dense_item<BM>(c, item, mtiles, ntiles, nt);
+      const ItemOrder o(item, mtiles, ntiles);
+      return Tile{dense_tile<BM>(c, o.m), o.nt * kCols};
     }
-    t.n = nt * kCols;
-    return t;
   };
   int item = begin + (blockIdx.x >> 3);
   if (item < end) {
@@ -859,7 +871,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
         for (int i = 0; i < MI; ++i) {
           const int at = MI * q + i;
           if (at == 2 * MI - kAhead) {
-            wait_vm<(S - 2) * (NX + NB)>();
+            if (kb >= S - 1) wait_vm<(S - 2) * (NX + NB)>();  // a tile's first S stages are here already
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             issue(ahead, slot);
 #pragma unroll
@@ -879,7 +891,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
     aim(cur);
 #pragma unroll
     for (int i = 0; i < S; ++i) issue(i, i);
-    wait_vm<(S - 1) * (NX + NB)>();
+    wait_vm<0>();
     asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int j = 0; j < 4; ++j) b[0][j] = wfrag(0, j, 0);
@@ -926,6 +938,9 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) xs[i][r] = c.x_scale[er[i][r] >= 0 && er[i][r] < c.x_rows ? er[i][r] : 0];
+      // With the scales, the next tile's first S stages are here: the steps that would
+      // wait for them need not wait for the stores below
+      wait_vm<0>();
       Channel ch[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) ch[n] = channel(c, ChannelBits{tb[n], bb[n]});
