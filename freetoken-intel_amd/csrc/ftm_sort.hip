@@ -287,6 +287,8 @@ struct RowVec {
       }
     }
   }
+  // ONCE: the row is not kept in the caches.
+  template <bool ONCE>
   __device__ __forceinline__ static void store(char* p, int64_t i, const float (&f)[N]) {
     if constexpr (N == 1) {
       store_scalar(p, i, DT, f[0]);
@@ -298,7 +300,8 @@ struct RowVec {
         else if constexpr (DT == FTM_DT_BF16) v[n] = pack_bf16x2(f[2 * n], f[2 * n + 1]);
         else v[n] = (uint32_t)f32_to_f16(f[2 * n]) | ((uint32_t)f32_to_f16(f[2 * n + 1]) << 16);
       }
-      ((Raw*)p)[i] = v;
+      if constexpr (ONCE) __builtin_nontemporal_store(v, (Raw*)p + i);
+      else ((Raw*)p)[i] = v;
     }
   }
 };
@@ -333,14 +336,15 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const char* rows, int64_
         for (int e = 0; e < N; ++e) acc[e] = fmaf(wt, v[e], acc[e]);
       }
     }
-    if (i < n) RowVec<OT, N>::store(out + t * out_stride, i, acc);
+    if (i < n) RowVec<OT, N>::template store<false>(out + t * out_stride, i, acc);
   }
 }
 
 // The gradients of out[t] = sum_j w[t, j] rows[row(t, j)]: grad_rows[row] = w g
 // (zeros on rows of no expert), grad_w[t, j] = g[t] . rows[row] (0 without an
 // expert), fp32 sums in a fixed order.  One workgroup a token; either may be
-// null.
+// null.  Bound by reading the rows and writing their gradients, which pass the
+// caches by: 8192 tokens of 8 rows of 2048 bf16 92 us, kept 113.
 template <int DT, int OT, int N>
 __global__ __launch_bounds__(256) void k_combine_grad(const char* g, int64_t g_stride, const char* rows,
                                                       int64_t row_stride, const void* w, int w_dt,
@@ -372,7 +376,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const char* g, int64_t g_s
           float v[N];
 #pragma unroll
           for (int e = 0; e < N; ++e) v[e] = r >= 0 ? to.w[j] * gv[e] : 0.0f;
-          V::store(grad_rows + (int64_t)(r < 0 ? ~r : r) * grad_stride, i, v);
+          V::template store<true>(grad_rows + (int64_t)(r < 0 ? ~r : r) * grad_stride, i, v);
         }
       }
       if (grad_w != nullptr) {

@@ -354,6 +354,10 @@ constexpr int kRow = 128;
 __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 typedef __attribute__((address_space(3))) void* LPtr;
 
+// Cache policy of what a kernel does not read again: nothing keeps it.  Results stored
+// so, 2048 tokens over 8 of 128 experts of 768 x 2048, bf16 67 us, kept 84.
+constexpr int kNT = 2;
+
 // The results of a row tile: N = 4 or 2 neighbouring channels from n0 on of one row
 // at a time, through a buffer that drops rows past the tile; channels past the
 // last take an offset past its end, so there is no branch around a store.
@@ -378,26 +382,26 @@ struct RowOut {
         if constexpr (N == 4)
           __builtin_amdgcn_raw_buffer_store_b128(
               (u32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])}, res, off, 0,
-              0);
+              kNT);
         else
-          __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(y[0]), __float_as_uint(y[1])}, res, off, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(y[0]), __float_as_uint(y[1])}, res, off, 0, kNT);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[i]), res, n0 + i < NO ? 4u * (at + i) : kOOB, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[i]), res, n0 + i < NO ? 4u * (at + i) : kOOB, 0, kNT);
       }
       return;
     }
     const uint32_t off = n0 < NO ? 2u * at : kOOB;
     if (vec) {
       if constexpr (N == 4)
-        __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, kNT);
       else
-        __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, kNT);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)half2(y[i], 0.0f), res, n0 + i < NO ? 2u * (at + i) : kOOB, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)half2(y[i], 0.0f), res, n0 + i < NO ? 2u * (at + i) : kOOB, 0, kNT);
     }
   }
 };
@@ -750,7 +754,7 @@ __device__ __forceinline__ int opaque_lane() {
   return l;
 }
 
-template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
+template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtiles, int ntiles) {
   constexpr int BM = 16 * MI * WM;
   constexpr int kX = BM * kRow, kStage = kX + 256 * kRow;
@@ -844,7 +848,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + i)), 16, (int)(woff[i] + k0), 0, 0,
-                                                 0);
+                                                 ONCE ? kNT : 0);
     };
     i32x4 acc[MI][4];
     u32x4 b[2][4], x[kAhead + 1];
@@ -1071,7 +1075,7 @@ hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, hipStream_t 
   return c.w_packed ? wide<XDT, 2, true>(c, x, x_stride, st) : wide<XDT, 2, false>(c, x, x_stride, st);
 }
 
-template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED>
+template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED, bool ONCE>
 hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
   constexpr int BM = 16 * MI * WM, lds = S * (BM + 256) * kRow;
   constexpr int resident = kCUs * (2 * lds <= 160 * 1024 ? 2 : 1);  // workgroups the chip holds at once
@@ -1079,22 +1083,24 @@ hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
   const int64_t mt = row_tiles(c, BM), nt = (out_cols(c) + cols - 1) / cols;
   if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
   static DeviceBits lds_set{0};
-  const auto kernel = k_w8a8_tile<WM, MI, S, PACKED, ACT, TAIL, GROUPED>;
+  const auto kernel = k_w8a8_tile<WM, MI, S, PACKED, ACT, TAIL, GROUPED, ONCE>;
   const hipError_t e = allow_lds(lds_set, (const void*)kernel, lds);
   if (e != hipSuccess) return e;
   const int64_t grid = mt * nt < resident ? (mt * nt + 7) / 8 * 8 : resident;  // the same for every XCD
   kernel<<<dim3((unsigned)grid), dim3(256 * WM), lds, st>>>(c, (int)mt, (int)nt);
   return hipGetLastError();
 }
-template <int WM, int MI, int S, bool ACT, bool GROUPED>
+template <int WM, int MI, int S, bool ACT, bool GROUPED, bool ONCE>
 hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
   if (c.K % 128 != 0 || c.K < 128 * S)
-    return c.w_packed ? tile<WM, MI, S, true, ACT, true, GROUPED>(c, st) : tile<WM, MI, S, false, ACT, true, GROUPED>(c, st);
-  return c.w_packed ? tile<WM, MI, S, true, ACT, false, GROUPED>(c, st) : tile<WM, MI, S, false, ACT, false, GROUPED>(c, st);
+    return c.w_packed ? tile<WM, MI, S, true, ACT, true, GROUPED, ONCE>(c, st)
+                      : tile<WM, MI, S, false, ACT, true, GROUPED, ONCE>(c, st);
+  return c.w_packed ? tile<WM, MI, S, true, ACT, false, GROUPED, ONCE>(c, st)
+                    : tile<WM, MI, S, false, ACT, false, GROUPED, ONCE>(c, st);
 }
-template <int WM, int MI, int S, bool GROUPED>
+template <int WM, int MI, int S, bool GROUPED, bool ONCE = false>
 hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
-  return c.act >= 0 ? tile<WM, MI, S, true, GROUPED>(c, st) : tile<WM, MI, S, false, GROUPED>(c, st);
+  return c.act >= 0 ? tile<WM, MI, S, true, GROUPED, ONCE>(c, st) : tile<WM, MI, S, false, GROUPED, ONCE>(c, st);
 }
 
 // us on MI355X beside each rule: 'split' 64 x 64 is k_w8a8_split's tile of 64
@@ -1145,6 +1151,10 @@ hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
   // 15.5, 512 (2560) 23 / 15.6; 4 of 32 of 2048 x 1536, 8 tokens (1632) 21.8 / 23.9,
   // 32 (1920) 28.9 / 28.9, 64 (2304) 32.3 / 29.3, 256 (4608) 48.5 / 29.4
   if (blocks < 8 * kCUs) return split<1, 2, 4, 2>(c, st);
+  // Mostly one tile an expert: its weights are not kept for another.  The layer of 8
+  // of 128 experts of 2048 x 768, 256 / 512 / 1024 / 2048 tokens 145 / 158 / 213 / 302,
+  // kept 155 / 168 / 209 / 279
+  if (seg <= 48) return tile<1, 4, 2, true, true>(c, st);
   // 64 / 128 tokens a tile, 2048 tokens over 128 experts (128 rows each) of 2048
   // x 1536 123 / 142, 4 of 32 (256 rows each) of 2880 x 5760 337 / 283
   return seg < 192 ? tile<1, 4, 2, true>(c, st) : tile<2, 4, 3, true>(c, st);
