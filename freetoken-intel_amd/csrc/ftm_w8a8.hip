@@ -355,7 +355,8 @@ __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 typedef __attribute__((address_space(3))) void* LPtr;
 
 // Cache policy of what a kernel does not read again: nothing keeps it.  Results stored
-// so, 2048 tokens over 8 of 128 experts of 768 x 2048, bf16 67 us, kept 84.
+// so leave the weights in the last cache: 2048 tokens over 8 of 128 experts of 768 x
+// 2048 (201 MB) again and again 67 us, kept 84; with cold weights 86 / 88.
 constexpr int kNT = 2;
 
 // The results of a row tile: N = 4 or 2 neighbouring channels from n0 on of one row
@@ -1108,14 +1109,15 @@ hipError_t tile(const ftm_w8a8& c, hipStream_t st) {
 
 // The split tile of up to 64 tokens whose columns give every CU one workgroup at
 // most (wider tiles read the tokens less often, but their CUs stay idle), or
-// none: 33-512 rows, 64 x 16 / 64 x 32 / 64 x 64 / tile 64: 64 of 4096 x 4096 7.8 /
-// 9.5 / 15.6 / 26, 128 13.8 / 10.0 / 15.8 / 26, 256 26 / 18.4 / 17.9 / 26, 512 50 /
-// 35 / 33 / 27, 64 of 4096 x 12288 25.6 / 22.4 / 19.3 / 38.
+// none: 64 x 16 / 64 x 32 / 64 x 64 / tile 64: 64 rows of 4096 x 4096 8.0 / 8.7 / 14.4 /
+// 25.5, 100 14.0 / 9.4 / 14.4 / 25.4, 160 20.2 / 16.5 / 15.3 / 25.5, 512 50.6 / 32.6 /
+// 31.9 / 27.0; 512 of 1408 x 2048 (1024 blocks) 18.2 / 12.0 / 11.8 / 13.7, 333 of 2048
+// x 4096 (1536) 28.9 / 18.5 / 22.0 / 16.6
 bool split64(const ftm_w8a8& c, int64_t row_tiles, hipStream_t st, hipError_t& e) {
   const int64_t blocks = row_tiles * ((c.N + 15) / 16);  // of 16 weight rows
   if (blocks <= kCUs) e = split<4, 1, 4, 3>(c, st);
   else if (blocks <= 2 * kCUs) e = split<4, 2, 4, 2>(c, st);
-  else if (blocks <= 6 * kCUs) e = split<4, 4, 4, 2>(c, st);
+  else if (blocks <= 4 * kCUs) e = split<4, 4, 4, 2>(c, st);
   else return false;
   return true;
 }
@@ -1127,8 +1129,9 @@ hipError_t dense(const ftm_w8a8& c, hipStream_t st) {
   // rows of 4096 x 4096 5.8 / 7.2, of 4096 x 12288 16.3 / 14.8
   if (M <= 16) return blocks <= 2 * kCUs ? split<1, 1, 4, 4>(c, st) : split<1, 1, 4, 2>(c, st);
   if (M <= 32) return blocks <= 2 * kCUs ? split<2, 1, 4, 3>(c, st) : split<2, 2, 4, 2>(c, st);
+  if (c.row_index != nullptr) return split<4, 4, 4, 2>(c, st);  // the tiles of a dense product take rows in order
   hipError_t e = hipSuccess;
-  if (c.row_index != nullptr || split64(c, (M + 63) / 64, st, e)) return c.row_index != nullptr ? split<4, 4, 4, 2>(c, st) : e;
+  if (split64(c, (M + 63) / 64, st, e)) return e;
   // The largest tile reads its operands least often, but a launch takes whole
   // rounds of them: rounds x the time of one, in that of a 256-token tile (1;
   // 128 tokens 0.6; two of 64 on a CU 0.68, one 0.58; 8192 rows of 8192 x 8192

@@ -4,11 +4,13 @@ plain arithmetic in 64 bits.
 Tolerances: the integer sum is exact; its rounding to fp32, the token scale and
 the channel scale (with the bias) are one rounding each, 2^-24 relative, and
 the output rounds once, by half a step of its type."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from ftmoe import _native as nat
 from ftmoe import quant
 from ftmoe.engine import MoeGraphRunner
 from ftmoe.kernel.fused_w8a8_linear import fused_w8a8_expert_forward, fused_w8a8_linear
@@ -259,6 +261,24 @@ def test_linear_activation(gpu, act, M, K, N, bias):
     assert got.shape == ref.shape
     err = (got.double() - ref).abs()
     assert (err <= tol + 1e-37).all(), float((err - tol).max())
+
+
+@pytest.mark.parametrize("M", [1, 5, 20, 40, 300])
+@pytest.mark.parametrize("K", [256, 52])
+def test_linear_row_index(gpu, M, K):
+    """The C call reads rows through an index without experts too; one that names none gives zeros."""
+    R, N = 70, 96
+    q, s, w, ws = codes((R, K), 1, gpu), scales((R,), 2, gpu), codes((N, K), 3, gpu), scales((N,), 4, gpu)
+    idx = torch.randint(0, R, (M,), generator=torch.Generator().manual_seed(M), dtype=torch.int32).to(gpu)
+    idx[M // 2] = R if M > 1 else -1
+    out = torch.full((M, N), 7.0, device=gpu)
+    c = nat.FtmW8A8(q.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), None, idx.data_ptr(),
+                    M, R, K, 0, N, K, 1, 0, nat.DT_F32, 0, nat.DT_F32, -1, 0.0, 0.0)
+    nat.launch("ftm_w8a8_linear", nat.lib().ftm_w8a8_linear, q, ctypes.byref(c))
+    at = idx.clamp(0, R - 1).long()
+    ref = w8a8_linear(q[at], s[at], w, ws, out_dtype=torch.float32)
+    ref[M // 2] = 0
+    assert torch.equal(out, ref)
 
 
 def test_linear_empty_and_refused(gpu):
