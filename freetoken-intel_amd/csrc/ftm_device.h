@@ -208,6 +208,14 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
 }
 
 // Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
+// A workgroup a row.  A launch counts the threads of one grid dimension in 32 bits,
+// so more than 2^20 rows go on in y; the last of those may be past the rows.
+inline dim3 row_grid(int64_t rows) {
+  const int64_t x = rows < (1 << 20) ? rows : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((rows + x - 1) / x));
+}
+__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // lanes (DPP row_shr, zeros shifted in), then the rows before.
 __device__ __forceinline__ int wave_prefix_sum(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);

@@ -227,9 +227,10 @@ struct TokenRows {
 // pairs (zeros where a pair has no expert).  Bound by the writes.
 template <class V>
 __global__ __launch_bounds__(256) void k_gather_tokens(const char* x, int64_t x_stride, int n, const int32_t* row_of_pair,
-                                                       int k, V* rows) {
-  const int64_t t = blockIdx.x;
-  const int P = (int)gridDim.x * k;
+                                                       int T, int k, V* rows) {
+  const int64_t t = grid_row();
+  if (t >= T) return;
+  const int P = T * k;
   const V* src = (const V*)(x + t * x_stride);
   for (int j0 = 0; j0 < k; j0 += 8) {
     const TokenRows to(row_of_pair, nullptr, 0, t * k + j0, k - j0, P);
@@ -248,12 +249,12 @@ hipError_t launch_gather(const void* x, int64_t x_stride, int elem, int H, const
                          void* rows, hipStream_t st) {
   const int64_t bytes = (int64_t)elem * H;
   const char* p = (const char*)x;
-  const dim3 grid((unsigned)T), wg(256);
+  const dim3 grid = row_grid(T), wg(256);
   if (((uintptr_t)x | (uintptr_t)rows | (uint64_t)x_stride | (uint64_t)bytes) % 16 == 0)
-    k_gather_tokens<u32x4><<<grid, wg, 0, st>>>(p, x_stride, (int)(bytes / 16), row_of_pair, k, (u32x4*)rows);
-  else if (elem == 4) k_gather_tokens<uint32_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, k, (uint32_t*)rows);
-  else if (elem == 2) k_gather_tokens<uint16_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, k, (uint16_t*)rows);
-  else k_gather_tokens<uint8_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, k, (uint8_t*)rows);
+    k_gather_tokens<u32x4><<<grid, wg, 0, st>>>(p, x_stride, (int)(bytes / 16), row_of_pair, T, k, (u32x4*)rows);
+  else if (elem == 4) k_gather_tokens<uint32_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, T, k, (uint32_t*)rows);
+  else if (elem == 2) k_gather_tokens<uint16_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, T, k, (uint16_t*)rows);
+  else k_gather_tokens<uint8_t><<<grid, wg, 0, st>>>(p, x_stride, H, row_of_pair, T, k, (uint8_t*)rows);
   return hipGetLastError();
 }
 
@@ -310,10 +311,11 @@ struct RowVec {
 // rounding; w null: ones.  One workgroup a token.  Bound by reading the rows.
 template <int DT, int OT, int N>
 __global__ __launch_bounds__(256) void k_combine_tokens(const char* rows, int64_t row_stride, const void* w, int w_dt,
-                                                        const int32_t* row_of_pair, int k, int n, char* out,
+                                                        const int32_t* row_of_pair, int T, int k, int n, char* out,
                                                         int64_t out_stride) {
-  const int64_t t = blockIdx.x;
-  const int P = (int)gridDim.x * k;
+  const int64_t t = grid_row();
+  if (t >= T) return;
+  const int P = T * k;
   // every lane takes part in each round of the loop (TokenRows asks lanes 0..7),
   // those past the row without loads
   for (int i0 = 0; i0 < n; i0 += 256) {
@@ -348,11 +350,12 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const char* rows, int64_
 template <int DT, int OT, int N>
 __global__ __launch_bounds__(256) void k_combine_grad(const char* g, int64_t g_stride, const char* rows,
                                                       int64_t row_stride, const void* w, int w_dt,
-                                                      const int32_t* row_of_pair, int k, int n, char* grad_rows,
+                                                      const int32_t* row_of_pair, int T, int k, int n, char* grad_rows,
                                                       int64_t grad_stride, void* grad_w) {
   __shared__ float part[4][8];
-  const int64_t t = blockIdx.x;
-  const int P = (int)gridDim.x * k;
+  const int64_t t = grid_row();
+  if (t >= T) return;
+  const int P = T * k;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int j0 = 0; j0 < k; j0 += 8) {
     const TokenRows to(row_of_pair, grad_rows != nullptr ? w : nullptr, w_dt, t * k + j0, k - j0, P);
@@ -426,12 +429,12 @@ hipError_t launch_combine(const void* rows, int dt, int64_t row_stride, const vo
   return row_types(dt, out_dt, [&](auto d, auto o) {
     constexpr int D = decltype(d)::value, O = decltype(o)::value, N = D == FTM_DT_F32 ? 4 : 8;
     const int64_t os = (int64_t)H * (O == FTM_DT_F32 ? 4 : 2);
-    const dim3 grid((unsigned)T), wg(256);
+    const dim3 grid = row_grid(T), wg(256);
     if (H % N == 0 && ((uintptr_t)rows | (uintptr_t)out | (uint64_t)row_stride) % 16 == 0)
-      k_combine_tokens<D, O, N><<<grid, wg, 0, st>>>((const char*)rows, row_stride, w, w_dt, row_of_pair, k, H / N,
+      k_combine_tokens<D, O, N><<<grid, wg, 0, st>>>((const char*)rows, row_stride, w, w_dt, row_of_pair, T, k, H / N,
                                                      (char*)out, os);
     else
-      k_combine_tokens<D, O, 1><<<grid, wg, 0, st>>>((const char*)rows, row_stride, w, w_dt, row_of_pair, k, H,
+      k_combine_tokens<D, O, 1><<<grid, wg, 0, st>>>((const char*)rows, row_stride, w, w_dt, row_of_pair, T, k, H,
                                                      (char*)out, os);
     return hipGetLastError();
   });
@@ -443,14 +446,14 @@ hipError_t launch_combine_grad(const void* g, int g_dt, int64_t g_stride, const 
   return row_types(dt, g_dt, [&](auto d, auto o) {
     constexpr int D = decltype(d)::value, O = decltype(o)::value, N = D == FTM_DT_F32 ? 4 : 8;
     const int64_t rs = (int64_t)H * (D == FTM_DT_F32 ? 4 : 2);
-    const dim3 grid((unsigned)T), wg(256);
+    const dim3 grid = row_grid(T), wg(256);
     const uint64_t read = grad_w != nullptr ? (uintptr_t)rows | (uint64_t)row_stride : 0;
     if (H % N == 0 && ((uintptr_t)g | (uint64_t)g_stride | read | (uintptr_t)grad_rows) % 16 == 0)
       k_combine_grad<D, O, N><<<grid, wg, 0, st>>>((const char*)g, g_stride, (const char*)rows, row_stride, w, w_dt,
-                                                   row_of_pair, k, H / N, (char*)grad_rows, rs, grad_w);
+                                                   row_of_pair, T, k, H / N, (char*)grad_rows, rs, grad_w);
     else
       k_combine_grad<D, O, 1><<<grid, wg, 0, st>>>((const char*)g, g_stride, (const char*)rows, row_stride, w, w_dt,
-                                                   row_of_pair, k, H, (char*)grad_rows, rs, grad_w);
+                                                   row_of_pair, T, k, H, (char*)grad_rows, rs, grad_w);
     return hipGetLastError();
   });
 }

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void k_quant_int8(const char* x, int64_t x_str
   __shared__ uint32_t wmax[4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * kRows + wave / WPR;
+  const int64_t row = grid_row() * kRows + wave / WPR;
   const int first = (wave % WPR) * 64 + lane;  // of this lane's vectors, WPR * 64 apart
   const bool live = row < rows;
   const char* src = x + (live ? row : 0) * x_stride;
@@ -153,10 +153,11 @@ __global__ __launch_bounds__(256) void k_quant_int8(const char* x, int64_t x_str
 
 // Any row length, stride and alignment: one workgroup per row, x read twice.
 template <int DT>
-__global__ __launch_bounds__(256) void k_quant_int8_any(const char* x, int64_t x_stride, int K, int8_t* q,
+__global__ __launch_bounds__(256) void k_quant_int8_any(const char* x, int64_t x_stride, int64_t rows, int K, int8_t* q,
                                                         int64_t q_stride, float* scale) {
   __shared__ uint32_t wmax[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = grid_row();
+  if (row >= rows) return;
   const void* src = x + row * x_stride;
   uint32_t m = 0;
   for (int k = threadIdx.x; k < K; k += 256) {
@@ -181,10 +182,10 @@ hipError_t quant_dt(const char* x, int64_t x_stride, int64_t rows, int K, int8_t
                        ((uintptr_t)q & 7u) == 0 && (q_stride & 7) == 0;
   const int vecs = K / kN;
   if (!aligned || vecs > 8 * 256) {
-    k_quant_int8_any<DT><<<dim3((unsigned)rows), dim3(256), 0, st>>>(x, x_stride, K, q, q_stride, scale);
+    k_quant_int8_any<DT><<<row_grid(rows), dim3(256), 0, st>>>(x, x_stride, rows, K, q, q_stride, scale);
     return hipGetLastError();
   }
-  const dim3 by4((unsigned)((rows + 3) / 4)), by1((unsigned)rows), wg(256);
+  const dim3 by4 = row_grid((rows + 3) / 4), by1 = row_grid(rows), wg(256);
   // one wave a row up to four loads a lane, else a workgroup a row
   if (vecs <= 64) k_quant_int8<DT, 1, 1><<<by4, wg, 0, st>>>(x, x_stride, rows, K, q, q_stride, scale);
   else if (vecs <= 128) k_quant_int8<DT, 1, 2><<<by4, wg, 0, st>>>(x, x_stride, rows, K, q, q_stride, scale);
@@ -990,14 +991,13 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
 // ------------------------------------------------------------------ any K and alignment
 // 16 tokens x 16 output channels a workgroup, bytes through LDS: for K not a
 // multiple of 16 and rows that are not 16-byte aligned.
-__global__ __launch_bounds__(256) void k_w8a8_any(ftm_w8a8 c, int mtiles, int ntiles) {
+__device__ __forceinline__ void any_item(const ftm_w8a8& c, int mt, int nt) {
   constexpr int KC = 64;
   __shared__ int8_t xs[16][KC + 4], ws[2][16][KC + 4];
-  const int item = blockIdx.x;
-  const RowTile rt = row_tile<16>(c, item / ntiles);
+  const RowTile rt = row_tile<16>(c, mt);
   if (rt.cnt <= 0) return;
   const bool act = c.act >= 0;
-  const int NO = out_cols(c), n0 = (item % ntiles) * 16;
+  const int NO = out_cols(c), n0 = nt * 16;
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
   int a = 0, b = 0;
   if (rt.e >= 0) {
@@ -1033,6 +1033,13 @@ __global__ __launch_bounds__(256) void k_w8a8_any(ftm_w8a8 c, int mtiles, int nt
   store_scalar(c.out, orow * NO + n0 + col, c.out_dtype, y);
 }
 
+__global__ __launch_bounds__(256) void k_w8a8_any(ftm_w8a8 c, int mtiles, int ntiles) {
+  const int64_t items = (int64_t)mtiles * ntiles;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) any_item(c, (int)(i / ntiles), (int)(i % ntiles));
+}
+
+constexpr int kMaxGroups = (1 << 24) - 1;  // workgroups of 256 threads that one grid dimension counts
+
 namespace {
 
 template <int MT, int NT, int NW, int S, bool PACKED>
@@ -1041,7 +1048,7 @@ hipError_t split(const ftm_w8a8& c, hipStream_t st) {
   constexpr int lds = ring > sums ? ring : sums;
   const int cols = c.act >= 0 ? 8 * NT : 16 * NT;
   const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + cols - 1) / cols;
-  if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
+  if (mt * nt > kMaxGroups) return hipErrorInvalidValue;
   static DeviceBits lds_set{0};
   const hipError_t e = allow_lds(lds_set, (const void*)k_w8a8_split<MT, NT, NW, S, PACKED>, lds);
   if (e != hipSuccess) return e;
@@ -1062,7 +1069,7 @@ hipError_t wide(const ftm_w8a8& c, const void* x, int64_t x_stride, hipStream_t 
   constexpr int S = NT == 1 ? 4 : 2, ring = 4 * S * NT * 16 * kRow;
   const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = ring + kWideRows * ((c.K + 127) / 128) * kRow;
   const int64_t mt = row_tiles(c, kWideRows), nt = (out_cols(c) + cols - 1) / cols;
-  if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
+  if (mt * nt > kMaxGroups) return hipErrorInvalidValue;
   static DeviceBits lds_set{0};
   const auto kernel = k_w8a8_wide<XDT, NT, S, PACKED>;
   const hipError_t e = allow_lds(lds_set, (const void*)kernel, ring + kWideRows * kWideK);
@@ -1183,8 +1190,8 @@ static bool aligned_call(const ftm_w8a8& c) {
 hipError_t launch_w8a8(const ftm_w8a8& c, hipStream_t st) {
   if (!aligned_call(c)) {
     const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + 15) / 16;
-    if (mt * nt > 0x7fffffff) return hipErrorInvalidValue;
-    k_w8a8_any<<<dim3((unsigned)(mt * nt)), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
+    const int64_t grid = mt * nt < kMaxGroups ? mt * nt : kMaxGroups;
+    k_w8a8_any<<<dim3((unsigned)grid), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
     return hipGetLastError();
   }
   return c.offsets != nullptr ? grouped(c, st) : dense(c, st);

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from .. import _native as nat
-from ..layout import rows_of
+from ..layout import row_stride, rows_of
 from ..moe.token_sort import ID_DTYPES
 from .w8a8_linear import activation_code, bias_of, scale_of, weight_of
 
@@ -71,7 +71,7 @@ def fused_w8a8_moe(
     need = L.ftm_w8a8_moe_workspace_bytes(T, k, E, H, I2 // 2)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     c = nat.FtmW8A8Moe(x.data_ptr(), ids.data_ptr(), w.data_ptr(), out.data_ptr(), wa.data_ptr(), sa.data_ptr(),
-                       nat.ptr(ba), wb.data_ptr(), sb.data_ptr(), nat.ptr(bb), x.stride(0) * x.element_size(), T, k, E,
+                       nat.ptr(ba), wb.data_ptr(), sb.data_ptr(), nat.ptr(bb), row_stride(x) * x.element_size(), T, k, E,
                        H, I2 // 2, dt, ID_DTYPES[ids.dtype], w_dt, packed_a, packed_b, sa_dt, ba_dt, sb_dt, bb_dt, act,
                        swiglu_alpha, swiglu_limit)
     nat.launch("ftm_w8a8_moe_forward", L.ftm_w8a8_moe_forward, x, ctypes.byref(c), ws.data_ptr(), need)

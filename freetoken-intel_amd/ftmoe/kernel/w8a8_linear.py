@@ -18,7 +18,7 @@ import torch
 
 from .. import _native as nat
 from ..layer import ACTIVATIONS
-from ..layout import rows_of
+from ..layout import row_stride, rows_of
 
 _DT = {torch.float32: nat.DT_F32, torch.float16: nat.DT_F16, torch.bfloat16: nat.DT_BF16}
 
@@ -46,7 +46,7 @@ def quantize_int8_token(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
     if x2.shape[0]:
         nat.launch("ftm_quant_int8", nat.lib().ftm_quant_int8, x2, x2.data_ptr(), dt, x2.shape[0], K,
-                   x2.stride(0) * x2.element_size(), q.data_ptr(), K, scale.data_ptr())
+                   row_stride(x2) * x2.element_size(), q.data_ptr(), K, scale.data_ptr())
     return q, scale
 
 
@@ -133,14 +133,15 @@ def _product(x, x_scale, weight, weight_scale, *, bias, out_dtype, offsets=None,
         scratch = torch.empty(at + 4 * M, dtype=torch.uint8, device=x.device).data_ptr()
         q, s, stride = scratch, scratch + at, K
     else:
-        q, s, stride = x.data_ptr(), x_scale.data_ptr(), x.stride(0)
+        x = x if row_stride(x) >= K else x.contiguous()  # rows over one another
+        q, s, stride = x.data_ptr(), x_scale.data_ptr(), row_stride(x)
     c = nat.FtmW8A8(q, s, w.data_ptr(), ws.data_ptr(), None if b is None else b.data_ptr(), out.data_ptr(),
                     None if offsets is None else offsets.data_ptr(), None if row_index is None else row_index.data_ptr(),
                     rows, M, stride, N * K, N, K, 1 if offsets is None else lead[0], packed, ws_dt, b_dt, out_dt, act,
                     alpha, limit)
     if x_scale is None:
         nat.launch("ftm_w8a8_linear_dynamic", nat.lib().ftm_w8a8_linear_dynamic, x, x.data_ptr(), x_dt,
-                   x.stride(0) * x.element_size(), ctypes.byref(c))
+                   row_stride(x) * x.element_size(), ctypes.byref(c))
     else:
         nat.launch("ftm_w8a8_linear", nat.lib().ftm_w8a8_linear, x, ctypes.byref(c))
     return out

@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
-from ..layout import rows_of
+from ..layout import row_stride, rows_of
 
 ID_DTYPES = {torch.int32: nat.ID_I32, torch.int64: nat.ID_I64}
 
@@ -81,7 +81,7 @@ def _gather(x: torch.Tensor, sort: TokenSort) -> torch.Tensor:
     rows = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
     if rows.numel() == 0:
         return rows
-    nat.launch("ftm_gather_tokens", nat.lib().ftm_gather_tokens, x, x.data_ptr(), x.stride(0) * size, size, H,
+    nat.launch("ftm_gather_tokens", nat.lib().ftm_gather_tokens, x, x.data_ptr(), row_stride(x) * size, size, H,
                sort.row_of_pair.data_ptr(), T, k, rows.data_ptr())
     return rows
 
@@ -95,7 +95,7 @@ def _combine(rows: torch.Tensor, w: Optional[torch.Tensor], sort: TokenSort, out
         return out
     w = w.contiguous() if w is not None else None
     nat.launch("ftm_combine_tokens", nat.lib().ftm_combine_tokens, rows, rows.data_ptr(), nat.dtype_code(rows.dtype),
-               rows.stride(0) * rows.element_size(), nat.ptr(w), nat.dtype_code(w.dtype) if w is not None else 0,
+               row_stride(rows) * rows.element_size(), nat.ptr(w), nat.dtype_code(w.dtype) if w is not None else 0,
                sort.row_of_pair.data_ptr(), T, k, H, out.data_ptr(), nat.dtype_code(out_dtype))
     return out
 
@@ -145,8 +145,8 @@ class _Combine(torch.autograd.Function):
         if T == 0 or H == 0:
             return grad_rows, None if grad_w is None else grad_w.zero_(), None, None
         nat.launch("ftm_combine_tokens_grad", nat.lib().ftm_combine_tokens_grad, rows, g.data_ptr(),
-                   nat.dtype_code(g.dtype), g.stride(0) * g.element_size(), rows.data_ptr(),
-                   nat.dtype_code(rows.dtype), rows.stride(0) * rows.element_size(), wc.data_ptr(),
+                   nat.dtype_code(g.dtype), row_stride(g) * g.element_size(), rows.data_ptr(),
+                   nat.dtype_code(rows.dtype), row_stride(rows) * rows.element_size(), wc.data_ptr(),
                    nat.dtype_code(w.dtype), row_of_pair.data_ptr(), T, k, H, nat.ptr(grad_rows), nat.ptr(grad_w))
         return grad_rows, grad_w, None, None
 

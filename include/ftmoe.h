@@ -271,8 +271,8 @@ int ftm_dequant(const ftm_proj* proj, int32_t slot, void* out, int32_t out_dtype
 
 /* Quantise rows x [rows, K] (x_stride bytes apart) to int8: scale[m] =
  * max_k |x[m, k]| * fp32(1 / 127) in fp32, the maximum taken as at least 1e-12
- * (the value of torch's amax / 127 on the GPU); q[m, k] = the whole number nearest x[m, k] / scale[m], ties to even (q_stride bytes
- * between rows).  A row with an infinity or NaN gets the scale NaN and codes 0. */
+ * (the value of torch's amax / 127 on the GPU); q[m, k] = the whole number nearest
+ * x[m, k] / scale[m], ties to even (q_stride bytes between rows).  A row with an infinity or NaN gets the scale NaN and codes 0. */
 int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride,
                    int8_t* q, int64_t q_stride, float* scale, void* stream);
 
@@ -343,8 +343,8 @@ int ftm_combine_tokens(const void* rows, int32_t dtype, int64_t row_stride, cons
                        const int32_t* row_of_pair, int32_t T, int32_t k, int32_t H, void* out, int32_t out_dtype,
                        void* stream);
 
-/* Its gradients for g = d out [T, H] (g_dtype, as out_dtype above): grad_rows[row_of_pair[t, j], :] = w[t, j]
- * g[t, :] (zeros without an expert), grad_w[t, j] = g[t] . rows[row] (w_dtype; 0
+/* Its gradients for g = d out [T, H] (g_dtype, as out_dtype above):
+ * grad_rows[row_of_pair[t, j], :] = w[t, j] g[t, :] (zeros without an expert), grad_w[t, j] = g[t] . rows[row] (w_dtype; 0
  * without an expert).  Either may be NULL (rows only serve grad_w, w grad_rows
  * and the dtype). */
 int ftm_combine_tokens_grad(const void* g, int32_t g_dtype, int64_t g_stride, const void* rows, int32_t dtype,

@@ -309,6 +309,24 @@ def test_rows_past_32_bits(gpu):
     assert torch.equal(gw[-9:], sgw) and torch.equal(gr[at], sgr[small.row_of_pair.reshape(-1).long()])
 
 
+def test_more_tokens_than_one_grid_dimension(gpu):
+    """2^24 tokens and more, a workgroup each."""
+    T, H, E = 2**24 + 70, 8, 4
+    ids = (torch.arange(T, device=gpu)[:, None] * 7 // 3) % E
+    sort = sort_tokens(ids, E)
+    x = torch.randn(T, H, generator=torch.Generator(device=gpu).manual_seed(6), device=gpu).to(torch.bfloat16)
+    rows = gather_tokens(x, sort)
+    assert torch.equal(rows, x[sort.token_of_row.long()])
+    w = torch.rand(T, 1, device=gpu)
+    rows.requires_grad_(), w.requires_grad_()
+    out = combine_tokens(rows, w, sort)
+    assert torch.equal(out.detach(), (x.float() * w.detach()).to(torch.bfloat16))
+    gr, gw = torch.autograd.grad(out, (rows, w), x)
+    assert torch.equal(gr, (x.float() * w.detach()).to(torch.bfloat16)[sort.token_of_row.long()])
+    ref = x.double().pow(2).sum(1, keepdim=True)
+    assert ((gw.double() - ref).abs() <= 9 * U * ref).all()
+
+
 def test_gradient_after_the_order_changed(gpu):
     """A write to the order between forward and backward is refused, not used."""
     sort = sort_tokens(routing(8, 2, 4, 3).to(gpu), 4)

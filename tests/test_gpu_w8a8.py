@@ -417,6 +417,34 @@ def test_rows_past_32_bits(gpu, K, N):
     assert torch.equal(w8a8_grouped_linear(q, s, off, w, ws, row_index=idx), ref)
 
 
+@pytest.mark.parametrize("M,K", [(2**24 + 70, 3), (2**24 + 70, 24), (2**20 + 70, 2064)])
+def test_more_rows_than_one_grid_dimension(gpu, M, K):
+    """A workgroup a row, or for four rows, past the threads that one dimension counts."""
+    x = torch.randn(M, K, generator=torch.Generator(device=gpu).manual_seed(5), device=gpu, dtype=torch.bfloat16)
+    q, s = quantize_int8_token(x)
+    at = torch.cat([torch.arange(0, 9), torch.arange(2**20 - 4, 2**20 + 4), torch.arange(M - 80, M)]).to(gpu)
+    rq, rs = exact_quantise(x[at])
+    assert torch.equal(q[at].cpu(), rq) and torch.equal(s[at].cpu(), rs)
+    for N in (2, 260) if K < 30 else (2,):  # 17.8 M items of 16 x 16 the second
+        w, ws = codes((N, K), 3, gpu), scales((N,), 4, gpu)
+        assert torch.equal(w8a8_linear(q, s, w, ws)[at], w8a8_linear(q[at], s[at], w, ws))
+
+
+def test_rows_over_one_another(gpu):
+    """Rows that share memory (expanded, overlapping), and a single row of any stride."""
+    w, ws = codes((40, 64), 3, gpu), scales((40,), 4, gpu)
+    one = torch.randn(1, 64, device=gpu)
+    q, s = quantize_int8_token(one)
+    for M in (3, 70):
+        assert torch.equal(w8a8_linear(q.expand(M, 64), s.expand(M), w, ws), w8a8_linear(q.repeat(M, 1), s.repeat(M), w, ws))
+        assert torch.equal(fused_w8a8_linear(one.expand(M, 64), w, ws), fused_w8a8_linear(one.repeat(M, 1), w, ws))
+    flat = codes((100,), 5, gpu)
+    lap = flat.as_strided((5, 64), (7, 1))
+    assert torch.equal(w8a8_linear(lap, s.repeat(5), w, ws), w8a8_linear(lap.clone(), s.repeat(5), w, ws))
+    odd = flat.as_strided((1, 64), (7, 1))
+    assert torch.equal(w8a8_linear(odd, s, w, ws), w8a8_linear(odd.clone(), s, w, ws))
+
+
 @pytest.mark.parametrize("N", [16384, 16400])
 def test_results_past_32_bits(gpu, N):
     M, K = 2**32 // (2 * N) + 300, 64
