@@ -1161,13 +1161,20 @@ hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
   // 15.5, 512 (2560) 23 / 15.6; 4 of 32 of 2048 x 1536, 8 tokens (1632) 21.8 / 23.9,
   // 32 (1920) 28.9 / 28.9, 64 (2304) 32.3 / 29.3, 256 (4608) 48.5 / 29.4
   if (blocks < 8 * kCUs) return split<1, 2, 4, 2>(c, st);
-  // Mostly one tile an expert: its weights are not kept for another.  The layer of 8
-  // of 128 experts of 2048 x 768, 256 / 512 / 1024 / 2048 tokens 145 / 158 / 213 / 302,
-  // kept 155 / 168 / 209 / 279
-  if (seg <= 48) return tile<1, 4, 2, true, true>(c, st);
-  // 64 / 128 tokens a tile, 2048 tokens over 128 experts (128 rows each) of 2048
-  // x 1536 123 / 142, 4 of 32 (256 rows each) of 2880 x 5760 337 / 283
-  return seg < 192 ? tile<1, 4, 2, true>(c, st) : tile<2, 4, 3, true>(c, st);
+  // Mostly one tile an expert: its weights are not kept for another, where a row's 128
+  // bytes are one line and no neighbour's copy needs the rest.  The layer of 8 of 128
+  // experts of 2048 x 768, 512 / 768 / 1024 tokens (32, 48, 64 rows an expert) 159 / 182 /
+  // 213, kept 169 / 192 / 208; of 4 of 32 of 2880 x 2880, 384 tokens 253 / 230
+  if (seg <= 48 && c.K % 128 == 0 && ((uintptr_t)c.w & 127u) == 0) return tile<1, 4, 2, true, true>(c, st);
+  // 64 / 128 tokens a tile: five of the first take the time of three of the second;
+  // an expert with an eighth more rows than the mean decides.  The same layers, 48 rows
+  // an expert 230 / 236, 64 208 / 198 and 298 / 245, 80 230 / 207, 96 243 / 220 and 307 /
+  // 263, 256 461 / 431 and 528 / 502, but 128 (one of 128 and a few rows more for half of
+  // the experts), down products alone 86 / 93; with fewer of them than CUs, 2 of 16 of
+  // 1024 x 512, 64 rows 41 / 45
+  const int64_t n = seg + seg / 8, n64 = (n + 63) / 64, n128 = (n + 127) / 128;
+  if (5 * n128 <= 3 * n64 && hit * n128 * ((c.N + 255) / 256) >= kCUs) return tile<2, 4, 3, true>(c, st);
+  return tile<1, 4, 2, true>(c, st);
 }
 
 }  // namespace

@@ -325,7 +325,8 @@ GROUPS = {
 
 
 @pytest.mark.parametrize("name", sorted(GROUPS))
-@pytest.mark.parametrize("K,N", [(64, 48), (272, 33), (256, 300), (40, 10), (384, 2100), (176, 1900)])
+@pytest.mark.parametrize("K,N", [(64, 48), (272, 33), (256, 300), (40, 10), (384, 2100), (176, 1900), (384, 7300),
+                                 (144, 7300)])
 @pytest.mark.parametrize("act", [None, "silu"])
 def test_grouped(gpu, name, K, N, act):
     """Every expert's rows are the dense product's bits, the rows of no expert zeros; packed
