@@ -760,9 +760,9 @@ template <int WM, int MI, int S, bool PACKED, bool ACT, bool TAIL, bool GROUPED,
 __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtiles, int ntiles) {
   constexpr int BM = 16 * MI * WM;
   constexpr int kX = BM * kRow, kStage = kX + 256 * kRow;
-  constexpr int NX = BM / 8 / (4 * WM), NB = 32 / (4 * WM);  // 1 KiB copies a wave and step: tokens, weights
+  constexpr int NX = (BM / 8 + 4 * WM - 1) / (4 * WM), NB = 32 / (4 * WM);  // 1 KiB copies a wave and step: tokens, weights
   constexpr int kCols = ACT ? 128 : 256;                     // output channels of the tile
-  constexpr int kAhead = 3;                                  // row blocks read ahead of their products
+  constexpr int kAhead = MI % 5 == 0 ? 4 : 3;                // row blocks read ahead of their products
   static_assert(2 * MI % (kAhead + 1) == 0, "a step leaves its row blocks where it found them");
   static_assert(kAhead <= MI && MI >= 4, "the next step's first weights take registers that are done");
   extern __shared__ char lds[];
@@ -808,11 +808,15 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
     Rsrc xres, wres;
     uint32_t xoff[NX], woff[NB];
     int ix[NX];  // rows of x that the copies read
+    auto xblock = [&](int i) __attribute__((always_inline)) {  // the waves' last may copy the last again
+      const int b = wave * NX + i;
+      return b < BM / 8 ? b : BM / 8 - 1;
+    };
     auto copy_rows = [&](const Tile& t) __attribute__((always_inline)) {
       const int lane = opaque_lane();
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
-        const int r = 8 * (wave * NX + i) + (lane >> 3), in = r < t.rt.cnt ? r : 0;
+        const int r = 8 * xblock(i) + (lane >> 3), in = r < t.rt.cnt ? r : 0;
         ix[i] = indexed ? c.row_index[t.rt.row0 + in] : in;
       }
     };
@@ -822,7 +826,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
                        (uint32_t)((indexed ? c.x_rows - 1 : (int64_t)t.rt.cnt - 1) * c.x_stride + K));
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
-        const int r = 8 * (wave * NX + i) + (lane >> 3);
+        const int r = 8 * xblock(i) + (lane >> 3);
         const bool ok = !indexed || (ix[i] >= 0 && ix[i] < c.x_rows);
         xoff[i] = (uint32_t)((ok ? ix[i] : 0) * c.x_stride) + 16u * (uint32_t)((lane & 7) ^ swz(r));
       }
@@ -846,7 +850,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
       char* st = lds + slot * kStage;
 #pragma unroll
       for (int i = 0; i < NX; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * (wave * NX + i)), 16, (int)(xoff[i] + k0), 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * xblock(i)), 16, (int)(xoff[i] + k0), 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + i)), 16, (int)(woff[i] + k0), 0, 0,
@@ -1166,14 +1170,20 @@ hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
   // experts of 2048 x 768, 512 / 768 / 1024 tokens (32, 48, 64 rows an expert) 159 / 182 /
   // 213, kept 169 / 192 / 208; of 4 of 32 of 2880 x 2880, 384 tokens 253 / 230
   if (seg <= 48 && c.K % 128 == 0 && ((uintptr_t)c.w & 127u) == 0) return tile<1, 4, 2, true, true>(c, st);
-  // 64 / 128 tokens a tile: five of the first take the time of three of the second;
-  // an expert with an eighth more rows than the mean decides.  The same layers, 48 rows
-  // an expert 230 / 236, 64 208 / 198 and 298 / 245, 80 230 / 207, 96 243 / 220 and 307 /
-  // 263, 256 461 / 431 and 528 / 502, but 128 (one of 128 and a few rows more for half of
-  // the experts), down products alone 86 / 93; with fewer of them than CUs, 2 of 16 of
+  // 64, 128 or 160 tokens a tile: tiles for experts of a fifth less to a fifth more
+  // rows than the mean, times that of one tile (16, 20 and 23).  The same layers, 64
+  // / 128 / 160 tokens: 64 rows an expert 212 / 200 / 209, 96 239 / 220 / 227 and 305 / 262
+  // / 269, 128 281 / 283 / 272 and 348 / 344 / 287, 188 346 / 342 / 363, 256 451 / 420 /
+  // 404 and 524 / 495 / 439; 48 230 / 236; with fewer tiles than CUs, 2 of 16 of
   // 1024 x 512, 64 rows 41 / 45
-  const int64_t n = seg + seg / 8, n64 = (n + 63) / 64, n128 = (n + 127) / 128;
-  if (5 * n128 <= 3 * n64 && hit * n128 * ((c.N + 255) / 256) >= kCUs) return tile<2, 4, 3, true>(c, st);
+  auto time = [&](int64_t rows, int64_t unit) {
+    int64_t n = 0;
+    for (int i = -3; i <= 3; i += 2) n += (seg + i * seg / 15 + rows - 1) / rows;
+    return n * unit;
+  };
+  const int64_t t64 = time(64, 16), t128 = time(128, 20), t160 = time(160, 23), nt = (c.N + 255) / 256;
+  if (t160 < t128 && t160 < t64 && hit * ((seg + 159) / 160) * nt >= kCUs) return tile<2, 5, 3, true>(c, st);
+  if (t128 < t64 && hit * ((seg + 127) / 128) * nt >= kCUs) return tile<2, 4, 3, true>(c, st);
   return tile<1, 4, 2, true>(c, st);
 }
 

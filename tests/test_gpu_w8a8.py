@@ -321,6 +321,7 @@ GROUPS = {
     "many": ([(7 * i) % 5 for i in range(512)], 2),
     "full": ([64] * 9, 0),
     "large": ([400, 3, 700, 256], 130),
+    "about_128": ([128, 140, 117, 96, 161, 130, 160, 129, 127], 5),
 }
 
 
