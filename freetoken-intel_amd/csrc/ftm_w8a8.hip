@@ -1170,20 +1170,15 @@ hipError_t grouped(const ftm_w8a8& c, hipStream_t st) {
   // experts of 2048 x 768, 512 / 768 / 1024 tokens (32, 48, 64 rows an expert) 159 / 182 /
   // 213, kept 169 / 192 / 208; of 4 of 32 of 2880 x 2880, 384 tokens 253 / 230
   if (seg <= 48 && c.K % 128 == 0 && ((uintptr_t)c.w & 127u) == 0) return tile<1, 4, 2, true, true>(c, st);
-  // 64, 128 or 160 tokens a tile: tiles for experts of a fifth less to a fifth more
-  // rows than the mean, times that of one tile (16, 20 and 23).  The same layers, 64
-  // / 128 / 160 tokens: 64 rows an expert 212 / 200 / 209, 96 239 / 220 / 227 and 305 / 262
-  // / 269, 128 281 / 283 / 272 and 348 / 344 / 287, 188 346 / 342 / 363, 256 451 / 420 /
-  // 404 and 524 / 495 / 439; 48 230 / 236; with fewer tiles than CUs, 2 of 16 of
-  // 1024 x 512, 64 rows 41 / 45
-  auto time = [&](int64_t rows, int64_t unit) {
-    int64_t n = 0;
-    for (int i = -3; i <= 3; i += 2) n += (seg + i * seg / 15 + rows - 1) / rows;
-    return n * unit;
-  };
-  const int64_t t64 = time(64, 16), t128 = time(128, 20), t160 = time(160, 23), nt = (c.N + 255) / 256;
-  if (t160 < t128 && t160 < t64 && hit * ((seg + 159) / 160) * nt >= kCUs) return tile<2, 5, 3, true>(c, st);
-  if (t128 < t64 && hit * ((seg + 127) / 128) * nt >= kCUs) return tile<2, 4, 3, true>(c, st);
+  // 64, 128 or 160 tokens a tile, the layers above: 64 rows an expert 212 / 200 / 209, 96
+  // 239 / 220 / 227 and 305 / 262 / 269, 188 346 / 342 / 363, 256 451 / 420 / 404 and 524 /
+  // 495 / 439, 1024 1467 / 1337 / 1306; 48 230 / 236; with fewer tiles than CUs, 2 of
+  // 16 of 1024 x 512, 64 rows 41 / 45.  Five tiles of 64 take the time of three of 128,
+  // for an expert with an eighth more rows than the mean; around 128 rows evenly routed
+  // 281 / 283 / 272, but 278 / 280 / 292 where the experts' rows differ more
+  const int64_t n = seg + seg / 8, n64 = (n + 63) / 64, n128 = (n + 127) / 128, nt = (c.N + 255) / 256;
+  if (seg >= 200 && hit * ((seg + 159) / 160) * nt >= kCUs) return tile<2, 5, 3, true>(c, st);
+  if (5 * n128 <= 3 * n64 && hit * n128 * nt >= kCUs) return tile<2, 4, 3, true>(c, st);
   return tile<1, 4, 2, true>(c, st);
 }
 
