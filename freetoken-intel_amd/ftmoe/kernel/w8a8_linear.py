@@ -130,8 +130,10 @@ def _product(x, x_scale, weight, weight_scale, *, bias, out_dtype, offsets=None,
         return out.zero_()
     if x_scale is None:  # codes, then the scales on a 4-byte border
         at = (M * K + 3) // 4 * 4
-        scratch = torch.empty(at + 4 * M, dtype=torch.uint8, device=x.device).data_ptr()
-        q, s, stride = scratch, scratch + at, K
+        # held until the native call has enqueued its kernels: what is freed earlier another
+        # thread may be given, and write, between the quantiser and the product
+        scratch = torch.empty(at + 4 * M, dtype=torch.uint8, device=x.device)
+        q, s, stride = scratch.data_ptr(), scratch.data_ptr() + at, K
     else:
         x = x if row_stride(x) >= K else x.contiguous()  # rows over one another
         q, s, stride = x.data_ptr(), x_scale.data_ptr(), row_stride(x)

@@ -2,6 +2,7 @@
 points check their arguments before they touch the HIP runtime, and the Python
 functions take no CPU tensor."""
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -166,3 +167,37 @@ def test_no_cpu_fallback():
                  lambda: combine_tokens(torch.zeros(8, 64), None, sort)):
         with pytest.raises(RuntimeError, match="ROCm device tensor"):
             call()
+
+
+# ------------------------------------------------------------------ what a call keeps and passes on
+def _record_calls(monkeypatch, run):
+    """The Python functions on CPU tensors, with ``run(args)`` in the place of the native call."""
+    monkeypatch.setattr(nat, "require_gpu", lambda t, name: None)
+    monkeypatch.setattr(nat, "launch", lambda what, fn, t, *args: run(args))
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_scratch_lives_until_the_native_call_has_returned(monkeypatch, M):
+    """The codes' and scales' scratch belongs to a tensor that is still held while the library
+    enqueues its kernels: memory given back before could be another thread's by then."""
+    made, calls = [], []
+    empty = torch.empty
+
+    def remembered(*a, **kw):
+        t = empty(*a, **kw)
+        made.append(weakref.ref(t))
+        return t
+
+    def run(args):
+        c = args[-1]._obj
+        for at, n in ((c.x, c.x_rows * c.K), (c.x_scale, 4 * c.x_rows)):
+            live = [t for t in (r() for r in made) if t is not None]
+            assert any(t.data_ptr() <= at and at + n <= t.data_ptr() + t.numel() * t.element_size() for t in live)
+        calls.append(c.K)
+
+    _record_calls(monkeypatch, run)
+    monkeypatch.setattr(torch, "empty", remembered)
+    x, w, s = torch.zeros(M, 64), torch.zeros(32, 64, dtype=torch.int8), torch.ones(32)
+    fused_w8a8_linear(x, w, s)
+    fused_w8a8_expert_forward(x, w, s, w[:, :16], s, intermediate=16)
+    assert calls == [64, 64, 16]
