@@ -1,6 +1,6 @@
 """(token, expert) pairs sorted by expert, tokens copied into that order, and
-rows back in token order with their router weights -- with gradients, so a
-trained router or trained experts can stand between the two.
+rows back in token order with their router weights -- with gradients (reverse
+mode), so a trained router or trained experts can stand between the two.
 
 The grouping that the layer kernels do inside
 (python/freetoken/kernel/triton/fused_moe.py:106-161), as operators: a stable
@@ -12,6 +12,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
@@ -100,12 +101,21 @@ def _combine(rows: torch.Tensor, w: Optional[torch.Tensor], sort: TokenSort, out
     return out
 
 
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """The kernels know nothing of forward mode: a tangent would be dropped."""
+    for t in tensors:
+        if t is not None and fwAD.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("gather_tokens and combine_tokens have no forward-mode derivative")
+
+
 def _first_only(backward):
-    """``backward``, refusing a second derivative; the wrapper that refuses it costs more
-    than a small backward itself, so it is passed only where one may follow."""
+    """``backward``, refusing a second derivative, in forward mode too; the wrapper that
+    refuses one in reverse mode costs more than a small backward itself, so it is passed
+    only where one may follow."""
     once = once_differentiable(backward)
 
     def run(ctx, g):
+        _refuse_tangents(g)
         return once(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
 
     return run
@@ -151,16 +161,22 @@ class _Combine(torch.autograd.Function):
         return grad_rows, grad_w, None, None
 
 
+def _recorded(*inputs: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to see the call."""
+    _refuse_tangents(*inputs)
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+
+
 def gather_tokens(x: torch.Tensor, sort: TokenSort) -> torch.Tensor:
     """``x [T, H]`` -> ``[T k, H]``: row r is token ``sort.token_of_row[r]``, zeros where
-    that is -1.  Any dtype of 1, 2 or 4 bytes; differentiable in x (fp32, fp16, bf16): a
-    token's gradient is the sum of its rows', in fp32, rounded once."""
+    that is -1.  Any dtype of 1, 2 or 4 bytes; differentiable in x (fp32, fp16, bf16; in
+    reverse mode, once): a token's gradient is the sum of its rows', in fp32, rounded once."""
     _check_sort(sort, x, "x")
     if x.dim() != 2 or x.shape[0] != sort.row_of_pair.shape[0]:
         raise ValueError(f"x must be [{sort.row_of_pair.shape[0]}, H], got {tuple(x.shape)}")
     if x.element_size() not in (1, 2, 4):
         raise TypeError(f"x must have elements of 1, 2 or 4 bytes, got {x.dtype}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _recorded(x):
         nat.dtype_code(x.dtype)
         return _Gather.apply(x, sort)
     return _gather(x, sort)
@@ -172,8 +188,8 @@ def combine_tokens(rows: torch.Tensor, topk_w: Optional[torch.Tensor], sort: Tok
     times the row of pair (t, j), pairs without an expert left out (their rows are not
     read); fp32 sums in order of j, rounded once.  ``rows`` and ``topk_w [T, k]`` in
     fp32, fp16 or bf16 (``topk_w`` None: ones), ``out_dtype`` the rows' (the default) or,
-    from fp32 rows, any of the three.  Differentiable in both: rows of no expert get zero
-    gradients, and so do their weights."""
+    from fp32 rows, any of the three.  Differentiable in both (in reverse mode, once): rows
+    of no expert get zero gradients, and so do their weights."""
     _check_sort(sort, rows, "rows")
     T, k = sort.row_of_pair.shape
     nat.dtype_code(rows.dtype)
@@ -188,7 +204,7 @@ def combine_tokens(rows: torch.Tensor, topk_w: Optional[torch.Tensor], sort: Tok
         nat.require_same_device(rows, (("topk_w", topk_w),))
         if tuple(topk_w.shape) != (T, k):
             raise ValueError(f"topk_w must be [{T}, {k}], got {tuple(topk_w.shape)}")
-    if torch.is_grad_enabled() and (rows.requires_grad or (topk_w is not None and topk_w.requires_grad)):
+    if _recorded(rows, topk_w):
         if topk_w is None:
             topk_w = torch.ones((T, k), dtype=torch.float32, device=rows.device)
         return _Combine.apply(rows, topk_w, sort, out_dtype)

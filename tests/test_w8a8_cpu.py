@@ -6,6 +6,7 @@ import weakref
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from ftmoe import _native as nat
 from ftmoe.kernel.fused_w8a8_linear import fused_w8a8_expert_forward, fused_w8a8_linear
@@ -201,3 +202,43 @@ def test_scratch_lives_until_the_native_call_has_returned(monkeypatch, M):
     fused_w8a8_linear(x, w, s)
     fused_w8a8_expert_forward(x, w, s, w[:, :16], s, intermediate=16)
     assert calls == [64, 64, 16]
+
+
+def _token_order(T=4, k=2):
+    ids = torch.arange(T * k, dtype=torch.int32).reshape(T, k)
+    return TokenSort(2, torch.tensor([0, T * k, T * k], dtype=torch.int32), ids, ids.reshape(-1), ids.reshape(-1) // k)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused(monkeypatch, grad_mode):
+    """A tangent is not dropped without a word (its derivative would be taken for zero): of the
+    tokens, of the rows, of the weights; an input without one passes."""
+    calls = []
+    _record_calls(monkeypatch, calls.append)
+    sort, x, rows, w = _token_order(), torch.randn(4, 8), torch.randn(8, 8), torch.rand(4, 2)
+    with fwAD.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = [fwAD.make_dual(t, torch.ones_like(t)) for t in (x, rows, w)]
+        for call in (lambda: gather_tokens(dual[0], sort), lambda: combine_tokens(dual[1], w, sort),
+                     lambda: combine_tokens(rows, dual[2], sort), lambda: combine_tokens(dual[1], None, sort)):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+        assert not calls
+        gather_tokens(x, sort), combine_tokens(rows, w, sort), combine_tokens(rows, None, sort)
+        assert len(calls) == 3
+
+
+def test_forward_mode_derivatives_of_gradients_are_refused(monkeypatch):
+    """A tangent of the upstream gradient, while the inputs have none."""
+    calls = []
+    _record_calls(monkeypatch, calls.append)
+    sort = _token_order()
+    x, rows, w = torch.randn(4, 8).requires_grad_(), torch.randn(8, 8).requires_grad_(), torch.rand(4, 2)
+    for out, leaf in ((gather_tokens(x, sort), x), (combine_tokens(rows, w, sort), rows)):
+        done = len(calls)
+        with fwAD.dual_level():
+            g = fwAD.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(out, leaf, g, retain_graph=True)
+        assert len(calls) == done
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
+        assert len(calls) == done + 1
