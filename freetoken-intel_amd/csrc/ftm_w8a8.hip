@@ -408,6 +408,14 @@ struct RowOut {
   }
 };
 
+// act(gate) up.  A NaN in either (the scale of its token or channel is one) is the
+// result; the clamps of act_fn would replace it by their limit.
+__device__ __forceinline__ float gated(int act, float g, float u, const ftm_w8a8& c) {
+  const float y = act_fn(act, g, u, c.act_alpha, c.act_limit);
+  if (act != FTM_ACT_RELU && act != FTM_ACT_SWIGLU_OAI) return y;
+  return __builtin_isunordered(g, u) ? __uint_as_float(0x7fc00000u) : y;
+}
+
 // f(activation) with the selection outside the loops (-1: none).
 template <class F>
 __device__ __forceinline__ void with_act(int act, F&& f) {
@@ -480,7 +488,7 @@ __device__ __forceinline__ void split_finish(const ftm_w8a8& c, const RowTile& r
       for (int r = 0; r < 4; ++r) {
         y[r] = scaled(u[r], k.xscale, channel(c, {k.t[r], k.b[r]}));
         if constexpr (A >= 0)
-          y[r] = act_fn(A, y[r], scaled(v[r], k.xscale, channel(c, {k.t[4 + r], k.b[4 + r]})), c.act_alpha, c.act_limit);
+          y[r] = gated(A, y[r], scaled(v[r], k.xscale, channel(c, {k.t[4 + r], k.b[4 + r]})), c);
         y[r] = k.live ? y[r] : 0.0f;
       }
       RowOut<4>(c, rt, out_cols(c), split_channel<NT>(c, n0, f, g)).store(16 * (f / NT) + m, y);
@@ -969,8 +977,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_w8a8_tile(ftm_w8a8 c, int mtile
             for (int n = 0; n < CN; ++n) {
               y[n] = scaled(acc[i][n][r], xs[i][r], ch[n]);
               if constexpr (ACT)
-                y[n] = act_fn(decltype(a)::value, y[n], scaled(acc[i][2 + n][r], xs[i][r], ch[2 + n]), c.act_alpha,
-                              c.act_limit);
+                y[n] = gated(decltype(a)::value, y[n], scaled(acc[i][2 + n][r], xs[i][r], ch[2 + n]), c);
               y[n] = live ? y[n] : 0.0f;
             }
             out.store(t0 + 16 * i + r, y);
@@ -1032,7 +1039,7 @@ __device__ __forceinline__ void any_item(const ftm_w8a8& c, int mt, int nt) {
   if (src >= 0) {
     const float s = c.x_scale[src];
     y = scaled(a, s, channel(c, rt.e, n0 + col));
-    if (act) y = act_fn(c.act, y, scaled(b, s, channel(c, rt.e, NO + n0 + col)), c.act_alpha, c.act_limit);
+    if (act) y = gated(c.act, y, scaled(b, s, channel(c, rt.e, NO + n0 + col)), c);
   }
   store_scalar(c.out, orow * NO + n0 + col, c.out_dtype, y);
 }
