@@ -1147,8 +1147,21 @@ hipError_t dense(const ftm_w8a8& c, hipStream_t st) {
   // rows of 4096 x 4096 5.8 / 7.2, of 4096 x 12288 16.3 / 14.8
   if (M <= 16) return blocks <= 2 * kCUs ? split<1, 1, 4, 4>(c, st) : split<1, 1, 4, 2>(c, st);
   if (M <= 32) return blocks <= 2 * kCUs ? split<2, 1, 4, 3>(c, st) : split<2, 2, 4, 2>(c, st);
-  if (c.row_index != nullptr) return split<4, 4, 4, 2>(c, st);  // the tiles of a dense product take rows in order
   hipError_t e = hipSuccess;
+  if (c.row_index != nullptr) {
+    // Through an index (a C call only; the tiles of a dense product take rows in order):
+    // 64 x 64 split tiles, as many rows a launch as one grid dimension counts
+    const int cols = out_cols(c), esz = c.out_dtype == FTM_DT_F32 ? 4 : 2, wide = c.act >= 0 ? 32 : 64;
+    const int64_t at_once = (int64_t)(kMaxGroups / ((cols + wide - 1) / wide)) * 64;
+    for (int64_t row = 0; row < M && e == hipSuccess; row += at_once) {
+      ftm_w8a8 part = c;
+      part.rows = M - row < at_once ? M - row : at_once;
+      part.row_index = c.row_index + row;
+      part.out = (char*)c.out + row * cols * esz;
+      e = split<4, 4, 4, 2>(part, st);
+    }
+    return e;
+  }
   if (split64(c, (M + 63) / 64, st, e)) return e;
   // The largest tile reads its operands least often, but a launch takes whole
   // rounds of them: rounds x the time of one, in that of a 256-token tile (1;

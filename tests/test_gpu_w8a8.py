@@ -281,6 +281,23 @@ def test_linear_row_index(gpu, M, K):
     assert torch.equal(out, ref)
 
 
+def test_linear_row_index_past_one_grid_dimension(gpu):
+    """More tiles than workgroups that one grid dimension counts, through an index without experts."""
+    R, K, N, M = 70, 16, 1, (2**24 - 1) * 64 + 100
+    q, s, w, ws = codes((R, K), 1, gpu), scales((R,), 2, gpu), codes((N, K), 3, gpu), scales((N,), 4, gpu)
+    idx = torch.arange(M, device=gpu, dtype=torch.int32).remainder_(R)
+    idx[-1] = -1
+    out = torch.full((M, N), 7.0, device=gpu, dtype=torch.bfloat16)
+    c = nat.FtmW8A8(q.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), None, idx.data_ptr(),
+                    M, R, K, 0, N, K, 1, 0, nat.DT_F32, 0, nat.DT_BF16, -1, 0.0, 0.0)
+    nat.launch("ftm_w8a8_linear", nat.lib().ftm_w8a8_linear, q, ctypes.byref(c))
+    ref = w8a8_linear(q, s, w, ws)
+    assert out[-1] == 0
+    for at in range(0, M - 1, 2**27):
+        part = slice(at, min(at + 2**27, M - 1))
+        assert torch.equal(out[part], ref[idx[part]])
+
+
 def test_linear_empty_and_refused(gpu):
     q, s, w, ws = codes((4, 64), 1, gpu), scales((4,), 2, gpu), codes((32, 64), 3, gpu), scales((32,), 4, gpu)
     assert w8a8_linear(q[:0], s[:0], w, ws).shape == (0, 32)
