@@ -414,3 +414,32 @@ def test_forward_and_backward_in_a_graph(gpu):
         torch.cuda.synchronize()
         eager = step()
         assert all(torch.equal(a, b) for a, b in zip(captured, eager)), seed
+
+
+# ------------------------------------------------------------------ many pairs
+@pytest.mark.parametrize("T,k,E", [(131072 + 9, 8, 60), (300000, 8, 1), (300000, 7, 511), (2**20 + 5, 8, 512)])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_sort_of_many_workgroups(gpu, T, k, E, dtype):
+    """More workgroups than read one another's counts."""
+    ids = routing(T, k, E, T + k, lo=-1, dtype=dtype)
+    check_sort(sort_tokens(ids.to(gpu), E), ids, E)
+
+
+def test_sort_time_is_proportional_to_the_pairs(gpu):
+    """Eight times the pairs of 4 M take about eight times as long (a cost for every two
+    workgroups would take 64 times): 24 leaves room for what the smaller one's caches gain."""
+    E, times = 64, []
+    for T in (2**19, 2**22):
+        ids = torch.arange(T * 8, device=gpu, dtype=torch.int32).reshape(T, 8).remainder_(E)
+        sort_tokens(ids, E)
+        best = math.inf
+        for _ in range(5):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            start.record()
+            sort_tokens(ids, E)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        times.append(best)
+    assert times[1] < 24 * times[0], times
