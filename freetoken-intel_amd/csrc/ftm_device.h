@@ -207,7 +207,6 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
   return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
 }
 
-// Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
 // A workgroup a row.  A launch counts the threads of one grid dimension in 32 bits,
 // so more than 2^20 rows go on in y; the last of those may be past the rows.
 inline dim3 row_grid(int64_t rows) {
@@ -216,6 +215,7 @@ inline dim3 row_grid(int64_t rows) {
 }
 __device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
+// Inclusive prefix sum over the wave: shifts by 1, 2, 4 and 8 inside each 16
 // lanes (DPP row_shr, zeros shifted in), then the rows before.
 __device__ __forceinline__ int wave_prefix_sum(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);

@@ -12,8 +12,11 @@
 //
 // Operands of v_mfma_i32_16x16x64_i8 (lane l): A[i][k] i = l % 16, B[k][j] j =
 // l % 16, both k = 16 (l / 16) + 0..15; D[i][j] j = l % 16, i = 4 (l / 16) +
-// 0..3.  The weights are A and the tokens B, so a lane's results are
-// neighbouring output channels of one token.
+// 0..3.  Where K is split over the waves the weights are A and the tokens B, so a
+// lane's results are neighbouring output channels of one token; in the LDS tiles
+// the tokens are A and the weights B, so a lane has four tokens of one channel a
+// block, and the order in which the weight rows are laid into LDS makes the
+// channels of its blocks neighbours.
 #include <type_traits>
 
 #include "ftm_layer.h"
@@ -356,8 +359,11 @@ __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 typedef __attribute__((address_space(3))) void* LPtr;
 
 // Cache policy of what a kernel does not read again: nothing keeps it.  Results stored
-// so leave the weights in the last cache: 2048 tokens over 8 of 128 experts of 768 x
-// 2048 (201 MB) again and again 67 us, kept 84; with cold weights 86 / 88.
+// so leave their place in the last cache to the weights.  Past / kept, four sets of
+// inputs in turn (none is in a cache): 4096 x 4096 x 12288 190 / 193 us, grouped down of
+// 2048 tokens of 8 of 128 experts of 768 x 2048 87 / 88, gate_up to fp32 129 / 133; one set
+// again and again: down 66 / 77.  In the expert layer the next kernel reads the results:
+// 512 tokens 172 / 175, but 2048 277 / 274, and of 4 of 32 of 2880 x 2880 467 / 460.
 constexpr int kNT = 2;
 
 // The results of a row tile: N = 4 or 2 neighbouring channels from n0 on of one row

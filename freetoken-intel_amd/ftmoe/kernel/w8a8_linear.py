@@ -8,7 +8,8 @@ same codes and scales, either plain int8 ``[N, K]``
 
 gfx950: int32 sums on the int8 matrix cores, exact for K up to 131071, so a
 result does not depend on the batch it is computed in; scales, bias and the
-gated activation are applied in fp32 in the same kernel and rounded once."""
+gated activation are applied in fp32 in the same kernel and rounded once.  For
+inference, like the other fused projections: autograd does not see the calls."""
 from __future__ import annotations
 
 import ctypes

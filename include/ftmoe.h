@@ -279,7 +279,7 @@ int ftm_quant_int8(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int6
 /* One product: out[m, n] = (sum_k x[i, k] w[n, k]) * x_scale[i] * w_scale[n]
  * (+ bias[n]), i = m or row_index[m], the sum exact in int32 (K <= 131071), one
  * rounding to out_dtype.  With act >= 0 the weight rows [0, N/2) are gate and
- * [N/2, N) up and out[m, n] = act(gate) * up, n < N/2.
+ * [N/2, N) up and out[m, n] = act(gate) * up, n < N/2 (NaN where either is).
  * Grouped (offsets not NULL): rows [offsets[e], offsets[e+1]) take weight e;
  * the other rows, and rows whose row_index names no row of x, become zeros. */
 typedef struct ftm_w8a8 {
