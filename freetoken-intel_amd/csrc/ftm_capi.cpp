@@ -242,6 +242,60 @@ W8a8MoeLayout w8a8_moe_layout(int T, int k, int E, int H, int I) {
   return w;
 }
 
+int check_w4a4(const ftm_w4a4* call) {
+  if (call == nullptr) return FTM_ERR_NULL;
+  const ftm_w4a4& c = *call;
+  if (c.K <= 0 || c.K % 32 != 0 || c.K > FTM_W4A4_MAX_K || c.N <= 0 || c.rows < 0 || c.rows > INT32_MAX ||
+      c.x_rows < 0 || c.x_rows > INT32_MAX || c.w_stride < 0 || c.w_scale_stride < 0)
+    return FTM_ERR_DIM;
+  if (!dt_ok(c.out_dtype) || (c.bias != nullptr && !dt_ok(c.bias_dtype))) return FTM_ERR_FORMAT;
+  if (c.act < -1 || c.act > FTM_ACT_SWIGLU_OAI) return FTM_ERR_FORMAT;
+  if (c.act >= 0 && c.N % 2 != 0) return FTM_ERR_DIM;
+  if (c.num_experts < 1 || c.num_experts > kMaxExperts || (c.offsets == nullptr && c.num_experts != 1))
+    return FTM_ERR_DIM;
+  if (c.num_experts > 1 && (c.w_stride < (int64_t)c.N * (c.K / 2) || c.w_scale_stride < (int64_t)c.N * (c.K / 32)))
+    return FTM_ERR_DIM;
+  if (c.rows == 0) return FTM_OK;
+  if (c.out == nullptr || c.w == nullptr || c.w_scale == nullptr) return FTM_ERR_NULL;
+  // without an index every row of the output is one of x
+  if (c.row_index == nullptr && c.x_rows < c.rows) return FTM_ERR_DIM;
+  if (c.x_rows == 0) return FTM_ERR_DIM;
+  if (c.x == nullptr || c.x_scale == nullptr) return FTM_ERR_NULL;
+  if ((((uintptr_t)c.x | (uintptr_t)c.w | (uint64_t)(c.num_experts > 1 ? c.w_stride : 0)) & 15u) != 0) return FTM_ERR_ALIGN;
+  if ((uintptr_t)c.out % dt_bytes(c.out_dtype) != 0 || (c.bias != nullptr && (uintptr_t)c.bias % dt_bytes(c.bias_dtype) != 0))
+    return FTM_ERR_ALIGN;
+  if ((((uintptr_t)c.offsets | (uintptr_t)c.row_index) & 3u) != 0) return FTM_ERR_ALIGN;
+  return FTM_OK;
+}
+
+// Workspace of ftm_w4a4_moe_forward.
+struct W4a4MoeLayout {
+  size_t offsets, row_of_pair, pair_of_row, token_of_row, xq, xs, hq, hs, h, y, sort, total;
+};
+W4a4MoeLayout w4a4_moe_layout(int T, int k, int E, int H, int I) {
+  W4a4MoeLayout w;
+  const size_t P = (size_t)T * k;
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o = align_up(o + bytes, 256);
+    return at;
+  };
+  w.offsets = take(4 * (size_t)(E + 1));
+  w.row_of_pair = take(4 * P);
+  w.pair_of_row = take(4 * P);
+  w.token_of_row = take(4 * P);
+  w.xq = take((size_t)T * (H / 2));
+  w.xs = take((size_t)T * (H / 32));
+  w.hq = take(P * (I / 2));
+  w.hs = take(P * (I / 32));
+  w.h = take(4 * P * I);
+  w.y = take(4 * P * H);
+  w.sort = take(sort_workspace_bytes((int64_t)P, E));
+  w.total = o;
+  return w;
+}
+
 int hip_rc(hipError_t e) { return e == hipSuccess ? FTM_OK : FTM_ERR_HIP; }
 
 }  // namespace
@@ -549,6 +603,82 @@ int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_by
                        L.total - L.sort, stream);
   if (rc == FTM_OK) rc = ftm_w8a8_linear_dynamic(c.x, c.dtype, c.x_stride, &a, stream);
   if (rc == FTM_OK) rc = ftm_w8a8_linear_dynamic(h, FTM_DT_F32, (int64_t)I * 4, &b, stream);
+  if (rc == FTM_OK)
+    rc = ftm_combine_tokens(y, FTM_DT_F32, (int64_t)H * 4, c.topk_w, c.topk_w_dtype, row_of_pair, T, k, H, c.out, c.dtype,
+                            stream);
+  return rc;
+}
+
+int ftm_quant_mxfp4(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride, uint8_t* blocks,
+                    uint8_t* scales, void* stream) {
+  if (!dt_ok(x_dtype)) return FTM_ERR_FORMAT;
+  if (rows < 0 || rows > INT32_MAX || K <= 0 || K % 32 != 0 || x_stride < 0) return FTM_ERR_DIM;
+  if (rows == 0) return FTM_OK;
+  if (x == nullptr || blocks == nullptr || scales == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)x | (uint64_t)x_stride) % dt_bytes(x_dtype) != 0 || ((uintptr_t)blocks & 3u) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_quant_mxfp4(x, x_dtype, rows, K, x_stride, blocks, scales, (hipStream_t)stream));
+}
+
+int ftm_w4a4_linear(const ftm_w4a4* call, void* stream) {
+  const int rc = check_w4a4(call);
+  if (rc != FTM_OK || call->rows == 0) return rc;
+  return hip_rc(launch_w4a4(*call, (hipStream_t)stream));
+}
+
+int ftm_w4a4_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w4a4* call, void* stream) {
+  const int rc = check_w4a4(call);
+  if (rc != FTM_OK) return rc;
+  if (!dt_ok(x_dtype)) return FTM_ERR_FORMAT;
+  if (x_stride < 0) return FTM_ERR_DIM;
+  if (call->rows == 0) return FTM_OK;
+  if (x == nullptr) return FTM_ERR_NULL;
+  if (((uintptr_t)x | (uint64_t)x_stride) % dt_bytes(x_dtype) != 0) return FTM_ERR_ALIGN;
+  return hip_rc(launch_w4a4_dynamic(*call, x, x_dtype, x_stride, (hipStream_t)stream));
+}
+
+size_t ftm_w4a4_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter) {
+  if (T <= 0 || k <= 0 || num_experts <= 0 || num_experts > kMaxExperts || hidden <= 0 || inter <= 0) return 0;
+  return w4a4_moe_layout(T, k, num_experts, hidden, inter).total;
+}
+
+int ftm_w4a4_moe_forward(const ftm_w4a4_moe* call, void* workspace, size_t ws_bytes, void* stream) {
+  if (call == nullptr) return FTM_ERR_NULL;
+  const ftm_w4a4_moe& c = *call;
+  const int T = c.T, k = c.k, E = c.num_experts, H = c.hidden, I = c.inter;
+  if (T < 0 || k <= 0 || E <= 0 || E > kMaxExperts || H <= 0 || I <= 0 || I > FTM_W4A4_MAX_K || H > FTM_W4A4_MAX_K ||
+      H % 32 != 0 || I % 32 != 0 || (int64_t)T * k >= INT32_MAX || c.x_stride < 0)
+    return FTM_ERR_DIM;
+  if (!dt_ok(c.dtype) || !dt_ok(c.topk_w_dtype) || c.act < 0) return FTM_ERR_FORMAT;
+  if (c.ids_dtype != FTM_ID_I32 && c.ids_dtype != FTM_ID_I64) return FTM_ERR_FORMAT;
+  if (T == 0) return FTM_OK;
+  if (c.x == nullptr || c.topk_ids == nullptr || c.topk_w == nullptr || c.out == nullptr) return FTM_ERR_NULL;
+  if (workspace == nullptr) return FTM_ERR_WORKSPACE;
+  if (((uintptr_t)workspace & 255u) != 0) return FTM_ERR_ALIGN;
+  const W4a4MoeLayout L = w4a4_moe_layout(T, k, E, H, I);
+  if (ws_bytes < L.total) return FTM_ERR_WORKSPACE;
+  char* ws = (char*)workspace;
+  const int P = T * k;
+  int32_t* offsets = (int32_t*)(ws + L.offsets);
+  int32_t* row_of_pair = (int32_t*)(ws + L.row_of_pair);
+  int32_t* pair_of_row = (int32_t*)(ws + L.pair_of_row);
+  int32_t* token_of_row = (int32_t*)(ws + L.token_of_row);
+  float *h = (float*)(ws + L.h), *y = (float*)(ws + L.y);
+  const ftm_w4a4 a = {ws + L.xq, (uint8_t*)(ws + L.xs), c.w13, c.w13_scale, c.w13_bias, h, offsets, token_of_row, P, T,
+                      (int64_t)2 * I * (H / 2), (int64_t)2 * I * (H / 32), 2 * I, H, E, c.w13_bias_dtype, FTM_DT_F32, c.act,
+                      c.act_alpha, c.act_limit};
+  const ftm_w4a4 b = {ws + L.hq, (uint8_t*)(ws + L.hs), c.w2, c.w2_scale, c.w2_bias, y, offsets, nullptr, P, P,
+                      (int64_t)H * (I / 2), (int64_t)H * (I / 32), H, I, E, c.w2_bias_dtype, FTM_DT_F32, -1, 0.0f, 0.0f};
+  // everything is checked before anything is launched
+  int rc = check_w4a4(&a);
+  if (rc == FTM_OK) rc = check_w4a4(&b);
+  if (rc != FTM_OK) return rc;
+  if (((uintptr_t)c.x | (uint64_t)c.x_stride | (uintptr_t)c.out) % dt_bytes(c.dtype) != 0 ||
+      (uintptr_t)c.topk_w % dt_bytes(c.topk_w_dtype) != 0 || (uintptr_t)c.topk_ids % (c.ids_dtype == FTM_ID_I64 ? 8 : 4) != 0)
+    return FTM_ERR_ALIGN;
+  rc = ftm_sort_tokens(c.topk_ids, c.ids_dtype, T, k, E, offsets, row_of_pair, pair_of_row, token_of_row, ws + L.sort,
+                       L.total - L.sort, stream);
+  if (rc == FTM_OK) rc = ftm_w4a4_linear_dynamic(c.x, c.dtype, c.x_stride, &a, stream);
+  if (rc == FTM_OK) rc = ftm_w4a4_linear_dynamic(h, FTM_DT_F32, (int64_t)I * 4, &b, stream);
   if (rc == FTM_OK)
     rc = ftm_combine_tokens(y, FTM_DT_F32, (int64_t)H * 4, c.topk_w, c.topk_w_dtype, row_of_pair, T, k, H, c.out, c.dtype,
                             stream);

@@ -216,6 +216,12 @@ hipError_t launch_quant_int8(const void* x, int dt, int64_t rows, int K, int64_t
 hipError_t launch_w8a8(const ftm_w8a8& call, hipStream_t st);
 // ... of x still wide (call.x and call.x_scale: scratch for its codes)
 hipError_t launch_w8a8_dynamic(const ftm_w8a8& call, const void* x, int x_dt, int64_t x_stride, hipStream_t st);
+// ftm_w4a4.hip (strides in bytes)
+hipError_t launch_quant_mxfp4(const void* x, int dt, int64_t rows, int K, int64_t x_stride, uint8_t* blocks,
+                              uint8_t* scales, hipStream_t st);
+hipError_t launch_w4a4(const ftm_w4a4& call, hipStream_t st);
+// ... of x still wide (call.x and call.x_scale: scratch for its codes)
+hipError_t launch_w4a4_dynamic(const ftm_w4a4& call, const void* x, int x_dt, int64_t x_stride, hipStream_t st);
 // ftm_sort.hip
 size_t sort_workspace_bytes(int64_t pairs, int E);
 hipError_t launch_sort(const void* ids, bool ids64, int64_t pairs, int k, int E, int32_t* offsets,

@@ -28,9 +28,12 @@ NEED = {
     "v_mfma_f32_16x16x32_bf16": 8,
     "v_mfma_i32_16x16x64_i8": 8,
     "v_mfma_f32_16x16x4_f32": 10,
-    "v_mfma_scale_f32_16x16x128_f8f6f4": 12,  # with an e4m3 operand (fp4 x fp4 would need fewer)
+    "v_mfma_scale_f32_16x16x128_f8f6f4": 12,  # with an e4m3 operand
     "v_mfma_f32_32x32x1_2b_f32": 18,
 }
+
+# The same where both operands are fp4 (cbsz:4 blgp:4), which take half the passes.
+NEED_FP4 = {"v_mfma_scale_f32_16x16x128_f8f6f4": 8}
 
 _FUNC = re.compile(r"\n(_Z\w+):[^\n]*\n(.*?)\.Lfunc_end", re.S)
 _RANGE = re.compile(r"([av])\[(\d+):(\d+)\]")
@@ -148,7 +151,8 @@ def check(path: str) -> list:
             if not args:
                 continue
             if op.startswith("v_mfma"):
-                need = NEED.get(op)
+                fp4 = "cbsz:4" in txt and "blgp:4" in txt
+                need = (NEED_FP4 if fp4 else NEED).get(op)
                 if need is None:
                     findings.append(f"{path}: {name}: '{txt}': no wait states known for {op}")
                     continue

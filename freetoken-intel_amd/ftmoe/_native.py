@@ -47,6 +47,7 @@ ID_I32 = 0
 ID_I64 = 1
 
 W8A8_MAX_K = 131071
+W4A4_MAX_K = 1 << 20
 
 ACT_SILU = 0
 ACT_GELU = 1
@@ -170,6 +171,26 @@ class FtmW8A8Moe(ctypes.Structure):
                 + [("act_alpha", ctypes.c_float), ("act_limit", ctypes.c_float)])
 
 
+class FtmW4A4(ctypes.Structure):
+    """``ftm_w4a4``: one MXFP4 x MXFP4 product, dense or grouped by expert."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "out", "offsets", "row_index")]
+                + [(n, ctypes.c_int64) for n in ("rows", "x_rows", "w_stride", "w_scale_stride")]
+                + [(n, ctypes.c_int32) for n in ("N", "K", "num_experts", "bias_dtype", "out_dtype", "act")]
+                + [("act_alpha", ctypes.c_float), ("act_limit", ctypes.c_float)])
+
+
+class FtmW4A4Moe(ctypes.Structure):
+    """``ftm_w4a4_moe``: one call of the routed experts, MXFP4 x MXFP4."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "topk_ids", "topk_w", "out", "w13", "w13_scale", "w13_bias", "w2",
+                                                "w2_scale", "w2_bias")]
+                + [("x_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("T", "k", "num_experts", "hidden", "inter", "dtype", "ids_dtype",
+                                                 "topk_w_dtype", "w13_bias_dtype", "w2_bias_dtype", "act")]
+                + [("act_alpha", ctypes.c_float), ("act_limit", ctypes.c_float)])
+
+
 # Every symbol include/ftmoe.h declares (tests check the export table against this).
 EXPORTED = (
     "ftm_version",
@@ -189,6 +210,11 @@ EXPORTED = (
     "ftm_w8a8_linear_dynamic",
     "ftm_w8a8_moe_workspace_bytes",
     "ftm_w8a8_moe_forward",
+    "ftm_quant_mxfp4",
+    "ftm_w4a4_linear",
+    "ftm_w4a4_linear_dynamic",
+    "ftm_w4a4_moe_workspace_bytes",
+    "ftm_w4a4_moe_forward",
     "ftm_sort_workspace_bytes",
     "ftm_sort_tokens",
     "ftm_gather_tokens",
@@ -265,6 +291,16 @@ def lib() -> ctypes.CDLL:
     L.ftm_w8a8_moe_workspace_bytes.argtypes = [i32] * 5
     L.ftm_w8a8_moe_forward.restype = ctypes.c_int
     L.ftm_w8a8_moe_forward.argtypes = [ctypes.POINTER(FtmW8A8Moe), vp, sz, vp]
+    L.ftm_quant_mxfp4.restype = ctypes.c_int
+    L.ftm_quant_mxfp4.argtypes = [vp, i32, i64, i32, i64, vp, vp, vp]
+    L.ftm_w4a4_linear.restype = ctypes.c_int
+    L.ftm_w4a4_linear.argtypes = [ctypes.POINTER(FtmW4A4), vp]
+    L.ftm_w4a4_linear_dynamic.restype = ctypes.c_int
+    L.ftm_w4a4_linear_dynamic.argtypes = [vp, i32, i64, ctypes.POINTER(FtmW4A4), vp]
+    L.ftm_w4a4_moe_workspace_bytes.restype = sz
+    L.ftm_w4a4_moe_workspace_bytes.argtypes = [i32] * 5
+    L.ftm_w4a4_moe_forward.restype = ctypes.c_int
+    L.ftm_w4a4_moe_forward.argtypes = [ctypes.POINTER(FtmW4A4Moe), vp, sz, vp]
     L.ftm_sort_workspace_bytes.restype = sz
     L.ftm_sort_workspace_bytes.argtypes = [i32, i32, i32]
     L.ftm_sort_tokens.restype = ctypes.c_int

@@ -314,6 +314,57 @@ int ftm_w8a8_linear(const ftm_w8a8* call, void* stream);
  * few rows the product quantises by itself and leaves the scratch as it is). */
 int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w8a8* call, void* stream);
 
+/* ---- MXFP4 activations x MXFP4 weights ----
+ * The reference has MXFP4 weights under wide activations only
+ * (python/freetoken/kernel/triton/fused_mxfp4_linear.py); these take the
+ * activations in the same format. */
+
+/* Quantise rows x [rows, K] (x_stride bytes apart, K a multiple of 32): of each block
+ * of 32, with a = max(max |x|, 1e-12), scale = e + 127 for the least whole number e with
+ * a <= 6 * 2^e, and per value the code of the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
+ * |x| / 2^e, ties to the smaller, with x's sign unless it is 0: the bytes of
+ * quantize_mxfp4_blocks (python/freetoken/kernel/triton/mxfp4_linear.py:79-111).  A
+ * block with an infinity or NaN gets the scale 255 (the format's NaN) and codes 0.
+ * blocks [rows, K/32, 16], 4-byte aligned; scales [rows, K/32]. */
+int ftm_quant_mxfp4(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride,
+                    uint8_t* blocks, uint8_t* scales, void* stream);
+
+/* One product: out[m, n] = sum over blocks b of 2^(x_scale[i, b] + w_scale[n, b] - 254)
+ * sum_k x[i, k] w[n, k] (+ bias[n]), i = m or row_index[m], fp32 sums, one rounding to
+ * out_dtype; a block with the scale 255 makes NaN.  With act >= 0 the weight rows [0, N/2) are gate and
+ * [N/2, N) up and out[m, n] = act(gate) * up, n < N/2 (NaN where either is).
+ * Grouped (offsets not NULL): rows [offsets[e], offsets[e+1]) take weight e;
+ * the other rows, and rows whose row_index names no row of x, become zeros. */
+typedef struct ftm_w4a4 {
+  const void* x;           /* [x_rows, K/32, 16], 16-byte aligned */
+  const uint8_t* x_scale;  /* [x_rows, K/32] */
+  const void* w;           /* [N, K/32, 16] per expert, 16-byte aligned */
+  const uint8_t* w_scale;  /* [N, K/32] per expert */
+  const void* bias;        /* [N] per expert, bias_dtype, or NULL */
+  void* out;               /* [rows, N] (act: [rows, N/2]), out_dtype */
+  const int32_t* offsets;  /* device [num_experts + 1], or NULL: one weight */
+  const int32_t* row_index;/* device [rows]: row of x of each output row, or NULL: the same row */
+  int64_t rows;            /* output rows */
+  int64_t x_rows;
+  int64_t w_stride;        /* bytes between the experts' weights, a multiple of 16 */
+  int64_t w_scale_stride;  /* bytes between the experts' scales */
+  int32_t N;
+  int32_t K;               /* a multiple of 32, <= FTM_W4A4_MAX_K */
+  int32_t num_experts;     /* <= 512; 1 without offsets */
+  int32_t bias_dtype;
+  int32_t out_dtype;
+  int32_t act;             /* FTM_ACT_*, or -1: none */
+  float act_alpha;         /* FTM_ACT_SWIGLU_OAI */
+  float act_limit;
+} ftm_w4a4;
+#define FTM_W4A4_MAX_K (1 << 20)
+int ftm_w4a4_linear(const ftm_w4a4* call, void* stream);
+
+/* ftm_quant_mxfp4 of x [call->x_rows, K] and ftm_w4a4_linear over its codes: call->x
+ * and call->x_scale are scratch for them (for few rows the product quantises by
+ * itself and leaves the scratch as it is). */
+int ftm_w4a4_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, const ftm_w4a4* call, void* stream);
+
 /* ---- (token, expert) pairs sorted by expert, and back ----
  * ids [T, k] int32 or int64 (ids_dtype: FTM_ID_*).  Pair p = t k + j.  The rows
  * of expert e, [offsets[e], offsets[e+1]), are its pairs in order of p; the
@@ -389,6 +440,41 @@ typedef struct ftm_w8a8_moe {
 } ftm_w8a8_moe;
 size_t ftm_w8a8_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter);
 int ftm_w8a8_moe_forward(const ftm_w8a8_moe* call, void* workspace, size_t ws_bytes, void* stream);
+
+/* Routed experts, MXFP4 x MXFP4: x [T, H] quantised, w13 with its activation, h
+ * quantised from fp32, w2, and the rows (fp32) weighted by topk_w [T, k] and summed in
+ * fp32, rounded once to dtype (x and out).  N and K of the weights are the layer's
+ * (w13 [2 inter, hidden], w2 [hidden, inter]; hidden and inter multiples of 32), experts
+ * side by side in memory.  The workspace needs no initial value; one call uses
+ * it at a time. */
+typedef struct ftm_w4a4_moe {
+  const void* x;            /* [T, hidden], x_stride bytes apart */
+  const void* topk_ids;     /* [T, k], ids_dtype; outside [0, E): no expert */
+  const void* topk_w;       /* [T, k], topk_w_dtype */
+  void* out;                /* [T, hidden] */
+  const void* w13;          /* [E, 2 inter, hidden/32, 16], 16-byte aligned */
+  const uint8_t* w13_scale; /* [E, 2 inter, hidden/32] */
+  const void* w13_bias;     /* [E, 2 inter] or NULL */
+  const void* w2;           /* [E, hidden, inter/32, 16], 16-byte aligned */
+  const uint8_t* w2_scale;  /* [E, hidden, inter/32] */
+  const void* w2_bias;      /* [E, hidden] or NULL */
+  int64_t x_stride;
+  int32_t T;
+  int32_t k;
+  int32_t num_experts;
+  int32_t hidden;
+  int32_t inter;
+  int32_t dtype;
+  int32_t ids_dtype;
+  int32_t topk_w_dtype;
+  int32_t w13_bias_dtype;
+  int32_t w2_bias_dtype;
+  int32_t act;              /* FTM_ACT_* */
+  float act_alpha;
+  float act_limit;
+} ftm_w4a4_moe;
+size_t ftm_w4a4_moe_workspace_bytes(int32_t T, int32_t k, int32_t num_experts, int32_t hidden, int32_t inter);
+int ftm_w4a4_moe_forward(const ftm_w4a4_moe* call, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---- offload slot pool (python/freetoken/moe/offload_cache.py:218-694) ---- */
 
