@@ -212,13 +212,356 @@ __global__ __launch_bounds__(256) void k_w4a4_any(ftm_w4a4 c, int mtiles, int nt
   }
 }
 
-hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
+// ------------------------------------------------------------------ operands
+// The eight scale bytes of one row and step of 256 K, nb >= 8 of them in the row, as
+// loaded (no alignment asked for; the last eight of the row where fewer are left) and as
+// the step's: bytes past K are 0.  Apart, because fitting would wait for the load.
+__device__ __forceinline__ u32x2 load_scales(const uint8_t* row, int step, int nb) {
+  u32x2 v;
+  __builtin_memcpy(&v, row + (8 * step + 8 <= nb ? 8 * step : nb - 8), 8);
+  return v;
+}
+__device__ __forceinline__ u32x2 fit_scales(u32x2 v, int step, int nb) {
+  const int past = 8 * step + 8 - nb;  // blocks of the step that are not there, up to 7
+  const uint64_t b = (((uint64_t)v.y << 32) | v.x) >> (past > 0 ? 8 * past : 0);
+  return (u32x2){(uint32_t)b, (uint32_t)(b >> 32)};
+}
+// Bytes g and 4 + g of eight: the scale operand of a lane of group g, byte q for the
+// step's q-th 128 K.
+__device__ __forceinline__ uint32_t scale_operand(u32x2 v, int g) {
+  return __builtin_amdgcn_perm(v.y, v.x, 0x0c0c0000u | (uint32_t)(0x0400 + 0x101 * g));
+}
+
+// Weight rows of a tile of NT blocks of 16: with an activation 8 gate rows and their 8
+// up rows a block.  Copies of 8 rows, a 16-byte piece a lane; rows past the last copy
+// it, what lies past the end of the last row is zeros.
+template <int NT>
+struct SplitWeights {
+  Rsrc res;
+  uint32_t off[2 * NT];
+  __device__ __forceinline__ SplitWeights(const char* w, int NO, int K, bool act, int n0, int ncol) {
+    const int lane = threadIdx.x & 63, Kb = K / 2;
+    res = make_rsrc(w + (int64_t)n0 * Kb, (uint32_t)((act ? NO : 0) + ncol) * (uint32_t)Kb);
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      int n = act ? 8 * (i >> 1) + (r & 7) : r;
+      n = n < ncol ? n : ncol - 1;
+      off[i] = (uint32_t)(n + (act && (i & 1) ? NO : 0)) * (uint32_t)Kb + 16u * (uint32_t)((lane & 7) ^ swz(r));
+    }
+  }
+  // The weight row of row r of the tile's, from the tile's first on.
+  __device__ __forceinline__ static int64_t row(int NO, bool act, int ncol, int r) {
+    int n = act ? 8 * (r >> 4) + (r & 7) : r;
+    n = n < ncol ? n : ncol - 1;
+    return n + (act && (r & 8) != 0 ? NO : 0);
+  }
+  // k0 past the rows: nothing is read
+  __device__ __forceinline__ void issue(char* at, uint32_t k0) const {
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LPtr)(at + 1024 * i), 16, (int)(off[i] + k0), 0, 0, 0);
+  }
+};
+constexpr int kMinK = 256;  // of the kernels that take the scales eight at a time
+
+// A wave's scales of R rows and its `per` steps from `lo` on, kept in LDS with scale_pitch
+// bytes between rows (an odd number of eights: 16 rows hit distinct banks).  A lane
+// has a row of each 64 (two lanes one of 32, in turn); `p` says where they begin.  The
+// first kFlight loads of each are under way when the copies of the operands are
+// requested (`then`), before any of them is waited for.
+__host__ __device__ inline int scale_pitch(int per) { return 8 * (per | 1); }
+template <int R>
+struct FillScales {
+  static constexpr int kRows = (R + 63) / 64, kTurns = R <= 32 ? 2 : 1, kFlight = kTurns == 2 ? 2 : 4;
+  const uint8_t* p[kRows];
+  __device__ __forceinline__ static int row(int i) {  // the lane's i-th
+    const int lane = threadIdx.x & 63, r = (kTurns == 2 ? lane & 31 : lane) + 64 * i;
+    return r < R ? r : R - 1;
+  }
+  template <class Then>
+  __device__ __forceinline__ void operator()(char* at, int lo, int per, int nb, Then&& then) const {
+    const int lane = threadIdx.x & 63, pitch = scale_pitch(per);
+    const int turn = kTurns == 2 ? lane >> 5 : 0, first = kTurns == 2 ? lane & 31 : lane;
+    const int last = (nb - 1) / 8, n = lo + per <= last + 1 ? per : last + 1 - lo;
+    for (int s0 = 0; s0 < n; s0 += kTurns * kFlight) {
+      u32x2 v[kRows][kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int s = s0 + kTurns * f + turn;
+          v[i][f] = load_scales(p[i], lo + (s < n ? s : n - 1), nb);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      if (s0 == 0) then();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int s = s0 + kTurns * f + turn, r = first + 64 * i;
+          if (s < n && r < R) *(u32x2*)(at + r * pitch + 8 * s) = fit_scales(v[i][f], lo + s, nb);
+        }
+    }
+  }
+};
+
+constexpr uint32_t kNowhere = 0x40000000u;  // added to an offset below 2^30: past every buffer
+
+// Piece q (128 K each) of row r of an LDS stage, for a lane of group g.
+__device__ __forceinline__ u32x4 stage_piece(const char* st, int r, int q, int g) {
+  return *(const u32x4*)(st + r * kRow + 16 * ((4 * q + g) ^ swz(r)));
+}
+
+// ------------------------------------------------------------------ K split over the waves
+// Biases of one 16 x 16 block's results of a lane: weight rows 4 g .. 4 g + 3 (with an
+// activation rows 0..7 of a block are gate channels, 8..15 their up rows, and only
+// lanes of the first eight have results).
+struct SplitBias {
+  uint32_t b[8];
+  __device__ __forceinline__ void request(const void* bias, int dt, int64_t at, bool act, int NO, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0;
+    if (bias == nullptr) return;
+    load_run<4>(bias, at, n, NO - 1, dt, b);
+    if (act) load_run<4>(bias, at + NO, n, NO - 1, dt, b + 4);
+  }
+  __device__ __forceinline__ float at(int i, int dt) const { return bits_to_f32(opaque_bits(b[i]), dt); }
+};
+
+template <int NT>
+__device__ __forceinline__ int split_channel(bool act, int n0, int block, int g) {
+  return n0 + (act ? 8 * (block % NT) + 4 * (g & 1) : 16 * (block % NT) + 4 * g);
+}
+
+// The waves' sums of the tile's MT x NT blocks, through LDS (which they may
+// overwrite): f(part, block, sums, sums of the up rows) for the blocks of this wave; a
+// lane's four sums are rows 4 g .. 4 g + 3 of token lane % 16.
+template <int MT, int NT, int NW, class F>
+__device__ __forceinline__ void split_sums(char* lds, const f32x4 (&acc)[MT][NT], bool act, F&& f) {
+  constexpr int kParts = (MT * NT + NW - 1) / NW;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x4* red = (f32x4*)lds;  // [NW][MT * NT][64]
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) {
+    const int b = p * NW + wave;
+    if (MT * NT % NW != 0 && b >= MT * NT) continue;
+    f32x4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      u += red[(w * MT * NT + b) * 64 + lane];
+      if (act) v += red[(w * MT * NT + b) * 64 + (lane | 32)];
+    }
+    f(p, b, u, v);
+  }
+}
+
+// A workgroup's tile of 16 MT tokens x 16 NT weight rows; each of the NW waves takes a
+// run of K over the whole tile through an LDS ring of its own (S stages of 256 K), and the
+// waves' sums meet in LDS.  No barrier in the K loop; a stage's slot is filled again as
+// soon as its operands are in registers.  For few rows, where the weights' stream is
+// all the time, and for grids too small for the tiles that share a ring.
+template <int MT, int NT, int NW, int S>
+__global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, int ntiles) {
+  constexpr int BM = 16 * MT, kStage = (MT + NT) * 16 * kRow;
+  constexpr int kParts = (MT * NT + NW - 1) / NW;
+  extern __shared__ char lds[];  // [NW][S][kStage], then the sums
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const RowTile rt = row_tile<BM>(c, item / ntiles);
+  if (rt.cnt <= 0) return;
+  const int NO = out_cols(c), nb = c.K / 32;
+  const bool act = c.act >= 0;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int cols = act ? 8 * NT : 16 * NT;  // output channels of the tile
+  const int n0 = (item % ntiles) * cols;
+  const int ncol = NO - n0 < cols ? NO - n0 : cols;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+  // The rows of x: of this wave's results, of its copies, and of its scales
+  const bool indexed = c.row_index != nullptr;
+  using Fill = FillScales<16 * (MT + NT)>;
+  int rr[kParts], rc[2 * MT], rs[Fill::kRows];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) rr[p] = 16 * ((p * NW + wave) / NT) + m;
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) rc[i] = 8 * i + (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < Fill::kRows; ++i) rs[i] = Fill::row(i);
+  auto known = [&](int r) { return rt.row0 + (r < rt.cnt ? r : 0); };
+  const bool none = rt.e < 0;
+  const int64_t x_rows = indexed ? c.x_rows : c.rows;
+  if (indexed && !none) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) rr[p] = rr[p] < rt.cnt ? c.row_index[known(rr[p])] : -1;
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) rc[i] = rc[i] < rt.cnt ? c.row_index[known(rc[i])] : -1;
+#pragma unroll
+    for (int i = 0; i < Fill::kRows; ++i) rs[i] = rs[i] < 16 * MT ? c.row_index[known(rs[i])] : 0;
+  } else {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) rr[p] = rr[p] < rt.cnt && !none ? (int)known(rr[p]) : -1;
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) rc[i] = rc[i] < rt.cnt ? rc[i] : -1;
+#pragma unroll
+    for (int i = 0; i < Fill::kRows; ++i) rs[i] = (int)known(rs[i]);
+  }
+  SplitBias bias[kParts];
+  auto request = [&] {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      bias[p].request(none ? nullptr : c.bias, c.bias_dtype, (int64_t)rt.e * c.N, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
+  };
+  const int nsteps = (nb + 7) / 8, per = (nsteps + NW - 1) / NW;
+  const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
+  if (!none && lo < hi) {
+    // rows past the tile and rows that are none are not copied; offsets from the tile's
+    // first token, or, read through an index, from x's
+    const uint32_t Kb = (uint32_t)c.K / 2;
+    const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
+    const SplitWeights<NT> weights((const char*)c.w + (int64_t)rt.e * c.w_stride, NO, c.K, act, n0, ncol);
+    uint32_t xoff[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int r = 8 * i + (lane >> 3);
+      const bool in = rc[i] >= 0 && rc[i] < (indexed ? x_rows : (int64_t)rt.cnt);
+      xoff[i] = in ? (uint32_t)rc[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+    }
+    Fill fill;
+#pragma unroll
+    for (int i = 0; i < Fill::kRows; ++i) {
+      const int r = Fill::row(i);
+      const int64_t n = n0 + SplitWeights<NT>::row(NO, act, ncol, r < 16 * MT ? 0 : r - 16 * MT);
+      fill.p[i] = r < 16 * MT ? c.x_scale + (int64_t)(rs[i] >= 0 && rs[i] < x_rows ? rs[i] : 0) * nb
+                              : c.w_scale + (int64_t)rt.e * c.w_scale_stride + n * nb;
+    }
+    char* ring = lds + wave * (S * kStage);
+    char* scales = lds + NW * S * kStage + wave * (MT + NT) * 16 * scale_pitch(per);
+    auto issue = [&](int step, int slot) __attribute__((always_inline)) {
+      const uint32_t k0 = step < hi ? (uint32_t)step * 128u : kNowhere;
+      char* st = ring + slot * kStage;
+      weights.issue(st + 2048 * MT, k0);
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * i), 16, (int)(xoff[i] + k0), 0, 0, 0);
+    };
+    fill(scales, lo, per, nb, [&] {
+      request();
+#pragma unroll
+      for (int u = 0; u < S; ++u) issue(lo + u, u);
+    });
+    const int pitch = scale_pitch(per);
+    int slot = 0;
+    for (int step = lo; step < hi; ++step) {
+      wait_vm<(S - 1) * 2 * (MT + NT)>();  // this step's copies have landed
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = ring + slot * kStage;
+      u32x4 w[2][NT], x[2][MT];
+      uint32_t sw[NT], sx[MT];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[q][j] = stage_piece(st, 16 * (MT + j) + m, q, g);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[q][i] = stage_piece(st, 16 * i + m, q, g);
+      }
+      auto scale = [&](int r) { return scale_operand(*(const u32x2*)(scales + r * pitch + 8 * (step - lo)), g); };
+#pragma unroll
+      for (int j = 0; j < NT; ++j) sw[j] = scale(16 * (MT + j) + m);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sx[i] = scale(16 * i + m);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the operands are here: the slot is free
+      __builtin_amdgcn_sched_barrier(0);
+      issue(step + S, slot);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          acc[i][j] = mfma_fp4<0, 0>(w[0][j], x[0][i], acc[i][j], sw[j], sx[i]);
+          acc[i][j] = mfma_fp4<1, 1>(w[1][j], x[1][i], acc[i][j], sw[j], sx[i]);
+        }
+      slot = slot == S - 1 ? 0 : slot + 1;
+    }
+    wait_vm<0>();  // the copies past the last step, before the sums take their place
+  } else {
+    request();
+  }
+  with_act(c.act, [&](auto a) {
+    constexpr int A = decltype(a)::value;
+    split_sums<MT, NT, NW>(lds, acc, A >= 0, [&](int p, int b, f32x4 u, f32x4 v) {
+      if (A >= 0 && g >= 2) return;
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = u[r] + bias[p].at(r, c.bias_dtype);
+        if constexpr (A >= 0) y[r] = gated(A, y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
+        y[r] = rr[p] >= 0 && rr[p] < x_rows ? y[r] : 0.0f;
+      }
+      RowOut<4>(c, rt, NO, split_channel<NT>(act, n0, b, g)).store(16 * (b / NT) + m, y);
+    });
+  });
+}
+
+namespace {
+
+hipError_t any(const ftm_w4a4& c, hipStream_t st) {
   const int64_t mt = row_tiles(c, 16), nt = (out_cols(c) + 15) / 16;
   const int64_t wgs = (mt * nt + 3) / 4, grid = wgs < kMaxGroups ? wgs : kMaxGroups;
   if (mt > INT32_MAX) return hipErrorInvalidValue;
   if (c.act >= 0) k_w4a4_any<true><<<dim3((unsigned)grid), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
   else k_w4a4_any<false><<<dim3((unsigned)grid), dim3(256), 0, st>>>(c, (int)mt, (int)nt);
   return hipGetLastError();
+}
+
+constexpr int kMaxLds = 160 * 1024;
+
+template <int MT, int NT, int NW, int S>
+int split_lds(const ftm_w4a4& c) {
+  constexpr int ring = NW * S * (MT + NT) * 16 * kRow, sums = NW * MT * NT * 1024;
+  const int nsteps = (c.K + 255) / 256, lds = ring + NW * (MT + NT) * 16 * scale_pitch((nsteps + NW - 1) / NW);
+  return lds > sums ? lds : sums;
+}
+template <int MT, int NT, int NW, int S>
+hipError_t split(const ftm_w4a4& c, hipStream_t st) {
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = split_lds<MT, NT, NW, S>(c);
+  const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + cols - 1) / cols;
+  if (mt * nt > kMaxGroups || lds > kMaxLds) return any(c, st);
+  static DeviceBits lds_set{0};
+  const hipError_t e = allow_lds(lds_set, (const void*)k_w4a4_split<MT, NT, NW, S>, kMaxLds);
+  if (e != hipSuccess) return e;
+  k_w4a4_split<MT, NT, NW, S><<<dim3((unsigned)(mt * nt)), dim3(64 * NW), lds, st>>>(c, (int)mt, (int)nt);
+  return hipGetLastError();
+}
+
+// Whether a tile's 32-bit offsets (below 2^30) reach its tokens (256 rows from its
+// first, or all of x where they are read through an index), its weight rows and its results.
+bool offsets_ok(const ftm_w4a4& c) {
+  const int64_t rows = c.row_index != nullptr ? c.x_rows : c.x_rows < 256 ? c.x_rows : 256;
+  const int64_t wrows = 256 + (c.act >= 0 ? c.N / 2 : 0), Kb = c.K / 2 + 256;
+  return rows * Kb < (int64_t)kNowhere && wrows * Kb < (int64_t)kNowhere && 4 * 256 * (int64_t)c.N < (int64_t)kNowhere;
+}
+
+}  // namespace
+
+hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
+  if (c.K < kMinK || !offsets_ok(c)) return any(c, st);
+  if (c.offsets != nullptr) return split<1, 2, 4, 2>(c, st);
+  const int64_t M = c.rows;
+  if (M <= 16) return split<1, 1, 4, 4>(c, st);
+  if (M <= 32) return split<2, 1, 4, 3>(c, st);
+  return split<4, 4, 4, 2>(c, st);
 }
 
 hipError_t launch_w4a4_dynamic(const ftm_w4a4& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {
