@@ -154,7 +154,7 @@ typedef __attribute__((address_space(3))) void* LPtr;
 // 512 tokens 172 / 175, but 2048 277 / 274, and of 4 of 32 of 2880 x 2880 467 / 460.
 constexpr int kNT = 2;
 
-// The results of a row tile: N = 4 or 2 neighbouring channels from n0 on of one row
+// The results of a row tile: N = 8, 4 or 2 neighbouring channels from n0 on of one row
 // at a time, through a buffer that drops rows past the tile; channels past the
 // last take an offset past its end, so there is no branch around a store.
 template <int N>
@@ -176,7 +176,13 @@ struct RowOut {
     if (dt == FTM_DT_F32) {
       const uint32_t off = n0 < NO ? 4u * at : kOOB;
       if (vec) {
-        if constexpr (N == 4)
+        if constexpr (N == 8) {
+#pragma unroll
+          for (int h = 0; h < 8; h += 4)
+            __builtin_amdgcn_raw_buffer_store_b128((u32x4){__float_as_uint(y[h]), __float_as_uint(y[h + 1]), __float_as_uint(y[h + 2]),
+                                                           __float_as_uint(y[h + 3])},
+                                                   res, n0 < NO ? off + 4u * h : kOOB, 0, kNT);
+        } else if constexpr (N == 4)
           __builtin_amdgcn_raw_buffer_store_b128(
               (u32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])}, res, off, 0,
               kNT);
@@ -191,7 +197,10 @@ struct RowOut {
     }
     const uint32_t off = n0 < NO ? 2u * at : kOOB;
     if (vec) {
-      if constexpr (N == 4)
+      if constexpr (N == 8)
+        __builtin_amdgcn_raw_buffer_store_b128((u32x4){half2(y[0], y[1]), half2(y[2], y[3]), half2(y[4], y[5]), half2(y[6], y[7])},
+                                               res, off, 0, kNT);
+      else if constexpr (N == 4)
         __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, kNT);
       else
         __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, kNT);

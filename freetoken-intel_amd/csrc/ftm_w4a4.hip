@@ -222,8 +222,8 @@ __device__ __forceinline__ u32x2 load_scales(const uint8_t* row, int step, int n
   return v;
 }
 __device__ __forceinline__ u32x2 fit_scales(u32x2 v, int step, int nb) {
-  const int past = 8 * step + 8 - nb;  // blocks of the step that are not there, up to 7
-  const uint64_t b = (((uint64_t)v.y << 32) | v.x) >> (past > 0 ? 8 * past : 0);
+  const int past = 8 * step + 8 - nb;  // blocks of the step that are not there
+  const uint64_t b = past < 8 ? (((uint64_t)v.y << 32) | v.x) >> (past > 0 ? 8 * past : 0) : 0;
   return (u32x2){(uint32_t)b, (uint32_t)(b >> 32)};
 }
 // Bytes g and 4 + g of eight: the scale operand of a lane of group g, byte q for the
@@ -514,6 +514,347 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, 
   });
 }
 
+// ------------------------------------------------------------------ LDS tiles
+// A tile is BM = 16 MI WM tokens x BN = 16 NJ WN weight rows (with an activation BN / 2 gate
+// rows and their up rows): WM WN waves of 16 MI tokens x 16 NJ weight rows each over the
+// whole K.  Codes go through a ring of S LDS stages of 256 K, filled by direct copies,
+// one barrier a step; scale bytes through registers into two slots of LDS, one step
+// ahead.  Few large waves: a step reads (16 MI + 16 NJ) rows of LDS a wave for 16 MI x 16 NJ
+// results, and with one wave a SIMD every other instruction is written into the
+// shadow of an MFMA (16 cycles), in the order in which it is to be issued.  A workgroup
+// takes one tile after another, and the copies run on from tile to tile.
+template <int WM, int WN, int MI, int NJ, int S, bool ACT, bool GROUPED, bool QOUT>
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8_t* out_scale, int mtiles, int ntiles) {
+  constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, kRows = BM + BN;
+  constexpr int kX = BM * kRow, kStage = kRows * kRow, kSlot = 8 * kRows;  // of codes, of scales
+  constexpr int NX = BM / 8 / kWaves, NB = BN / 8 / kWaves, ND = NX + NB;  // 1 KiB copies a wave and step
+  constexpr int NR = (kRows + kThreads - 1) / kThreads;  // rows whose scales a thread carries
+  constexpr int kCols = ACT ? BN / 2 : BN;               // output channels of the tile
+  constexpr int CN = ACT ? NJ / 2 : NJ;                  // neighbouring ones of a lane
+  constexpr int kAhead = 3;                              // row blocks read ahead of their products
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies of 8 rows, as many for each wave");
+  static_assert(2 * MI % (kAhead + 1) == 0 && kAhead <= MI && NJ >= 4 && NJ % 4 == 0 && (NJ % MI == 0 || MI % NJ == 0),
+                "the order of the reads");
+  extern __shared__ char lds[];  // [S][kStage], then [2][kSlot]
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int NO = out_cols(c), nb = c.K / 32;
+  const uint32_t Kb = (uint32_t)c.K / 2;
+  const int nsteps = (nb + 7) / 8, nrun = nsteps > S ? nsteps : S;  // steps past K multiply zeros
+  const bool indexed = GROUPED && c.row_index != nullptr;
+
+  // this workgroup's items: every (workgroups per XCD)-th of its XCD's run
+  using Scan = std::conditional_t<GROUPED, RowScan<BM>, int>;
+  const Scan scan = [&] {
+    if constexpr (GROUPED) return RowScan<BM>(c);
+    else return 0;
+  }();
+  int row_tiles = mtiles;
+  if constexpr (GROUPED) row_tiles = scan.total;
+  const int items = row_tiles * ntiles, xcd = blockIdx.x & 7, rem = items & 7;
+  const int begin = xcd * (items >> 3) + (xcd < rem ? xcd : rem), end = begin + (items >> 3) + (xcd < rem ? 1 : 0);
+  struct Tile {
+    RowTile rt;
+    int n;  // first output channel
+  };
+  auto tile_at = [&](int item) __attribute__((always_inline)) {
+    if constexpr (GROUPED) {
+      const auto x = scan.expert(item / ntiles);
+      const ItemOrder o(item - x.before * ntiles, x.tiles, ntiles);
+      return Tile{scan.tile(x, o.m), o.nt * kCols};
+    } else {
+      const ItemOrder o(item, mtiles, ntiles);
+      return Tile{dense_tile<BM>(c, o.m), o.nt * kCols};
+    }
+  };
+  // Weight row of the tile's LDS row r: wave r / (16 NJ) of the columns; its operand block
+  // j, operand row o is channel NJ o + j, so that a lane's results are neighbours
+  // (with an activation: NJ / 2 o + j of gate, j < NJ / 2, and of up); rows past the last copy it
+  auto weight_row = [&](int r, int cols) __attribute__((always_inline)) {
+    const int j = (r >> 4) % NJ, o = r & 15;
+    int n = r / (16 * NJ) * (kCols / WN) + CN * o + j % CN;
+    n = n < cols ? n : cols - 1;
+    return n + (ACT && j >= CN ? NO : 0);
+  };
+  int item = begin + (blockIdx.x >> 3);
+  if (item < end) {
+    Tile cur = tile_at(item);
+    // Rows of x that the wave's copies and the thread's scales read, asked for a tile
+    // ahead: waiting for them waits for every copy before them.
+    int ix[NX], is[NR];
+    auto rows_of = [&](const Tile& t) __attribute__((always_inline)) {
+      const int lane = opaque_lane();
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int r = 8 * (wave * NX + i) + (lane >> 3);
+        ix[i] = indexed ? c.row_index[t.rt.row0 + (r < t.rt.cnt ? r : 0)] : r;
+      }
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int r = 64 * wave + lane + kThreads * i;
+        is[i] = indexed ? c.row_index[t.rt.row0 + (r < t.rt.cnt ? r : 0)] : r;
+      }
+    };
+    // Offsets of a wave's copies: 8 rows each, a 16-byte piece a lane, swizzled; tokens
+    // from the tile's first row, or, read through an index, from x's; weights from the tile's
+    // first gate row.  Rows past the tile are not copied.
+    Rsrc xres, wres;
+    uint32_t xoff[NX], woff[NB];
+    auto aim = [&](const Tile& t) __attribute__((always_inline)) {
+      const int lane = opaque_lane();
+      xres = make_rsrc((const char*)c.x + (indexed ? 0 : t.rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : t.rt.cnt) * Kb);
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int r = 8 * (wave * NX + i) + (lane >> 3);
+        const bool in = r < t.rt.cnt && (!indexed || (ix[i] >= 0 && ix[i] < c.x_rows));
+        xoff[i] = in ? (uint32_t)ix[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+      }
+      const int cols = NO - t.n < kCols ? NO - t.n : kCols;
+      wres = make_rsrc((const char*)c.w + (int64_t)t.rt.e * c.w_stride + (int64_t)t.n * Kb, (uint32_t)((ACT ? NO : 0) + cols) * Kb);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int r = 8 * (wave * NB + i) + (lane >> 3);
+        woff[i] = (uint32_t)weight_row(r, cols) * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r));
+      }
+    };
+    // copy d of the wave's: tokens, then weights
+    auto copy = [&](int d, uint32_t k0, char* st) __attribute__((always_inline)) {
+      if (d < NX)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * (wave * NX + d)), 16, (int)(xoff[d < NX ? d : 0] + k0), 0, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + d - NX)), 16,
+                                                 (int)(woff[d < NX ? 0 : d - NX] + k0), 0, 0, 0);
+    };
+    auto k_of = [&](int kb) { return (uint32_t)(kb < nsteps ? kb : nsteps - 1) * 128u; };
+    // Scales: a thread's rows, the eight bytes of the step after next under way
+    const uint8_t* srow[NR];
+    u32x2 sraw[NR];
+    auto saim = [&](const Tile& t) __attribute__((always_inline)) {
+      const int cols = NO - t.n < kCols ? NO - t.n : kCols;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        int r = 64 * wave + opaque_lane() + kThreads * i;
+        r = r < kRows ? r : kRows - 1;
+        const int64_t s = indexed ? (is[i] >= 0 && is[i] < c.x_rows ? is[i] : 0) : t.rt.row0 + (r < t.rt.cnt ? r : 0);
+        const uint8_t* w = c.w_scale + (int64_t)t.rt.e * c.w_scale_stride + (int64_t)(t.n + weight_row(r >= BM ? r - BM : 0, cols)) * nb;
+        srow[i] = r < BM ? c.x_scale + s * nb : w;
+      }
+    };
+    auto load_s = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) sraw[i] = load_scales(srow[i], kb < nsteps ? kb : nsteps - 1, nb);
+    };
+    // bytes b0 b4 b1 b5 b2 b6 b3 b7: group g's two are neighbours
+    auto store_s = [&](int kb, int slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const u32x2 v = fit_scales(sraw[i], kb, nb);
+        const int r = (int)threadIdx.x + kThreads * i;
+        if (kRows % kThreads == 0 || r < kRows)
+          *(u32x2*)(lds + S * kStage + slot * kSlot + 8 * r) =
+              (u32x2){__builtin_amdgcn_perm(v.y, v.x, 0x05010400u), __builtin_amdgcn_perm(v.y, v.x, 0x07030602u)};
+      }
+    };
+    f32x4 acc[MI][NJ];
+    u32x4 b[2][NJ], x[kAhead + 1];
+    uint32_t sx[MI], sb[NJ], sn[NJ];
+    auto xfrag = [&](int slot, int at) __attribute__((always_inline)) {
+      return stage_piece(lds + slot * kStage, 16 * (wm * MI + at % MI) + m, at / MI, g);
+    };
+    auto wfrag = [&](int slot, int j, int q) __attribute__((always_inline)) {
+      return stage_piece(lds + slot * kStage, BM + 16 * (wn * NJ + j) + m, q, g);
+    };
+    auto sfrag = [&](int slot, int r) __attribute__((always_inline)) {
+      return (uint32_t)*(const uint16_t*)(lds + S * kStage + slot * kSlot + 8 * r + 2 * g);
+    };
+    // Products of step kb, whose first operands are in registers; the rest is read
+    // kAhead row blocks ahead.  Once every wave has read the last of them, the stage's slot
+    // takes the copies of the step S later (`k0`: its place in the tile that the copies
+    // are at), and the first operands of the next step, whose copies have landed, are
+    // read under the products left.
+    auto step = [&](int kb, int snext, int sload, uint32_t k0, int slot, int par) __attribute__((always_inline)) {
+      const int next = slot == S - 1 ? 0 : slot + 1;
+      constexpr int kLast = 2 * MI - kAhead, kSlots = kAhead * NJ;
+#pragma unroll
+      for (int at = 0; at < 2 * MI; ++at) {
+        const int q = at / MI, i = at % MI;
+        if (at == kLast) {
+          // the next step's copies have landed (a tile's first S stages are here already)
+          if (kb >= S - 1) wait_vm<(S - 2) * ND + NR>();
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (q == 0) acc[i][j] = mfma_fp4<0, 0>(x[at % (kAhead + 1)], b[0][j], acc[i][j], sx[i], sb[j]);
+          else acc[i][j] = mfma_fp4<1, 1>(x[at % (kAhead + 1)], b[1][j], acc[i][j], sx[i], sb[j]);
+          __builtin_amdgcn_sched_barrier(0);
+          const int a = at + kAhead;
+          if (j == 0 && a < 2 * MI) x[a % (kAhead + 1)] = xfrag(slot, a);
+          if (j == 1 && a < MI) sx[a] = sfrag(par, 16 * (wm * MI + a) + m);
+          if (q == 0) {  // the second half's weights, spread over the row blocks
+            constexpr int kPer = NJ > MI ? NJ / MI : 1, kEvery = MI > NJ ? MI / NJ : 1;
+            if (i % kEvery == 0 && j >= 2 && j < 2 + kPer) b[1][i / kEvery * kPer + j - 2] = wfrag(slot, i / kEvery * kPer + j - 2, 1);
+          }
+          if (at >= kLast) {
+            const int t = (at - kLast) * NJ + j;
+            if (j == 0) x[a % (kAhead + 1)] = xfrag(next, a - 2 * MI);
+            if (j == 1) sx[a - 2 * MI] = sfrag(1 - par, 16 * (wm * MI + a - 2 * MI) + m);
+#pragma unroll
+            for (int n = 0; n < NJ; ++n) {
+              if (n * kSlots / NJ == t) {
+                b[0][n] = wfrag(next, n, 0);
+                sn[n] = sfrag(1 - par, BM + 16 * (wn * NJ + n) + m);
+              }
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+              if (d * kSlots / ND == t) copy(d, k0, lds + slot * kStage);
+          }
+        }
+        if (at == 0) store_s(snext, 1 - par);
+        if (at == 0) load_s(sload);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) sb[j] = sn[j];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    rows_of(cur);
+    aim(cur);
+    saim(cur);
+    load_s(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) copy(d, k_of(s), lds + s * kStage);
+    store_s(0, 0);
+    load_s(1);
+    wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      b[0][j] = wfrag(0, j, 0);
+      sb[j] = sfrag(0, BM + 16 * (wn * NJ + j) + m);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      x[i] = xfrag(0, i);
+      sx[i] = sfrag(0, 16 * (wm * MI + i) + m);
+    }
+    int slot = 0, par = 0;
+    for (;;) {
+      const int after = item + (int)(gridDim.x >> 3);
+      const Tile next = after < end ? tile_at(after) : cur;  // (the last tile's copies go on over it: nothing reads them)
+      rows_of(next);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+      for (int kb = 0; kb < nrun; ++kb) {
+        if (kb == nrun - S) aim(next);  // from here on the copies are the next tile's
+        if (kb == nrun - 2) saim(next);
+        const int ahead = kb + S < nrun ? kb + S : kb + S - nrun;
+        step(kb, kb + 1 < nrun ? kb + 1 : 0, kb + 2 < nrun ? kb + 2 : kb + 2 - nrun, k_of(ahead), slot, par);
+        slot = slot == S - 1 ? 0 : slot + 1;
+        par = 1 - par;
+      }
+      // A lane has tokens 16 i + 4 g + r (r 0..3) and CN neighbouring channels from n0 on
+      // (with an activation, and their up rows)
+      const int el = opaque_lane(), em = el & 15, eg = el >> 4;
+      const int n0 = cur.n + wn * (kCols / WN) + CN * em;
+      const int t0 = 16 * wm * MI + 4 * eg;
+      uint32_t live = ~0u;  // bit 4 i + r: the row is one of x
+      if (indexed) {
+        int er[MI][4];
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) er[i][r] = c.row_index[cur.rt.row0 + (t0 + 16 * i + r < cur.rt.cnt ? t0 + 16 * i + r : 0)];
+        live = 0;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) live |= er[i][r] >= 0 && er[i][r] < c.x_rows ? 1u << (4 * i + r) : 0u;
+      }
+      uint32_t bb[NJ];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) bb[n] = 0;
+      if (c.bias != nullptr) {
+        const int64_t at = (int64_t)cur.rt.e * c.N;
+        load_run<CN>(c.bias, at, n0, NO - 1, c.bias_dtype, bb);
+        if constexpr (ACT) load_run<CN>(c.bias, at + NO, n0, NO - 1, c.bias_dtype, bb + CN);
+      }
+      // With the biases, the next tile's first S stages are here: the steps that would
+      // wait for them need not wait for the stores below
+      wait_vm<0>();
+      float bias[NJ];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) bias[n] = bits_to_f32(opaque_bits(bb[n]), c.bias_dtype);
+      with_act(ACT ? c.act : -1, [&](auto a) __attribute__((always_inline)) {
+        constexpr int A = decltype(a)::value;
+        const RowOut<CN> out(c, cur.rt, NO, n0);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          // one row block after the other, so that their results do not all sit in
+          // registers at once
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) asm volatile("" : "+v"(acc[i][j]) : : "memory");
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float y[CN];
+#pragma unroll
+            for (int n = 0; n < CN; ++n) {
+              y[n] = acc[i][n][r] + bias[n];
+              if constexpr (ACT) y[n] = gated(A, y[n], acc[i][CN + n][r] + bias[CN + n], c);
+              if constexpr (GROUPED) y[n] = (live >> (4 * i + r)) & 1u ? y[n] : 0.0f;
+            }
+            const int t = t0 + 16 * i + r;
+            if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
+              uint32_t top = 0;
+#pragma unroll
+              for (int n = 0; n < CN; ++n) {
+                const uint32_t b = __float_as_uint(y[n]) & 0x7fffffffu;
+                top = b > top ? b : top;
+              }
+              top = quad_max(top);
+              auto with = [&](uint32_t o) { top = o > top ? o : top; };
+              with((uint32_t)dpp_i<kDppHalfMirror>((int)top));
+              if constexpr (CN == 2) with((uint32_t)dpp_i<kDppMirror>((int)top));
+              const uint32_t byte = mx_scale_byte(top);
+              const float s = __uint_as_float(byte << 23);
+              uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, towards_zero<FTM_DT_F32>(y[0]), towards_zero<FTM_DT_F32>(y[1]), s, 0);
+              if constexpr (CN == 4)
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, towards_zero<FTM_DT_F32>(y[2]), towards_zero<FTM_DT_F32>(y[3]), s, 1);
+              w = byte == 255u ? 0u : positive_zeros(w);
+              if (t < cur.rt.cnt && n0 < NO) {
+                const int64_t row = cur.rt.row0 + t;
+                if constexpr (CN == 4) *(uint16_t*)((char*)c.out + (row * NO + n0) / 2) = (uint16_t)w;
+                else *((uint8_t*)c.out + (row * NO + n0) / 2) = (uint8_t)w;
+                if ((em & (32 / CN - 1)) == 0) out_scale[(row * NO + n0) / 32] = (uint8_t)byte;
+              }
+            } else {
+              out.store(t, y);
+            }
+          }
+        }
+      });
+      if (after >= end) break;
+      cur = next;
+      item = after;
+    }
+    wait_vm<0>();  // the copies past the last step, before the LDS is given back
+  }
+  if constexpr (GROUPED && !QOUT) {  // rows of no expert
+    const int head = scan.head(), tail = scan.tail(), none = head + ((int)c.rows - tail);
+    for (int z = blockIdx.x; z < none; z += gridDim.x) {
+      const int64_t row = z < head ? z : tail + (z - head);
+      for (int n = threadIdx.x; n < NO; n += kThreads) store_scalar(c.out, row * NO + n, c.out_dtype, 0.0f);
+    }
+  }
+}
+
 namespace {
 
 hipError_t any(const ftm_w4a4& c, hipStream_t st) {
@@ -545,6 +886,31 @@ hipError_t split(const ftm_w4a4& c, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int WM, int WN, int MI, int NJ, int S, bool ACT, bool GROUPED, bool QOUT>
+hipError_t tile(const ftm_w4a4& c, uint8_t* out_scale, hipStream_t st) {
+  constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, lds = S * (BM + BN) * kRow + 16 * (BM + BN);
+  static_assert(lds <= kMaxLds, "fits a CU");
+  constexpr int resident = kCUs * (2 * lds <= kMaxLds ? 2 : 1);  // workgroups the chip holds at once
+  const int cols = ACT ? BN / 2 : BN;
+  const int64_t mt = row_tiles(c, BM), nt = (out_cols(c) + cols - 1) / cols;
+  if (mt * nt > INT32_MAX) return hipErrorInvalidValue;
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w4a4_tile<WM, WN, MI, NJ, S, ACT, GROUPED, QOUT>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, lds);
+  if (e != hipSuccess) return e;
+  const int64_t grid = mt * nt < resident ? (mt * nt + 7) / 8 * 8 : resident;  // the same for every XCD
+  kernel<<<dim3((unsigned)grid), dim3(64 * WM * WN), lds, st>>>(c, out_scale, (int)mt, (int)nt);
+  return hipGetLastError();
+}
+template <int WM, int WN, int MI, int NJ, int S>
+hipError_t tile(const ftm_w4a4& c, hipStream_t st) {
+  if (c.offsets != nullptr)
+    return c.act >= 0 ? tile<WM, WN, MI, NJ, S, true, true, false>(c, nullptr, st)
+                      : tile<WM, WN, MI, NJ, S, false, true, false>(c, nullptr, st);
+  return c.act >= 0 ? tile<WM, WN, MI, NJ, S, true, false, false>(c, nullptr, st)
+                    : tile<WM, WN, MI, NJ, S, false, false, false>(c, nullptr, st);
+}
+
 // Whether a tile's 32-bit offsets (below 2^30) reach its tokens (256 rows from its
 // first, or all of x where they are read through an index), its weight rows and its results.
 bool offsets_ok(const ftm_w4a4& c) {
@@ -557,10 +923,17 @@ bool offsets_ok(const ftm_w4a4& c) {
 
 hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
   if (c.K < kMinK || !offsets_ok(c)) return any(c, st);
-  if (c.offsets != nullptr) return split<1, 2, 4, 2>(c, st);
+  if (c.offsets != nullptr) {
+    const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
+    if (seg >= 128) return tile<2, 2, 4, 8, 3>(c, st);
+    if (seg >= 16) return tile<1, 4, 4, 4, 3>(c, st);
+    return split<1, 2, 4, 2>(c, st);
+  }
   const int64_t M = c.rows;
   if (M <= 16) return split<1, 1, 4, 4>(c, st);
   if (M <= 32) return split<2, 1, 4, 3>(c, st);
+  if (M > 1024 && c.row_index == nullptr) return tile<2, 2, 8, 8, 2>(c, st);
+  if (M > 512 && c.row_index == nullptr) return tile<2, 2, 4, 8, 3>(c, st);
   return split<4, 4, 4, 2>(c, st);
 }
 
