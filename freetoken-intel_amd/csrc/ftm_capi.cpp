@@ -675,6 +675,8 @@ int ftm_w4a4_moe_forward(const ftm_w4a4_moe* call, void* workspace, size_t ws_by
   if (((uintptr_t)c.x | (uint64_t)c.x_stride | (uintptr_t)c.out) % dt_bytes(c.dtype) != 0 ||
       (uintptr_t)c.topk_w % dt_bytes(c.topk_w_dtype) != 0 || (uintptr_t)c.topk_ids % (c.ids_dtype == FTM_ID_I64 ? 8 : 4) != 0)
     return FTM_ERR_ALIGN;
+  hipError_t e = hipSuccess;
+  if (launch_w4a4_moe_few(c, (uint8_t*)(ws + L.hq), (uint8_t*)(ws + L.hs), (hipStream_t)stream, e)) return hip_rc(e);
   rc = ftm_sort_tokens(c.topk_ids, c.ids_dtype, T, k, E, offsets, row_of_pair, pair_of_row, token_of_row, ws + L.sort,
                        L.total - L.sort, stream);
   if (rc == FTM_OK) rc = ftm_w4a4_linear_dynamic(c.x, c.dtype, c.x_stride, &a, stream);

@@ -514,6 +514,328 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, 
   });
 }
 
+// ------------------------------------------------------------------ few tokens
+constexpr int kFewRows = 16;    // of one workgroup: the columns of a 16 x 16 product
+constexpr int kFewPairs = 256;  // (token, expert) pairs of a layer: four a lane
+
+// The pairs of one expert, found by every wave for itself.  Workgroups come by pair: the
+// one of the expert's pair number 0, cap, 2 cap .. takes that pair and the next cap - 1
+// of the same expert, the others leave.  list[0 .. cnt) are the pairs; cnt 0: nothing to do.
+struct FewPairs {
+  int e, cnt;
+  __device__ __forceinline__ FewPairs(const void* ids, bool ids64, int P, int E, int p, int cap, int* list) {
+    const int lane = threadIdx.x & 63;
+    int id[kFewPairs / 64];
+#pragma unroll
+    for (int i = 0; i < kFewPairs / 64; ++i) {
+      const int at = lane + 64 * i;
+      id[i] = -1;
+      if (at < P) {
+        const int64_t v = ids64 ? ((const int64_t*)ids)[at] : (int64_t)((const int32_t*)ids)[at];
+        id[i] = v >= 0 && v < E ? (int)v : -1;
+      }
+    }
+    e = -1;
+#pragma unroll
+    for (int i = 0; i < kFewPairs / 64; ++i)
+      if ((p >> 6) == i) e = __builtin_amdgcn_readlane(id[i], p & 63);
+    cnt = 0;
+    if (e < 0) return;
+    uint64_t mine[kFewPairs / 64];
+    int before = 0, all = 0;  // matches before p, and of all pairs
+#pragma unroll
+    for (int i = 0; i < kFewPairs / 64; ++i) {
+      mine[i] = __ballot(id[i] == e);
+      all += __popcll(mine[i]);
+      if ((p >> 6) > i) before += __popcll(mine[i]);
+      if ((p >> 6) == i) before += __popcll(mine[i] & ((1ull << (p & 63)) - 1));
+    }
+    if (before % cap != 0) return;
+    cnt = all - before < cap ? all - before : cap;
+    int base = -before;
+#pragma unroll
+    for (int i = 0; i < kFewPairs / 64; ++i) {
+      const int r = base + __popcll(mine[i] & ((1ull << lane) - 1));
+      if (id[i] == e && r >= 0 && r < cap) list[r] = lane + 64 * i;
+      base += __popcll(mine[i]);
+    }
+  }
+};
+
+struct FewCall {
+  const char* x;          // wide rows
+  int64_t x_stride;
+  const char* w;          // of expert 0
+  const uint8_t* w_scale;
+  const void* bias;
+  int64_t w_stride, w_scale_stride;
+  int N, K, bias_dtype, act;
+  float act_alpha, act_limit;
+  int cap;                // rows of a workgroup, at most
+  // dense: the product's rows, dtype and result
+  int64_t rows;
+  void* out;
+  int out_dtype;
+  // a layer's first product: its pairs, and h quantised, a row a pair
+  const void* ids;
+  int ids64, P, E, k;
+  uint8_t *hq, *hs;
+};
+
+// Up to 16 tokens whose values are still wide: a workgroup quantises them itself, each wave
+// the K that it multiplies, while its weights are under way, and multiplies them by a
+// tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.  A layer's first
+// product (MOE) finds the tokens of its expert in the ids, and quantises its 32
+// channels of h, one block, in the epilogue.
+template <int XDT, int NT, int NW, int S, bool MOE>
+__global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
+  using V = Vec8<XDT>;
+  constexpr int kStage = NT * 16 * kRow, kParts = (NT + NW - 1) / NW, kBatch = 4;
+  extern __shared__ char lds[];  // [NW] of: ring [S][kStage], codes [per][cap][kRow], scales of weights and tokens; then the sums
+  __shared__ int lists[NW][kFewRows];
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nt = blockIdx.x % ntiles;
+  const bool act = MOE || c.act >= 0;
+  const int NO = act ? c.N / 2 : c.N, K = c.K, nb = K / 32, cap = c.cap;
+  int e = 0, cnt = cap;
+  if constexpr (MOE) {
+    const FewPairs pairs(c.ids, c.ids64 != 0, c.P, c.E, blockIdx.x / ntiles, cap, lists[wave]);
+    e = pairs.e;
+    cnt = pairs.cnt;
+    if (cnt == 0) return;
+  }
+  const int cols = act ? 8 * NT : 16 * NT, n0 = nt * cols, ncol = NO - n0 < cols ? NO - n0 : cols;
+  f32x4 acc[1][NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[0][j] = (f32x4){0, 0, 0, 0};
+  SplitBias bias[kParts];
+  auto request = [&] {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      bias[p].request(c.bias, c.bias_dtype, (int64_t)e * c.N, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
+  };
+  const int nsteps = (nb + 7) / 8, per = (nsteps + NW - 1) / NW, pitch = scale_pitch(per);
+  const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
+  if (lo < hi) {
+    const SplitWeights<NT> weights(c.w + (int64_t)e * c.w_stride, NO, K, act, n0, ncol);
+    char* ring = lds + wave * (S * kStage + per * cap * kRow + (16 * NT + cap) * pitch);
+    char* codes = ring + S * kStage;
+    char* scales = codes + per * cap * kRow;  // of the weights, then of the tokens
+    char* xscales = scales + 16 * NT * pitch;
+    auto issue = [&](int step, int slot) __attribute__((always_inline)) {
+      weights.issue(ring + slot * kStage, step < hi ? (uint32_t)step * 128u : kNowhere);
+    };
+    FillScales<16 * NT> fill;
+#pragma unroll
+    for (int i = 0; i < fill.kRows; ++i)
+      fill.p[i] = c.w_scale + (int64_t)e * c.w_scale_stride + (n0 + SplitWeights<NT>::row(NO, act, ncol, fill.row(i))) * nb;
+    // half a wave takes 256 values of one row: of this wave's one step two rows at a time,
+    // else two steps of one
+    const int half = lane >> 5, l32 = lane & 31, n = hi - lo, hp = (n + 1) / 2;
+    const int turns = n == 1 ? (cnt + 1) / 2 : cnt * hp;
+    auto row_of = [&](int t) { return n == 1 ? 2 * t + half : t / hp; };
+    auto step_of = [&](int t) { return n == 1 ? 0 : 2 * (t % hp) + half; };
+    V v[kBatch];
+    auto load = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = t0 + i, r = row_of(t), s = step_of(t), k = 256 * (lo + s) + 8 * l32;
+        if (t < turns && r < cnt && s < n && k < K) {
+          const int64_t row = MOE ? lists[wave][r] / c.k : r;
+          v[i].load(c.x + row * c.x_stride + (int64_t)(k / 8) * V::kBytes);
+        } else {
+          v[i].zero();
+        }
+      }
+    };
+    auto quantise = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = t0 + i, r = row_of(t), s = step_of(t);
+        const uint32_t byte = mx_scale_byte(quad_max(v[i].max_bits()));
+        const uint32_t w = mx_codes<XDT>(v[i], byte);
+        if (t < turns && r < cnt && s < n) {
+          *(uint32_t*)(codes + (s * cap + r) * kRow + 16 * ((l32 >> 2) ^ swz(r)) + 4 * (l32 & 3)) = w;
+          if ((l32 & 3) == 0) *(uint8_t*)(xscales + r * pitch + 8 * s + (l32 >> 2)) = (uint8_t)byte;
+        }
+      }
+    };
+    fill(scales, lo, per, nb, [&] {
+      request();
+      load(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < S; ++u) issue(lo + u, u);
+    });
+    quantise(0);
+    for (int t = kBatch; t < turns; t += kBatch) {
+      load(t);
+      quantise(t);
+    }
+    __builtin_amdgcn_wave_barrier();
+    const int xr = m < cnt ? m : 0;
+    int slot = 0;
+    for (int step = lo; step < hi; ++step) {
+      wait_vm<(S - 1) * 2 * NT>();  // this step's copies have landed
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const char* st = ring + slot * kStage;
+      u32x4 w[2][NT], x[2];
+      uint32_t sw[NT];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[q][j] = stage_piece(st, 16 * j + m, q, g);
+        x[q] = stage_piece(codes + (step - lo) * cap * kRow, xr, q, g);
+      }
+      auto scale = [&](const char* at, int r) { return scale_operand(*(const u32x2*)(at + r * pitch + 8 * (step - lo)), g); };
+#pragma unroll
+      for (int j = 0; j < NT; ++j) sw[j] = scale(scales, 16 * j + m);
+      const uint32_t sx = scale(xscales, xr);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the operands are here: the slot is free
+      __builtin_amdgcn_sched_barrier(0);
+      issue(step + S, slot);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        acc[0][j] = mfma_fp4<0, 0>(w[0][j], x[0], acc[0][j], sw[j], sx);
+        acc[0][j] = mfma_fp4<1, 1>(w[1][j], x[1], acc[0][j], sw[j], sx);
+      }
+      slot = slot == S - 1 ? 0 : slot + 1;
+    }
+    wait_vm<0>();  // the copies past the last step, before the sums take their place
+  } else {
+    request();
+  }
+  constexpr int kSums = NW * NT * 1024, kPitch = 36;  // h: [16][kPitch] behind the sums
+  float* h = (float*)(lds + kSums);
+  with_act(c.act, [&](auto a) {
+    constexpr int A = decltype(a)::value;
+    split_sums<1, NT, NW>(lds, acc, A >= 0, [&](int p, int b, f32x4 u, f32x4 v) {
+      if (A >= 0 && g >= 2) return;
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = u[r] + bias[p].at(r, c.bias_dtype);
+        if constexpr (A >= 0) y[r] = gated(A, y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
+      }
+      if constexpr (MOE) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) h[m * kPitch + 8 * b + 4 * g + r] = y[r];
+      } else {
+        RowOut<4>(c, RowTile{0, cnt, 0}, NO, split_channel<NT>(act, n0, b, g)).store(m, y);
+      }
+    });
+  });
+  if constexpr (MOE) {
+    static_assert(NT == 4, "a tile is one block of h");
+    __syncthreads();
+    const int row = lane >> 2, part = lane & 3;
+    if (wave != 0) return;
+    Vec8<FTM_DT_F32> v;
+    v.load((const char*)(h + row * kPitch + 8 * part));
+    const uint32_t byte = mx_scale_byte(quad_max(v.max_bits()));
+    const uint32_t codes = mx_codes<FTM_DT_F32>(v, byte);
+    if (row >= cnt) return;
+    const int64_t at = (int64_t)lists[0][row] * (NO / 32) + nt;
+    *(uint32_t*)(c.hq + at * 16 + 4 * part) = codes;
+    if (part == 0) c.hs[at] = (uint8_t)byte;
+  }
+}
+
+// A layer's second product and sum for few tokens: one token x 16 output channels a
+// workgroup.  The steps of 256 K of the token's experts, one expert behind the other, are
+// split over the waves; a step's results are weighted by its expert's weight and added
+// up in fp32, the waves' sums in order, so the order is the same in each call.  h comes
+// from memory (every lane of a group the same block), the weights through LDS.
+template <int NW, int S>
+__global__ __launch_bounds__(64 * NW) void k_w4a4_few_down(ftm_w4a4_moe c, const uint8_t* hq, const uint8_t* hs, int ntiles) {
+  __shared__ __attribute__((aligned(1024))) char ring[NW][S][16 * kRow];
+  __shared__ float sums[NW][16];
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = xcd_item(blockIdx.x, gridDim.x);  // the tokens of a column side by side: they share weights
+  const int t = item % c.T, n0 = item / c.T * 16, H = c.hidden, nb = c.inter / 32, Kb = c.inter / 2;
+  const int ns = (nb + 7) / 8;
+  // lane j: the token's j-th expert and its weight
+  int e = -1;
+  float wt = 0.0f;
+  if (lane < c.k) {
+    const int64_t at = (int64_t)t * c.k + lane;
+    const int64_t v = c.ids_dtype == FTM_ID_I64 ? ((const int64_t*)c.topk_ids)[at] : (int64_t)((const int32_t*)c.topk_ids)[at];
+    e = v >= 0 && v < c.num_experts ? (int)v : -1;
+    wt = load_scalar(c.topk_w, at, c.topk_w_dtype);
+  }
+  const uint64_t valid = __ballot(e >= 0);
+  const int total = __popcll(valid) * ns, per = (total + NW - 1) / NW;
+  const int lo = wave * per, hi = lo + per < total ? lo + per : total;
+  const int ncol = H - n0 < 16 ? H - n0 : 16, row = m < ncol ? m : ncol - 1;
+  f32x4 sum = {0, 0, 0, 0};
+  uint64_t left = valid;  // the experts from this wave's first on
+  int s = lo;             // its step within the first of them
+  for (; s >= ns && left != 0; s -= ns) left &= left - 1;
+  for (int u0 = lo; u0 < hi; u0 += S) {
+    u32x4 h[S][2];
+    u32x2 sh[S], sw[S];
+    float wj[S];
+    int at[S];
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      if (u0 + u >= hi) break;
+      const int j = __builtin_ctzll(left), ej = __builtin_amdgcn_readlane(e, j);
+      wj[u] = readlane_f(wt, j);
+      at[u] = s;
+      const Rsrc res = make_rsrc((const char*)c.w2 + ((int64_t)ej * H + n0) * Kb, (uint32_t)(ncol * Kb));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + (lane >> 3), in = r < ncol ? r : ncol - 1;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LPtr)(ring[wave][u] + 1024 * i), 16,
+                                                 in * Kb + 128 * s + 16 * ((lane & 7) ^ swz(r)), 0, 0, 0);
+      }
+      const int64_t pair = (int64_t)t * c.k + j;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int b = 8 * s + 4 * q + g;
+        h[u][q] = *(const u32x4*)(hq + (pair * nb + (b < nb ? b : nb - 1)) * 16);
+      }
+      sh[u] = load_scales(hs + pair * nb, s, nb);
+      sw[u] = load_scales(c.w2_scale + ((int64_t)ej * H + n0 + row) * nb, s, nb);
+      if (++s == ns) {
+        s = 0;
+        left &= left - 1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      if (u0 + u >= hi) break;
+      asm volatile("" : "+v"(sw[u]) : : "memory");  // requested behind the step's copies: with it they have landed
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t a = scale_operand(fit_scales(sw[u], at[u], nb), g), b = scale_operand(fit_scales(sh[u], at[u], nb), g);
+      f32x4 d = mfma_fp4<0, 0>(stage_piece(ring[wave][u], m, 0, g), h[u][0], (f32x4){0, 0, 0, 0}, a, b);
+      d = mfma_fp4<1, 1>(stage_piece(ring[wave][u], m, 1, g), h[u][1], d, a, b);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[r] = fmaf(wj[u], d[r], sum[r]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slots are free
+  }
+  if (m == 0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[wave][4 * g + r] = sum[r];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 || n0 + (int)threadIdx.x >= H) return;
+  const int n = n0 + threadIdx.x;
+  float y = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) y += sums[w][threadIdx.x];
+  if (c.w2_bias != nullptr)
+    for (uint64_t b = valid; b != 0; b &= b - 1) {
+      const int j = __builtin_ctzll(b);
+      y = fmaf(readlane_f(wt, j), load_scalar(c.w2_bias, (int64_t)__builtin_amdgcn_readlane(e, j) * H + n, c.w2_bias_dtype), y);
+    }
+  store_scalar(c.out, (int64_t)t * H + n, c.dtype, y);
+}
+
 // ------------------------------------------------------------------ LDS tiles
 // A tile is BM = 16 MI WM tokens x BN = 16 NJ WN weight rows (with an activation BN / 2 gate
 // rows and their up rows): WM WN waves of 16 MI tokens x 16 NJ weight rows each over the
@@ -937,7 +1259,63 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
   return split<4, 4, 4, 2>(c, st);
 }
 
+namespace {
+
+template <int NT, int NW, int S>
+int few_lds(int K, int cap) {
+  const int per = ((K + 255) / 256 + NW - 1) / NW;
+  const int lds = NW * (S * NT * 16 * kRow + per * cap * kRow + (16 * NT + cap) * scale_pitch(per));
+  constexpr int sums = NW * NT * 1024 + 16 * 36 * 4;
+  return lds > sums ? lds : sums;
+}
+template <int XDT, int NT, int NW, int S, bool MOE>
+hipError_t few(const FewCall& c, hipStream_t st) {
+  const int lds = few_lds<NT, NW, S>(c.K, c.cap);
+  const bool act = MOE || c.act >= 0;
+  const int cols = act ? 8 * NT : 16 * NT, ntiles = ((act ? c.N / 2 : c.N) + cols - 1) / cols;
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w4a4_few<XDT, NT, NW, S, MOE>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)((MOE ? c.P : 1) * ntiles)), dim3(64 * NW), lds, st>>>(c, ntiles);
+  return hipGetLastError();
+}
+template <int NT, int NW, int S, bool MOE>
+hipError_t few(const FewCall& c, int dt, hipStream_t st) {
+  if (dt == FTM_DT_F32) return few<FTM_DT_F32, NT, NW, S, MOE>(c, st);
+  if (dt == FTM_DT_F16) return few<FTM_DT_F16, NT, NW, S, MOE>(c, st);
+  return few<FTM_DT_BF16, NT, NW, S, MOE>(c, st);
+}
+
+}  // namespace
+
+// A layer of few tokens in two kernels, if it is one: hq and hs hold h, a row a pair.
+bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStream_t st, hipError_t& e) {
+  const int P = c.T * c.k, H = c.hidden, I = c.inter, cap = c.T < kFewRows ? c.T : kFewRows;
+  if (c.T > kFewRows || P > kFewPairs || c.k > 64 || H < kMinK || I < kMinK) return false;
+  if ((((uintptr_t)c.x | (uint64_t)c.x_stride) & 15u) != 0) return false;
+  if ((int64_t)2 * I * (H / 2) + 256 >= (int64_t)kNowhere) return false;
+  const FewCall f = {(const char*)c.x, c.x_stride, (const char*)c.w13, c.w13_scale, c.w13_bias, (int64_t)2 * I * (H / 2),
+                     (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
+                     c.topk_ids, c.ids_dtype == FTM_ID_I64, P, c.num_experts, c.k, hq, hs};
+  constexpr int kRoom = kMaxLds - 1024;  // beside the lists
+  if (few_lds<4, 8, 2>(H, cap) <= kRoom && H > 8 * 256) e = few<4, 8, 2, true>(f, c.dtype, st);
+  else if (few_lds<4, 8, 1>(H, cap) <= kRoom) e = few<4, 8, 1, true>(f, c.dtype, st);
+  else return false;
+  if (e != hipSuccess) return true;
+  const int ntiles = (H + 15) / 16;
+  k_w4a4_few_down<8, 4><<<dim3((unsigned)(ntiles * c.T)), dim3(512), 0, st>>>(c, hq, hs, ntiles);
+  e = hipGetLastError();
+  return true;
+}
+
 hipError_t launch_w4a4_dynamic(const ftm_w4a4& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {
+  if (c.offsets == nullptr && c.row_index == nullptr && c.rows <= 4 && c.rows * c.K <= 16384 && c.K >= kMinK && offsets_ok(c) &&
+      (((uintptr_t)x | (uint64_t)x_stride) & 15u) == 0) {
+    const FewCall f = {(const char*)x, x_stride, (const char*)c.w, c.w_scale, c.bias, 0, 0, c.N, c.K, c.bias_dtype, c.act, c.act_alpha,
+                       c.act_limit, (int)c.rows, c.rows, c.out, c.out_dtype, nullptr, 0, 0, 1, 1, nullptr, nullptr};
+    return few<1, 4, 4, false>(f, dt, st);
+  }
   const hipError_t e = launch_quant_mxfp4(x, dt, c.x_rows, c.K, x_stride, (uint8_t*)const_cast<void*>(c.x),
                                           const_cast<uint8_t*>(c.x_scale), st);
   return e != hipSuccess ? e : launch_w4a4(c, st);
