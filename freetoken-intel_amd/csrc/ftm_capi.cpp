@@ -663,7 +663,7 @@ int ftm_w4a4_moe_forward(const ftm_w4a4_moe* call, void* workspace, size_t ws_by
   int32_t* pair_of_row = (int32_t*)(ws + L.pair_of_row);
   int32_t* token_of_row = (int32_t*)(ws + L.token_of_row);
   float *h = (float*)(ws + L.h), *y = (float*)(ws + L.y);
-  const ftm_w4a4 a = {ws + L.xq, (uint8_t*)(ws + L.xs), c.w13, c.w13_scale, c.w13_bias, h, offsets, token_of_row, P, T,
+  const ftm_w4a4 a = {ws + L.xq, (uint8_t*)(ws + L.xs), c.w13, c.w13_scale, c.w13_bias, ws + L.hq, offsets, token_of_row, P, T,
                       (int64_t)2 * I * (H / 2), (int64_t)2 * I * (H / 32), 2 * I, H, E, c.w13_bias_dtype, FTM_DT_F32, c.act,
                       c.act_alpha, c.act_limit};
   const ftm_w4a4 b = {ws + L.hq, (uint8_t*)(ws + L.hs), c.w2, c.w2_scale, c.w2_bias, y, offsets, nullptr, P, P,
@@ -679,8 +679,9 @@ int ftm_w4a4_moe_forward(const ftm_w4a4_moe* call, void* workspace, size_t ws_by
   if (launch_w4a4_moe_few(c, (uint8_t*)(ws + L.hq), (uint8_t*)(ws + L.hs), (hipStream_t)stream, e)) return hip_rc(e);
   rc = ftm_sort_tokens(c.topk_ids, c.ids_dtype, T, k, E, offsets, row_of_pair, pair_of_row, token_of_row, ws + L.sort,
                        L.total - L.sort, stream);
-  if (rc == FTM_OK) rc = ftm_w4a4_linear_dynamic(c.x, c.dtype, c.x_stride, &a, stream);
-  if (rc == FTM_OK) rc = ftm_w4a4_linear_dynamic(h, FTM_DT_F32, (int64_t)I * 4, &b, stream);
+  if (rc == FTM_OK) rc = ftm_quant_mxfp4(c.x, c.dtype, T, H, c.x_stride, (uint8_t*)(ws + L.xq), (uint8_t*)(ws + L.xs), stream);
+  if (rc == FTM_OK) rc = hip_rc(launch_w4a4_quantised(a, h, (uint8_t*)(ws + L.hs), (hipStream_t)stream));
+  if (rc == FTM_OK) rc = hip_rc(launch_w4a4(b, (hipStream_t)stream));
   if (rc == FTM_OK)
     rc = ftm_combine_tokens(y, FTM_DT_F32, (int64_t)H * 4, c.topk_w, c.topk_w_dtype, row_of_pair, T, k, H, c.out, c.dtype,
                             stream);

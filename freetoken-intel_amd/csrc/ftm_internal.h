@@ -220,6 +220,8 @@ hipError_t launch_w8a8_dynamic(const ftm_w8a8& call, const void* x, int x_dt, in
 hipError_t launch_quant_mxfp4(const void* x, int dt, int64_t rows, int K, int64_t x_stride, uint8_t* blocks,
                               uint8_t* scales, hipStream_t st);
 hipError_t launch_w4a4(const ftm_w4a4& call, hipStream_t st);
+// Grouped and gated, the result quantised (call.out: blocks; h: scratch)
+hipError_t launch_w4a4_quantised(const ftm_w4a4& call, float* h, uint8_t* out_scale, hipStream_t st);
 // A layer of few tokens in two kernels, where it is one (else false, and nothing is launched)
 bool launch_w4a4_moe_few(const ftm_w4a4_moe& call, uint8_t* hq, uint8_t* hs, hipStream_t st, hipError_t& e);
 // ... of x still wide (call.x and call.x_scale: scratch for its codes)

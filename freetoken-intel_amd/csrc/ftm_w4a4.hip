@@ -160,6 +160,26 @@ hipError_t launch_quant_mxfp4(const void* x, int dt, int64_t rows, int K, int64_
   return quant<FTM_DT_BF16, 1>(p, x_stride, rows, K, b, scales, st);
 }
 
+// ------------------------------------------------------------------ activation
+// 1 / (1 + e^-z) from the hardware's 2^t and 1 / t, one step of fp32 off each.  Rounding
+// t = -z log2(e) moves e^-z by |z| 2^-24 at most, as much as half a step of z does.  In
+// fp32's own division and exponential the epilogue of a tile took half as long as its
+// products (clamped gate, 8192 rows of 2880 x 5760: 231 us, so 139).
+__device__ __forceinline__ float sigmoid_of(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+// act(gate) up, the same in every kernel here; NaN where either is.
+template <int A, class C>
+__device__ __forceinline__ float act_gated(float g, float u, const C& c) {
+  if constexpr (A == FTM_ACT_SILU) return g * sigmoid_of(g) * u;
+  if constexpr (A == FTM_ACT_SWIGLU_OAI) {
+    g = g > c.act_limit ? c.act_limit : g;
+    u = u > c.act_limit ? c.act_limit : u < -c.act_limit ? -c.act_limit : u;
+    return (u + 1.0f) * (g * sigmoid_of(c.act_alpha * g));
+  }
+  return gated(A, g, u, c);
+}
+
 // ------------------------------------------------------------------ any size
 // 16 tokens x 16 output channels a wave, operands straight from memory with 64-bit
 // addresses.  Weights are A and tokens B, so a lane has four neighbouring channels of
@@ -204,8 +224,10 @@ __global__ __launch_bounds__(256) void k_w4a4_any(ftm_w4a4 c, int mtiles, int nt
       if (src >= 0) {
         const int64_t at = (int64_t)rt.e * c.N + n;
         y = acc[0][r] + (c.bias != nullptr ? load_scalar(c.bias, at, c.bias_dtype) : 0.0f);
-        if constexpr (ACT)
-          y = gated(c.act, y, acc[1][r] + (c.bias != nullptr ? load_scalar(c.bias, at + NO, c.bias_dtype) : 0.0f), c);
+        if constexpr (ACT) {
+          const float u = acc[1][r] + (c.bias != nullptr ? load_scalar(c.bias, at + NO, c.bias_dtype) : 0.0f), g = y;
+          with_act(c.act, [&](auto a) { y = act_gated<decltype(a)::value>(g, u, c); });
+        }
       }
       store_scalar(c.out, (rt.row0 + m) * NO + n, c.out_dtype, y);
     }
@@ -506,7 +528,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         y[r] = u[r] + bias[p].at(r, c.bias_dtype);
-        if constexpr (A >= 0) y[r] = gated(A, y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
+        if constexpr (A >= 0) y[r] = act_gated<A>(y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
         y[r] = rr[p] >= 0 && rr[p] < x_rows ? y[r] : 0.0f;
       }
       RowOut<4>(c, rt, NO, split_channel<NT>(act, n0, b, g)).store(16 * (b / NT) + m, y);
@@ -717,7 +739,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         y[r] = u[r] + bias[p].at(r, c.bias_dtype);
-        if constexpr (A >= 0) y[r] = gated(A, y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
+        if constexpr (A >= 0) y[r] = act_gated<A>(y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
       }
       if constexpr (MOE) {
 #pragma unroll
@@ -1129,8 +1151,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
 #pragma unroll
             for (int n = 0; n < CN; ++n) {
               y[n] = acc[i][n][r] + bias[n];
-              if constexpr (ACT) y[n] = gated(A, y[n], acc[i][CN + n][r] + bias[CN + n], c);
-              if constexpr (GROUPED) y[n] = (live >> (4 * i + r)) & 1u ? y[n] : 0.0f;
+              if constexpr (ACT) y[n] = act_gated<A>(y[n], acc[i][CN + n][r] + bias[CN + n], c);
             }
             const int t = t0 + 16 * i + r;
             if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
@@ -1158,6 +1179,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
               }
             } else {
               out.store(t, y);
+              if constexpr (GROUPED) {  // a row whose index names none: zeros over it
+                if (!((live >> (4 * i + r)) & 1u)) {
+                  const float zero[CN] = {};
+                  out.store(t, zero);
+                }
+              }
             }
           }
         }
@@ -1307,6 +1334,24 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
   k_w4a4_few_down<8, 4><<<dim3((unsigned)(ntiles * c.T)), dim3(512), 0, st>>>(c, hq, hs, ntiles);
   e = hipGetLastError();
   return true;
+}
+
+// Rows sorted by expert through a gated activation, the result quantised: out holds its
+// blocks [rows, N / 64, 16] and out_scale their scales.  On tiles the epilogue does it,
+// else (h: scratch, fp32 [rows, N / 2]) a kernel of its own; rows of no expert are then
+// those of zeros, on tiles left as they were.
+hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale, hipStream_t st) {
+  const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
+  if (c.K >= kMinK && offsets_ok(c) && seg >= 16) {
+    if (seg >= 128) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
+    return tile<1, 4, 4, 4, 3, true, true, true>(c, out_scale, st);
+  }
+  ftm_w4a4 wide = c;
+  wide.out = h;
+  wide.out_dtype = FTM_DT_F32;
+  const hipError_t e = launch_w4a4(wide, st);
+  const int I = out_cols(c);
+  return e != hipSuccess ? e : launch_quant_mxfp4(h, FTM_DT_F32, c.rows, I, (int64_t)I * 4, (uint8_t*)c.out, out_scale, st);
 }
 
 hipError_t launch_w4a4_dynamic(const ftm_w4a4& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {

@@ -99,7 +99,8 @@ def gated_close(got, gu, mag, name, dtype, n, **kw):
     """act(gate) * up of sums that may be off by n roundings of mag: the largest change at the
     corners of that box, 16 roundings of fp32 for the activation (of gelu relative to g u: its
     1 + erf cancels; of swiglu_oai to g (u + 1) with its 1 not cancelled), one of the output.  Where
-    exp(-g) exceeds fp32 (2^128) the sigmoid is 0 instead of less than 2^-128."""
+    1 + exp(-g) exceeds 2^126 its reciprocal is below fp32's normal numbers and becomes 0, so the
+    result is off by less than 2^-126 of its factors."""
     e = n * U * mag
     (g, u), (eg, eu) = gu.chunk(2, dim=1), e.chunk(2, dim=1)
     ref = act(name, g, u, **kw)
@@ -108,7 +109,7 @@ def gated_close(got, gu, mag, name, dtype, n, **kw):
         for b in (-1, 1):
             off = torch.maximum(off, (act(name, g + a * eg, u + b * eu, **kw) - ref).abs())
     size = ref.abs() + ((g * u).abs() if name == "gelu" else g.abs() if name == "swiglu_oai" else 0)
-    bound = 2 * off + 16 * U * size + half_step(dtype) * ref.abs() + tiny(dtype) + g.abs() * (u.abs() + 1) * 2.0 ** -127
+    bound = 2 * off + 16 * U * size + half_step(dtype) * ref.abs() + tiny(dtype) + g.abs() * (u.abs() + 1) * 2.0 ** -126
     bad = far(got, ref, bound, dtype)
     assert got.dtype == dtype and not bad.any(), f"{int(bad.sum())} of {bad.numel()} out of tolerance"
 
@@ -486,7 +487,7 @@ def layer_reference(x, w1, w2, ids, wt, name, b1=None, b2=None, K=0, **kw):
             for a in (-1, 1):
                 for b in (-1, 1):
                     off = torch.maximum(off, (act(name, g + a * eg, u + b * eu, **kw) - h).abs())
-            off = 2 * off + 16 * U * (h.abs() + (g.abs() if name == "swiglu_oai" else 0)) + 2.0 ** -140
+            off = 2 * off + 16 * U * (h.abs() + (g.abs() if name == "swiglu_oai" else 0)) + g.abs() * (u.abs() + 1) * 2.0 ** -126
             ex = quantised(h)
             q = code_values(h, ex)
             dq = torch.zeros_like(q)
