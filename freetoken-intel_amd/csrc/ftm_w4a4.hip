@@ -289,22 +289,23 @@ constexpr int kMinK = 256;  // of the kernels that take the scales eight at a ti
 
 // A wave's scales of R rows and its `per` steps from `lo` on, kept in LDS with scale_pitch
 // bytes between rows (an odd number of eights: 16 rows hit distinct banks).  A lane
-// has a row of each 64 (two lanes one of 32, in turn); `p` says where they begin.  The
+// has a row of each 64 (of 32 or 16 rows two or four lanes one, in turn); `p` says where they begin.  The
 // first kFlight loads of each are under way when the copies of the operands are
 // requested (`then`), before any of them is waited for.
 __host__ __device__ inline int scale_pitch(int per) { return 8 * (per | 1); }
 template <int R>
 struct FillScales {
-  static constexpr int kRows = (R + 63) / 64, kTurns = R <= 32 ? 2 : 1, kFlight = kTurns == 2 ? 2 : 4;
+  static constexpr int kRows = (R + 63) / 64, kTurns = R <= 16 ? 4 : R <= 32 ? 2 : 1, kFlight = kTurns > 1 ? 2 : 4;
+  static constexpr int kWidth = 64 / kTurns;
   const uint8_t* p[kRows];
   __device__ __forceinline__ static int row(int i) {  // the lane's i-th
-    const int lane = threadIdx.x & 63, r = (kTurns == 2 ? lane & 31 : lane) + 64 * i;
+    const int r = (threadIdx.x & (kWidth - 1)) + 64 * i;
     return r < R ? r : R - 1;
   }
   template <class Then>
   __device__ __forceinline__ void operator()(char* at, int lo, int per, int nb, Then&& then) const {
     const int lane = threadIdx.x & 63, pitch = scale_pitch(per);
-    const int turn = kTurns == 2 ? lane >> 5 : 0, first = kTurns == 2 ? lane & 31 : lane;
+    const int turn = lane / kWidth, first = lane & (kWidth - 1);
     const int last = (nb - 1) / 8, n = lo + per <= last + 1 ? per : last + 1 - lo;
     for (int s0 = 0; s0 < n; s0 += kTurns * kFlight) {
       u32x2 v[kRows][kFlight];
@@ -761,6 +762,250 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
     if (row >= cnt) return;
     const int64_t at = (int64_t)lists[0][row] * (NO / 32) + nt;
     *(uint32_t*)(c.hq + at * 16 + 4 * part) = codes;
+    if (part == 0) c.hs[at] = (uint8_t)byte;
+  }
+}
+
+// ------------------------------------------------------------------ columns over the waves
+// Up to 16 MT rows of one expert x 64 weight rows: the rows' codes and scales over the whole K
+// in LDS, for all four waves; each wave streams 16 weight rows through a ring of its
+// own (S stages of 256 K) and finishes its results alone.  Where an expert has few rows and
+// there are blocks for every CU: against K split over the waves there are no sums to
+// exchange, the rows are held once, and a workgroup's ring holds most of its weights.
+// Call is a product (codes in hand) or a layer's first (FewCall: wide tokens, which the
+// workgroup quantises, its 32 channels of h quantised in the epilogue).
+template <int XDT, int MT, int S, class Call>
+__global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
+  constexpr bool MOE = std::is_same_v<Call, FewCall>;
+  constexpr int kStage = 16 * kRow, kTurns = 4 / MT;
+  extern __shared__ char lds[];  // [4][S][kStage], codes [nsteps][rows][kRow], scales of the rows, and of each wave's weights
+  __shared__ int lists[MOE ? 4 : 1][kFewRows];
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int K = c.K, nb = K / 32, nsteps = (nb + 7) / 8, pitch = scale_pitch(nsteps);
+  int e, cnt, nt;
+  RowTile rt = {0, 0, 0};
+  int R = 16 * MT;  // rows of the codes in LDS
+  if constexpr (MOE) {
+    nt = blockIdx.x % ntiles;
+    const FewPairs pairs(c.ids, c.ids64 != 0, c.P, c.E, blockIdx.x / ntiles, c.cap, lists[wave]);
+    e = pairs.e;
+    cnt = pairs.cnt;
+    R = c.cap;
+  } else {
+    const int item = xcd_item(blockIdx.x, gridDim.x);
+    nt = item % ntiles;
+    rt = row_tile<16 * MT>(c, item / ntiles);
+    e = rt.e;
+    cnt = rt.cnt;
+  }
+  if (cnt <= 0) return;
+  const bool act = MOE || c.act >= 0;
+  const int NO = act ? c.N / 2 : c.N;
+  const int cols = act ? 8 : 16, n0 = nt * 4 * cols + wave * cols, ncol = NO - n0 < cols ? NO - n0 : cols;
+  if constexpr (!MOE) {
+    if (e < 0) {  // rows of no expert
+      const float zero[4] = {};
+      const RowOut<4> out(c, rt, NO, n0 + 4 * (act ? g & 1 : g));
+      if (ncol > 0 && (!act || g < 2)) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) out.store(16 * i + m, zero);
+      }
+      return;
+    }
+  }
+  char* ring = lds + wave * (S * kStage);
+  char* codes = lds + 4 * S * kStage;
+  char* xscales = codes + nsteps * R * kRow;
+  char* scales = xscales + (R + 16 * wave) * pitch;
+  bool live[MT];  // of this lane's results
+#pragma unroll
+  for (int i = 0; i < MT; ++i) live[i] = true;
+  const SplitWeights<1> weights((const char*)c.w + (int64_t)e * c.w_stride, NO, K, act, n0 < NO ? n0 : 0, ncol > 0 ? ncol : 1);
+  auto issue = [&](int step, int slot) __attribute__((always_inline)) {
+    weights.issue(ring + slot * kStage, step < nsteps && ncol > 0 ? (uint32_t)step * 128u : kNowhere);
+  };
+  FillScales<16> fill;
+  fill.p[0] = c.w_scale + (int64_t)e * c.w_scale_stride +
+              ((n0 < NO ? n0 : 0) + SplitWeights<1>::row(NO, act, ncol > 0 ? ncol : 1, fill.row(0))) * nb;
+  SplitBias bias;
+  auto request = [&] {
+    bias.request(c.bias, c.bias_dtype, (int64_t)e * c.N, act, NO, n0 + 4 * (act ? g & 1 : g));
+  };
+  if constexpr (MOE) {
+    using V = Vec8<XDT>;
+    constexpr int kBatch = 4;
+    // half a wave takes 256 values of one row; the (row, step) pairs in turn over the half waves
+    const int l32 = lane & 31, turns = cnt * nsteps;
+    V v[kBatch];
+    auto load = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = t0 + 8 * i, r = t / nsteps, k = 256 * (t % nsteps) + 8 * l32;
+        if (t < turns && k < K) v[i].load(c.x + (int64_t)(lists[wave][r] / c.k) * c.x_stride + (int64_t)(k / 8) * V::kBytes);
+        else v[i].zero();
+      }
+    };
+    auto quantise = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = t0 + 8 * i, r = t / nsteps, s = t % nsteps;
+        const uint32_t byte = mx_scale_byte(quad_max(v[i].max_bits()));
+        const uint32_t w = mx_codes<XDT>(v[i], byte);
+        if (t < turns) {
+          *(uint32_t*)(codes + (s * R + r) * kRow + 16 * ((l32 >> 2) ^ swz(r)) + 4 * (l32 & 3)) = w;
+          if ((l32 & 3) == 0) *(uint8_t*)(xscales + r * pitch + 8 * s + (l32 >> 2)) = (uint8_t)byte;
+        }
+      }
+    };
+    const int first = 2 * wave + (lane >> 5);
+    fill(scales, 0, nsteps, nb, [&] {
+      request();
+      load(first);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < S; ++u) issue(u, u);
+    });
+    quantise(first);
+    for (int t = first + 8 * kBatch; t - (lane >> 5) < turns; t += 8 * kBatch) {
+      load(t);
+      quantise(t);
+    }
+    __syncthreads();
+  } else {
+    // The rows of x: of the copies, of the scales, of the results
+    const bool indexed = c.row_index != nullptr;
+    const int64_t x_rows = indexed ? c.x_rows : c.rows;
+    const uint32_t Kb = (uint32_t)K / 2;
+    int rc[2 * MT], rr[MT], rs = lane & (16 * MT - 1);
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) rc[i] = 8 * i + (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) rr[i] = 16 * i + m;
+    auto in_tile = [&](int r) { return r < cnt ? r : 0; };
+    int ic[2 * MT], ir[MT], is = in_tile(rs);
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) ic[i] = in_tile(rc[i]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) ir[i] = in_tile(rr[i]);
+    if (indexed) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) ic[i] = c.row_index[rt.row0 + ic[i]];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) ir[i] = c.row_index[rt.row0 + ir[i]];
+      is = c.row_index[rt.row0 + is];
+    } else {
+      is += (int)rt.row0;
+    }
+    const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
+    uint32_t xoff[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const bool in = rc[i] < cnt && ic[i] >= 0 && ic[i] < (indexed ? x_rows : (int64_t)cnt);
+      xoff[i] = in ? (uint32_t)ic[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(rc[i])) : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) live[i] = !indexed || (ir[i] >= 0 && ir[i] < x_rows);
+    const uint8_t* xs = c.x_scale + (int64_t)(is >= 0 && is < x_rows ? is : 0) * nb;
+    const int turn = kTurns * wave + lane / (16 * MT);
+    u32x2 own[2];  // the lane's row at steps turn and turn + 4 kTurns: the first
+    fill(scales, 0, nsteps, nb, [&] {
+      request();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int s = turn + 4 * kTurns * i;
+        own[i] = load_scales(xs, s < nsteps ? s : nsteps - 1, nb);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      for (int s = wave; s < nsteps; s += 4)
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(codes + (s * R + 8 * i) * kRow), 16, (int)(xoff[i] + 128u * s), 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < S; ++u) issue(u, u);
+    });
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = turn + 4 * kTurns * i;
+      if (s < nsteps) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(own[i], s, nb);
+    }
+    for (int s = turn + 8 * kTurns; s < nsteps; s += 4 * kTurns) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(load_scales(xs, s, nb), s, nb);
+    wait_vm<2 * S>();  // the rows' copies have landed
+    __syncthreads();
+  }
+  f32x4 acc[MT];
+  int xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    acc[i] = (f32x4){0, 0, 0, 0};
+    xr[i] = 16 * i + m < cnt ? 16 * i + m : 0;
+  }
+  int slot = 0;
+  for (int step = 0; step < nsteps; ++step) {
+    wait_vm<(S - 1) * 2>();  // this step's copies have landed
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const char* st = ring + slot * kStage;
+    u32x4 w[2], x[MT][2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      w[q] = stage_piece(st, m, q, g);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[i][q] = stage_piece(codes + step * R * kRow, xr[i], q, g);
+    }
+    auto scale = [&](const char* at, int r) { return scale_operand(*(const u32x2*)(at + r * pitch + 8 * step), g); };
+    const uint32_t sw = scale(scales, m);
+    uint32_t sx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx[i] = scale(xscales, xr[i]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the operands are here: the slot is free
+    __builtin_amdgcn_sched_barrier(0);
+    issue(step + S, slot);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = mfma_fp4<0, 0>(w[0], x[i][0], acc[i], sw, sx[i]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = mfma_fp4<1, 1>(w[1], x[i][1], acc[i], sw, sx[i]);
+    slot = slot == S - 1 ? 0 : slot + 1;
+  }
+  wait_vm<0>();  // the copies past the last step, before the LDS is given back
+  if constexpr (MOE) __syncthreads();  // the rows' codes make place for h
+  float* h = (float*)codes;  // [16][36]
+  with_act(c.act, [&](auto a) {
+    constexpr int A = decltype(a)::value;
+    if constexpr (!MOE || A >= 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[r] = acc[i][r] + bias.at(r, c.bias_dtype);
+          if constexpr (A >= 0) {  // the up rows are the lanes 32 on
+            const float u = __shfl_xor(acc[i][r], 32) + bias.at(4 + r, c.bias_dtype);
+            y[r] = act_gated<A>(y[r], u, c);
+          }
+          y[r] = live[i] ? y[r] : 0.0f;
+        }
+        if (A >= 0 && g >= 2) continue;
+        if constexpr (MOE) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) h[m * 36 + 8 * wave + 4 * g + r] = y[r];
+        } else if (ncol > 0) {
+          RowOut<4>(c, rt, NO, n0 + 4 * (act ? g & 1 : g)).store(16 * i + m, y);
+        }
+      }
+    }
+  });
+  if constexpr (MOE) {
+    __syncthreads();
+    const int row = lane >> 2, part = lane & 3;
+    if (wave != 0) return;
+    Vec8<FTM_DT_F32> v;
+    v.load((const char*)(h + row * 36 + 8 * part));
+    const uint32_t byte = mx_scale_byte(quad_max(v.max_bits()));
+    const uint32_t q = mx_codes<FTM_DT_F32>(v, byte);
+    if (row >= cnt) return;
+    const int64_t at = (int64_t)lists[0][row] * (NO / 32) + nt;
+    *(uint32_t*)(c.hq + at * 16 + 4 * part) = q;
     if (part == 0) c.hs[at] = (uint8_t)byte;
   }
 }
@@ -1235,6 +1480,21 @@ hipError_t split(const ftm_w4a4& c, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int S>
+int cols_lds(int K, int rows);
+template <int MT, int S>
+hipError_t cols(const ftm_w4a4& c, hipStream_t st) {
+  const int per = c.act >= 0 ? 32 : 64, lds = cols_lds<S>(c.K, 16 * MT);
+  const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + per - 1) / per;
+  if (mt * nt > kMaxGroups || lds > kMaxLds - 1024) return split<MT, 2, 4, 2>(c, st);
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w4a4_cols<-1, MT, S, ftm_w4a4>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (int)nt);
+  return hipGetLastError();
+}
+
 template <int WM, int WN, int MI, int NJ, int S, bool ACT, bool GROUPED, bool QOUT>
 hipError_t tile(const ftm_w4a4& c, uint8_t* out_scale, hipStream_t st) {
   constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, lds = S * (BM + BN) * kRow + 16 * (BM + BN);
@@ -1276,7 +1536,7 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
     const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
     if (seg >= 128) return tile<2, 2, 4, 8, 3>(c, st);
     if (seg >= 16) return tile<1, 4, 4, 4, 3>(c, st);
-    return split<1, 2, 4, 2>(c, st);
+    return cols<1, 4>(c, st);
   }
   const int64_t M = c.rows;
   if (M <= 16) return split<1, 1, 4, 4>(c, st);
@@ -1314,6 +1574,28 @@ hipError_t few(const FewCall& c, int dt, hipStream_t st) {
   return few<FTM_DT_BF16, NT, NW, S, MOE>(c, st);
 }
 
+template <int S>
+int cols_lds(int K, int rows) {
+  const int nsteps = (K + 255) / 256, codes = nsteps * rows * kRow, pitch = scale_pitch(nsteps);
+  return 4 * S * 16 * kRow + (codes > 16 * 36 * 4 ? codes : 16 * 36 * 4) + (rows + 64) * pitch;
+}
+template <int XDT, int S>
+hipError_t cols_moe(const FewCall& c, hipStream_t st) {
+  const int ntiles = c.N / 64;
+  static DeviceBits lds_set{0};
+  const auto kernel = k_w4a4_cols<XDT, 1, S, FewCall>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)(c.P * ntiles)), dim3(256), cols_lds<S>(c.K, c.cap), st>>>(c, ntiles);
+  return hipGetLastError();
+}
+template <int S>
+hipError_t cols_moe(const FewCall& c, int dt, hipStream_t st) {
+  if (dt == FTM_DT_F32) return cols_moe<FTM_DT_F32, S>(c, st);
+  if (dt == FTM_DT_F16) return cols_moe<FTM_DT_F16, S>(c, st);
+  return cols_moe<FTM_DT_BF16, S>(c, st);
+}
+
 }  // namespace
 
 // A layer of few tokens in two kernels, if it is one: hq and hs hold h, a row a pair.
@@ -1326,7 +1608,8 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
                      (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
                      c.topk_ids, c.ids_dtype == FTM_ID_I64, P, c.num_experts, c.k, hq, hs};
   constexpr int kRoom = kMaxLds - 1024;  // beside the lists
-  if (few_lds<4, 8, 2>(H, cap) <= kRoom && H > 8 * 256) e = few<4, 8, 2, true>(f, c.dtype, st);
+  if (cols_lds<6>(H, cap) <= kRoom) e = cols_moe<6>(f, c.dtype, st);
+  else if (few_lds<4, 8, 2>(H, cap) <= kRoom && H > 8 * 256) e = few<4, 8, 2, true>(f, c.dtype, st);
   else if (few_lds<4, 8, 1>(H, cap) <= kRoom) e = few<4, 8, 1, true>(f, c.dtype, st);
   else return false;
   if (e != hipSuccess) return true;
