@@ -171,18 +171,41 @@ struct RowOut {
   __device__ __forceinline__ uint32_t half2(float a, float b) const {
     return dt == FTM_DT_BF16 ? pack_bf16x2(a, b) : (uint32_t)f32_to_f16(a) | ((uint32_t)f32_to_f16(b) << 16);
   }
+  // All N in one store (where vec says so) of a type known beforehand.
+  template <int DT>
+  __device__ __forceinline__ void store_vec(int row, const float (&y)[N]) const {
+    const uint32_t at = (uint32_t)(row * NO + n0);
+    if constexpr (DT == FTM_DT_F32) {
+      const uint32_t off = n0 < NO ? 4u * at : kOOB;
+      if constexpr (N == 2) {
+        __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(y[0]), __float_as_uint(y[1])}, res, off, 0, kNT);
+      } else {
+#pragma unroll
+        for (int h = 0; h < N; h += 4)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              (u32x4){__float_as_uint(y[h]), __float_as_uint(y[h + 1]), __float_as_uint(y[h + 2]), __float_as_uint(y[h + 3])}, res,
+              n0 < NO ? off + 4u * h : kOOB, 0, kNT);
+      }
+    } else {
+      const uint32_t off = n0 < NO ? 2u * at : kOOB;
+      auto half2 = [](float a, float b) {
+        return DT == FTM_DT_BF16 ? pack_bf16x2(a, b) : (uint32_t)f32_to_f16(a) | ((uint32_t)f32_to_f16(b) << 16);
+      };
+      if constexpr (N == 8)
+        __builtin_amdgcn_raw_buffer_store_b128((u32x4){half2(y[0], y[1]), half2(y[2], y[3]), half2(y[4], y[5]), half2(y[6], y[7])},
+                                               res, off, 0, kNT);
+      else if constexpr (N == 4)
+        __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, kNT);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, kNT);
+    }
+  }
   __device__ __forceinline__ void store(int row, const float (&y)[N]) const {
     const uint32_t at = (uint32_t)(row * NO + n0);
     if (dt == FTM_DT_F32) {
       const uint32_t off = n0 < NO ? 4u * at : kOOB;
       if (vec) {
-        if constexpr (N == 8) {
-#pragma unroll
-          for (int h = 0; h < 8; h += 4)
-            __builtin_amdgcn_raw_buffer_store_b128((u32x4){__float_as_uint(y[h]), __float_as_uint(y[h + 1]), __float_as_uint(y[h + 2]),
-                                                           __float_as_uint(y[h + 3])},
-                                                   res, n0 < NO ? off + 4u * h : kOOB, 0, kNT);
-        } else if constexpr (N == 4)
+        if constexpr (N == 4)
           __builtin_amdgcn_raw_buffer_store_b128(
               (u32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])}, res, off, 0,
               kNT);
@@ -197,10 +220,7 @@ struct RowOut {
     }
     const uint32_t off = n0 < NO ? 2u * at : kOOB;
     if (vec) {
-      if constexpr (N == 8)
-        __builtin_amdgcn_raw_buffer_store_b128((u32x4){half2(y[0], y[1]), half2(y[2], y[3]), half2(y[4], y[5]), half2(y[6], y[7])},
-                                               res, off, 0, kNT);
-      else if constexpr (N == 4)
+      if constexpr (N == 4)
         __builtin_amdgcn_raw_buffer_store_b64((u32x2){half2(y[0], y[1]), half2(y[2], y[3])}, res, off, 0, kNT);
       else
         __builtin_amdgcn_raw_buffer_store_b32(half2(y[0], y[1]), res, off, 0, kNT);

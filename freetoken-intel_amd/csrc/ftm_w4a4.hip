@@ -767,17 +767,18 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
 }
 
 // ------------------------------------------------------------------ columns over the waves
-// Up to 16 MT rows of one expert x 64 weight rows: the rows' codes and scales over the whole K
+// Up to RW rows of one expert x 64 weight rows: the rows' codes and scales over the whole K
 // in LDS, for all four waves; each wave streams 16 weight rows through a ring of its
 // own (S stages of 256 K) and finishes its results alone.  Where an expert has few rows and
 // there are blocks for every CU: against K split over the waves there are no sums to
 // exchange, the rows are held once, and a workgroup's ring holds most of its weights.
 // Call is a product (codes in hand) or a layer's first (FewCall: wide tokens, which the
 // workgroup quantises, its 32 channels of h quantised in the epilogue).
-template <int XDT, int MT, int S, class Call>
+template <int XDT, int RW, int S, class Call>
 __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
   constexpr bool MOE = std::is_same_v<Call, FewCall>;
-  constexpr int kStage = 16 * kRow, kTurns = 4 / MT;
+  constexpr int MT = (RW + 15) / 16, NC = RW / 8, kStage = 16 * kRow, kTurns = 64 / RW;
+  static_assert(RW == 8 || RW % 16 == 0, "copies of 8 rows");
   extern __shared__ char lds[];  // [4][S][kStage], codes [nsteps][rows][kRow], scales of the rows, and of each wave's weights
   __shared__ int lists[MOE ? 4 : 1][kFewRows];
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -785,7 +786,7 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
   const int K = c.K, nb = K / 32, nsteps = (nb + 7) / 8, pitch = scale_pitch(nsteps);
   int e, cnt, nt;
   RowTile rt = {0, 0, 0};
-  int R = 16 * MT;  // rows of the codes in LDS
+  int R = RW;  // rows of the codes in LDS
   if constexpr (MOE) {
     nt = blockIdx.x % ntiles;
     const FewPairs pairs(c.ids, c.ids64 != 0, c.P, c.E, blockIdx.x / ntiles, c.cap, lists[wave]);
@@ -795,7 +796,7 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
   } else {
     const int item = xcd_item(blockIdx.x, gridDim.x);
     nt = item % ntiles;
-    rt = row_tile<16 * MT>(c, item / ntiles);
+    rt = row_tile<RW>(c, item / ntiles);
     e = rt.e;
     cnt = rt.cnt;
   }
@@ -873,64 +874,63 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
     }
     __syncthreads();
   } else {
-    // The rows of x: of the copies, of the scales, of the results
+    // The tile's rows of x by scalar loads: a vector load would be waited for with every
+    // copy before it, and the weights are to be under way first.
     const bool indexed = c.row_index != nullptr;
     const int64_t x_rows = indexed ? c.x_rows : c.rows;
     const uint32_t Kb = (uint32_t)K / 2;
-    int rc[2 * MT], rr[MT], rs = lane & (16 * MT - 1);
+    int row[RW];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) rc[i] = 8 * i + (lane >> 3);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) rr[i] = 16 * i + m;
-    auto in_tile = [&](int r) { return r < cnt ? r : 0; };
-    int ic[2 * MT], ir[MT], is = in_tile(rs);
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) ic[i] = in_tile(rc[i]);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) ir[i] = in_tile(rr[i]);
-    if (indexed) {
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) ic[i] = c.row_index[rt.row0 + ic[i]];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) ir[i] = c.row_index[rt.row0 + ir[i]];
-      is = c.row_index[rt.row0 + is];
-    } else {
-      is += (int)rt.row0;
+    for (int i = 0; i < RW; ++i) {
+      const int64_t at = rt.row0 + (i < cnt ? i : cnt - 1);
+      row[i] = indexed ? c.row_index[at] : (int)at;
     }
-    const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
-    uint32_t xoff[2 * MT];
+    // row r of them, the same for the lanes of a group
+    auto row_at = [&](int r, int first, int n) __attribute__((always_inline)) {
+      int v = row[first];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const bool in = rc[i] < cnt && ic[i] >= 0 && ic[i] < (indexed ? x_rows : (int64_t)cnt);
-      xoff[i] = in ? (uint32_t)ic[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(rc[i])) : kNowhere;
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) live[i] = !indexed || (ir[i] >= 0 && ir[i] < x_rows);
-    const uint8_t* xs = c.x_scale + (int64_t)(is >= 0 && is < x_rows ? is : 0) * nb;
-    const int turn = kTurns * wave + lane / (16 * MT);
-    u32x2 own[2];  // the lane's row at steps turn and turn + 4 kTurns: the first
+      for (int i = 1; i < n; ++i) v = r == first + i ? row[first + i] : v;
+      return v;
+    };
     fill(scales, 0, nsteps, nb, [&] {
       request();
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int s = turn + 4 * kTurns * i;
-        own[i] = load_scales(xs, s < nsteps ? s : nsteps - 1, nb);
-      }
       __builtin_amdgcn_sched_barrier(0);
-      for (int s = wave; s < nsteps; s += 4)
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(codes + (s * R + 8 * i) * kRow), 16, (int)(xoff[i] + 128u * s), 0, 0, 0);
 #pragma unroll
       for (int u = 0; u < S; ++u) issue(u, u);
     });
+    // the rows' copies; rows past the tile and rows that are none are not copied
+    const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
+    uint32_t xoff[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = 8 * i + (lane >> 3), v = row_at(r, 8 * i, 8);
+      const bool in = r < cnt && v >= 0 && v < x_rows;
+      xoff[i] = in ? (uint32_t)(indexed ? v : r) * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+    }
+    const int rs = lane & (RW - 1), vs = row_at(rs, 0, RW), turn = kTurns * wave + lane / RW;
+    const uint8_t* xs = c.x_scale + (int64_t)(vs >= 0 && vs < x_rows ? vs : 0) * nb;
+    u32x2 own[2];  // the lane's row at steps turn and turn + 4 kTurns
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = turn + 4 * kTurns * i;
+      own[i] = load_scales(xs, s < nsteps ? s : nsteps - 1, nb);
+    }
+    for (int s = wave; s < nsteps; s += 4)
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(codes + (s * R + 8 * i) * kRow), 16, (int)(xoff[i] + 128u * s), 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = 16 * i + (RW == 8 ? m & 7 : m), v = row_at(r, 16 * i, RW < 16 ? RW : 16);
+      live[i] = v >= 0 && v < x_rows;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int s = turn + 4 * kTurns * i;
       if (s < nsteps) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(own[i], s, nb);
     }
     for (int s = turn + 8 * kTurns; s < nsteps; s += 4 * kTurns) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(load_scales(xs, s, nb), s, nb);
-    wait_vm<2 * S>();  // the rows' copies have landed
+    wait_vm<0>();  // the rows' copies have landed, and the first weights
     __syncthreads();
   }
   f32x4 acc[MT];
@@ -1122,9 +1122,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   constexpr int kCols = ACT ? BN / 2 : BN;               // output channels of the tile
   constexpr int CN = ACT ? NJ / 2 : NJ;                  // neighbouring ones of a lane
   constexpr int kAhead = 3;                              // row blocks read ahead of their products
+  constexpr int kLast = 2 * MI - kAhead;                 // from this one on they are the next step's
+  constexpr int kNextX = MI < kAhead ? MI : kAhead;      // row blocks whose scales are read a step ahead
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies of 8 rows, as many for each wave");
-  static_assert(2 * MI % (kAhead + 1) == 0 && kAhead <= MI && NJ >= 4 && NJ % 4 == 0 && (NJ % MI == 0 || MI % NJ == 0),
-                "the order of the reads");
+  constexpr int kSecond = MI < kLast ? MI : kLast;       // row blocks that read the second half's weights
+  static_assert(2 * MI % (kAhead + 1) == 0 && NJ % 4 == 0 && NJ % kSecond == 0, "the order of the reads");
   extern __shared__ char lds[];  // [S][kStage], then [2][kSlot]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1248,7 +1250,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
     };
     f32x4 acc[MI][NJ];
     u32x4 b[2][NJ], x[kAhead + 1];
-    uint32_t sx[MI], sb[NJ], sn[NJ];
+    uint32_t sx[MI], sb[NJ], nx[kNextX], sn[NJ];
     auto xfrag = [&](int slot, int at) __attribute__((always_inline)) {
       return stage_piece(lds + slot * kStage, 16 * (wm * MI + at % MI) + m, at / MI, g);
     };
@@ -1265,7 +1267,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
     // read under the products left.
     auto step = [&](int kb, int snext, int sload, uint32_t k0, int slot, int par) __attribute__((always_inline)) {
       const int next = slot == S - 1 ? 0 : slot + 1;
-      constexpr int kLast = 2 * MI - kAhead, kSlots = kAhead * NJ;
+      constexpr int kSlots = kAhead * NJ;
+      // the next step's first weights take registers that are free from the second half on
+      constexpr int kFirstB = MI > kLast ? (MI - kLast) * NJ : 0;
 #pragma unroll
       for (int at = 0; at < 2 * MI; ++at) {
         const int q = at / MI, i = at % MI;
@@ -1283,20 +1287,20 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
           const int a = at + kAhead;
           if (j == 0 && a < 2 * MI) x[a % (kAhead + 1)] = xfrag(slot, a);
           if (j == 1 && a < MI) sx[a] = sfrag(par, 16 * (wm * MI + a) + m);
-          if (q == 0) {  // the second half's weights, spread over the row blocks
-            constexpr int kPer = NJ > MI ? NJ / MI : 1, kEvery = MI > NJ ? MI / NJ : 1;
-            if (i % kEvery == 0 && j >= 2 && j < 2 + kPer) b[1][i / kEvery * kPer + j - 2] = wfrag(slot, i / kEvery * kPer + j - 2, 1);
+          if (at < kSecond) {  // the second half's weights, before the slot is given away
+            constexpr int kPer = NJ / kSecond;
+#pragma unroll
+            for (int n = 0; n < kPer; ++n)
+              if (j == (2 + n) % NJ) b[1][at * kPer + n] = wfrag(slot, at * kPer + n, 1);
           }
           if (at >= kLast) {
             const int t = (at - kLast) * NJ + j;
             if (j == 0) x[a % (kAhead + 1)] = xfrag(next, a - 2 * MI);
-            if (j == 1) sx[a - 2 * MI] = sfrag(1 - par, 16 * (wm * MI + a - 2 * MI) + m);
+            if (j == 1 && at - kLast < kNextX) nx[at - kLast] = sfrag(1 - par, 16 * (wm * MI + at - kLast) + m);
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
-              if (n * kSlots / NJ == t) {
-                b[0][n] = wfrag(next, n, 0);
-                sn[n] = sfrag(1 - par, BM + 16 * (wn * NJ + n) + m);
-              }
+              if (kFirstB + n * (kSlots - kFirstB) / NJ == t) b[0][n] = wfrag(next, n, 0);
+              if (n * kSlots / NJ == t) sn[n] = sfrag(1 - par, BM + 16 * (wn * NJ + n) + m);
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -1308,6 +1312,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) sb[j] = sn[j];
+#pragma unroll
+      for (int i = 0; i < kNextX; ++i) sx[i] = nx[i];
       __builtin_amdgcn_sched_barrier(0);
     };
     rows_of(cur);
@@ -1328,10 +1334,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       sb[j] = sfrag(0, BM + 16 * (wn * NJ + j) + m);
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      x[i] = xfrag(0, i);
-      sx[i] = sfrag(0, 16 * (wm * MI + i) + m);
-    }
+    for (int i = 0; i < kAhead; ++i) x[i] = xfrag(0, i);
+#pragma unroll
+    for (int i = 0; i < kNextX; ++i) sx[i] = sfrag(0, 16 * (wm * MI + i) + m);
     int slot = 0, par = 0;
     for (;;) {
       const int after = item + (int)(gridDim.x >> 3);
@@ -1381,59 +1386,99 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       float bias[NJ];
 #pragma unroll
       for (int n = 0; n < NJ; ++n) bias[n] = bits_to_f32(opaque_bits(bb[n]), c.bias_dtype);
-      with_act(ACT ? c.act : -1, [&](auto a) __attribute__((always_inline)) {
-        constexpr int A = decltype(a)::value;
-        const RowOut<CN> out(c, cur.rt, NO, n0);
+      // The activation in place of the gate's sums, then the results by their type: a path
+      // is as long as the work, not as all types and activations together (instructions that
+      // a tile runs once are fetched anew: 128 x 256 results took 3.9 us, so %RESULTS%)
+      if constexpr (ACT) {
+        with_act(c.act, [&](auto a) __attribute__((always_inline)) {
+          if constexpr (decltype(a)::value >= 0) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+              for (int n = 0; n < CN; ++n) {
+                f32x4 y = acc[i][n], u = acc[i][CN + n];
+                asm volatile("" : "+v"(y), "+v"(u) : : "memory");  // one block after the other
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = act_gated<decltype(a)::value>(y[r] + bias[n], u[r] + bias[CN + n], c);
+                asm volatile("" : "+v"(y) : : "memory");
+                acc[i][n] = y;
+              }
+          }
+        });
+      }
+      auto each_row = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
           // one row block after the other, so that their results do not all sit in
           // registers at once
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) asm volatile("" : "+v"(acc[i][j]) : : "memory");
+          for (int n = 0; n < CN; ++n) asm volatile("" : "+v"(acc[i][n]) : : "memory");
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float y[CN];
 #pragma unroll
-            for (int n = 0; n < CN; ++n) {
-              y[n] = acc[i][n][r] + bias[n];
-              if constexpr (ACT) y[n] = act_gated<A>(y[n], acc[i][CN + n][r] + bias[CN + n], c);
-            }
-            const int t = t0 + 16 * i + r;
-            if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
-              uint32_t top = 0;
-#pragma unroll
-              for (int n = 0; n < CN; ++n) {
-                const uint32_t b = __float_as_uint(y[n]) & 0x7fffffffu;
-                top = b > top ? b : top;
-              }
-              top = quad_max(top);
-              auto with = [&](uint32_t o) { top = o > top ? o : top; };
-              with((uint32_t)dpp_i<kDppHalfMirror>((int)top));
-              if constexpr (CN == 2) with((uint32_t)dpp_i<kDppMirror>((int)top));
-              const uint32_t byte = mx_scale_byte(top);
-              const float s = __uint_as_float(byte << 23);
-              uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, towards_zero<FTM_DT_F32>(y[0]), towards_zero<FTM_DT_F32>(y[1]), s, 0);
-              if constexpr (CN == 4)
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, towards_zero<FTM_DT_F32>(y[2]), towards_zero<FTM_DT_F32>(y[3]), s, 1);
-              w = byte == 255u ? 0u : positive_zeros(w);
-              if (t < cur.rt.cnt && n0 < NO) {
-                const int64_t row = cur.rt.row0 + t;
-                if constexpr (CN == 4) *(uint16_t*)((char*)c.out + (row * NO + n0) / 2) = (uint16_t)w;
-                else *((uint8_t*)c.out + (row * NO + n0) / 2) = (uint8_t)w;
-                if ((em & (32 / CN - 1)) == 0) out_scale[(row * NO + n0) / 32] = (uint8_t)byte;
-              }
-            } else {
-              out.store(t, y);
-              if constexpr (GROUPED) {  // a row whose index names none: zeros over it
-                if (!((live >> (4 * i + r)) & 1u)) {
-                  const float zero[CN] = {};
-                  out.store(t, zero);
-                }
-              }
-            }
+            for (int n = 0; n < CN; ++n) y[n] = ACT ? acc[i][n][r] : acc[i][n][r] + bias[n];
+            f(t0 + 16 * i + r, y);
           }
         }
-      });
+      };
+      if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
+        each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int n = 0; n < CN; ++n) {
+            const uint32_t b = __float_as_uint(y[n]) & 0x7fffffffu;
+            top = b > top ? b : top;
+          }
+          top = quad_max(top);
+          auto with = [&](uint32_t o) { top = o > top ? o : top; };
+          with((uint32_t)dpp_i<kDppHalfMirror>((int)top));
+          if constexpr (CN == 2) with((uint32_t)dpp_i<kDppMirror>((int)top));
+          const uint32_t byte = mx_scale_byte(top);
+          const float s = __uint_as_float(byte << 23);
+          uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, towards_zero<FTM_DT_F32>(y[0]), towards_zero<FTM_DT_F32>(y[1]), s, 0);
+          if constexpr (CN == 4)
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, towards_zero<FTM_DT_F32>(y[2]), towards_zero<FTM_DT_F32>(y[3]), s, 1);
+          w = byte == 255u ? 0u : positive_zeros(w);
+          if (t < cur.rt.cnt && n0 < NO) {
+            const int64_t row = cur.rt.row0 + t;
+            if constexpr (CN == 4) *(uint16_t*)((char*)c.out + (row * NO + n0) / 2) = (uint16_t)w;
+            else *((uint8_t*)c.out + (row * NO + n0) / 2) = (uint8_t)w;
+            if ((em & (32 / CN - 1)) == 0) out_scale[(row * NO + n0) / 32] = (uint8_t)byte;
+          }
+        });
+      } else {
+        constexpr int ON = CN == 8 ? 4 : CN;  // of a store of any alignment
+        const RowOut<CN> out(c, cur.rt, NO, n0);
+        if (out.vec && c.out_dtype == FTM_DT_BF16) {
+          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_BF16>(t, y); });
+        } else if (out.vec && c.out_dtype == FTM_DT_F32) {
+          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F32>(t, y); });
+        } else if (out.vec) {
+          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F16>(t, y); });
+        } else {
+          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int o = 0; o < CN; o += ON) {
+              float z[ON];
+#pragma unroll
+              for (int n = 0; n < ON; ++n) z[n] = y[o + n];
+              RowOut<ON>(c, cur.rt, NO, n0 + o).store(t, z);
+            }
+          });
+        }
+        if constexpr (GROUPED) {  // rows whose index names none: zeros over them
+          if (live != ~0u) {
+            wait_vm<0>();  // behind the results
+            for (int o = 0; o < CN; ++o)
+              for (int t = 0; t < 4 * MI; ++t) {
+                const int row = t0 + 16 * (t >> 2) + (t & 3);
+                if (!((live >> t) & 1u) && row < cur.rt.cnt && n0 + o < NO)
+                  store_scalar(c.out, (cur.rt.row0 + row) * NO + n0 + o, c.out_dtype, 0.0f);
+              }
+          }
+        }
+      }
       if (after >= end) break;
       cur = next;
       item = after;
@@ -1481,14 +1526,17 @@ hipError_t split(const ftm_w4a4& c, hipStream_t st) {
 }
 
 template <int S>
-int cols_lds(int K, int rows);
-template <int MT, int S>
+int cols_lds(int K, int rows) {
+  const int nsteps = (K + 255) / 256, codes = nsteps * rows * kRow, pitch = scale_pitch(nsteps);
+  return 4 * S * 16 * kRow + (codes > 16 * 36 * 4 ? codes : 16 * 36 * 4) + (rows + 64) * pitch;
+}
+template <int RW, int S>
 hipError_t cols(const ftm_w4a4& c, hipStream_t st) {
-  const int per = c.act >= 0 ? 32 : 64, lds = cols_lds<S>(c.K, 16 * MT);
-  const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + per - 1) / per;
-  if (mt * nt > kMaxGroups || lds > kMaxLds - 1024) return split<MT, 2, 4, 2>(c, st);
+  const int per = c.act >= 0 ? 32 : 64, lds = cols_lds<S>(c.K, RW);
+  const int64_t mt = row_tiles(c, RW), nt = (out_cols(c) + per - 1) / per;
+  if (mt * nt > kMaxGroups || lds > kMaxLds - 1024) return split<1, 2, 4, 2>(c, st);
   static DeviceBits lds_set{0};
-  const auto kernel = k_w4a4_cols<-1, MT, S, ftm_w4a4>;
+  const auto kernel = k_w4a4_cols<-1, RW, S, ftm_w4a4>;
   const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
   if (e != hipSuccess) return e;
   kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (int)nt);
@@ -1535,8 +1583,8 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
   if (c.offsets != nullptr) {
     const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
     if (seg >= 128) return tile<2, 2, 4, 8, 3>(c, st);
-    if (seg >= 16) return tile<1, 4, 4, 4, 3>(c, st);
-    return cols<1, 4>(c, st);
+    if (seg >= 16) return tile<2, 2, 2, 4, 6>(c, st);
+    return seg <= 4 ? cols<8, 3>(c, st) : cols<16, 3>(c, st);
   }
   const int64_t M = c.rows;
   if (M <= 16) return split<1, 1, 4, 4>(c, st);
@@ -1574,16 +1622,11 @@ hipError_t few(const FewCall& c, int dt, hipStream_t st) {
   return few<FTM_DT_BF16, NT, NW, S, MOE>(c, st);
 }
 
-template <int S>
-int cols_lds(int K, int rows) {
-  const int nsteps = (K + 255) / 256, codes = nsteps * rows * kRow, pitch = scale_pitch(nsteps);
-  return 4 * S * 16 * kRow + (codes > 16 * 36 * 4 ? codes : 16 * 36 * 4) + (rows + 64) * pitch;
-}
 template <int XDT, int S>
 hipError_t cols_moe(const FewCall& c, hipStream_t st) {
   const int ntiles = c.N / 64;
   static DeviceBits lds_set{0};
-  const auto kernel = k_w4a4_cols<XDT, 1, S, FewCall>;
+  const auto kernel = k_w4a4_cols<XDT, 16, S, FewCall>;
   const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
   if (e != hipSuccess) return e;
   kernel<<<dim3((unsigned)(c.P * ntiles)), dim3(256), cols_lds<S>(c.K, c.cap), st>>>(c, ntiles);
@@ -1627,7 +1670,7 @@ hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale
   const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
   if (c.K >= kMinK && offsets_ok(c) && seg >= 16) {
     if (seg >= 128) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
-    return tile<1, 4, 4, 4, 3, true, true, true>(c, out_scale, st);
+    return tile<2, 2, 2, 4, 6, true, true, true>(c, out_scale, st);
   }
   ftm_w4a4 wide = c;
   wide.out = h;
