@@ -1118,16 +1118,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, kRows = BM + BN;
   constexpr int kX = BM * kRow, kStage = kRows * kRow, kSlot = 8 * kRows;  // of codes, of scales
   constexpr int NX = BM / 8 / kWaves, NB = BN / 8 / kWaves, ND = NX + NB;  // 1 KiB copies a wave and step
-  constexpr int NR = (kRows + kThreads - 1) / kThreads;  // rows whose scales a thread carries
+  constexpr int NR = 2;                                  // rows whose scales a thread carries: of x, of the weights
+  static_assert(NX <= 8 && BN <= kThreads, "rows of scales");
   constexpr int kCols = ACT ? BN / 2 : BN;               // output channels of the tile
   constexpr int CN = ACT ? NJ / 2 : NJ;                  // neighbouring ones of a lane
-  constexpr int kAhead = 3;                              // row blocks read ahead of their products
+  constexpr int kAhead = MI >= 4 ? 7 : 2 * MI - 1;       // row blocks read ahead of their products
   constexpr int kLast = 2 * MI - kAhead;                 // from this one on they are the next step's
   constexpr int kNextX = MI < kAhead ? MI : kAhead;      // row blocks whose scales are read a step ahead
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies of 8 rows, as many for each wave");
   constexpr int kSecond = MI < kLast ? MI : kLast;       // row blocks that read the second half's weights
   static_assert(2 * MI % (kAhead + 1) == 0 && NJ % 4 == 0 && NJ % kSecond == 0, "the order of the reads");
-  extern __shared__ char lds[];  // [S][kStage], then [2][kSlot]
+  extern __shared__ char lds[];  // [S][kStage], [2][kSlot], the rows of x [BM]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -1135,6 +1136,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   const uint32_t Kb = (uint32_t)c.K / 2;
   const int nsteps = (nb + 7) / 8, nrun = nsteps > S ? nsteps : S;  // steps past K multiply zeros
   const bool indexed = GROUPED && c.row_index != nullptr;
+  int32_t* const index = (int32_t*)(lds + S * kStage + 2 * kSlot);
 
   // this workgroup's items: every (workgroups per XCD)-th of its XCD's run
   using Scan = std::conditional_t<GROUPED, RowScan<BM>, int>;
@@ -1172,22 +1174,21 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   int item = begin + (blockIdx.x >> 3);
   if (item < end) {
     Tile cur = tile_at(item);
-    // Rows of x that the wave's copies and the thread's scales read, asked for a tile
-    // ahead: waiting for them waits for every copy before them.
-    int ix[NX], is[NR];
-    auto rows_of = [&](const Tile& t) __attribute__((always_inline)) {
-      const int lane = opaque_lane();
+    // The next tile's rows of x, where they are read through an index, are copied to LDS a
+    // tile ahead: a load of them into registers would be waited for with every copy
+    // before it.  They are there from step S on; a shorter tile waits for them.
+    auto copy_index = [&](const Tile& t) __attribute__((always_inline)) {
+      if (!indexed || wave != 0) return;
+      const Rsrc res = make_rsrc(c.row_index + t.rt.row0, 4u * (uint32_t)t.rt.cnt);
 #pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int r = 8 * (wave * NX + i) + (lane >> 3);
-        ix[i] = indexed ? c.row_index[t.rt.row0 + (r < t.rt.cnt ? r : 0)] : r;
-      }
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const int r = 64 * wave + lane + kThreads * i;
-        is[i] = indexed ? c.row_index[t.rt.row0 + (r < t.rt.cnt ? r : 0)] : r;
-      }
+      for (int i = 0; i < BM / 64; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LPtr)(index + 64 * i), 4, 4 * lane + 256 * i, 0, 0, 0);
     };
+    auto index_here = [&] {
+      wait_vm<0>();
+      asm volatile("s_barrier" ::: "memory");
+    };
+    const bool index_late = indexed && nrun < 2 * S;
     // Offsets of a wave's copies: 8 rows each, a 16-byte piece a lane, swizzled; tokens
     // from the tile's first row, or, read through an index, from x's; weights from the tile's
     // first gate row.  Rows past the tile are not copied.
@@ -1199,8 +1200,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         const int r = 8 * (wave * NX + i) + (lane >> 3);
-        const bool in = r < t.rt.cnt && (!indexed || (ix[i] >= 0 && ix[i] < c.x_rows));
-        xoff[i] = in ? (uint32_t)ix[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+        const int ix = indexed ? index[r] : r;
+        const bool in = r < t.rt.cnt && ix >= 0 && (!indexed || ix < c.x_rows);
+        xoff[i] = in ? (uint32_t)ix * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
       }
       const int cols = NO - t.n < kCols ? NO - t.n : kCols;
       wres = make_rsrc((const char*)c.w + (int64_t)t.rt.e * c.w_stride + (int64_t)t.n * Kb, (uint32_t)((ACT ? NO : 0) + cols) * Kb);
@@ -1210,28 +1212,31 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
         woff[i] = (uint32_t)weight_row(r, cols) * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r));
       }
     };
-    // copy d of the wave's: tokens, then weights
+    // copy d of the wave's: tokens, then weights.  The sum is kept at its place: all of
+    // them ahead would stand between two products.
     auto copy = [&](int d, uint32_t k0, char* st) __attribute__((always_inline)) {
-      if (d < NX)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * (wave * NX + d)), 16, (int)(xoff[d < NX ? d : 0] + k0), 0, 0, 0);
-      else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + d - NX)), 16,
-                                                 (int)(woff[d < NX ? 0 : d - NX] + k0), 0, 0, 0);
+      uint32_t at;
+      asm volatile("v_add_u32 %0, %1, %2" : "=v"(at) : "v"(d < NX ? xoff[d < NX ? d : 0] : woff[d < NX ? 0 : d - NX]), "s"(k0));
+      if (d < NX) __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(st + 1024 * (wave * NX + d)), 16, (int)at, 0, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (LPtr)(st + kX + 1024 * (wave * NB + d - NX)), 16, (int)at, 0, 0, 0);
     };
     auto k_of = [&](int kb) { return (uint32_t)(kb < nsteps ? kb : nsteps - 1) * 128u; };
-    // Scales: a thread's rows, the eight bytes of the step after next under way
+    // Scales: a thread's rows, one of x (of those that its wave copies) and one of the
+    // weights, the eight bytes of the step after next under way
     const uint8_t* srow[NR];
     u32x2 sraw[NR];
     auto saim = [&](const Tile& t) __attribute__((always_inline)) {
-      const int cols = NO - t.n < kCols ? NO - t.n : kCols;
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        int r = 64 * wave + opaque_lane() + kThreads * i;
-        r = r < kRows ? r : kRows - 1;
-        const int64_t s = indexed ? (is[i] >= 0 && is[i] < c.x_rows ? is[i] : 0) : t.rt.row0 + (r < t.rt.cnt ? r : 0);
-        const uint8_t* w = c.w_scale + (int64_t)t.rt.e * c.w_scale_stride + (int64_t)(t.n + weight_row(r >= BM ? r - BM : 0, cols)) * nb;
-        srow[i] = r < BM ? c.x_scale + s * nb : w;
+      const int cols = NO - t.n < kCols ? NO - t.n : kCols, l = opaque_lane();
+      int r = 8 * NX * wave + (l < 8 * NX ? l : 0);
+      r = r < t.rt.cnt ? r : 0;
+      int64_t x = t.rt.row0 + r;
+      if (indexed) {
+        const int ix = index[r];
+        x = ix >= 0 && ix < c.x_rows ? ix : 0;
       }
+      srow[0] = c.x_scale + x * nb;
+      const int wr = (64 * wave + l) & (BN - 1);
+      srow[1] = c.w_scale + (int64_t)t.rt.e * c.w_scale_stride + (int64_t)(t.n + weight_row(wr, cols)) * nb;
     };
     auto load_s = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
@@ -1239,26 +1244,39 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
     };
     // bytes b0 b4 b1 b5 b2 b6 b3 b7: group g's two are neighbours
     auto store_s = [&](int kb, int slot) __attribute__((always_inline)) {
+      char* at = lds + S * kStage + slot * kSlot;
+      if (8 * kb + 8 > nb) {  // not all of the step's blocks are there
+#pragma unroll
+        for (int i = 0; i < NR; ++i) sraw[i] = fit_scales(sraw[i], kb, nb);
+      }
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const u32x2 v = fit_scales(sraw[i], kb, nb);
-        const int r = (int)threadIdx.x + kThreads * i;
-        if (kRows % kThreads == 0 || r < kRows)
-          *(u32x2*)(lds + S * kStage + slot * kSlot + 8 * r) =
-              (u32x2){__builtin_amdgcn_perm(v.y, v.x, 0x05010400u), __builtin_amdgcn_perm(v.y, v.x, 0x07030602u)};
+        const u32x2 v = sraw[i];
+        const int r = i == 0 ? 8 * NX * wave + lane : BM + ((64 * wave + lane) & (BN - 1));
+        if (i == 1 || NX == 8 || lane < 8 * NX)
+          *(u32x2*)(at + 8 * r) = (u32x2){__builtin_amdgcn_perm(v.y, v.x, 0x05010400u), __builtin_amdgcn_perm(v.y, v.x, 0x07030602u)};
       }
     };
     f32x4 acc[MI][NJ];
     u32x4 b[2][NJ], x[kAhead + 1];
     uint32_t sx[MI], sb[NJ], nx[kNextX], sn[NJ];
+    // The swizzle of row 16 i + m is that of row m: a base for each half of a stage and
+    // operand, the row block as an immediate
+    const uint32_t piece[2] = {16u * (uint32_t)(g ^ swz(m)), 16u * (uint32_t)((4 + g) ^ swz(m))};
+    const uint32_t xbase = (uint32_t)((16 * wm * MI + m) * kRow), wbase = (uint32_t)((BM + 16 * wn * NJ + m) * kRow);
+    const uint32_t sxbase = (uint32_t)(S * kStage + 8 * (16 * wm * MI + m) + 2 * g);
+    const uint32_t swbase = (uint32_t)(S * kStage + 8 * (BM + 16 * wn * NJ + m) + 2 * g);
     auto xfrag = [&](int slot, int at) __attribute__((always_inline)) {
-      return stage_piece(lds + slot * kStage, 16 * (wm * MI + at % MI) + m, at / MI, g);
+      return *(const u32x4*)(lds + (xbase + piece[at / MI] + (uint32_t)(slot * kStage)) + at % MI * 16 * kRow);
     };
     auto wfrag = [&](int slot, int j, int q) __attribute__((always_inline)) {
-      return stage_piece(lds + slot * kStage, BM + 16 * (wn * NJ + j) + m, q, g);
+      return *(const u32x4*)(lds + (wbase + piece[q] + (uint32_t)(slot * kStage)) + j * 16 * kRow);
     };
-    auto sfrag = [&](int slot, int r) __attribute__((always_inline)) {
-      return (uint32_t)*(const uint16_t*)(lds + S * kStage + slot * kSlot + 8 * r + 2 * g);
+    auto xscale = [&](int slot, int i) __attribute__((always_inline)) {
+      return (uint32_t)*(const uint16_t*)(lds + (sxbase + (uint32_t)(slot * kSlot)) + 128 * i);
+    };
+    auto wscale = [&](int slot, int j) __attribute__((always_inline)) {
+      return (uint32_t)*(const uint16_t*)(lds + (swbase + (uint32_t)(slot * kSlot)) + 128 * j);
     };
     // Products of step kb, whose first operands are in registers; the rest is read
     // kAhead row blocks ahead.  Once every wave has read the last of them, the stage's slot
@@ -1286,7 +1304,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
           __builtin_amdgcn_sched_barrier(0);
           const int a = at + kAhead;
           if (j == 0 && a < 2 * MI) x[a % (kAhead + 1)] = xfrag(slot, a);
-          if (j == 1 && a < MI) sx[a] = sfrag(par, 16 * (wm * MI + a) + m);
+          if (j == 1 && a < MI) sx[a] = xscale(par, a);
           if (at < kSecond) {  // the second half's weights, before the slot is given away
             constexpr int kPer = NJ / kSecond;
 #pragma unroll
@@ -1296,11 +1314,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
           if (at >= kLast) {
             const int t = (at - kLast) * NJ + j;
             if (j == 0) x[a % (kAhead + 1)] = xfrag(next, a - 2 * MI);
-            if (j == 1 && at - kLast < kNextX) nx[at - kLast] = sfrag(1 - par, 16 * (wm * MI + at - kLast) + m);
+            if (j == 1 && at - kLast < kNextX) nx[at - kLast] = xscale(1 - par, at - kLast);
 #pragma unroll
             for (int n = 0; n < NJ; ++n) {
               if (kFirstB + n * (kSlots - kFirstB) / NJ == t) b[0][n] = wfrag(next, n, 0);
-              if (n * kSlots / NJ == t) sn[n] = sfrag(1 - par, BM + 16 * (wn * NJ + n) + m);
+              if (n * kSlots / NJ == t) sn[n] = wscale(1 - par, n);
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -1316,7 +1334,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       for (int i = 0; i < kNextX; ++i) sx[i] = nx[i];
       __builtin_amdgcn_sched_barrier(0);
     };
-    rows_of(cur);
+    if (indexed) {
+      copy_index(cur);
+      index_here();
+    }
     aim(cur);
     saim(cur);
     load_s(0);
@@ -1331,23 +1352,26 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       b[0][j] = wfrag(0, j, 0);
-      sb[j] = sfrag(0, BM + 16 * (wn * NJ + j) + m);
+      sb[j] = wscale(0, j);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) x[i] = xfrag(0, i);
 #pragma unroll
-    for (int i = 0; i < kNextX; ++i) sx[i] = sfrag(0, 16 * (wm * MI + i) + m);
+    for (int i = 0; i < kNextX; ++i) sx[i] = xscale(0, i);
     int slot = 0, par = 0;
     for (;;) {
       const int after = item + (int)(gridDim.x >> 3);
       const Tile next = after < end ? tile_at(after) : cur;  // (the last tile's copies go on over it: nothing reads them)
-      rows_of(next);
+      copy_index(next);
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
       for (int kb = 0; kb < nrun; ++kb) {
-        if (kb == nrun - S) aim(next);  // from here on the copies are the next tile's
+        if (kb == nrun - S) {
+          if (index_late) index_here();
+          aim(next);  // from here on the copies are the next tile's
+        }
         if (kb == nrun - 2) saim(next);
         const int ahead = kb + S < nrun ? kb + S : kb + S - nrun;
         step(kb, kb + 1 < nrun ? kb + 1 : 0, kb + 2 < nrun ? kb + 2 : kb + 2 - nrun, k_of(ahead), slot, par);
@@ -1545,7 +1569,7 @@ hipError_t cols(const ftm_w4a4& c, hipStream_t st) {
 
 template <int WM, int WN, int MI, int NJ, int S, bool ACT, bool GROUPED, bool QOUT>
 hipError_t tile(const ftm_w4a4& c, uint8_t* out_scale, hipStream_t st) {
-  constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, lds = S * (BM + BN) * kRow + 16 * (BM + BN);
+  constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN, lds = S * (BM + BN) * kRow + 16 * (BM + BN) + 4 * BM;
   static_assert(lds <= kMaxLds, "fits a CU");
   constexpr int resident = kCUs * (2 * lds <= kMaxLds ? 2 : 1);  // workgroups the chip holds at once
   const int cols = ACT ? BN / 2 : BN;
