@@ -1410,97 +1410,91 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       float bias[NJ];
 #pragma unroll
       for (int n = 0; n < NJ; ++n) bias[n] = bits_to_f32(opaque_bits(bb[n]), c.bias_dtype);
-      // The activation in place of the gate's sums, then the results by their type: a path
-      // is as long as the work, not as all types and activations together (instructions that
-      // a tile runs once are fetched anew: 128 x 256 results took 3.9 us, so %RESULTS%)
-      if constexpr (ACT) {
-        with_act(c.act, [&](auto a) __attribute__((always_inline)) {
-          if constexpr (decltype(a)::value >= 0) {
+      // A path for each activation and type, as long as its work: instructions that a tile
+      // runs once are fetched anew, and a path that jumped over the other types' stores
+      // took 3.9 us for 128 x 256 results, so 1.3
+      const RowOut<CN> out(c, cur.rt, NO, n0);
+      with_act(ACT ? c.act : -1, [&](auto a) __attribute__((always_inline)) {
+        constexpr int A = decltype(a)::value;
+        if constexpr (ACT == (A >= 0)) {
+          auto each_row = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i) {
+              // one row block after the other, so that their results do not all sit in
+              // registers at once
+              f32x4 v[NJ];
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) {
+                v[j] = acc[i][j];
+                asm volatile("" : "+v"(v[j]) : : "memory");
+              }
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                float y[CN];
+#pragma unroll
+                for (int n = 0; n < CN; ++n) {
+                  y[n] = v[n][r] + bias[n];
+                  if constexpr (ACT) y[n] = act_gated<A>(y[n], v[CN + n][r] + bias[CN + n], c);
+                }
+                f(t0 + 16 * i + r, y);
+              }
+            }
+          };
+          if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
+            each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
+              uint32_t top = 0;
 #pragma unroll
               for (int n = 0; n < CN; ++n) {
-                f32x4 y = acc[i][n], u = acc[i][CN + n];
-                asm volatile("" : "+v"(y), "+v"(u) : : "memory");  // one block after the other
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = act_gated<decltype(a)::value>(y[r] + bias[n], u[r] + bias[CN + n], c);
-                asm volatile("" : "+v"(y) : : "memory");
-                acc[i][n] = y;
+                const uint32_t b = __float_as_uint(y[n]) & 0x7fffffffu;
+                top = b > top ? b : top;
               }
-          }
-        });
-      }
-      auto each_row = [&](auto f) __attribute__((always_inline)) {
+              top = quad_max(top);
+              auto with = [&](uint32_t o) { top = o > top ? o : top; };
+              with((uint32_t)dpp_i<kDppHalfMirror>((int)top));
+              if constexpr (CN == 2) with((uint32_t)dpp_i<kDppMirror>((int)top));
+              const uint32_t byte = mx_scale_byte(top);
+              const float s = __uint_as_float(byte << 23);
+              uint32_t w =
+                  __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, towards_zero<FTM_DT_F32>(y[0]), towards_zero<FTM_DT_F32>(y[1]), s, 0);
+              if constexpr (CN == 4)
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, towards_zero<FTM_DT_F32>(y[2]), towards_zero<FTM_DT_F32>(y[3]), s, 1);
+              w = byte == 255u ? 0u : positive_zeros(w);
+              if (t < cur.rt.cnt && n0 < NO) {
+                const int64_t row = cur.rt.row0 + t;
+                if constexpr (CN == 4) *(uint16_t*)((char*)c.out + (row * NO + n0) / 2) = (uint16_t)w;
+                else *((uint8_t*)c.out + (row * NO + n0) / 2) = (uint8_t)w;
+                if ((em & (32 / CN - 1)) == 0) out_scale[(row * NO + n0) / 32] = (uint8_t)byte;
+              }
+            });
+          } else if (out.vec && c.out_dtype == FTM_DT_BF16) {
+            each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_BF16>(t, y); });
+          } else if (out.vec && c.out_dtype == FTM_DT_F32) {
+            each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F32>(t, y); });
+          } else if (out.vec) {
+            each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F16>(t, y); });
+          } else {
+            constexpr int ON = CN == 8 ? 4 : CN;  // of a store of any alignment
+            each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          // one row block after the other, so that their results do not all sit in
-          // registers at once
+              for (int o = 0; o < CN; o += ON) {
+                float z[ON];
 #pragma unroll
-          for (int n = 0; n < CN; ++n) asm volatile("" : "+v"(acc[i][n]) : : "memory");
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float y[CN];
-#pragma unroll
-            for (int n = 0; n < CN; ++n) y[n] = ACT ? acc[i][n][r] : acc[i][n][r] + bias[n];
-            f(t0 + 16 * i + r, y);
+                for (int n = 0; n < ON; ++n) z[n] = y[o + n];
+                RowOut<ON>(c, cur.rt, NO, n0 + o).store(t, z);
+              }
+            });
           }
         }
-      };
-      if constexpr (QOUT) {  // a block of 32 is 32 / CN neighbouring lanes
-        each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int n = 0; n < CN; ++n) {
-            const uint32_t b = __float_as_uint(y[n]) & 0x7fffffffu;
-            top = b > top ? b : top;
-          }
-          top = quad_max(top);
-          auto with = [&](uint32_t o) { top = o > top ? o : top; };
-          with((uint32_t)dpp_i<kDppHalfMirror>((int)top));
-          if constexpr (CN == 2) with((uint32_t)dpp_i<kDppMirror>((int)top));
-          const uint32_t byte = mx_scale_byte(top);
-          const float s = __uint_as_float(byte << 23);
-          uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, towards_zero<FTM_DT_F32>(y[0]), towards_zero<FTM_DT_F32>(y[1]), s, 0);
-          if constexpr (CN == 4)
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, towards_zero<FTM_DT_F32>(y[2]), towards_zero<FTM_DT_F32>(y[3]), s, 1);
-          w = byte == 255u ? 0u : positive_zeros(w);
-          if (t < cur.rt.cnt && n0 < NO) {
-            const int64_t row = cur.rt.row0 + t;
-            if constexpr (CN == 4) *(uint16_t*)((char*)c.out + (row * NO + n0) / 2) = (uint16_t)w;
-            else *((uint8_t*)c.out + (row * NO + n0) / 2) = (uint8_t)w;
-            if ((em & (32 / CN - 1)) == 0) out_scale[(row * NO + n0) / 32] = (uint8_t)byte;
-          }
-        });
-      } else {
-        constexpr int ON = CN == 8 ? 4 : CN;  // of a store of any alignment
-        const RowOut<CN> out(c, cur.rt, NO, n0);
-        if (out.vec && c.out_dtype == FTM_DT_BF16) {
-          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_BF16>(t, y); });
-        } else if (out.vec && c.out_dtype == FTM_DT_F32) {
-          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F32>(t, y); });
-        } else if (out.vec) {
-          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) { out.template store_vec<FTM_DT_F16>(t, y); });
-        } else {
-          each_row([&](int t, const float(&y)[CN]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int o = 0; o < CN; o += ON) {
-              float z[ON];
-#pragma unroll
-              for (int n = 0; n < ON; ++n) z[n] = y[o + n];
-              RowOut<ON>(c, cur.rt, NO, n0 + o).store(t, z);
+      });
+      if constexpr (GROUPED && !QOUT) {  // rows whose index names none: zeros over them
+        if (live != ~0u) {
+          wait_vm<0>();  // behind the results
+          for (int o = 0; o < CN; ++o)
+            for (int t = 0; t < 4 * MI; ++t) {
+              const int row = t0 + 16 * (t >> 2) + (t & 3);
+              if (!((live >> t) & 1u) && row < cur.rt.cnt && n0 + o < NO)
+                store_scalar(c.out, (cur.rt.row0 + row) * NO + n0 + o, c.out_dtype, 0.0f);
             }
-          });
-        }
-        if constexpr (GROUPED) {  // rows whose index names none: zeros over them
-          if (live != ~0u) {
-            wait_vm<0>();  // behind the results
-            for (int o = 0; o < CN; ++o)
-              for (int t = 0; t < 4 * MI; ++t) {
-                const int row = t0 + 16 * (t >> 2) + (t & 3);
-                if (!((live >> t) & 1u) && row < cur.rt.cnt && n0 + o < NO)
-                  store_scalar(c.out, (cur.rt.row0 + row) * NO + n0 + o, c.out_dtype, 0.0f);
-              }
-          }
         }
       }
       if (after >= end) break;
@@ -1606,16 +1600,20 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
   if (c.K < kMinK || !offsets_ok(c)) return any(c, st);
   if (c.offsets != nullptr) {
     const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
-    if (seg >= 128) return tile<2, 2, 4, 8, 3>(c, st);
-    if (seg >= 16) return tile<2, 2, 2, 4, 6>(c, st);
+    if (seg >= 200) return tile<2, 2, 8, 8, 2>(c, st);
+    if (seg >= 96) return tile<2, 2, 4, 8, 3>(c, st);
+    if (seg >= 16) return tile<2, 2, 2, 8, 3>(c, st);
     return seg <= 4 ? cols<8, 3>(c, st) : cols<16, 3>(c, st);
   }
   const int64_t M = c.rows;
+  const auto blocks = [&](int rows, int cols) { return ((M + rows - 1) / rows) * ((c.N + cols - 1) / cols); };
   if (M <= 16) return split<1, 1, 4, 4>(c, st);
   if (M <= 32) return split<2, 1, 4, 3>(c, st);
-  if (M > 1024 && c.row_index == nullptr) return tile<2, 2, 8, 8, 2>(c, st);
-  if (M > 512 && c.row_index == nullptr) return tile<2, 2, 4, 8, 3>(c, st);
-  return split<4, 4, 4, 2>(c, st);
+  if (blocks(32, 32) <= 640 || c.row_index != nullptr) return split<2, 2, 4, 2>(c, st);
+  if (blocks(64, 64) <= kCUs) return split<4, 4, 8, 1>(c, st);
+  if (blocks(256, 256) >= 192) return tile<2, 2, 8, 8, 2>(c, st);
+  if (blocks(128, 256) >= 192) return tile<2, 2, 4, 8, 3>(c, st);
+  return tile<2, 2, 4, 4, 4>(c, st);
 }
 
 namespace {
@@ -1693,8 +1691,9 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
 hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale, hipStream_t st) {
   const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
   if (c.K >= kMinK && offsets_ok(c) && seg >= 16) {
-    if (seg >= 128) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
-    return tile<2, 2, 2, 4, 6, true, true, true>(c, out_scale, st);
+    if (seg >= 200) return tile<2, 2, 8, 8, 2, true, true, true>(c, out_scale, st);
+    if (seg >= 96) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
+    return tile<2, 2, 2, 8, 3, true, true, true>(c, out_scale, st);
   }
   ftm_w4a4 wide = c;
   wide.out = h;
