@@ -874,63 +874,61 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
     }
     __syncthreads();
   } else {
-    // The tile's rows of x by scalar loads: a vector load would be waited for with every
-    // copy before it, and the weights are to be under way first.
+    // The rows of x: of the copies, of the scales, of the results
     const bool indexed = c.row_index != nullptr;
     const int64_t x_rows = indexed ? c.x_rows : c.rows;
     const uint32_t Kb = (uint32_t)K / 2;
-    int row[RW];
+    const int rs = lane & (RW - 1), turn = kTurns * wave + lane / RW;
+    auto in_tile = [&](int r) { return r < cnt ? r : 0; };
+    int ic[NC], ir[MT], is = in_tile(rs);
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int64_t at = rt.row0 + (i < cnt ? i : cnt - 1);
-      row[i] = indexed ? c.row_index[at] : (int)at;
+    for (int i = 0; i < NC; ++i) ic[i] = in_tile(8 * i + (lane >> 3));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) ir[i] = in_tile(16 * i + m);
+    if (indexed) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) ic[i] = c.row_index[rt.row0 + ic[i]];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) ir[i] = c.row_index[rt.row0 + ir[i]];
+      is = c.row_index[rt.row0 + is];
+    } else {
+      is += (int)rt.row0;
     }
-    // row r of them, the same for the lanes of a group
-    auto row_at = [&](int r, int first, int n) __attribute__((always_inline)) {
-      int v = row[first];
-#pragma unroll
-      for (int i = 1; i < n; ++i) v = r == first + i ? row[first + i] : v;
-      return v;
-    };
-    fill(scales, 0, nsteps, nb, [&] {
-      request();
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < S; ++u) issue(u, u);
-    });
-    // the rows' copies; rows past the tile and rows that are none are not copied
+    // rows past the tile and rows that are none are not copied
     const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
     uint32_t xoff[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int r = 8 * i + (lane >> 3), v = row_at(r, 8 * i, 8);
-      const bool in = r < cnt && v >= 0 && v < x_rows;
-      xoff[i] = in ? (uint32_t)(indexed ? v : r) * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+      const int r = 8 * i + (lane >> 3);
+      const bool in = r < cnt && ic[i] >= 0 && ic[i] < (indexed ? x_rows : (int64_t)cnt);
+      xoff[i] = in ? (uint32_t)ic[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
     }
-    const int rs = lane & (RW - 1), vs = row_at(rs, 0, RW), turn = kTurns * wave + lane / RW;
-    const uint8_t* xs = c.x_scale + (int64_t)(vs >= 0 && vs < x_rows ? vs : 0) * nb;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) live[i] = !indexed || (ir[i] >= 0 && ir[i] < x_rows);
+    const uint8_t* xs = c.x_scale + (int64_t)(is >= 0 && is < x_rows ? is : 0) * nb;
     u32x2 own[2];  // the lane's row at steps turn and turn + 4 kTurns
+    fill(scales, 0, nsteps, nb, [&] {
+      request();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = turn + 4 * kTurns * i;
-      own[i] = load_scales(xs, s < nsteps ? s : nsteps - 1, nb);
-    }
-    for (int s = wave; s < nsteps; s += 4)
+      for (int i = 0; i < 2; ++i) {
+        const int s = turn + 4 * kTurns * i;
+        own[i] = load_scales(xs, s < nsteps ? s : nsteps - 1, nb);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      for (int s = wave; s < nsteps; s += 4)
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(codes + (s * R + 8 * i) * kRow), 16, (int)(xoff[i] + 128u * s), 0, 0, 0);
+        for (int i = 0; i < NC; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (LPtr)(codes + (s * R + 8 * i) * kRow), 16, (int)(xoff[i] + 128u * s), 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int r = 16 * i + (RW == 8 ? m & 7 : m), v = row_at(r, 16 * i, RW < 16 ? RW : 16);
-      live[i] = v >= 0 && v < x_rows;
-    }
+      for (int u = 0; u < S; ++u) issue(u, u);
+    });
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int s = turn + 4 * kTurns * i;
       if (s < nsteps) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(own[i], s, nb);
     }
     for (int s = turn + 8 * kTurns; s < nsteps; s += 4 * kTurns) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(load_scales(xs, s, nb), s, nb);
-    wait_vm<0>();  // the rows' copies have landed, and the first weights
+    wait_vm<2 * S>();  // the rows' copies have landed
     __syncthreads();
   }
   f32x4 acc[MT];
@@ -1603,7 +1601,7 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
     if (seg >= 200) return tile<2, 2, 8, 8, 2>(c, st);
     if (seg >= 96) return tile<2, 2, 4, 8, 3>(c, st);
     if (seg >= 16) return tile<2, 2, 2, 8, 3>(c, st);
-    return seg <= 4 ? cols<8, 3>(c, st) : cols<16, 3>(c, st);
+    return seg <= 4 ? cols<8, 2>(c, st) : cols<16, 2>(c, st);
   }
   const int64_t M = c.rows;
   const auto blocks = [&](int rows, int cols) { return ((M + rows - 1) / rows) * ((c.N + cols - 1) / cols); };
