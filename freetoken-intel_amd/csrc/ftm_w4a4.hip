@@ -1671,13 +1671,13 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
                      (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
                      c.topk_ids, c.ids_dtype == FTM_ID_I64, P, c.num_experts, c.k, hq, hs};
   constexpr int kRoom = kMaxLds - 1024;  // beside the lists
-  if (cols_lds<6>(H, cap) <= kRoom) e = cols_moe<6>(f, c.dtype, st);
+  if (cols_lds<2>(H, cap) <= kRoom) e = cols_moe<2>(f, c.dtype, st);
   else if (few_lds<4, 8, 2>(H, cap) <= kRoom && H > 8 * 256) e = few<4, 8, 2, true>(f, c.dtype, st);
   else if (few_lds<4, 8, 1>(H, cap) <= kRoom) e = few<4, 8, 1, true>(f, c.dtype, st);
   else return false;
   if (e != hipSuccess) return true;
   const int ntiles = (H + 15) / 16;
-  k_w4a4_few_down<8, 4><<<dim3((unsigned)(ntiles * c.T)), dim3(512), 0, st>>>(c, hq, hs, ntiles);
+  k_w4a4_few_down<8, 3><<<dim3((unsigned)(ntiles * c.T)), dim3(512), 0, st>>>(c, hq, hs, ntiles);
   e = hipGetLastError();
   return true;
 }
