@@ -253,6 +253,7 @@ int check_w4a4(const ftm_w4a4* call) {
   if (c.act >= 0 && c.N % 2 != 0) return FTM_ERR_DIM;
   if (c.num_experts < 1 || c.num_experts > kMaxExperts || (c.offsets == nullptr && c.num_experts != 1))
     return FTM_ERR_DIM;
+  if (c.row_index != nullptr && c.offsets == nullptr) return FTM_ERR_DIM;
   if (c.num_experts > 1 && (c.w_stride < (int64_t)c.N * (c.K / 2) || c.w_scale_stride < (int64_t)c.N * (c.K / 32)))
     return FTM_ERR_DIM;
   if (c.rows == 0) return FTM_OK;

@@ -75,7 +75,7 @@ __device__ __forceinline__ float dequant_elem(const ProjSlot& W, int n, int k) {
 }
 
 // MXFP4 in row order: eight codes a lane, the LUT value by conversion (exact, at scale 1)
-// and the same fp32 product as above.  Bound by its stores: 8192 x 4096 to fp32 %T us, one
+// and the same fp32 product as above.  Bound by its stores: 8192 x 4096 to fp32 25 us, one
 // element a lane 74.
 template <int DT>
 __global__ __launch_bounds__(kBlock) void k_dequant_mxfp4(const uint32_t* codes, const uint8_t* scales, int64_t words, char* out) {

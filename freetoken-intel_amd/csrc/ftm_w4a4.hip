@@ -164,7 +164,7 @@ hipError_t launch_quant_mxfp4(const void* x, int dt, int64_t rows, int K, int64_
 // 1 / (1 + e^-z) from the hardware's 2^t and 1 / t, one step of fp32 off each.  Rounding
 // t = -z log2(e) moves e^-z by |z| 2^-24 at most, as much as half a step of z does.  In
 // fp32's own division and exponential the epilogue of a tile took half as long as its
-// products (clamped gate, 8192 rows of 2880 x 5760: 231 us, so 139).
+// products (clamped gate, 8192 rows of 2880 x 5760: 231 us, so 213).
 __device__ __forceinline__ float sigmoid_of(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
@@ -412,62 +412,32 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
-  // The rows of x: of this wave's results, of its copies, and of its scales
-  const bool indexed = c.row_index != nullptr;
   using Fill = FillScales<16 * (MT + NT)>;
-  int rr[kParts], rc[2 * MT], rs[Fill::kRows];
-#pragma unroll
-  for (int p = 0; p < kParts; ++p) rr[p] = 16 * ((p * NW + wave) / NT) + m;
-#pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) rc[i] = 8 * i + (lane >> 3);
-#pragma unroll
-  for (int i = 0; i < Fill::kRows; ++i) rs[i] = Fill::row(i);
-  auto known = [&](int r) { return rt.row0 + (r < rt.cnt ? r : 0); };
-  const bool none = rt.e < 0;
-  const int64_t x_rows = indexed ? c.x_rows : c.rows;
-  if (indexed && !none) {
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) rr[p] = rr[p] < rt.cnt ? c.row_index[known(rr[p])] : -1;
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) rc[i] = rc[i] < rt.cnt ? c.row_index[known(rc[i])] : -1;
-#pragma unroll
-    for (int i = 0; i < Fill::kRows; ++i) rs[i] = rs[i] < 16 * MT ? c.row_index[known(rs[i])] : 0;
-  } else {
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) rr[p] = rr[p] < rt.cnt && !none ? (int)known(rr[p]) : -1;
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) rc[i] = rc[i] < rt.cnt ? rc[i] : -1;
-#pragma unroll
-    for (int i = 0; i < Fill::kRows; ++i) rs[i] = (int)known(rs[i]);
-  }
   SplitBias bias[kParts];
   auto request = [&] {
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
-      bias[p].request(none ? nullptr : c.bias, c.bias_dtype, (int64_t)rt.e * c.N, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
+      bias[p].request(c.bias, c.bias_dtype, 0, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
   };
   const int nsteps = (nb + 7) / 8, per = (nsteps + NW - 1) / NW;
   const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
-  if (!none && lo < hi) {
-    // rows past the tile and rows that are none are not copied; offsets from the tile's
-    // first token, or, read through an index, from x's
+  if (lo < hi) {
+    // rows past the tile are not copied; offsets from its first token
     const uint32_t Kb = (uint32_t)c.K / 2;
-    const Rsrc xres = make_rsrc((const char*)c.x + (indexed ? 0 : rt.row0 * Kb), (uint32_t)(indexed ? c.x_rows : rt.cnt) * Kb);
-    const SplitWeights<NT> weights((const char*)c.w + (int64_t)rt.e * c.w_stride, NO, c.K, act, n0, ncol);
+    const Rsrc xres = make_rsrc((const char*)c.x + rt.row0 * Kb, (uint32_t)rt.cnt * Kb);
+    const SplitWeights<NT> weights((const char*)c.w, NO, c.K, act, n0, ncol);
     uint32_t xoff[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
       const int r = 8 * i + (lane >> 3);
-      const bool in = rc[i] >= 0 && rc[i] < (indexed ? x_rows : (int64_t)rt.cnt);
-      xoff[i] = in ? (uint32_t)rc[i] * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
+      xoff[i] = r < rt.cnt ? (uint32_t)r * Kb + 16u * (uint32_t)((lane & 7) ^ swz(r)) : kNowhere;
     }
     Fill fill;
 #pragma unroll
     for (int i = 0; i < Fill::kRows; ++i) {
       const int r = Fill::row(i);
       const int64_t n = n0 + SplitWeights<NT>::row(NO, act, ncol, r < 16 * MT ? 0 : r - 16 * MT);
-      fill.p[i] = r < 16 * MT ? c.x_scale + (int64_t)(rs[i] >= 0 && rs[i] < x_rows ? rs[i] : 0) * nb
-                              : c.w_scale + (int64_t)rt.e * c.w_scale_stride + n * nb;
+      fill.p[i] = r < 16 * MT ? c.x_scale + (rt.row0 + (r < rt.cnt ? r : 0)) * nb : c.w_scale + n * nb;
     }
     char* ring = lds + wave * (S * kStage);
     char* scales = lds + NW * S * kStage + wave * (MT + NT) * 16 * scale_pitch(per);
@@ -530,7 +500,6 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, 
       for (int r = 0; r < 4; ++r) {
         y[r] = u[r] + bias[p].at(r, c.bias_dtype);
         if constexpr (A >= 0) y[r] = act_gated<A>(y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
-        y[r] = rr[p] >= 0 && rr[p] < x_rows ? y[r] : 0.0f;
       }
       RowOut<4>(c, rt, NO, split_channel<NT>(act, n0, b, g)).store(16 * (b / NT) + m, y);
     });
@@ -605,30 +574,19 @@ struct FewCall {
   uint8_t *hq, *hs;
 };
 
-// Up to 16 tokens whose values are still wide: a workgroup quantises them itself, each wave
-// the K that it multiplies, while its weights are under way, and multiplies them by a
-// tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.  A layer's first
-// product (MOE) finds the tokens of its expert in the ids, and quantises its 32
-// channels of h, one block, in the epilogue.
-template <int XDT, int NT, int NW, int S, bool MOE>
-__global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
+// Up to 16 tokens whose values are still wide, one weight: a workgroup quantises them
+// itself, each wave the K that it multiplies, while its weights are under way, and
+// multiplies them by a tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.
+template <int XDT, int NT, int NW, int S>
+__global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
   using V = Vec8<XDT>;
   constexpr int kStage = NT * 16 * kRow, kParts = (NT + NW - 1) / NW, kBatch = 4;
-  extern __shared__ char lds[];  // [NW] of: ring [S][kStage], codes [per][cap][kRow], scales of weights and tokens; then the sums
-  __shared__ int lists[NW][kFewRows];
+  extern __shared__ char lds[];  // [NW] of: ring [S][kStage], codes [per][cnt][kRow], scales of weights and tokens; then the sums
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt = blockIdx.x % ntiles;
-  const bool act = MOE || c.act >= 0;
-  const int NO = act ? c.N / 2 : c.N, K = c.K, nb = K / 32, cap = c.cap;
-  int e = 0, cnt = cap;
-  if constexpr (MOE) {
-    const FewPairs pairs(c.ids, c.ids64 != 0, c.P, c.E, blockIdx.x / ntiles, cap, lists[wave]);
-    e = pairs.e;
-    cnt = pairs.cnt;
-    if (cnt == 0) return;
-  }
-  const int cols = act ? 8 * NT : 16 * NT, n0 = nt * cols, ncol = NO - n0 < cols ? NO - n0 : cols;
+  const bool act = c.act >= 0;
+  const int NO = act ? c.N / 2 : c.N, K = c.K, nb = K / 32, cnt = c.cap;
+  const int cols = act ? 8 * NT : 16 * NT, n0 = blockIdx.x * cols, ncol = NO - n0 < cols ? NO - n0 : cols;
   f32x4 acc[1][NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[0][j] = (f32x4){0, 0, 0, 0};
@@ -636,15 +594,15 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
   auto request = [&] {
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
-      bias[p].request(c.bias, c.bias_dtype, (int64_t)e * c.N, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
+      bias[p].request(c.bias, c.bias_dtype, 0, act, NO, split_channel<NT>(act, n0, p * NW + wave, g));
   };
   const int nsteps = (nb + 7) / 8, per = (nsteps + NW - 1) / NW, pitch = scale_pitch(per);
   const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
   if (lo < hi) {
-    const SplitWeights<NT> weights(c.w + (int64_t)e * c.w_stride, NO, K, act, n0, ncol);
-    char* ring = lds + wave * (S * kStage + per * cap * kRow + (16 * NT + cap) * pitch);
+    const SplitWeights<NT> weights(c.w, NO, K, act, n0, ncol);
+    char* ring = lds + wave * (S * kStage + per * cnt * kRow + (16 * NT + cnt) * pitch);
     char* codes = ring + S * kStage;
-    char* scales = codes + per * cap * kRow;  // of the weights, then of the tokens
+    char* scales = codes + per * cnt * kRow;  // of the weights, then of the tokens
     char* xscales = scales + 16 * NT * pitch;
     auto issue = [&](int step, int slot) __attribute__((always_inline)) {
       weights.issue(ring + slot * kStage, step < hi ? (uint32_t)step * 128u : kNowhere);
@@ -652,7 +610,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
     FillScales<16 * NT> fill;
 #pragma unroll
     for (int i = 0; i < fill.kRows; ++i)
-      fill.p[i] = c.w_scale + (int64_t)e * c.w_scale_stride + (n0 + SplitWeights<NT>::row(NO, act, ncol, fill.row(i))) * nb;
+      fill.p[i] = c.w_scale + (n0 + SplitWeights<NT>::row(NO, act, ncol, fill.row(i))) * nb;
     // half a wave takes 256 values of one row: of this wave's one step two rows at a time,
     // else two steps of one
     const int half = lane >> 5, l32 = lane & 31, n = hi - lo, hp = (n + 1) / 2;
@@ -665,8 +623,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
       for (int i = 0; i < kBatch; ++i) {
         const int t = t0 + i, r = row_of(t), s = step_of(t), k = 256 * (lo + s) + 8 * l32;
         if (t < turns && r < cnt && s < n && k < K) {
-          const int64_t row = MOE ? lists[wave][r] / c.k : r;
-          v[i].load(c.x + row * c.x_stride + (int64_t)(k / 8) * V::kBytes);
+          v[i].load(c.x + r * c.x_stride + (int64_t)(k / 8) * V::kBytes);
         } else {
           v[i].zero();
         }
@@ -679,7 +636,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
         const uint32_t byte = mx_scale_byte(quad_max(v[i].max_bits()));
         const uint32_t w = mx_codes<XDT>(v[i], byte);
         if (t < turns && r < cnt && s < n) {
-          *(uint32_t*)(codes + (s * cap + r) * kRow + 16 * ((l32 >> 2) ^ swz(r)) + 4 * (l32 & 3)) = w;
+          *(uint32_t*)(codes + (s * cnt + r) * kRow + 16 * ((l32 >> 2) ^ swz(r)) + 4 * (l32 & 3)) = w;
           if ((l32 & 3) == 0) *(uint8_t*)(xscales + r * pitch + 8 * s + (l32 >> 2)) = (uint8_t)byte;
         }
       }
@@ -710,7 +667,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
       for (int q = 0; q < 2; ++q) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) w[q][j] = stage_piece(st, 16 * j + m, q, g);
-        x[q] = stage_piece(codes + (step - lo) * cap * kRow, xr, q, g);
+        x[q] = stage_piece(codes + (step - lo) * cnt * kRow, xr, q, g);
       }
       auto scale = [&](const char* at, int r) { return scale_operand(*(const u32x2*)(at + r * pitch + 8 * (step - lo)), g); };
 #pragma unroll
@@ -730,8 +687,6 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
   } else {
     request();
   }
-  constexpr int kSums = NW * NT * 1024, kPitch = 36;  // h: [16][kPitch] behind the sums
-  float* h = (float*)(lds + kSums);
   with_act(c.act, [&](auto a) {
     constexpr int A = decltype(a)::value;
     split_sums<1, NT, NW>(lds, acc, A >= 0, [&](int p, int b, f32x4 u, f32x4 v) {
@@ -742,28 +697,9 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c, int ntiles) {
         y[r] = u[r] + bias[p].at(r, c.bias_dtype);
         if constexpr (A >= 0) y[r] = act_gated<A>(y[r], v[r] + bias[p].at(4 + r, c.bias_dtype), c);
       }
-      if constexpr (MOE) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) h[m * kPitch + 8 * b + 4 * g + r] = y[r];
-      } else {
-        RowOut<4>(c, RowTile{0, cnt, 0}, NO, split_channel<NT>(act, n0, b, g)).store(m, y);
-      }
+      RowOut<4>(c, RowTile{0, cnt, 0}, NO, split_channel<NT>(act, n0, b, g)).store(m, y);
     });
   });
-  if constexpr (MOE) {
-    static_assert(NT == 4, "a tile is one block of h");
-    __syncthreads();
-    const int row = lane >> 2, part = lane & 3;
-    if (wave != 0) return;
-    Vec8<FTM_DT_F32> v;
-    v.load((const char*)(h + row * kPitch + 8 * part));
-    const uint32_t byte = mx_scale_byte(quad_max(v.max_bits()));
-    const uint32_t codes = mx_codes<FTM_DT_F32>(v, byte);
-    if (row >= cnt) return;
-    const int64_t at = (int64_t)lists[0][row] * (NO / 32) + nt;
-    *(uint32_t*)(c.hq + at * 16 + 4 * part) = codes;
-    if (part == 0) c.hs[at] = (uint8_t)byte;
-  }
 }
 
 // ------------------------------------------------------------------ columns over the waves
@@ -1521,7 +1457,7 @@ hipError_t any(const ftm_w4a4& c, hipStream_t st) {
   return hipGetLastError();
 }
 
-constexpr int kMaxLds = 160 * 1024;
+constexpr int kMaxLds = 160 * 1024, kListLds = 1024;  // of which k_w4a4_cols has its lists
 
 template <int MT, int NT, int NW, int S>
 int split_lds(const ftm_w4a4& c) {
@@ -1530,14 +1466,18 @@ int split_lds(const ftm_w4a4& c) {
   return lds > sums ? lds : sums;
 }
 template <int MT, int NT, int NW, int S>
+bool split_fits(const ftm_w4a4& c) {
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT;
+  return split_lds<MT, NT, NW, S>(c) <= kMaxLds && row_tiles(c, 16 * MT) * ((out_cols(c) + cols - 1) / cols) <= kMaxGroups;
+}
+template <int MT, int NT, int NW, int S>
 hipError_t split(const ftm_w4a4& c, hipStream_t st) {
-  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, lds = split_lds<MT, NT, NW, S>(c);
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT;
   const int64_t mt = row_tiles(c, 16 * MT), nt = (out_cols(c) + cols - 1) / cols;
-  if (mt * nt > kMaxGroups || lds > kMaxLds) return any(c, st);
   static DeviceBits lds_set{0};
   const hipError_t e = allow_lds(lds_set, (const void*)k_w4a4_split<MT, NT, NW, S>, kMaxLds);
   if (e != hipSuccess) return e;
-  k_w4a4_split<MT, NT, NW, S><<<dim3((unsigned)(mt * nt)), dim3(64 * NW), lds, st>>>(c, (int)mt, (int)nt);
+  k_w4a4_split<MT, NT, NW, S><<<dim3((unsigned)(mt * nt)), dim3(64 * NW), split_lds<MT, NT, NW, S>(c), st>>>(c, (int)mt, (int)nt);
   return hipGetLastError();
 }
 
@@ -1547,15 +1487,19 @@ int cols_lds(int K, int rows) {
   return 4 * S * 16 * kRow + (codes > 16 * 36 * 4 ? codes : 16 * 36 * 4) + (rows + 64) * pitch;
 }
 template <int RW, int S>
+bool cols_fits(const ftm_w4a4& c) {
+  const int per = c.act >= 0 ? 32 : 64;
+  return cols_lds<S>(c.K, RW) <= kMaxLds - kListLds && row_tiles(c, RW) * ((out_cols(c) + per - 1) / per) <= kMaxGroups;
+}
+template <int RW, int S>
 hipError_t cols(const ftm_w4a4& c, hipStream_t st) {
-  const int per = c.act >= 0 ? 32 : 64, lds = cols_lds<S>(c.K, RW);
+  const int per = c.act >= 0 ? 32 : 64;
   const int64_t mt = row_tiles(c, RW), nt = (out_cols(c) + per - 1) / per;
-  if (mt * nt > kMaxGroups || lds > kMaxLds - 1024) return split<1, 2, 4, 2>(c, st);
   static DeviceBits lds_set{0};
   const auto kernel = k_w4a4_cols<-1, RW, S, ftm_w4a4>;
-  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - kListLds);
   if (e != hipSuccess) return e;
-  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), lds, st>>>(c, (int)nt);
+  kernel<<<dim3((unsigned)(mt * nt)), dim3(256), cols_lds<S>(c.K, RW), st>>>(c, (int)nt);
   return hipGetLastError();
 }
 
@@ -1575,13 +1519,10 @@ hipError_t tile(const ftm_w4a4& c, uint8_t* out_scale, hipStream_t st) {
   kernel<<<dim3((unsigned)grid), dim3(64 * WM * WN), lds, st>>>(c, out_scale, (int)mt, (int)nt);
   return hipGetLastError();
 }
-template <int WM, int WN, int MI, int NJ, int S>
+template <int WM, int WN, int MI, int NJ, int S, bool GROUPED>
 hipError_t tile(const ftm_w4a4& c, hipStream_t st) {
-  if (c.offsets != nullptr)
-    return c.act >= 0 ? tile<WM, WN, MI, NJ, S, true, true, false>(c, nullptr, st)
-                      : tile<WM, WN, MI, NJ, S, false, true, false>(c, nullptr, st);
-  return c.act >= 0 ? tile<WM, WN, MI, NJ, S, true, false, false>(c, nullptr, st)
-                    : tile<WM, WN, MI, NJ, S, false, false, false>(c, nullptr, st);
+  return c.act >= 0 ? tile<WM, WN, MI, NJ, S, true, GROUPED, false>(c, nullptr, st)
+                    : tile<WM, WN, MI, NJ, S, false, GROUPED, false>(c, nullptr, st);
 }
 
 // Whether a tile's 32-bit offsets (below 2^30) reach its tokens (256 rows from its
@@ -1594,52 +1535,84 @@ bool offsets_ok(const ftm_w4a4& c) {
 
 }  // namespace
 
-hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
-  if (c.K < kMinK || !offsets_ok(c)) return any(c, st);
-  if (c.offsets != nullptr) {
-    const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
-    if (seg >= 200) return tile<2, 2, 8, 8, 2>(c, st);
-    if (seg >= 96) return tile<2, 2, 4, 8, 3>(c, st);
-    if (seg >= 16) return tile<2, 2, 2, 8, 3>(c, st);
-    return seg <= 4 ? cols<8, 2>(c, st) : cols<16, 2>(c, st);
-  }
+// Rows an expert with rows has, if all have the same.
+static int64_t rows_an_expert(const ftm_w4a4& c) {
+  const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts;
+  return (c.rows + hit - 1) / hit;
+}
+constexpr int kTileRows = 8, kLargeRows = 96;  // an expert: from these on tiles of 64 x 256, of 256 x 256
+
+// By the rows an expert has.  In us, for 128 experts of [2 x 768, 2048], of [2048, 768], and 32
+// of [2 x 2880, 2880]:
+//                   1 row               4 rows              8 rows              64 rows      96 rows             128 rows
+//   cols of 8       38.5  24.0  60.9    50.1  32.8  80.7    60.5  43.6  102.7
+//   cols of 16      40.9  23.0  64.4    49.4  28.7  78.0    57.8  35.5   90.6
+//   tiles 64 x 256                                          53.6  30.3   83.8   71.8  48.9   90.2  57.2  139.8   100.2  67.0
+//   tiles 256 x 256                                                             92.3  57.8   92.8  58.6  128.4    94.3  60.6
+// Tiles of 128 x 256 (94.2, 53.6, 133.0 at 96 rows) gain less than 7% and only there.  Where
+// the codes of few rows do not fit the LDS (K above 13 thousand) it is tiles too.
+static hipError_t grouped(const ftm_w4a4& c, hipStream_t st) {
+  const int64_t seg = rows_an_expert(c);
+  if (seg >= kLargeRows) return tile<2, 2, 8, 8, 2, true>(c, st);
+  if (seg <= 2 && cols_fits<8, 2>(c)) return cols<8, 2>(c, st);
+  if (seg < kTileRows && cols_fits<16, 2>(c)) return cols<16, 2>(c, st);
+  return tile<2, 2, 2, 8, 3, true>(c, st);
+}
+
+// Blocks that the chip holds at once take one another's time; of the tiles, the least time of
+// all rounds is taken, a round of 256 workgroups being 4, 7 and 9 (13, 23.5 and 30 us at K = 4096).
+// In us, M x N x K:
+//   16 x 16 (K over four waves) against 32 x 16:  16 x 4096 x 4096 4.1, 4.9; 16 x 12288 x 4096 9.0, 11.9
+//   32 x 16 against 32 x 32:  32 x 4096 x 4096 5.1, 5.5; x 12288 11.3, 8.9; x 5760 x 2880 6.9, 5.8
+//   32 x 32 against 64 x 64 (eight waves):  512 blocks 9.4, 11.5; 528 9.6, 8.1; 540 12.7, 10.3; 768 13.9, 11.5
+//   32 x 32 against tiles, K = 11008 where 64 x 64 does not fit:  640 blocks 28.3, 32.0; 1024 39.8, 32.9
+//   64 x 64 against tiles of 128 x 128:  256 blocks 12.3, 15.5; 270 18.1, 13.4; 384 21.1, 15.7
+//   tiles of 128 x 128, 128 x 256 and 256 x 256:  1024 x 4096 x 4096 18.5, 25.0, 29.7; 2048 x 4096 x 4096
+//   31.2, 29.0, 31.5; 1024 x 12288 x 4096 42.3, 46.2, 33.0; 2048 x 12288 x 4096 78.4, 71.6, 64.1
+static hipError_t dense(const ftm_w4a4& c, hipStream_t st) {
   const int64_t M = c.rows;
   const auto blocks = [&](int rows, int cols) { return ((M + rows - 1) / rows) * ((c.N + cols - 1) / cols); };
-  if (M <= 16) return split<1, 1, 4, 4>(c, st);
-  if (M <= 32) return split<2, 1, 4, 3>(c, st);
-  if (blocks(32, 32) <= 640 || c.row_index != nullptr) return split<2, 2, 4, 2>(c, st);
-  if (blocks(64, 64) <= kCUs) return split<4, 4, 8, 1>(c, st);
-  if (blocks(256, 256) >= 192) return tile<2, 2, 8, 8, 2>(c, st);
-  if (blocks(128, 256) >= 192) return tile<2, 2, 4, 8, 3>(c, st);
-  return tile<2, 2, 4, 4, 4>(c, st);
+  if (M <= 16 && split_fits<1, 1, 4, 4>(c)) return split<1, 1, 4, 4>(c, st);
+  if (M <= 32 && blocks(32, 16) <= kCUs && split_fits<2, 1, 4, 3>(c)) return split<2, 1, 4, 3>(c, st);
+  const bool few64 = blocks(64, 64) <= kCUs && split_fits<4, 4, 8, 1>(c);
+  if ((blocks(32, 32) <= 2 * kCUs || (blocks(32, 32) <= 3 * kCUs && !few64)) && split_fits<2, 2, 4, 2>(c))
+    return split<2, 2, 4, 2>(c, st);
+  if (few64) return split<4, 4, 8, 1>(c, st);
+  const auto time = [&](int rows, int cols, int each) { return (blocks(rows, cols) + kCUs - 1) / kCUs * each; };
+  const int64_t t128 = time(128, 128, 4), t256 = time(128, 256, 7), t512 = time(256, 256, 9);
+  if (t128 <= t256 && t128 <= t512) return tile<2, 2, 4, 4, 4, false>(c, st);
+  return t256 <= t512 ? tile<2, 2, 4, 8, 3, false>(c, st) : tile<2, 2, 8, 8, 2, false>(c, st);
+}
+
+hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
+  if (c.K < kMinK || !offsets_ok(c)) return any(c, st);
+  return c.offsets != nullptr ? grouped(c, st) : dense(c, st);
 }
 
 namespace {
 
 template <int NT, int NW, int S>
-int few_lds(int K, int cap) {
+int few_lds(int K, int rows) {
   const int per = ((K + 255) / 256 + NW - 1) / NW;
-  const int lds = NW * (S * NT * 16 * kRow + per * cap * kRow + (16 * NT + cap) * scale_pitch(per));
-  constexpr int sums = NW * NT * 1024 + 16 * 36 * 4;
+  const int lds = NW * (S * NT * 16 * kRow + per * rows * kRow + (16 * NT + rows) * scale_pitch(per));
+  constexpr int sums = NW * NT * 1024;
   return lds > sums ? lds : sums;
 }
-template <int XDT, int NT, int NW, int S, bool MOE>
+template <int XDT, int NT, int NW, int S>
 hipError_t few(const FewCall& c, hipStream_t st) {
-  const int lds = few_lds<NT, NW, S>(c.K, c.cap);
-  const bool act = MOE || c.act >= 0;
-  const int cols = act ? 8 * NT : 16 * NT, ntiles = ((act ? c.N / 2 : c.N) + cols - 1) / cols;
+  const int cols = c.act >= 0 ? 8 * NT : 16 * NT, NO = c.act >= 0 ? c.N / 2 : c.N;
   static DeviceBits lds_set{0};
-  const auto kernel = k_w4a4_few<XDT, NT, NW, S, MOE>;
-  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  const auto kernel = k_w4a4_few<XDT, NT, NW, S>;
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds);
   if (e != hipSuccess) return e;
-  kernel<<<dim3((unsigned)((MOE ? c.P : 1) * ntiles)), dim3(64 * NW), lds, st>>>(c, ntiles);
+  kernel<<<dim3((unsigned)((NO + cols - 1) / cols)), dim3(64 * NW), few_lds<NT, NW, S>(c.K, c.cap), st>>>(c);
   return hipGetLastError();
 }
-template <int NT, int NW, int S, bool MOE>
+template <int NT, int NW, int S>
 hipError_t few(const FewCall& c, int dt, hipStream_t st) {
-  if (dt == FTM_DT_F32) return few<FTM_DT_F32, NT, NW, S, MOE>(c, st);
-  if (dt == FTM_DT_F16) return few<FTM_DT_F16, NT, NW, S, MOE>(c, st);
-  return few<FTM_DT_BF16, NT, NW, S, MOE>(c, st);
+  if (dt == FTM_DT_F32) return few<FTM_DT_F32, NT, NW, S>(c, st);
+  if (dt == FTM_DT_F16) return few<FTM_DT_F16, NT, NW, S>(c, st);
+  return few<FTM_DT_BF16, NT, NW, S>(c, st);
 }
 
 template <int XDT, int S>
@@ -1647,7 +1620,7 @@ hipError_t cols_moe(const FewCall& c, hipStream_t st) {
   const int ntiles = c.N / 64;
   static DeviceBits lds_set{0};
   const auto kernel = k_w4a4_cols<XDT, 16, S, FewCall>;
-  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - 1024);
+  const hipError_t e = allow_lds(lds_set, (const void*)kernel, kMaxLds - kListLds);
   if (e != hipSuccess) return e;
   kernel<<<dim3((unsigned)(c.P * ntiles)), dim3(256), cols_lds<S>(c.K, c.cap), st>>>(c, ntiles);
   return hipGetLastError();
@@ -1661,7 +1634,10 @@ hipError_t cols_moe(const FewCall& c, int dt, hipStream_t st) {
 
 }  // namespace
 
-// A layer of few tokens in two kernels, if it is one: hq and hs hold h, a row a pair.
+// A layer of few tokens in two kernels, if it is one: hq and hs hold h, a row a pair.  Against
+// the kernels of any layer (sort, quantise, product, quantise, product, sum), in us: 128 experts of 768
+// at 1 token 11.9, 28.3, at 16 tokens 49.4, 82.8; 32 of 2880 at 1 token 19.3, 39.4, at 16 tokens 108.7,
+// 123.9.  The limit is the 16 columns of a product: an expert's tokens are one workgroup's.
 bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStream_t st, hipError_t& e) {
   const int P = c.T * c.k, H = c.hidden, I = c.inter, cap = c.T < kFewRows ? c.T : kFewRows;
   if (c.T > kFewRows || P > kFewPairs || c.k > 64 || H < kMinK || I < kMinK) return false;
@@ -1670,11 +1646,8 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
   const FewCall f = {(const char*)c.x, c.x_stride, (const char*)c.w13, c.w13_scale, c.w13_bias, (int64_t)2 * I * (H / 2),
                      (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
                      c.topk_ids, c.ids_dtype == FTM_ID_I64, P, c.num_experts, c.k, hq, hs};
-  constexpr int kRoom = kMaxLds - 1024;  // beside the lists
-  if (cols_lds<2>(H, cap) <= kRoom) e = cols_moe<2>(f, c.dtype, st);
-  else if (few_lds<4, 8, 2>(H, cap) <= kRoom && H > 8 * 256) e = few<4, 8, 2, true>(f, c.dtype, st);
-  else if (few_lds<4, 8, 1>(H, cap) <= kRoom) e = few<4, 8, 1, true>(f, c.dtype, st);
-  else return false;
+  if (cols_lds<2>(H, cap) > kMaxLds - kListLds) return false;
+  e = cols_moe<2>(f, c.dtype, st);
   if (e != hipSuccess) return true;
   const int ntiles = (H + 15) / 16;
   k_w4a4_few_down<8, 3><<<dim3((unsigned)(ntiles * c.T)), dim3(512), 0, st>>>(c, hq, hs, ntiles);
@@ -1687,8 +1660,13 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
 // else (h: scratch, fp32 [rows, N / 2]) a kernel of its own; rows of no expert are then
 // those of zeros, on tiles left as they were.
 hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale, hipStream_t st) {
-  const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts, seg = (c.rows + hit - 1) / hit;
-  if (c.K >= kMinK && offsets_ok(c) && seg >= 16) {
+  const int64_t seg = rows_an_expert(c);
+  // In us, tiles of 64 x 256, 128 x 256 and 256 x 256, with the quantisation in the epilogue, for 128
+  // experts of [2 x 768, 2048] and 32 of [2 x 2880, 2880]: 64 rows an expert 72.9, 79.7, 110.8 and
+  // 119.3, 122.1, 124.8; 96 rows 91.5, 91.8, 113.5 and 139.8, 129.9, 149.3; 128 rows 102.3, 96.9, 114.6
+  // and 172.2, 144.8, 159.6; 200 rows 134.2, 134.8, 140.6 and 227.0, 176.9, 171.2; 256 rows 166.6, 145.5,
+  // 142.4 and 267.5, 207.1, 197.8.
+  if (c.K >= kMinK && offsets_ok(c) && seg >= kTileRows) {
     if (seg >= 200) return tile<2, 2, 8, 8, 2, true, true, true>(c, out_scale, st);
     if (seg >= 96) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
     return tile<2, 2, 2, 8, 3, true, true, true>(c, out_scale, st);
@@ -1701,12 +1679,16 @@ hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale
   return e != hipSuccess ? e : launch_quant_mxfp4(h, FTM_DT_F32, c.rows, I, (int64_t)I * 4, (uint8_t*)c.out, out_scale, st);
 }
 
+// Few values: each workgroup of the product quantises them all, and one launch does.  In us,
+// against the quantiser and the product (and the gap between them, which is not in these
+// figures): 2 x 1536 x 2048 4.9, 5.7; 8 x 1536 x 2048 7.1, 7.5; 4 x 4096 x 4096 7.5, 8.0;
+// 8 x 4096 x 4096 11.9, 7.8; 1 x 4096 x 11008 10.5, 10.6; 2 x 4096 x 11008 12.2, 10.9.
 hipError_t launch_w4a4_dynamic(const ftm_w4a4& c, const void* x, int dt, int64_t x_stride, hipStream_t st) {
-  if (c.offsets == nullptr && c.row_index == nullptr && c.rows <= 4 && c.rows * c.K <= 16384 && c.K >= kMinK && offsets_ok(c) &&
+  if (c.offsets == nullptr && c.rows <= 8 && c.rows * c.K <= 16384 && c.K >= kMinK && offsets_ok(c) &&
       (((uintptr_t)x | (uint64_t)x_stride) & 15u) == 0) {
     const FewCall f = {(const char*)x, x_stride, (const char*)c.w, c.w_scale, c.bias, 0, 0, c.N, c.K, c.bias_dtype, c.act, c.act_alpha,
                        c.act_limit, (int)c.rows, c.rows, c.out, c.out_dtype, nullptr, 0, 0, 1, 1, nullptr, nullptr};
-    return few<1, 4, 4, false>(f, dt, st);
+    return few<1, 4, 4>(f, dt, st);
   }
   const hipError_t e = launch_quant_mxfp4(x, dt, c.x_rows, c.K, x_stride, (uint8_t*)const_cast<void*>(c.x),
                                           const_cast<uint8_t*>(c.x_scale), st);

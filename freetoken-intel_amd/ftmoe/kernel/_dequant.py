@@ -16,7 +16,6 @@ def dequant(proj: Proj, *, out_dtype: torch.dtype, transpose: bool = False, slot
         nat.require_gpu(t, "weight")
     shape = (proj.K, proj.N) if transpose else (proj.N, proj.K)
     out = torch.empty(shape, dtype=out_dtype, device=proj.device)
-    rc = nat.lib().ftm_dequant(ctypes.byref(proj.c()), int(slot), out.data_ptr(), nat.dtype_code(out_dtype),
-                               1 if transpose else 0, torch.cuda.current_stream(proj.device).cuda_stream)
-    nat.check(rc, "ftm_dequant")
+    nat.launch("ftm_dequant", nat.lib().ftm_dequant, out, ctypes.byref(proj.c()), int(slot), out.data_ptr(),
+               nat.dtype_code(out_dtype), 1 if transpose else 0)
     return out

@@ -330,7 +330,7 @@ int ftm_quant_mxfp4(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int
                     uint8_t* blocks, uint8_t* scales, void* stream);
 
 /* One product: out[m, n] = sum over blocks b of 2^(x_scale[i, b] + w_scale[n, b] - 254)
- * sum_k x[i, k] w[n, k] (+ bias[n]), i = m or row_index[m], fp32 sums, one rounding to
+ * sum_k x[i, k] w[n, k] (+ bias[n]), i = m or (grouped) row_index[m], fp32 sums, one rounding to
  * out_dtype; a block with the scale 255 makes NaN.  With act >= 0 the weight rows [0, N/2) are gate and
  * [N/2, N) up and out[m, n] = act(gate) * up, n < N/2 (NaN where either is).
  * Grouped (offsets not NULL): rows [offsets[e], offsets[e+1]) take weight e;
@@ -343,7 +343,7 @@ typedef struct ftm_w4a4 {
   const void* bias;        /* [N] per expert, bias_dtype, or NULL */
   void* out;               /* [rows, N] (act: [rows, N/2]), out_dtype */
   const int32_t* offsets;  /* device [num_experts + 1], or NULL: one weight */
-  const int32_t* row_index;/* device [rows]: row of x of each output row, or NULL: the same row */
+  const int32_t* row_index;/* grouped: device [rows], row of x of each output row; or NULL: the same row */
   int64_t rows;            /* output rows */
   int64_t x_rows;
   int64_t w_stride;        /* bytes between the experts' weights, a multiple of 16 */

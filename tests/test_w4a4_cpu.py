@@ -38,9 +38,9 @@ BAD_DIM = (dict(K=0), dict(K=48), dict(K=nat.W4A4_MAX_K + 32), dict(N=0), dict(r
            dict(x_rows=-1), dict(x_rows=3), dict(num_experts=0), dict(num_experts=2), dict(offsets=P, num_experts=513),
            dict(offsets=P, num_experts=2, w_stride=32 * 32 - 16, w_scale_stride=64),
            dict(offsets=P, num_experts=2, w_stride=32 * 32, w_scale_stride=63), dict(act=nat.ACT_SILU, N=31),
-           dict(row_index=P, x_rows=0), dict(w_stride=-1), dict(w_scale_stride=-1))
+           dict(row_index=P), dict(offsets=P, row_index=P, x_rows=0), dict(w_stride=-1), dict(w_scale_stride=-1))
 BAD_FORMAT = (dict(out_dtype=9), dict(bias=P, bias_dtype=9), dict(act=4), dict(act=-2))
-BAD_ALIGN = (dict(x=P + 8), dict(w=P + 8), dict(out=P + 1), dict(bias=P + 1, bias_dtype=nat.DT_BF16), dict(row_index=P + 2),
+BAD_ALIGN = (dict(x=P + 8), dict(w=P + 8), dict(out=P + 1), dict(bias=P + 1, bias_dtype=nat.DT_BF16), dict(offsets=P, row_index=P + 2),
              dict(offsets=P + 2), dict(offsets=P, num_experts=2, w_stride=32 * 32 + 8, w_scale_stride=64))
 
 
