@@ -220,7 +220,8 @@ def test_quantiser_layouts(gpu, dtype):
 SHAPES = [(1, 1, 32), (1, 16, 64), (1, 1536, 2048), (2, 33, 96), (3, 100, 256), (4, 4096, 4096), (5, 24, 128),
           (15, 130, 1056), (16, 2048, 768), (17, 64, 512), (31, 4100, 512), (33, 4096, 2880), (64, 1024, 1024),
           (65, 200, 320), (100, 4096, 4096), (128, 256, 256), (200, 999, 736), (256, 8192, 640), (333, 5760, 2880),
-          (513, 1024, 4096), (1000, 4097, 160), (1025, 2304, 1408), (2048, 4096, 1024)]
+          (513, 1024, 4096), (1000, 4097, 160), (1025, 2304, 1408), (2048, 4096, 1024), (20, 5760, 352),
+          (90, 5800, 288), (150, 5760, 288), (1100, 11990, 288)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -236,7 +237,7 @@ def test_linear(gpu, M, N, K):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 64, 8192), (7, 48, 11008), (40, 64, 16384), (3, 32, 65536), (20, 40, 131072),
-                                   (300, 300, 32768)])
+                                   (300, 300, 32768), (256, 4096, 11008)])
 def test_linear_long_k(gpu, M, N, K):
     x, xs = operand((M, K), K, gpu)
     w, ws = operand((N, K), N, gpu)
@@ -277,7 +278,8 @@ def test_linear_edge_scales(gpu, M, K):
 
 @pytest.mark.parametrize("name", ["silu", "gelu", "relu", "swiglu_oai"])
 @pytest.mark.parametrize("M,N,K", [(1, 2, 32), (1, 128, 256), (3, 30, 96), (4, 1536, 2048), (16, 66, 512), (33, 200, 640),
-                                   (64, 512, 256), (129, 1030, 352), (300, 4096, 512), (700, 2880, 1024)])
+                                   (64, 512, 256), (129, 1030, 352), (300, 4096, 512), (700, 2880, 1024),
+                                   (2050, 4100, 288), (1100, 12010, 256)])
 def test_linear_gated(gpu, name, M, N, K):
     x, xs = operand((M, K), M, gpu, spread=2)
     w, ws = operand((N, K), N, gpu, spread=2)
@@ -330,7 +332,7 @@ def test_linear_layouts(gpu):
 # ------------------------------------------------------------------ quantiser and product
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 1536, 2048), (1, 7, 32), (2, 100, 96), (3, 4096, 4096), (4, 64, 8192), (6, 50, 1056),
-                                   (16, 48, 416), (17, 300, 11008), (70, 256, 512), (300, 520, 352)])
+                                   (8, 66, 2048), (9, 66, 1024), (16, 48, 416), (17, 300, 11008), (70, 256, 512), (300, 520, 352)])
 def test_fused_linear(gpu, dtype, M, N, K):
     """The bits of the quantiser and the product in two calls' definition."""
     g = torch.Generator(device=gpu).manual_seed(M + N)
@@ -395,7 +397,8 @@ def grouped_reference(x, offsets, w, index=None, bias=None):
 @pytest.mark.parametrize("sizes,N,K", [
     ([0, 1, 0], 33, 64), ([3, 0, 5, 1, 17], 48, 96), ([1] * 12, 1536, 2048), ([16, 15, 33, 0, 64], 130, 416),
     ([40, 7, 90, 128, 129], 520, 352), ([100] * 9, 2048, 768), ([300, 500, 1, 0, 223], 768, 1056),
-    ([70] * 40, 600, 512), ([190] * 12, 1024, 256), ([0, 0, 700], 5760, 2880)])
+    ([70] * 40, 600, 512), ([190] * 12, 1024, 256), ([0, 0, 700], 5760, 2880), ([1, 0, 9, 0, 0, 0], 77, 320),
+    ([3, 9, 0, 5, 17, 1], 70, 416), ([6] * 20, 640, 256), ([1, 2, 0, 3], 48, 32768), ([5, 8, 6], 34, 16384)])
 @pytest.mark.parametrize("through", [False, True])
 def test_grouped(gpu, sizes, N, K, through):
     E, P = len(sizes), sum(sizes)
@@ -530,7 +533,7 @@ def routing(T, k, E, seed, dev, dtype=torch.int32):
     (2, 3, 5, 160, 64, "relu", True), (3, 4, 32, 2880, 2880, "swiglu_oai", True), (7, 2, 16, 1024, 512, "silu", False),
     (8, 8, 64, 512, 320, "silu", True), (16, 8, 256, 256, 512, "silu", False), (17, 4, 8, 384, 160, "swiglu_oai", True),
     (16, 1, 1, 256, 128, "silu", False), (33, 6, 60, 512, 1408, "gelu", False), (150, 4, 6, 544, 288, "silu", True),
-    (400, 2, 4, 256, 512, "swiglu_oai", True)])
+    (400, 2, 4, 256, 512, "swiglu_oai", True), (16, 1, 2, 14336, 256, "silu", True), (16, 16, 40, 256, 256, "relu", True)])
 def test_moe(gpu, T, k, E, H, I, name, bias):
     w1, s1, w2, s2, b1, b2 = layer(E, H, I, T + H, gpu, bias)
     dtype = (torch.bfloat16, torch.float16, torch.float32)[T % 3]
@@ -611,6 +614,21 @@ def test_expert_forward(gpu, M):
         fused_w4a4_expert_forward(x, w1[0], s1[0], w2[0], s2[0], intermediate=95)
 
 
+@pytest.mark.parametrize("T", [3, 16, 40])
+def test_moe_layouts(gpu, T):
+    """Tokens with rows apart, from a border of 2 bytes, and tables that are not contiguous."""
+    w1, s1, w2, s2, b1, b2 = layer(8, 256, 256, 9, gpu, True)
+    wide = torch.randn(T, 3 * 256, device=gpu).to(torch.bfloat16)
+    ids, wt = routing(T, 3, 8, 2, gpu)
+    for x in (wide[:, 256:512], wide[:, 1:257], wide.t().contiguous().t()[:, :256]):
+        want = fused_w4a4_moe(x.contiguous(), w1, s1, w2, s2, ids, wt, w1_bias=b1, w2_bias=b2)
+        got = fused_w4a4_moe(x, w1, s1, w2, s2, ids.t().contiguous().t(), wt.t().contiguous().t(), w1_bias=b1, w2_bias=b2)
+        if x.data_ptr() % 16 == 0:
+            assert torch.equal(got, want)
+        ref, bound = layer_reference(values(*quantize_mxfp4(x)), values(w1, s1), values(w2, s2), ids, wt, "silu", b1, b2)
+        layer_close(got, ref, bound, torch.bfloat16)
+
+
 def test_moe_refusals(gpu):
     w1, s1, w2, s2, _, _ = layer(2, 64, 32, 1, gpu)
     x, ids, wt = torch.randn(3, 64, device=gpu), torch.zeros(3, 1, dtype=torch.int32, device=gpu), torch.ones(3, 1, device=gpu)
@@ -660,6 +678,67 @@ def test_captured_and_replayed(gpu, T):
             outs.append(run(*sets[n % 4]))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[n % 4]) for n, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("sizes", [[1, 0, 3], [9, 4, 6, 0], [40, 0, 70], [300, 5, 90]])
+def test_products_captured_and_replayed(gpu, sizes):
+    """Quantiser, dense and grouped products in one graph, replayed over other values and other
+    offsets, with eager calls between the replays."""
+    E, P, K, N = len(sizes), sum(sizes), 288, 130
+    w, ws = operand((E, N, K), 3, gpu)
+    sets = []
+    for n in range(3):
+        cuts = torch.tensor(sizes[n:] + sizes[:n]).cumsum(0)
+        sets.append((torch.randn(P, K, device=gpu), torch.cat([torch.zeros(1), cuts]).to(torch.int32).to(gpu)))
+
+    def run(x, offsets):
+        q, s = quantize_mxfp4(x)
+        return (w4a4_grouped_linear(q, s, offsets, w, ws), w4a4_linear(q, s, w[0], ws[0], activation="silu"),
+                fused_w4a4_linear(x, w[1], ws[1]))
+
+    want = [run(*a) for a in sets]
+    x, offsets = (t.clone() for t in sets[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(x, offsets)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, offsets)
+    for n in range(6):
+        for dst, src in zip((x, offsets), sets[n % 3]):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[n % 3]))
+        assert all(torch.equal(a, b) for a, b in zip(run(*sets[(n + 1) % 3]), want[(n + 1) % 3]))
+
+
+def test_far_offsets(gpu):
+    """Operands and results past 2^31 bytes, and rows that an index finds past 2^30."""
+    M, K, N = 2 ** 21 + 5, 1024, 640
+    part, parts = operand((997, K), 1, gpu)
+    x, xs = part.repeat(M // 997 + 1, 1, 1)[:M], parts.repeat(M // 997 + 1, 1)[:M]
+    w, ws = operand((3, N, K), 2, gpu)
+    rows = torch.tensor([0, 1, 2 ** 19 + 1, 2 ** 20, 2 ** 20 + 255, M - 300, M - 2, M - 1], device=gpu)
+    v = values(w, ws)
+    got = w4a4_linear(x, xs, w[0], ws[0], out_dtype=torch.float32)
+    y, mag = product(values(x[rows], xs[rows]), v[0])
+    close(got[rows], y, mag, torch.float32, roundings(K))
+    del got
+    offsets = torch.tensor([0, 2 ** 19 + 1, 2 ** 20, M], dtype=torch.int32, device=gpu)
+    got = w4a4_grouped_linear(x, xs, offsets, w, ws, out_dtype=torch.float32)
+    for r in rows.tolist():
+        e = 0 if r < 2 ** 19 + 1 else 1 if r < 2 ** 20 else 2
+        y, mag = product(values(x[r:r + 1], xs[r:r + 1]), v[e])
+        close(got[r:r + 1], y, mag, torch.float32, roundings(K))
+    del got
+    index = rows.to(torch.int32)
+    offsets = torch.tensor([0, 3, 4, 8], dtype=torch.int32, device=gpu)
+    y, mag, live = grouped_reference(values(x[rows], xs[rows]), offsets, v)
+    close(w4a4_grouped_linear(x, xs, offsets, w, ws, row_index=index, out_dtype=torch.float32), y, mag, torch.float32, roundings(K))
+    assert live.all()
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 50, 64), (3, 66, 288), (20, 70, 256), (70, 130, 352), (300, 300, 256)])
