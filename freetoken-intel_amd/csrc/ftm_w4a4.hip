@@ -730,9 +730,10 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
     cnt = pairs.cnt;
     R = c.cap;
   } else {
-    const int item = xcd_item(blockIdx.x, gridDim.x);
-    nt = item % ntiles;
-    rt = row_tile<RW>(c, item / ntiles);
+    // Neighbours on other XCDs: the tiles that have rows come first, and a run of items for each XCD would leave those
+    // of the last runs idle (16 tokens of 8 of 128 experts, gate_up, 38.4 us, so 26.7).  No weight is read twice.
+    nt = blockIdx.x % ntiles;
+    rt = row_tile<RW>(c, blockIdx.x / ntiles);
     e = rt.e;
     cnt = rt.cnt;
   }
@@ -1540,15 +1541,18 @@ static int64_t rows_an_expert(const ftm_w4a4& c) {
   const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts;
   return (c.rows + hit - 1) / hit;
 }
-constexpr int kTileRows = 8, kLargeRows = 96;  // an expert: from these on tiles of 64 x 256, of 256 x 256
+constexpr int kTileRows = 16, kLargeRows = 96;  // an expert: from these on tiles of 64 x 256, of 256 x 256
 
 // By the rows an expert has.  In us, for 128 experts of [2 x 768, 2048], of [2048, 768], and 32
 // of [2 x 2880, 2880]:
-//                   1 row               4 rows              8 rows              64 rows      96 rows             128 rows
-//   cols of 8       38.5  24.0  60.9    50.1  32.8  80.7    60.5  43.6  102.7
-//   cols of 16      40.9  23.0  64.4    49.4  28.7  78.0    57.8  35.5   90.6
-//   tiles 64 x 256                                          53.6  30.3   83.8   71.8  48.9   90.2  57.2  139.8   100.2  67.0
-//   tiles 256 x 256                                                             92.3  57.8   92.8  58.6  128.4    94.3  60.6
+//                     1 row              4 rows             8 rows             12 rows
+//   cols of 8         26.7  15.3  40.1   41.0  23.6  61.6   49.2  33.3  79.4   58.0  42.5  97.8
+//   cols of 16        26.4  14.8  42.7   41.9  21.4  61.8   48.3  27.6  71.4   51.0  31.9  79.2
+//   tiles 64 x 256                       51.3  28.3         53.5  29.7  83.7   54.2  30.6  84.0
+//                     16 rows            64 rows            96 rows            128 rows
+//   cols of 16        56.8  36.6
+//   tiles 64 x 256    57.4  33.6         71.8  48.9         90.2  57.2  139.8  100.2  67.0
+//   tiles 256 x 256                      92.3  57.8         92.8  58.6  128.4   94.3  60.6
 // Tiles of 128 x 256 (94.2, 53.6, 133.0 at 96 rows) gain less than 7% and only there.  Where
 // the codes of few rows do not fit the LDS (K above 13 thousand) it is tiles too.
 static hipError_t grouped(const ftm_w4a4& c, hipStream_t st) {
@@ -1666,7 +1670,8 @@ hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale
   // 119.3, 122.1, 124.8; 96 rows 91.5, 91.8, 113.5 and 139.8, 129.9, 149.3; 128 rows 102.3, 96.9, 114.6
   // and 172.2, 144.8, 159.6; 200 rows 134.2, 134.8, 140.6 and 227.0, 176.9, 171.2; 256 rows 166.6, 145.5,
   // 142.4 and 267.5, 207.1, 197.8.
-  if (c.K >= kMinK && offsets_ok(c) && seg >= kTileRows) {
+  // Below, the columns' kernel and the quantiser: at 8 rows 48.3 and 4.2 against 53.5 for the tiles.
+  if (c.K >= kMinK && offsets_ok(c) && seg >= 8) {
     if (seg >= 200) return tile<2, 2, 8, 8, 2, true, true, true>(c, out_scale, st);
     if (seg >= 96) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
     return tile<2, 2, 2, 8, 3, true, true, true>(c, out_scale, st);
