@@ -1639,13 +1639,17 @@ hipError_t cols_moe(const FewCall& c, int dt, hipStream_t st) {
 }  // namespace
 
 // A layer of few tokens in two kernels, if it is one: hq and hs hold h, a row a pair.  Against
-// the kernels of any layer (sort, quantise, product, quantise, product, sum), in us: 128 experts of 768
-// at 1 token 11.9, 28.3, at 16 tokens 49.4, 82.8; 32 of 2880 at 1 token 19.3, 39.4, at 16 tokens 108.7,
-// 123.9.  The limit is the 16 columns of a product: an expert's tokens are one workgroup's.
+// the kernels of any layer (sort, quantise, product, quantise, product, sum; without the gaps
+// between six launches), in us: 16 experts of 512 at 16 tokens 11.9, 25.8; 128 of 768 at 1 token 11.9, 27.6,
+// at 16 49.1, 62.0; 32 of 2880 at 1 token 18.9, 34.4, at 8 75.1, 78.9, at 16 108.5, 92.9.  The
+// limits are the 16 columns of a product, for an expert's tokens are one workgroup's, and what the
+// second product reads again, an expert's weights once for each of its tokens: at least 64 MB of it (32
+// of 2880 from 13 tokens on) and the kernels of any layer are faster.
 bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStream_t st, hipError_t& e) {
   const int P = c.T * c.k, H = c.hidden, I = c.inter, cap = c.T < kFewRows ? c.T : kFewRows;
   if (c.T > kFewRows || P > kFewPairs || c.k > 64 || H < kMinK || I < kMinK) return false;
   if ((((uintptr_t)c.x | (uint64_t)c.x_stride) & 15u) != 0) return false;
+  if ((int64_t)(P - (P < c.num_experts ? P : c.num_experts)) * H * (I / 2) > (64 << 20)) return false;
   if ((int64_t)2 * I * (H / 2) + 256 >= (int64_t)kNowhere) return false;
   const FewCall f = {(const char*)c.x, c.x_stride, (const char*)c.w13, c.w13_scale, c.w13_bias, (int64_t)2 * I * (H / 2),
                      (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
@@ -1670,8 +1674,9 @@ hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale
   // 119.3, 122.1, 124.8; 96 rows 91.5, 91.8, 113.5 and 139.8, 129.9, 149.3; 128 rows 102.3, 96.9, 114.6
   // and 172.2, 144.8, 159.6; 200 rows 134.2, 134.8, 140.6 and 227.0, 176.9, 171.2; 256 rows 166.6, 145.5,
   // 142.4 and 267.5, 207.1, 197.8.
-  // Below, the columns' kernel and the quantiser: at 8 rows 48.3 and 4.2 against 53.5 for the tiles.
-  if (c.K >= kMinK && offsets_ok(c) && seg >= 8) {
+  // Below 12, the columns' kernel and the quantiser: at 8 rows 48.3 + 4.2 against 55.1 on tiles, 71.4 + 4.2 against
+  // 82.6; at 12 rows 51.0 + 4.2 against 55.4, 79.2 + 4.2 against 83.6, and one launch more.
+  if (c.K >= kMinK && offsets_ok(c) && seg >= 12) {
     if (seg >= 200) return tile<2, 2, 8, 8, 2, true, true, true>(c, out_scale, st);
     if (seg >= 96) return tile<2, 2, 4, 8, 3, true, true, true>(c, out_scale, st);
     return tile<2, 2, 2, 8, 3, true, true, true>(c, out_scale, st);
