@@ -391,7 +391,9 @@ __device__ __forceinline__ void split_sums(char* lds, const f32x4 (&acc)[MT][NT]
 // run of K over the whole tile through an LDS ring of its own (S stages of 256 K), and the
 // waves' sums meet in LDS.  No barrier in the K loop; a stage's slot is filled again as
 // soon as its operands are in registers.  For few rows, where the weights' stream is
-// all the time, and for grids too small for the tiles that share a ring.
+// all the time, and for grids too small for the tiles that share a ring.  Bound by the
+// chain of a launch, a ring's first round trip and the sums: 16 x 4096 x 4096 4.1 us, 32 x 4096 x
+// 11008 7.9 us (3.0 TB/s of weights).
 template <int MT, int NT, int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, int ntiles) {
   constexpr int BM = 16 * MT, kStage = (MT + NT) * 16 * kRow;
@@ -577,6 +579,7 @@ struct FewCall {
 // Up to 16 tokens whose values are still wide, one weight: a workgroup quantises them
 // itself, each wave the K that it multiplies, while its weights are under way, and
 // multiplies them by a tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.
+// Bound by two round trips one behind the other: 1 x 1536 x 2048 5.3 us.
 template <int XDT, int NT, int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
   using V = Vec8<XDT>;
@@ -709,7 +712,11 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
 // there are blocks for every CU: against K split over the waves there are no sums to
 // exchange, the rows are held once, and a workgroup's ring holds most of its weights.
 // Call is a product (codes in hand) or a layer's first (FewCall: wide tokens, which the
-// workgroup quantises, its 32 channels of h quantised in the epilogue).
+// workgroup quantises, its 32 channels of h quantised in the epilogue).  Bound by the
+// weights' stream with the chain before it (offsets, index, rows): 16 tokens of 8 of 128 experts,
+// gate_up, 26.7 us, 138 MB of weights at 5.2 TB/s; a layer's 8 tokens of 4 of 32 of 2880 41 us, 184 MB at
+// 4.5 TB/s.  K split over two groups of four waves lost (38.4 to 48.7 us, on the
+// item order of that time), for the chain is then paid for half the weights.
 template <int XDT, int RW, int S, class Call>
 __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
   constexpr bool MOE = std::is_same_v<Call, FewCall>;
@@ -949,7 +956,11 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
 // workgroup.  The steps of 256 K of the token's experts, one expert behind the other, are
 // split over the waves; a step's results are weighted by its expert's weight and added
 // up in fp32, the waves' sums in order, so the order is the same in each call.  h comes
-// from memory (every lane of a group the same block), the weights through LDS.
+// from memory (every lane of a group the same block), the weights through LDS.  Bound by
+// the workgroups' chains, of which two rounds are resident: 128 experts at 1 token 3.4 us, 32 of 2880 at
+// 8 tokens 31 us (82 MB from memory, 141 MB into LDS).  One workgroup for all tokens of its
+// channels, so that weights are read once, lost: 34 us there, 128 experts at 16 tokens 19.0 to
+// 25.9.
 template <int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_few_down(ftm_w4a4_moe c, const uint8_t* hq, const uint8_t* hs, int ntiles) {
   __shared__ __attribute__((aligned(1024))) char ring[NW][S][16 * kRow];
@@ -1046,7 +1057,9 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few_down(ftm_w4a4_moe c, const
 // ahead.  Few large waves: a step reads (16 MI + 16 NJ) rows of LDS a wave for 16 MI x 16 NJ
 // results, and with one wave a SIMD every other instruction is written into the
 // shadow of an MFMA (16 cycles), in the order in which it is to be issued.  A workgroup
-// takes one tile after another, and the copies run on from tile to tile.
+// takes one tile after another, and the copies run on from tile to tile.  Bound by power and
+// MFMA issue where a tile is large (4096 x 12288 x 4096 105 to 109 us, 3.9 POP/s; MFMA busy 44 % of the
+// cycles), by the copies of a step where it is small.
 template <int WM, int WN, int MI, int NJ, int S, bool ACT, bool GROUPED, bool QOUT>
 __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8_t* out_scale, int mtiles, int ntiles) {
   constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
