@@ -533,7 +533,8 @@ def routing(T, k, E, seed, dev, dtype=torch.int32):
     (2, 3, 5, 160, 64, "relu", True), (3, 4, 32, 2880, 2880, "swiglu_oai", True), (7, 2, 16, 1024, 512, "silu", False),
     (8, 8, 64, 512, 320, "silu", True), (16, 8, 256, 256, 512, "silu", False), (17, 4, 8, 384, 160, "swiglu_oai", True),
     (16, 1, 1, 256, 128, "silu", False), (33, 6, 60, 512, 1408, "gelu", False), (150, 4, 6, 544, 288, "silu", True),
-    (400, 2, 4, 256, 512, "swiglu_oai", True), (16, 1, 2, 14336, 256, "silu", True), (16, 16, 40, 256, 256, "relu", True)])
+    (400, 2, 4, 256, 512, "swiglu_oai", True), (16, 1, 2, 14336, 256, "silu", True), (16, 2, 2, 2880, 1600, "silu", False),
+    (15, 4, 32, 2880, 2880, "swiglu_oai", True), (16, 16, 40, 256, 256, "relu", True)])
 def test_moe(gpu, T, k, E, H, I, name, bias):
     w1, s1, w2, s2, b1, b2 = layer(E, H, I, T + H, gpu, bias)
     dtype = (torch.bfloat16, torch.float16, torch.float32)[T % 3]
