@@ -373,21 +373,28 @@ def stream_of(t) -> int:
 
 
 _raw_stream = None  # device index -> its current stream, without a Stream object around it
+_current_device = None
+
+
+def _bind() -> None:
+    global _raw_stream, _current_device
+    import torch
+
+    _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def launch(what: str, fn, t, *args) -> None:
     """``fn(*args, stream)`` on the current stream of ``t``'s device, which is made
     current for the call; raises :class:`FtmError` for an error code."""
-    global _raw_stream
-    import torch
-
     if _raw_stream is None:
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                              lambda i: torch.cuda.current_stream(i).cuda_stream)
-    index = t.device.index
-    if index == torch.cuda.current_device():
+        _bind()
+    index = t.get_device()
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
+        import torch
+
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc < 0:
@@ -396,8 +403,9 @@ def launch(what: str, fn, t, *args) -> None:
 
 def require_same_device(t, others) -> None:
     """``others``: (name, tensor or None) pairs that have to be on ``t``'s device."""
+    index = t.get_device()
     for name, o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != index:
             require_gpu(o, name)
             raise ValueError(f"{name} is on {o.device}, expected {t.device}")
 

@@ -63,7 +63,7 @@ def fused_w4a4_moe(
         raise ValueError(f"w2_blocks must be {[E, H, I2 // 2 // _QBLOCK, 16]} for {I2} rows of w1, got {tuple(wb.shape)}")
     ba, ba_dt = bias_of(w1_bias, wa.shape[:2], "w1_bias")
     bb, bb_dt = bias_of(w2_bias, wb.shape[:2], "w2_bias")
-    out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+    out = torch.empty(T, H, dtype=x.dtype, device=x.device)
     if T == 0:
         return out
     x, ids, w = rows_of(x), topk_ids.contiguous(), topk_w.contiguous()

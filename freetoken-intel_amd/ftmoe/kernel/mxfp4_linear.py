@@ -28,7 +28,7 @@ def dequantize_mxfp4_blocks(blocks: torch.Tensor, scales: torch.Tensor, *,
     nat.require_gpu(scales, "weight")
     *lead, nb = scales.shape
     blocks, scales = blocks.contiguous(), scales.contiguous()
-    out = torch.empty((*lead, nb * 32), dtype=out_dtype, device=blocks.device)
+    out = torch.empty(*lead, nb * 32, dtype=out_dtype, device=blocks.device)
     p = nat.FtmProj(blocks.data_ptr(), scales.data_ptr(), None, None, 0, 0, 0, 0, FORMATS["mxfp4"], nat.DT_F32, nat.DT_BF16,
                     32, math.prod(lead), nb * 32, 1, 0)
     nat.launch("ftm_dequant", nat.lib().ftm_dequant, out, ctypes.byref(p), 0, out.data_ptr(), nat.dtype_code(out_dtype), 0)

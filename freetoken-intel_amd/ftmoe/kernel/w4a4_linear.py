@@ -41,8 +41,8 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"x must be [..., K] with K a multiple of {_QBLOCK}, got {tuple(x.shape)}")
     lead, K = x.shape[:-1], x.shape[-1]
     x2 = rows_of(x if x.dim() == 2 else x.reshape(-1, K))
-    blocks = torch.empty((*lead, K // _QBLOCK, 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, K // _QBLOCK), dtype=torch.uint8, device=x.device)
+    blocks = torch.empty(*lead, K // _QBLOCK, 16, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*lead, K // _QBLOCK, dtype=torch.uint8, device=x.device)
     if x2.shape[0]:
         nat.launch("ftm_quant_mxfp4", nat.lib().ftm_quant_mxfp4, x2, x2.data_ptr(), dt, x2.shape[0], K,
                    row_stride(x2) * x2.element_size(), blocks.data_ptr(), scales.data_ptr())
@@ -51,15 +51,17 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mxfp4_of(blocks: torch.Tensor, scales: torch.Tensor, lead: int, name: str) -> tuple[torch.Tensor, torch.Tensor]:
     """(blocks, scales) as the kernels take them; ``lead`` dimensions before K/32."""
-    for n, t in ((f"{name}_blocks", blocks), (f"{name}_scales", scales)):
-        if t.dtype != torch.uint8:
-            raise TypeError(f"{n} must be uint8, got {t.dtype}")
-    if blocks.dim() != lead + 2 or blocks.shape[-1] != 16 or blocks.shape[-2] == 0:
-        raise ValueError(f"{name}_blocks must be {['...'] * lead + ['K/32', 16]}, got {tuple(blocks.shape)}")
-    if scales.shape != blocks.shape[:-1]:
-        raise ValueError(f"{name}_scales must be {list(blocks.shape[:-1])}, got {tuple(scales.shape)}")
-    if _QBLOCK * blocks.shape[-2] > nat.W4A4_MAX_K:
-        raise ValueError(f"K={_QBLOCK * blocks.shape[-2]} exceeds {nat.W4A4_MAX_K}")
+    if blocks.dtype != torch.uint8:
+        raise TypeError(f"{name}_blocks must be uint8, got {blocks.dtype}")
+    if scales.dtype != torch.uint8:
+        raise TypeError(f"{name}_scales must be uint8, got {scales.dtype}")
+    shape = blocks.shape
+    if len(shape) != lead + 2 or shape[-1] != 16 or shape[-2] == 0:
+        raise ValueError(f"{name}_blocks must be {['...'] * lead + ['K/32', 16]}, got {tuple(shape)}")
+    if scales.shape != shape[:-1]:
+        raise ValueError(f"{name}_scales must be {list(shape[:-1])}, got {tuple(scales.shape)}")
+    if _QBLOCK * shape[-2] > nat.W4A4_MAX_K:
+        raise ValueError(f"K={_QBLOCK * shape[-2]} exceeds {nat.W4A4_MAX_K}")
     return _aligned(blocks), scales.contiguous()
 
 
@@ -92,8 +94,8 @@ def _product(x, x_scales, weight_blocks, weight_scales, *, bias, out_dtype, offs
         if N % 2:
             raise ValueError(f"a gated activation needs an even number of weight rows (gate, then up), got {N}")
     rows = M if row_index is None else row_index.shape[0]
-    out = torch.empty((rows, N // 2 if act >= 0 else N), dtype=out_dtype, device=x.device)
-    if out.numel() == 0:
+    out = torch.empty(rows, N // 2 if act >= 0 else N, dtype=out_dtype, device=x.device)
+    if rows == 0 or N == 0:
         return out
     if M == 0:  # an index into no rows
         return out.zero_()
