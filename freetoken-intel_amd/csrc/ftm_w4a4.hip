@@ -714,7 +714,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
 // Call is a product (codes in hand) or a layer's first (FewCall: wide tokens, which the
 // workgroup quantises, its 32 channels of h quantised in the epilogue).  Bound by the
 // weights' stream with the chain before it (offsets, index, rows): 16 tokens of 8 of 128 experts,
-// gate_up, 26.7 us, 138 MB of weights at 5.2 TB/s; a layer's 8 tokens of 4 of 32 of 2880 41 us, 184 MB at
+// gate_up, 26.7 us, 110 MB of weights at 4.1 TB/s; a layer's 8 tokens of 4 of 32 of 2880 41 us, 184 MB at
 // 4.5 TB/s.  K split over two groups of four waves lost (38.4 to 48.7 us, on the
 // item order of that time), for the chain is then paid for half the weights.
 template <int XDT, int RW, int S, class Call>
