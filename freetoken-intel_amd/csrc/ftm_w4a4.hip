@@ -292,7 +292,7 @@ constexpr int kMinK = 256;  // of the kernels that take the scales eight at a ti
 // has a row of each 64 (of 32 or 16 rows two or four lanes one, in turn); `p` says where they begin.  The
 // first kFlight loads of each are under way when the copies of the operands are
 // requested (`then`), before any of them is waited for.
-__host__ __device__ inline int scale_pitch(int per) { return 8 * (per | 1); }
+__host__ __device__ constexpr int scale_pitch(int per) { return 8 * (per | 1); }
 template <int R>
 struct FillScales {
   static constexpr int kRows = (R + 63) / 64, kTurns = R <= 16 ? 4 : R <= 32 ? 2 : 1, kFlight = kTurns > 1 ? 2 : 4;
@@ -398,7 +398,7 @@ template <int MT, int NT, int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_split(ftm_w4a4 c, int mtiles, int ntiles) {
   constexpr int BM = 16 * MT, kStage = (MT + NT) * 16 * kRow;
   constexpr int kParts = (MT * NT + NW - 1) / NW;
-  extern __shared__ char lds[];  // [NW][S][kStage], then the sums
+  extern __shared__ __attribute__((aligned(kRow))) char lds[];  // [NW][S][kStage], then the sums
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const RowTile rt = row_tile<BM>(c, item / ntiles);
   if (rt.cnt <= 0) return;
@@ -576,6 +576,14 @@ struct FewCall {
   uint8_t *hq, *hs;
 };
 
+// LDS of one wave of k_w4a4_few: its ring, the codes of `rows` tokens over its `per` steps, the
+// scales of its weights and of the tokens.  Whole stage rows: the scales of an odd number of rows end in the
+// middle of 16 bytes, and the next wave's ring takes 16-byte copies and reads.
+template <int NT, int S>
+__host__ __device__ constexpr int few_wave_lds(int per, int rows) {
+  return (S * NT * 16 * kRow + per * rows * kRow + (16 * NT + rows) * scale_pitch(per) + kRow - 1) / kRow * kRow;
+}
+
 // Up to 16 tokens whose values are still wide, one weight: a workgroup quantises them
 // itself, each wave the K that it multiplies, while its weights are under way, and
 // multiplies them by a tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.
@@ -584,7 +592,7 @@ template <int XDT, int NT, int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
   using V = Vec8<XDT>;
   constexpr int kStage = NT * 16 * kRow, kParts = (NT + NW - 1) / NW, kBatch = 4;
-  extern __shared__ char lds[];  // [NW] of: ring [S][kStage], codes [per][cnt][kRow], scales of weights and tokens; then the sums
+  extern __shared__ __attribute__((aligned(kRow))) char lds[];  // [NW] of: ring [S][kStage], codes [per][cnt][kRow], scales of weights and tokens; then the sums
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool act = c.act >= 0;
@@ -603,7 +611,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
   const int lo = wave * per, hi = lo + per < nsteps ? lo + per : nsteps;
   if (lo < hi) {
     const SplitWeights<NT> weights(c.w, NO, K, act, n0, ncol);
-    char* ring = lds + wave * (S * kStage + per * cnt * kRow + (16 * NT + cnt) * pitch);
+    char* ring = lds + wave * few_wave_lds<NT, S>(per, cnt);
     char* codes = ring + S * kStage;
     char* scales = codes + per * cnt * kRow;  // of the weights, then of the tokens
     char* xscales = scales + 16 * NT * pitch;
@@ -722,7 +730,7 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
   constexpr bool MOE = std::is_same_v<Call, FewCall>;
   constexpr int MT = (RW + 15) / 16, NC = RW / 8, kStage = 16 * kRow, kTurns = 64 / RW;
   static_assert(RW == 8 || RW % 16 == 0, "copies of 8 rows");
-  extern __shared__ char lds[];  // [4][S][kStage], codes [nsteps][rows][kRow], scales of the rows, and of each wave's weights
+  extern __shared__ __attribute__((aligned(kRow))) char lds[];  // [4][S][kStage], codes [nsteps][rows][kRow], scales of the rows, and of each wave's weights
   __shared__ int lists[MOE ? 4 : 1][kFewRows];
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1076,7 +1084,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies of 8 rows, as many for each wave");
   constexpr int kSecond = MI < kLast ? MI : kLast;       // row blocks that read the second half's weights
   static_assert(2 * MI % (kAhead + 1) == 0 && NJ % 4 == 0 && NJ % kSecond == 0, "the order of the reads");
-  extern __shared__ char lds[];  // [S][kStage], [2][kSlot], the rows of x [BM]
+  extern __shared__ __attribute__((aligned(kRow))) char lds[];  // [S][kStage], [2][kSlot], the rows of x [BM]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -1608,10 +1616,18 @@ hipError_t launch_w4a4(const ftm_w4a4& c, hipStream_t st) {
 
 namespace {
 
+constexpr bool few_rings_aligned() {
+  for (int rows = 1; rows <= kFewRows; ++rows)
+    for (int per = 1; per <= 16; ++per)
+      if (few_wave_lds<1, 4>(per, rows) % kRow != 0) return false;
+  return true;
+}
+static_assert(few_rings_aligned(), "each wave's ring begins on a stage row's border");
+
 template <int NT, int NW, int S>
 int few_lds(int K, int rows) {
   const int per = ((K + 255) / 256 + NW - 1) / NW;
-  const int lds = NW * (S * NT * 16 * kRow + per * rows * kRow + (16 * NT + rows) * scale_pitch(per));
+  const int lds = NW * few_wave_lds<NT, S>(per, rows);
   constexpr int sums = NW * NT * 1024;
   return lds > sums ? lds : sums;
 }

@@ -347,6 +347,23 @@ def test_fused_linear(gpu, dtype, M, N, K):
     assert torch.equal(fused_w4a4_linear(wide, w, ws, bias=bias), fused_w4a4_linear(x, w, ws, bias=bias))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 80, 288), (1, 80, 2048), (1, 33, 16384), (3, 130, 800), (3, 48, 5440), (5, 80, 1056),
+                                   (5, 40, 3232), (7, 48, 1024), (7, 100, 2336)])
+def test_fused_linear_odd_tokens(gpu, dtype, M, N, K):
+    """The one-launch product of an odd number of tokens, whose scales end in the middle of 16
+    bytes of LDS, with K over two to four waves of one to sixteen steps."""
+    assert M <= 8 and M * K <= 16384 and K >= 256
+    g = torch.Generator(device=gpu).manual_seed(K + M)
+    x = torch.randn(M, K, generator=g, device=gpu).to(dtype)
+    w, ws = operand((N, K), N + K, gpu)
+    y, mag = product(values(*quantize_mxfp4(x)), values(w, ws))
+    got = fused_w4a4_linear(x, w, ws, out_dtype=torch.float32)
+    close(got, y, mag, torch.float32, roundings(K))
+    for m in range(M):  # a token's result does not depend on how many there are
+        assert torch.equal(fused_w4a4_linear(x[m:m + 1], w, ws, out_dtype=torch.float32), got[m:m + 1])
+
+
 @pytest.mark.parametrize("M", [1, 3, 12, 100])
 def test_fused_linear_not_finite(gpu, M):
     x = torch.randn(M, 256, device=gpu)
