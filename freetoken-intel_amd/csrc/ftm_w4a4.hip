@@ -1026,11 +1026,12 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few_down(ftm_w4a4_moe c, const
         left &= left - 1;
       }
     }
+    wait_vm<0>();  // the steps' copies have landed
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < S; ++u) {
       if (u0 + u >= hi) break;
-      asm volatile("" : "+v"(sw[u]) : : "memory");  // requested behind the step's copies: with it they have landed
-      __builtin_amdgcn_sched_barrier(0);
       const uint32_t a = scale_operand(fit_scales(sw[u], at[u], nb), g), b = scale_operand(fit_scales(sh[u], at[u], nb), g);
       f32x4 d = mfma_fp4<0, 0>(stage_piece(ring[wave][u], m, 0, g), h[u][0], (f32x4){0, 0, 0, 0}, a, b);
       d = mfma_fp4<1, 1>(stage_piece(ring[wave][u], m, 1, g), h[u][1], d, a, b);
