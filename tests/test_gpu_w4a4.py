@@ -647,6 +647,147 @@ def test_moe_layouts(gpu, T):
         layer_close(got, ref, bound, torch.bfloat16)
 
 
+# A layer of few tokens in two kernels: hidden and inter from 256 on, up to 16 tokens
+def two_kernels(x, w1, s1, w2, s2, ids, wt, name="silu", b1=None, b2=None):
+    """fused_w4a4_moe, and that its call is of two kernels: they leave the sort's tables, with which the workspace
+    begins, as they were."""
+    (T, H), k, (E, I2) = x.shape, ids.shape[1], w1.shape[:2]
+    got = fused_w4a4_moe(x, w1, s1, w2, s2, ids, wt, activation=name, w1_bias=b1, w2_bias=b2)
+    L, out = nat.lib(), torch.empty_like(x)
+    need = L.ftm_w4a4_moe_workspace_bytes(T, k, E, H, I2 // 2)
+    ws = torch.full((need,), 0xA5, dtype=torch.uint8, device=x.device)
+    dt = lambda b: 0 if b is None else nat.dtype_code(b.dtype)  # noqa: E731
+    c = nat.FtmW4A4Moe(x.data_ptr(), ids.data_ptr(), wt.data_ptr(), out.data_ptr(), w1.data_ptr(), s1.data_ptr(), nat.ptr(b1),
+                       w2.data_ptr(), s2.data_ptr(), nat.ptr(b2), H * x.element_size(), T, k, E, H, I2 // 2,
+                       nat.dtype_code(x.dtype), nat.ID_I64 if ids.dtype == torch.int64 else nat.ID_I32, nat.dtype_code(wt.dtype),
+                       dt(b1), dt(b2), {"silu": nat.ACT_SILU, "swiglu_oai": nat.ACT_SWIGLU_OAI}[name], 1.702, 7.0)
+    nat.launch("ftm_w4a4_moe_forward", L.ftm_w4a4_moe_forward, x, ctypes.byref(c), ws.data_ptr(), need)
+    assert (ws[:4 * (E + 1)] == 0xA5).all(), "not the two kernels"
+    assert torch.equal(out.view(torch.uint8), got.view(torch.uint8))
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 5, 16])
+def test_two_kernels_odd_routing(gpu, T, dtype):
+    """No expert at all, one expert for all pairs (48 of 16 tokens), the same expert twice, ids far outside."""
+    w1, s1, w2, s2, b1, b2 = layer(4, 288, 320, 8, gpu, True)
+    g = torch.Generator().manual_seed(T)
+    x, wt = torch.randn(T, 288, generator=g).to(dtype).to(gpu), torch.rand(T, 3, generator=g).to(gpu)
+    v = values(*quantize_mxfp4(x)), values(w1, s1), values(w2, s2)
+    for ids in (torch.full((T, 3), -1), torch.full((T, 3), 2), torch.tensor([[1, 3, 1]]).repeat(T, 1),
+                torch.tensor([[9, 0, -7]]).repeat(T, 1), torch.tensor([[2 ** 32 + 1, 3, -2 ** 32]]).repeat(T, 1)):
+        ids = ids.to(gpu) if ids.abs().max() > 2 ** 31 else ids.to(torch.int32).to(gpu)
+        got = two_kernels(x, w1, s1, w2, s2, ids, wt, "silu", b1, b2)
+        ref, bound = layer_reference(*v, ids, wt, "silu", b1, b2)
+        layer_close(got, ref, bound, dtype)
+        if not ((ids >= 0) & (ids < 4)).any():
+            assert (got == 0).all()
+        assert (two_kernels(x, w1, s1, w2, s2, ids, torch.zeros_like(wt), "silu", b1, b2) == 0).all()
+
+
+@pytest.mark.parametrize("T,k,E,name", [(16, 16, 1, "silu"), (16, 16, 3, "swiglu_oai"), (4, 64, 5, "silu"), (1, 64, 2, "silu"),
+                                        (16, 12, 2, "silu"), (9, 28, 40, "swiglu_oai")])
+def test_two_kernels_many_pairs(gpu, T, k, E, name):
+    """Up to 256 pairs, an expert's more than a workgroup takes: the pairs that begin a chunk lie in
+    any lane of the ids."""
+    w1, s1, w2, s2, b1, b2 = layer(E, 256, 288, T + k, gpu, True)
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(T, 256, generator=g).to(torch.bfloat16).to(gpu)
+    ids = torch.randint(-1, E + 1, (T, k), generator=g).to(gpu) if E > 1 else torch.zeros(T, k, dtype=torch.int64, device=gpu)
+    wt = torch.softmax(torch.randn(T, k, generator=g), dim=1).to(gpu)
+    got = two_kernels(x, w1, s1, w2, s2, ids, wt, name, b1, b2)
+    ref, bound = layer_reference(values(*quantize_mxfp4(x)), values(w1, s1), values(w2, s2), ids, wt, name, b1, b2)
+    layer_close(got, ref, bound, torch.bfloat16)
+    assert torch.equal(got, two_kernels(x, w1, s1, w2, s2, ids, wt, name, b1, b2))
+
+
+@pytest.mark.parametrize("T", [2, 16])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_two_kernels_not_finite(gpu, T, bad):
+    """A token that is not finite has NaN results, no other token's change, of the same expert neither; a NaN
+    weight of a pair without an expert is not read; a NaN scale of a weight is that of its expert's tokens."""
+    w1, s1, w2, s2, _, _ = layer(4, 288, 256, 8, gpu)
+    x = torch.randn(T, 288, generator=torch.Generator().manual_seed(T)).to(gpu)
+    ids, wt = routing(T, 2, 4, 5, gpu)
+    ids[:, 0] = 2
+    want = two_kernels(x, w1, s1, w2, s2, ids, wt)
+    assert not want.isnan().any()
+    odd = x.clone()
+    odd[1, 7] = bad
+    got = two_kernels(odd, w1, s1, w2, s2, ids, wt)
+    assert got[1].isnan().all() and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+    ids[0, 1] = -1
+    one = two_kernels(x, w1, s1, w2, s2, ids, wt)
+    wt[0, 1] = math.nan
+    assert torch.equal(two_kernels(x, w1, s1, w2, s2, ids, wt), one)
+    ids[:, 0], ids[:, 1], ids[1, 1] = 0, 1, 3
+    wt[0, 1] = 0.5
+    want = two_kernels(x, w1, s1, w2, s2, ids, wt)
+    s2 = s2.clone()
+    s2[3, 40, 1] = 255
+    got = two_kernels(x, w1, s1, w2, s2, ids, wt)
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[1, 40] = True
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], want[~nan])
+
+
+@pytest.mark.parametrize("T", [1, 6, 16])
+def test_two_kernels_is_its_parts(gpu, T):
+    """Against the operators called one by one, with experts that come twice in a token."""
+    w1, s1, w2, s2, b1, b2 = layer(8, 288, 352, 2, gpu, True)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, 288, generator=g).to(torch.bfloat16).to(gpu)
+    ids, wt = torch.randint(0, 8, (T, 6), generator=g).to(torch.int32).to(gpu), torch.rand(T, 6, generator=g).to(gpu)
+    sort = sort_tokens(ids, 8)
+    q, s = quantize_mxfp4(x)
+    h = w4a4_grouped_linear(q, s, sort.offsets, w1, s1, row_index=sort.token_of_row, bias=b1, activation="silu",
+                            out_dtype=torch.float32)
+    hq, hs = quantize_mxfp4(h)
+    y = w4a4_grouped_linear(hq, hs, sort.offsets, w2, s2, bias=b2, out_dtype=torch.float32)
+    parts = combine_tokens(y, wt, sort, out_dtype=torch.bfloat16)
+    got = two_kernels(x, w1, s1, w2, s2, ids, wt, "silu", b1, b2)
+    ref, bound = layer_reference(values(q, s), values(w1, s1), values(w2, s2), ids, wt, "silu", b1, b2)
+    layer_close(parts, ref, bound, torch.bfloat16)
+    layer_close(got, ref, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [1, 8, 16])
+def test_two_kernels_captured_and_replayed(gpu, T):
+    """In a graph, replayed over other tokens and ids (experts that come often, and no expert) between eager calls;
+    then on two streams at once."""
+    w1, s1, w2, s2, b1, b2 = layer(8, 256, 288, 6, gpu, True)
+    run = lambda x, i, w: fused_w4a4_moe(x, w1, s1, w2, s2, i, w, w1_bias=b1, w2_bias=b2)  # noqa: E731
+    sets, want = [], []
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        ids = torch.randint(-1, (8, 2, 9, 1)[seed], (T, 3), generator=g).to(torch.int32).to(gpu)
+        sets.append((torch.randn(T, 256, generator=g).to(torch.bfloat16).to(gpu), ids, torch.rand(T, 3, generator=g).to(gpu)))
+        want.append(two_kernels(sets[-1][0], w1, s1, w2, s2, *sets[-1][1:], "silu", b1, b2))
+    x, ids, wt = (t.clone() for t in sets[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(x, ids, wt)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, ids, wt)
+    for n in range(8):
+        for dst, src in zip((x, ids, wt), sets[n % 4]):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[n % 4])
+        assert torch.equal(run(*sets[(n + 1) % 4]), want[(n + 1) % 4])
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for n in range(16):
+        with torch.cuda.stream(streams[n % 2]):
+            outs.append(run(*sets[n % 4]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[n % 4]) for n, o in enumerate(outs))
+
+
 def test_moe_refusals(gpu):
     w1, s1, w2, s2, _, _ = layer(2, 64, 32, 1, gpu)
     x, ids, wt = torch.randn(3, 64, device=gpu), torch.zeros(3, 1, dtype=torch.int32, device=gpu), torch.ones(3, 1, device=gpu)
