@@ -276,6 +276,26 @@ def test_linear_edge_scales(gpu, M, K):
     close(got[keep], y[keep], mag[keep], torch.float32, roundings(K))
 
 
+@pytest.mark.parametrize("M", [1, 4, 20, 70, 400])
+@pytest.mark.parametrize("K", [64, 416, 1024])
+def test_linear_largest_scales(gpu, M, K):
+    """The value of a product with the scales 253 and 254, the largest that are numbers, in the weight, in
+    x, and where the other operand's block brings the product back into fp32's range."""
+    x, xs = operand((M, K), 1, gpu)
+    w, ws = operand((50, K), 2, gpu)
+    xs[:, 0] = 40          # 2^-87: the first block's products are small ...
+    ws[11, 0], ws[12, 0] = 254, 253  # ... but for these, of 2^40 and 2^39
+    xs[M // 2, 1] = 254
+    ws[:, 1] = 30
+    vx, vw = values(x, xs), values(w, ws)
+    y, mag = product(vx, vw)
+    assert mag.max() < 2.0 ** 100 and (mag[:, 11] > 2.0 ** 30).all() and (mag[M // 2] > 2.0 ** 20).all()
+    close(w4a4_linear(x, xs, w, ws, out_dtype=torch.float32), y, mag, torch.float32, roundings(K))
+    offsets = torch.tensor([0, M], dtype=torch.int32, device=gpu)
+    got = w4a4_grouped_linear(x, xs, offsets, w[None], ws[None], out_dtype=torch.float32)
+    close(got, y, mag, torch.float32, roundings(K))
+
+
 @pytest.mark.parametrize("name", ["silu", "gelu", "relu", "swiglu_oai"])
 @pytest.mark.parametrize("M,N,K", [(1, 2, 32), (1, 128, 256), (3, 30, 96), (4, 1536, 2048), (16, 66, 512), (33, 200, 640),
                                    (64, 512, 256), (129, 1030, 352), (300, 4096, 512), (700, 2880, 1024),
