@@ -1085,6 +1085,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "copies of 8 rows, as many for each wave");
   constexpr int kSecond = MI < kLast ? MI : kLast;       // row blocks that read the second half's weights
   static_assert(2 * MI % (kAhead + 1) == 0 && NJ % 4 == 0 && NJ % kSecond == 0, "the order of the reads");
+  static_assert(MI <= 8, "a bit for each of a lane's rows");
+  constexpr uint32_t kAllRows = ~0u >> (32 - 4 * MI);
   extern __shared__ __attribute__((aligned(kRow))) char lds[];  // [S][kStage], [2][kSlot], the rows of x [BM]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1340,7 +1342,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
       const int el = opaque_lane(), em = el & 15, eg = el >> 4;
       const int n0 = cur.n + wn * (kCols / WN) + CN * em;
       const int t0 = 16 * wm * MI + 4 * eg;
-      uint32_t live = ~0u;  // bit 4 i + r: the row is one of x
+      uint32_t live = kAllRows;  // bit 4 i + r: the row is one of x
       if (indexed) {
         int er[MI][4];
 #pragma unroll
@@ -1444,7 +1446,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_w4a4_tile(ftm_w4a4 c, uint8
         }
       });
       if constexpr (GROUPED && !QOUT) {  // rows whose index names none: zeros over them
-        if (live != ~0u) {
+        if (live != kAllRows) {
           wait_vm<0>();  // behind the results
           for (int o = 0; o < CN; ++o)
             for (int t = 0; t < 4 * MI; ++t) {
