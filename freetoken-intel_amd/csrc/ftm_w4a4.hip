@@ -108,46 +108,33 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   return b > v ? b : v;
 }
 
-// Four lanes a block, NV blocks' parts a lane, 256 lanes apart.  x is read once and in
-// whole lines; bound by HBM.  FLAT: rows side by side in memory, taken as one.
-template <int DT, int NV, bool FLAT, bool ALIGNED>
+// Four lanes a block, eight values a lane.  x is read once and in whole lines, from any border of its
+// elements; bound by HBM.  FLAT: rows side by side in memory, taken as one.
+template <int DT, bool FLAT>
 __global__ __launch_bounds__(256) void k_quant_mxfp4(const char* x, int64_t x_stride, int64_t rows, int K, int per_row,
                                                      uint32_t* blocks, uint8_t* scales) {
   const int64_t wg = grid_row(), vecs = FLAT ? rows * (K / 8) : K / 8;
   const int64_t row = FLAT ? 0 : wg / per_row;
   if (row >= rows) return;
-  const int64_t first = (FLAT ? wg : wg - row * per_row) * (256 * NV) + threadIdx.x;
-  const char* src = x + row * x_stride;
-  const int64_t at = row * (K / 8);
-  Vec8<DT> v[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t k = first + 256 * i;
-    if (k >= vecs) v[i].zero();
-    else if constexpr (ALIGNED) v[i].load(src + k * Vec8<DT>::kBytes);
-    else v[i].load_any(src + k * Vec8<DT>::kBytes);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t k = first + 256 * i;
-    const uint32_t byte = mx_scale_byte(quad_max(v[i].max_bits()));
-    const uint32_t w = mx_codes<DT>(v[i], byte);
-    if (k >= vecs) continue;
-    blocks[at + k] = w;
-    if ((threadIdx.x & 3) == 0) scales[(at + k) >> 2] = (uint8_t)byte;
-  }
+  const int64_t k = (FLAT ? wg : wg - row * per_row) * 256 + threadIdx.x;
+  Vec8<DT> v;
+  if (k < vecs) v.load_any(x + row * x_stride + k * Vec8<DT>::kBytes);
+  else v.zero();
+  const uint32_t byte = mx_scale_byte(quad_max(v.max_bits()));
+  const uint32_t w = mx_codes<DT>(v, byte);
+  if (k >= vecs) return;
+  const int64_t at = row * (K / 8) + k;
+  blocks[at] = w;
+  if ((threadIdx.x & 3) == 0) scales[at >> 2] = (uint8_t)byte;
 }
 
-template <int DT, int NV>
+template <int DT>
 hipError_t quant(const char* x, int64_t x_stride, int64_t rows, int K, uint32_t* blocks, uint8_t* scales, hipStream_t st) {
-  const int64_t row_bytes = (int64_t)K / 8 * Vec8<DT>::kBytes;
-  const bool flat = x_stride == row_bytes || rows == 1, aligned = (((uintptr_t)x | (uint64_t)(rows > 1 ? x_stride : 0)) & 15u) == 0;
-  const int per_row = (K / 8 + 256 * NV - 1) / (256 * NV);
-  const dim3 grid = row_grid(flat ? (rows * (K / 8) + 256 * NV - 1) / (256 * NV) : rows * per_row), wg(256);
-  if (flat && aligned) k_quant_mxfp4<DT, NV, true, true><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
-  else if (flat) k_quant_mxfp4<DT, NV, true, false><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
-  else if (aligned) k_quant_mxfp4<DT, NV, false, true><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
-  else k_quant_mxfp4<DT, NV, false, false><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
+  const bool flat = x_stride == (int64_t)K / 8 * Vec8<DT>::kBytes || rows == 1;
+  const int per_row = (K / 8 + 255) / 256;
+  const dim3 grid = row_grid(flat ? (rows * (K / 8) + 255) / 256 : rows * per_row), wg(256);
+  if (flat) k_quant_mxfp4<DT, true><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
+  else k_quant_mxfp4<DT, false><<<grid, wg, 0, st>>>(x, x_stride, rows, K, per_row, blocks, scales);
   return hipGetLastError();
 }
 
@@ -155,9 +142,9 @@ hipError_t launch_quant_mxfp4(const void* x, int dt, int64_t rows, int K, int64_
                               uint8_t* scales, hipStream_t st) {
   const char* p = (const char*)x;
   uint32_t* b = (uint32_t*)blocks;
-  if (dt == FTM_DT_F32) return quant<FTM_DT_F32, 1>(p, x_stride, rows, K, b, scales, st);
-  if (dt == FTM_DT_F16) return quant<FTM_DT_F16, 1>(p, x_stride, rows, K, b, scales, st);
-  return quant<FTM_DT_BF16, 1>(p, x_stride, rows, K, b, scales, st);
+  if (dt == FTM_DT_F32) return quant<FTM_DT_F32>(p, x_stride, rows, K, b, scales, st);
+  if (dt == FTM_DT_F16) return quant<FTM_DT_F16>(p, x_stride, rows, K, b, scales, st);
+  return quant<FTM_DT_BF16>(p, x_stride, rows, K, b, scales, st);
 }
 
 // ------------------------------------------------------------------ activation
@@ -566,8 +553,7 @@ struct FewCall {
   int N, K, bias_dtype, act;
   float act_alpha, act_limit;
   int cap;                // rows of a workgroup, at most
-  // dense: the product's rows, dtype and result
-  int64_t rows;
+  // dense: the product's result
   void* out;
   int out_dtype;
   // a layer's first product: its pairs, and h quantised, a row a pair
@@ -1684,7 +1670,7 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
   if ((int64_t)(P - (P < c.num_experts ? P : c.num_experts)) * H * (I / 2) > (64 << 20)) return false;
   if ((int64_t)2 * I * (H / 2) + 256 >= (int64_t)kNowhere) return false;
   const FewCall f = {(const char*)c.x, c.x_stride, (const char*)c.w13, c.w13_scale, c.w13_bias, (int64_t)2 * I * (H / 2),
-                     (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, 0, nullptr, 0,
+                     (int64_t)2 * I * (H / 32), 2 * I, H, c.w13_bias_dtype, c.act, c.act_alpha, c.act_limit, cap, nullptr, 0,
                      c.topk_ids, c.ids_dtype == FTM_ID_I64, P, c.num_experts, c.k, hq, hs};
   if (cols_lds<2>(H, cap) > kMaxLds - kListLds) return false;
   e = cols_moe<2>(f, c.dtype, st);
@@ -1729,7 +1715,7 @@ hipError_t launch_w4a4_dynamic(const ftm_w4a4& c, const void* x, int dt, int64_t
   if (c.offsets == nullptr && c.rows <= 8 && c.rows * c.K <= 16384 && c.K >= kMinK && offsets_ok(c) &&
       (((uintptr_t)x | (uint64_t)x_stride) & 15u) == 0) {
     const FewCall f = {(const char*)x, x_stride, (const char*)c.w, c.w_scale, c.bias, 0, 0, c.N, c.K, c.bias_dtype, c.act, c.act_alpha,
-                       c.act_limit, (int)c.rows, c.rows, c.out, c.out_dtype, nullptr, 0, 0, 1, 1, nullptr, nullptr};
+                       c.act_limit, (int)c.rows, c.out, c.out_dtype, nullptr, 0, 0, 1, 1, nullptr, nullptr};
     return few<1, 4, 4>(f, dt, st);
   }
   const hipError_t e = launch_quant_mxfp4(x, dt, c.x_rows, c.K, x_stride, (uint8_t*)const_cast<void*>(c.x),
