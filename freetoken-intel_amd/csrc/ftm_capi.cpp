@@ -290,8 +290,7 @@ W4a4MoeLayout w4a4_moe_layout(int T, int k, int E, int H, int I) {
   w.xs = take((size_t)T * (H / 32));
   w.hq = take(P * (I / 2));
   w.hs = take(P * (I / 32));
-  w.h = take(4 * P * I);
-  w.y = take(4 * P * H);
+  w.h = w.y = take(4 * P * (I > H ? I : H));  // h is quantised before the second product writes y
   w.sort = take(sort_workspace_bytes((int64_t)P, E));
   w.total = o;
   return w;

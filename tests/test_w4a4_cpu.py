@@ -98,6 +98,16 @@ def test_moe_arguments():
     assert call(T=0, x=None) == nat.OK
 
 
+@pytest.mark.parametrize("T,k,E,H,I", [(2048, 4, 32, 2880, 2880), (2048, 8, 128, 2048, 768), (512, 2, 16, 1024, 4096)])
+def test_moe_workspace_holds_fp32_rows_once(T, k, E, H, I):
+    """h is dead when the second product writes its rows, so one buffer holds both: beside it the codes and
+    scales of x and h, the tables (three of the pairs, the offsets, the sort's) and borders of 256 bytes."""
+    L, P = nat.lib(), T * k
+    need = L.ftm_w4a4_moe_workspace_bytes(T, k, E, H, I)
+    rest = T * (H // 2 + H // 32) + P * (I // 2 + I // 32) + 12 * P + 4 * (E + 1) + L.ftm_sort_workspace_bytes(T, k, E)
+    assert 4 * P * max(H, I) + rest <= need <= 4 * P * max(H, I) + rest + 12 * 256
+
+
 def test_no_cpu_tensors():
     x = torch.zeros(2, 64)
     b, s = torch.zeros(2, 2, 16, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8)
