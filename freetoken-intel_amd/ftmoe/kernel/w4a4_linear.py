@@ -30,11 +30,14 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``x [..., K]`` (fp32, fp16 or bf16; K a multiple of 32) -> (uint8 blocks
-    ``[..., K/32, 16]``, uint8 e8m0 scales ``[..., K/32]``): the bytes of
-    :func:`~ftmoe.quant.quantize_mxfp4_blocks`.  A block's scale is the least power of two 2^e with
+    ``[..., K/32, 16]``, uint8 e8m0 scales ``[..., K/32]``).  A block's scale is the least power of two 2^e with
     max |x| <= 6 * 2^e (the maximum taken as at least 1e-12); a value's code the nearest
     of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to |x| / 2^e, ties to the smaller.  A block with an
-    infinity or NaN gets the scale 255 (NaN) and codes 0: its products are NaN, and so are its values."""
+    infinity or NaN gets the scale 255 (NaN) and codes 0: its products are NaN, and so are its values.
+
+    The rule of :func:`~ftmoe.quant.quantize_mxfp4_blocks`, and its bytes for every other block of bf16 or fp16; in
+    fp32 that function finds e by a logarithm, which rounds to a whole number where the maximum is a few
+    steps above 6 * 2^e (up to 33, where 2^e is far from 1): there it keeps e, this has e + 1."""
     nat.require_gpu(x, "x")
     dt = _dt(x.dtype, "x")
     if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % _QBLOCK != 0:

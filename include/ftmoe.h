@@ -322,9 +322,11 @@ int ftm_w8a8_linear_dynamic(const void* x, int32_t x_dtype, int64_t x_stride, co
 /* Quantise rows x [rows, K] (x_stride bytes apart, K a multiple of 32): of each block
  * of 32, with a = max(max |x|, 1e-12), scale = e + 127 for the least whole number e with
  * a <= 6 * 2^e, and per value the code of the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
- * |x| / 2^e, ties to the smaller, with x's sign unless it is 0: the bytes of
- * quantize_mxfp4_blocks (python/freetoken/kernel/triton/mxfp4_linear.py:79-111).  A
- * block with an infinity or NaN gets the scale 255 (the format's NaN) and codes 0.
+ * |x| / 2^e, ties to the smaller, with x's sign unless it is 0: the rule of
+ * quantize_mxfp4_blocks (python/freetoken/kernel/triton/mxfp4_linear.py:79-111), and its bytes
+ * but for two kinds of block.  One with an infinity or NaN gets the scale 255 (the format's NaN)
+ * and codes 0.  An fp32 one whose a is a few fp32 steps above 6 * 2^e (up to 33, where 2^e is far
+ * from 1) gets e + 1, where the logarithm there rounds to e.
  * blocks [rows, K/32, 16], 4-byte aligned; scales [rows, K/32]. */
 int ftm_quant_mxfp4(const void* x, int32_t x_dtype, int64_t rows, int32_t K, int64_t x_stride,
                     uint8_t* blocks, uint8_t* scales, void* stream);

@@ -170,6 +170,22 @@ def test_quantiser_scales(gpu, dtype):
         assert torch.equal(s.cpu(), rs) and torch.equal(b.cpu(), rb)
 
 
+@pytest.mark.parametrize("e", [-40, -8, -1, 0, 1, 10, 40, 100])
+def test_quantiser_fp32_above_the_largest_code(gpu, e):
+    """fp32 maxima next to 6 2^e: the scale by whole numbers; the bytes of the torch function but in the few
+    steps above, where its logarithm may round to e."""
+    steps = torch.arange(-40, 41, dtype=torch.int32)
+    x = torch.zeros(len(steps), 32)
+    x[:, 5] = (torch.tensor(6.0 * 2.0 ** e).view(torch.int32) + steps).view(torch.float32)
+    x[:, 9] = -x[:, 5] / 3
+    b, s = (t.cpu() for t in quantize_mxfp4(x.to(gpu)))
+    assert torch.equal(s[:, 0].int(), torch.where(steps > 0, e + 1, e).int() + 127)
+    rb, rs = quant.quantize_mxfp4_blocks(x)
+    same = (steps <= 0) | (steps > 33)
+    assert torch.equal(s[same], rs[same]) and torch.equal(b[same], rb[same])
+    assert (rs[~same] <= s[~same]).all()
+
+
 def test_quantiser_fp32_next_to_ties(gpu):
     """fp32 has values one step over a border, which go up."""
     v = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
