@@ -278,7 +278,9 @@ constexpr int kMinK = 256;  // of the kernels that take the scales eight at a ti
 // bytes between rows (an odd number of eights: 16 rows hit distinct banks).  A lane
 // has a row of each 64 (of 32 or 16 rows two or four lanes one, in turn); `p` says where they begin.  The
 // first kFlight loads of each are under way when the copies of the operands are
-// requested (`then`), before any of them is waited for.
+// requested (`then`), before any of them is waited for.  As compiled a fill ends with a
+// wait for all that is under way, these copies too, whether the loop over the rest of the
+// scales runs or not: all stages of a ring have landed when its first is used.
 __host__ __device__ constexpr int scale_pitch(int per) { return 8 * (per | 1); }
 template <int R>
 struct FillScales {
@@ -571,9 +573,10 @@ __host__ __device__ constexpr int few_wave_lds(int per, int rows) {
 }
 
 // Up to 16 tokens whose values are still wide, one weight: a workgroup quantises them
-// itself, each wave the K that it multiplies, while its weights are under way, and
+// itself, each wave the K that it multiplies, requested together with its scales and the first S stages of
+// its weights (and quantised when these have landed: FillScales), and
 // multiplies them by a tile of 16 NT weight rows, K split over the waves as in k_w4a4_split.
-// Bound by two round trips one behind the other: 1 x 1536 x 2048 5.3 us.
+// Bound by two round trips one behind the other: 1 x 1536 x 2048 5.1 us.
 template <int XDT, int NT, int NW, int S>
 __global__ __launch_bounds__(64 * NW) void k_w4a4_few(FewCall c) {
   using V = Vec8<XDT>;
@@ -867,7 +870,7 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
     }
     for (int s = turn + 8 * kTurns; s < nsteps; s += 4 * kTurns) *(u32x2*)(xscales + rs * pitch + 8 * s) = fit_scales(load_scales(xs, s, nb), s, nb);
     wait_vm<2 * S>();  // the rows' copies have landed
-    __syncthreads();
+    __syncthreads();   // (compiled with a wait for the ring's as well)
   }
   f32x4 acc[MT];
   int xr[MT];
@@ -951,7 +954,7 @@ __global__ __launch_bounds__(256) void k_w4a4_cols(Call c, int ntiles) {
 // split over the waves; a step's results are weighted by its expert's weight and added
 // up in fp32, the waves' sums in order, so the order is the same in each call.  h comes
 // from memory (every lane of a group the same block), the weights through LDS.  Bound by
-// the workgroups' chains, of which two rounds are resident: 128 experts at 1 token 3.4 us, 32 of 2880 at
+// the workgroups' chains, of which two rounds are resident: 128 experts at 1 token 4.4 us, 32 of 2880 at
 // 8 tokens 31 us (82 MB from memory, 141 MB into LDS).  One workgroup for all tokens of its
 // channels, so that weights are read once, lost: 34 us there, 128 experts at 16 tokens 19.0 to
 // 25.9.
@@ -1051,7 +1054,9 @@ __global__ __launch_bounds__(64 * NW) void k_w4a4_few_down(ftm_w4a4_moe c, const
 // one barrier a step; scale bytes through registers into two slots of LDS, one step
 // ahead.  Few large waves: a step reads (16 MI + 16 NJ) rows of LDS a wave for 16 MI x 16 NJ
 // results, and with one wave a SIMD every other instruction is written into the
-// shadow of an MFMA (16 cycles), in the order in which it is to be issued.  A workgroup
+// shadow of an MFMA (16 cycles), in the order in which it is to be issued.  So it is compiled for
+// 256 x 256; of the others the compiler takes some steps of a tile apart and puts their copies in one burst
+// before their products: the first of 64 x 256, the last of 128 x 256, the last two of 128 x 128.  A workgroup
 // takes one tile after another, and the copies run on from tile to tile.  Bound by power and
 // MFMA issue where a tile is large (4096 x 12288 x 4096 105 to 109 us, 3.9 POP/s; MFMA busy 44 % of the
 // cycles), by the copies of a step where it is small.
@@ -1546,23 +1551,27 @@ bool offsets_ok(const ftm_w4a4& c) {
 
 }  // namespace
 
-// Rows an expert with rows has, if all have the same.
+// The mean rows of the experts that can have any.
 static int64_t rows_an_expert(const ftm_w4a4& c) {
   const int64_t hit = c.rows < c.num_experts ? c.rows : c.num_experts;
   return (c.rows + hit - 1) / hit;
 }
 constexpr int kTileRows = 16, kLargeRows = 96;  // an expert: from these on tiles of 64 x 256, of 256 x 256
 
-// By the rows an expert has.  In us, for 128 experts of [2 x 768, 2048], of [2048, 768], and 32
-// of [2 x 2880, 2880]:
+// By the rows an expert has.  In us, for 128 experts of [2 x 768, 2048] through an index, of [2048, 768], and 32
+// of [2 x 2880, 2880] through an index, by the mean rows of an expert; their popularity is uneven (at a mean of
+// 256 rows 25 to 1000), so that of few rows not all are hit, and of many most tiles of 256 are partly filled:
 //                     1 row              4 rows             8 rows             12 rows
-//   cols of 8         26.7  15.3  40.1   41.0  23.6  61.6   49.2  33.3  79.4   58.0  42.5  97.8
-//   cols of 16        26.4  14.8  42.7   41.9  21.4  61.8   48.3  27.6  71.4   51.0  31.9  79.2
-//   tiles 64 x 256                       51.3  28.3         53.5  29.7  83.7   54.2  30.6  84.0
+//   cols of 8         25.0  15.3  41.2   40.7  23.4  61.4   49.8  33.4  79.2   58.2  42.3  97.8
+//   cols of 16        24.4  14.9  44.7   41.7  21.5  61.7   48.2  27.6  71.4   51.6  33.3  77.7
+//   tiles 64 x 256                       50.0  28.4  79.8   51.8  30.4  82.7   53.4  31.8  82.4
 //                     16 rows            64 rows            96 rows            128 rows
-//   cols of 16        56.8  36.6
-//   tiles 64 x 256    57.4  33.6         71.8  48.9         90.2  57.2  139.8  100.2  67.0
-//   tiles 256 x 256                      92.3  57.8         92.8  58.6  128.4   94.3  60.6
+//   cols of 16        56.8  36.8  88.7
+//   tiles 64 x 256    56.7  34.1  84.2   68.8  48.8 117.1   84.5  57.8 136.6   94.3  66.8
+//   tiles 256 x 256                      90.4  57.0 109.8   90.5  58.4 128.9   92.3  59.7
+// The same rows for every expert, gate_up, 128 experts and 32: tiles of 64 at 64 rows 52.0 and 78.0, of 256 70.0 and
+// 96.0; at 96 rows 75.0 and 123.0, 71.5 and 98.0; at 128 rows 77.0 and 125.4, 73.3 and 99.5.  At 16 rows cols of
+// 16 would be the faster there, 48.0 and 69.5, tiles of 64 50.1 and 74.3.
 // Tiles of 128 x 256 (94.2, 53.6, 133.0 at 96 rows) gain less than 7% and only there.  Where
 // the codes of few rows do not fit the LDS (K above 13 thousand) it is tiles too.
 static hipError_t grouped(const ftm_w4a4& c, hipStream_t st) {
@@ -1687,8 +1696,8 @@ bool launch_w4a4_moe_few(const ftm_w4a4_moe& c, uint8_t* hq, uint8_t* hs, hipStr
 // those of zeros, on tiles left as they were.
 hipError_t launch_w4a4_quantised(const ftm_w4a4& c, float* h, uint8_t* out_scale, hipStream_t st) {
   const int64_t seg = rows_an_expert(c);
-  // In us, tiles of 64 x 256, 128 x 256 and 256 x 256, with the quantisation in the epilogue, for 128
-  // experts of [2 x 768, 2048] and 32 of [2 x 2880, 2880]: 64 rows an expert 72.9, 79.7, 110.8 and
+  // In us, on uneven popularity as above, tiles of 64 x 256, 128 x 256 and 256 x 256, with the quantisation in the
+  // epilogue, for 128 experts of [2 x 768, 2048] and 32 of [2 x 2880, 2880]: 64 rows an expert 72.9, 79.7, 110.8 and
   // 119.3, 122.1, 124.8; 96 rows 91.5, 91.8, 113.5 and 139.8, 129.9, 149.3; 128 rows 102.3, 96.9, 114.6
   // and 172.2, 144.8, 159.6; 200 rows 134.2, 134.8, 140.6 and 227.0, 176.9, 171.2; 256 rows 166.6, 145.5,
   // 142.4 and 267.5, 207.1, 197.8.
